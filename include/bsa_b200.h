@@ -188,6 +188,77 @@ int bsa_forward_noalloc(const void* q, const void* k, const void* v, int dtype, 
                         int rope_dh, int rope_dw, int rope_T, int rope_H, int rope_W, void* q_rot, void* k_rot,
                         int32_t* block_indices, void* out, const int64_t* out_strides, void* stream);
 
+/* ---- dense side of the attention hook ----
+ * q/k norm with rotary positions, attention over key intervals, and an 8-bit key/value cache.  Tensors are
+ * [B, H, S, D] with element strides (sb, sh, ss) and d contiguous, D a multiple of 8 up to 128; bases and
+ * strides are multiples of 16 bytes.
+ *
+ * bsa_norm_rope: q/k RMSNorm (blocks.py:55-73) and 3-axis rotary positions (rope_3d.py:107-128) of one or two
+ * tensors in one launch: y = R(start + s) (w * x * rsqrt(mean(x^2) + eps)), fp32 throughout, rounded once.
+ * w0 / w1 (w_dtype, [D]; NULL: no norm), rope (NULL: no rotation) as in bsa_mean_pool; the tokens of x stand at
+ * places start .. start + S - 1 of the rope grid.  x1 NULL: one tensor.  Outputs are contiguous.
+ * bsa_norm_rope_backward: gradients dx (contiguous) of the inputs and dw ([D] fp32, NULL: none) of the weights
+ * from the outputs' gradients g; scratch (bsa_norm_rope_backward_scratch_bytes(D)) is needed for the weights'.
+ * Sums are taken in a fixed order. */
+int bsa_norm_rope(const void* x0, const int64_t* x0_strides, int H0, const void* w0, void* y0, const void* x1,
+                  const int64_t* x1_strides, int H1, const void* w1, void* y1, int dtype, int w_dtype, int B, int S,
+                  int D, float eps, const float* rope, int rope_dt, int rope_dh, int rope_dw, int rope_T, int rope_H,
+                  int rope_W, int start, void* stream);
+int64_t bsa_norm_rope_backward_scratch_bytes(int D);
+int bsa_norm_rope_backward(const void* x0, const int64_t* x0_strides, const void* g0, const int64_t* g0_strides, int H0,
+                           const void* w0, void* dx0, float* dw0, const void* x1, const int64_t* x1_strides,
+                           const void* g1, const int64_t* g1_strides, int H1, const void* w1, void* dx1, float* dw1,
+                           int dtype, int w_dtype, int B, int S, int D, float eps, const float* rope, int rope_dt,
+                           int rope_dh, int rope_dw, int rope_T, int rope_H, int rope_W, int start, void* scratch,
+                           void* stream);
+
+/* bsa_attention_ranges: key intervals for bsa_masked_attention.  ranges ([batch, Sq] pairs, 8-byte aligned)
+ * receives the keys [lo, hi) of every row, table ([batch, ceil(Sq / 128)] quadruples, 16-byte aligned) what the
+ * kernels need of each 128 rows.  given (NULL: none): the caller's own intervals, clamped to [0, Sk].  Else:
+ * documents (q_offsets, k_offsets: [documents + 1] int32 each, ascending, shared by the batch) or lengths
+ * (q_lengths, k_lengths: [batch], each optional; k_add is added to every key length) or one document.  Query i'
+ * of a document of qn queries and kn keys stands at key place a = i' + kn - qn and sees a + 1 keys (causal) or
+ * all; with a prefix (prefix, or prefixes[document or batch entry]) rows at a < prefix see exactly the prefix.
+ * Rows outside every document or behind their length see nothing. */
+int bsa_attention_ranges(int32_t* ranges, int32_t* table, int batch, int Sq, int Sk, const int32_t* given, int causal,
+                         int prefix, const int32_t* prefixes, const int32_t* q_offsets, const int32_t* k_offsets,
+                         int documents, const int32_t* q_lengths, const int32_t* k_lengths, int k_add, void* stream);
+
+/* bsa_masked_attention: softmax attention of q [B, H, Sq, D] over k, v [B, Hk, Sk, D] (H a multiple of Hk: head
+ * h reads key head h / (H / Hk)), fp16 or bf16.  ranges / table (both NULL: every key) hold ranges_batch (1 or B)
+ * entries.  softcap > 0: scores are softcap * tanh(s / softcap).  A row without keys gives zeros, and -inf in lse
+ * ([B, H, Sq] fp32, natural logarithm, NULL: not wanted).  scratch: bsa_masked_attention_scratch_bytes() bytes
+ * (0: none needed).  Scores of unseen keys never count, whatever they hold; so do values of keys that no row
+ * of the same 256 rows sees.  A value that is infinite or NaN and seen by one row can reach another row of
+ * the same tile. */
+int64_t bsa_masked_attention_scratch_bytes(int B, int H, int Sq, int Sk, int D);
+int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype, int B, int H, int Hk, int Sq, int Sk,
+                         int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         const int32_t* ranges, const int32_t* table, int ranges_batch, float sm_scale, float softcap,
+                         void* out, const int64_t* out_strides, float* lse, void* scratch, void* stream);
+
+/* 8-bit key/value cache: codes [B, Hk, capacity, D] e4m3, contiguous, 16-byte aligned; scales
+ * [B, Hk, capacity / 64] fp32, each the smallest power of two that keeps the block's codes within 448 (0: a block
+ * of zeros); lengths [B] int32: tokens held.  capacity is a multiple of 64.
+ * bsa_kv8_append: n new tokens (fp16 or bf16; counts [B]: only the first counts[b] of them) behind those held;
+ * lengths advance.  Tokens past the capacity are dropped and reported by bsa_device_error (BSA_ERR_INDEX).
+ * Rows behind the last token keep what they hold.
+ * bsa_kv8_unpack: held tokens, then n fresh ones, then zeros, as [B, Hk, rows, D] in dtype.
+ * bsa_kv8_attention: q [B, H, Sq, D] over the held tokens, straight from the codes; causal: query i sees
+ * lengths[b] - Sq + i + 1 tokens.  Meant for few rows (H / Hk * Sq up to about 64): 16 rows are one pass over the
+ * codes.  scratch: bsa_kv8_attention_scratch_bytes() bytes (0: none needed). */
+int bsa_kv8_append(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
+                   int capacity, int D, const void* k, const void* v, int dtype, int n, const int64_t* k_strides,
+                   const int64_t* v_strides, const int32_t* counts, void* stream);
+int bsa_kv8_unpack(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
+                   int capacity, int D, const void* k, const void* v, int dtype, int n, const int64_t* k_strides,
+                   const int64_t* v_strides, void* k_out, void* v_out, int rows, void* stream);
+int64_t bsa_kv8_attention_scratch_bytes(int B, int H, int Hk, int Sq, int capacity, int D);
+int bsa_kv8_attention(const void* q, int dtype, int B, int H, int Sq, const int64_t* q_strides, const void* k_codes,
+                      const float* k_scale, const void* v_codes, const float* v_scale, const int32_t* lengths, int Hk,
+                      int capacity, int D, int causal, float sm_scale, void* out, const int64_t* out_strides,
+                      void* scratch, void* stream);
+
 /* ---- peer exchange helpers (sequence-parallel all-to-all over NVLink by the copy engines) ----
  * No counterpart in the reference (the MLX port has no multi-GPU path; the upstream PyTorch model
  * used NCCL all-to-all).  These are the only allocating entry points: the exchange owns a few

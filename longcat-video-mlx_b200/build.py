@@ -18,8 +18,9 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "longcat_video", "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libbsa_b200.so")
-SOURCES = ["bsa_capi.cu", "bsa_attn.cu", "bsa_score.cu", "bsa_route.cu", "bsa_noalloc.cu", "bsa_xfer.cu"]
-HEADERS = ["bsa_ptx.cuh", "bsa_kernels.h", "bsa_select.cuh"]
+SOURCES = ["bsa_capi.cu", "bsa_attn.cu", "bsa_score.cu", "bsa_route.cu", "bsa_noalloc.cu", "bsa_xfer.cu",
+           "bsa_dense_capi.cu", "bsa_normrope.cu", "bsa_ranges.cu", "bsa_kv8.cu", "bsa_dense.cu"]
+HEADERS = ["bsa_ptx.cuh", "bsa_kernels.h", "bsa_select.cuh", "bsa_dense.h", "bsa_dense.cuh", "bsa_rows.cuh"]
 
 
 def nvcc_path() -> str:
@@ -42,7 +43,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
+    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "--threads", "0",
            "-shared", "-Xcompiler", "-fPIC", "-I", os.path.join(REPO, "include"),
            "-o", LIB_PATH + ".tmp"] + [os.path.join(CSRC, f) for f in SOURCES]
     if verbose:

@@ -12,6 +12,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
+#include "bsa_dense.h"
 #include "bsa_kernels.h"
 
 namespace {
@@ -262,6 +263,7 @@ int set_error(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
 }  // namespace bsa
 
 extern "C" {
@@ -282,7 +284,10 @@ int bsa_device_error(int clear) {
   const int a = bsa::attn_device_error(clear);
   const int s = bsa::score_device_error(clear);
   const int r = bsa::route_device_error(clear);
-  return a ? a : (s ? s : r);
+  const int c = bsa::cache_device_error(clear);
+  const int d = bsa::dense_device_error(clear);
+  const int first = a ? a : (s ? s : r);
+  return first ? first : (c ? c : d);
 }
 
 int bsa_mean_pool(const void* x, int dtype, int B, int H, int S, int D, int64_t sb, int64_t sh, int64_t ss, int T,

@@ -1,0 +1,546 @@
+// Dense attention over key intervals, forward, on sm_100a (tcgen05 + TMA + TMEM).
+//
+//   z_ij = s_ij = sm_scale q_i . k_j, or cap tanh(s_ij / cap);   p_ij = 2^(z_ij log2(e) - m_i) for j in [lo_i, hi_i)
+//   o_i = sum_j p_ij v_j / l_i,  l_i = sum_j p_ij,  lse_i = ln sum_j e^z_ij        (0 and -inf for an empty row)
+//
+// One pass over the keys with a running maximum and sum, scores and output accumulators in tensor memory.
+// A CTA takes up to two query tiles of 128 rows of one head: while the softmax warps of one tile work on its
+// scores, the tensor cores run the other tile's products, and each key and value tile is loaded once for both.
+//     S_t[128 x 128] = Q_t K^T         A = Q_t, B = K, both in shared memory
+//     O_t[128 x D]  += P_t V           A = P_t in tensor memory, over the scores it came from; B = V
+// TMEM: S_0, S_1, O_0, O_1 of 128 columns each.
+//
+// Roles (320 threads, one CTA to an SM):
+//   warps 0-3, 4-7 : softmax of tile 0, 1; a thread owns one row, so neither maximum nor sum leaves it
+//   warp 8         : issues every product, in the order S_0(0) S_1(0) [P_0 V, S_0(j+1), P_1 V, S_1(j+1)] ...;
+//                    products of one thread run in order, so S_t(j+1) may overwrite the P_t(j) that was read
+//                    before it, and its arrival also says that O_t holds all of P_t V up to j
+//   warp 9         : loads; one ring for K and V tiles in the order of their use
+// The maximum is raised, and O and l rescaled, only when a score exceeds it by more than 2^8: P stays within
+// fp16's range and rounding is relative, so the result is as exact as with the true maximum.
+// P is rounded to the input type for the tensor cores; l is summed from the fp32 values.
+//
+// Masked places never reach a result: scores are replaced by -inf whatever they hold, and V rows that no row
+// of the CTA sees are zeroed in shared memory (0 * NaN would be NaN).  Tiles outside the union of the rows'
+// intervals are not loaded; tiles inside all of them are not compared.
+// Every wait is bounded (bsa_ptx.cuh).
+#include <climits>
+#include <mutex>
+#include "bsa_dense.cuh"
+
+namespace bsa {
+namespace dense {
+
+__device__ int g_dense_err;
+
+constexpr int kThreads = 320;
+constexpr float kRescale = 8.f;  // log2
+constexpr uint32_t kTmemCols = 512;
+__host__ __device__ constexpr uint32_t col_s(int t) { return 128u * static_cast<uint32_t>(t); }
+__host__ __device__ constexpr uint32_t col_o(int t) { return 256u + 128u * static_cast<uint32_t>(t); }
+
+template <int DP>
+struct Smem {
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kTiles = (2 + kStages) * tile_bytes<DP>();
+  uint64_t q_full;
+  uint64_t full[kStages], empty[kStages];
+  uint64_t fix;
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t drain;
+  uint32_t tmem;
+  int abort_flag;
+};
+template <int DP>
+constexpr int smem_bytes() { return Smem<DP>::kTiles + static_cast<int>(sizeof(Smem<DP>)) + 1024; }
+
+struct Params {
+  const int2* ranges;  // [Bm][Sq], null: all keys
+  const int4* table;   // [Bm][q_tiles]
+  int Bm, H, G, Sq, Sk, D;
+  int q_tiles;         // tiles of 128 rows
+  int per_cta;         // 1 or 2 query tiles
+  int groups;          // CTAs along the rows
+  int splits;          // CTAs along the keys
+  float scale_log2;    // sm_scale log2(e)
+  float cap_in;        // 2 sm_scale log2(e) / cap
+  float cap_log2;      // cap log2(e)
+  void* out;
+  long long ob, oh, os;
+  float* lse;
+  float* part;         // splits > 1: [splits][B * H * Sq][D + 1]: o, then lse in log2
+  long long rows;      // B * H * Sq
+};
+
+template <int DP, bool kBF16, bool kCap>
+__global__ void __launch_bounds__(kThreads, 1)
+    dense_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  using S = Smem<DP>;
+  constexpr int kStages = S::kStages;
+  constexpr int kBytes = tile_bytes<DP>();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + 2 * kBytes;
+  S& ss = *reinterpret_cast<S*>(smem + S::kTiles);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // (b, h) outside, then the rows, the last tiles first (they see the most keys under a causal mask), then splits
+  int item = blockIdx.x;
+  const int split = item % p.splits;
+  item /= p.splits;
+  const int grp = p.groups - 1 - item % p.groups;
+  const int bh = item / p.groups;
+  const int b = bh / p.H, h = bh - b * p.H;
+  const int hk = h / p.G;
+  const int tile0 = grp * p.per_cta;
+  const int tiles = min(p.per_cta, p.q_tiles - tile0);
+  const int bm = p.Bm > 1 ? b : 0;
+  int4 tab[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    tab[t] = make_int4(INT_MAX, 0, 0, 0);
+    if (t < tiles) tab[t] = p.table ? p.table[bm * p.q_tiles + tile0 + t] : make_int4(0, p.Sk, 0, p.Sk);
+  }
+  const int lo_u = min(tab[0].x, tab[1].x), hi_u = max(tab[0].y, tab[1].y);
+  int n0 = 0, n1 = 0;
+  if (lo_u < hi_u) {
+    n0 = lo_u / kTile;
+    n1 = (hi_u + kTile - 1) / kTile;
+    if (p.splits > 1) {
+      const int per = (n1 - n0 + p.splits - 1) / p.splits;
+      n0 = min(n1, n0 + split * per);
+      n1 = min(n1, n0 + per);
+    }
+  }
+  const int steps = n1 - n0;
+
+  if (tid == 0) {
+    mbar_init(&ss.q_full, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&ss.full[i], 1);
+      mbar_init(&ss.empty[i], 1);
+    }
+    mbar_init(&ss.fix, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&ss.s_full[t], 1);
+      mbar_init(&ss.p_full[t], 4);
+      mbar_init(&ss.o_full[t], 1);
+    }
+    mbar_init(&ss.drain, 1);
+    ss.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&ss.tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ss.tmem;
+  volatile int* abort_flag = &ss.abort_flag;
+  int* err = &g_dense_err;
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------ loads
+    if (steps > 0) {
+      if (lane == 0) {
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        mbar_arrive_expect_tx(&ss.q_full, static_cast<uint32_t>(tiles * kBytes));
+        for (int t = 0; t < tiles; ++t)
+          load_tile<DP>(sQ + t * kBytes, &tm_q, &ss.q_full, (tile0 + t) * kTile, h, b);
+      }
+      int slot = 0, issued = 0, fixes = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; i < 2 * steps && ok; ++i) {
+        if (issued >= kStages) {
+          ok = mbar_wait(&ss.empty[slot], phase ^ 1u, abort_flag, err, 301);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        const int row = (n0 + (i >> 1)) * kTile;
+        uint8_t* dst = sKV + slot * kBytes;
+        // V rows of this tile that no row of the CTA sees, but the tensor holds
+        const bool fix = (i & 1) && (row < lo_u || min(row + kTile, p.Sk) > hi_u);
+        if (!fix) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&ss.full[slot], kBytes);
+            load_tile<DP>(dst, (i & 1) ? &tm_v : &tm_k, &ss.full[slot], row, hk, b);
+          }
+        } else {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&ss.fix, kBytes);
+            load_tile<DP>(dst, &tm_v, &ss.fix, row, hk, b);
+          }
+          __syncwarp();
+          ok = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 302);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          ++fixes;
+          for (int r = 0; r < kTile; ++r)
+            if (row + r < lo_u || row + r >= hi_u) zero_row<DP>(dst, r, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss.full[slot]);
+        }
+        ++issued;
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok && lane == 0) {
+        // wind-down after an expired wait: no load into this CTA's shared memory may still be in flight
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&ss.q_full, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+        }
+        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          while (!mbar_try_wait(&ss.full[i % kStages], static_cast<uint32_t>((i / kStages) & 1)) &&
+                 globaltimer_ns() - t0 < kWaitLimitNs) {
+          }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ products
+    if (lane == 0 && steps > 0) {
+      constexpr uint32_t kIdQK = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
+      constexpr uint32_t kIdPV = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
+      const uint32_t qb = smem_u32(sQ), kvb = smem_u32(sKV);
+      auto qk = [&](int t, int slot) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+          umma_ss(tmem + col_s(t), desc_d(qb + t * kBytes, kk), desc_d(kvb + slot * kBytes, kk), kIdQK, kk > 0);
+        umma_commit(&ss.s_full[t]);
+      };
+      int slot = 0;
+      uint32_t phase = 0;
+      auto next = [&] {
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      };
+      bool ok = mbar_wait(&ss.q_full, 0, abort_flag, err, 311) && mbar_wait(&ss.full[0], 0, abort_flag, err, 312);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < tiles; ++t) qk(t, 0);
+        umma_commit(&ss.empty[0]);
+        next();
+      }
+      for (int j = 0; j < steps && ok; ++j) {
+        const int vs = slot;
+        ok = mbar_wait(&ss.full[vs], phase, abort_flag, err, 313);
+        if (!ok) break;
+        next();
+        const int ks = slot;
+        const uint32_t kphase = phase;
+        const bool more = j + 1 < steps;
+        for (int t = 0; t < tiles; ++t) {
+          ok = mbar_wait(&ss.p_full[t], static_cast<uint32_t>(j & 1), abort_flag, err, 314);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ts(tmem + col_o(t), tmem + col_s(t) + 8 * kk, desc_rows(kvb + vs * kBytes, kk), kIdPV, j > 0 || kk > 0);
+          if (more) {
+            if (t == 0) ok = mbar_wait(&ss.full[ks], kphase, abort_flag, err, 315);
+            if (!ok) break;
+            tc_fence_after();
+            qk(t, ks);
+          } else {
+            umma_commit(&ss.o_full[t]);
+          }
+        }
+        if (!ok) break;
+        umma_commit(&ss.empty[vs]);
+        if (more) {
+          umma_commit(&ss.empty[ks]);
+          next();
+        }
+      }
+      // teardown: this thread's products complete before the tensor memory is released
+      umma_commit(&ss.drain);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(&ss.drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const int t = warp >> 2;
+    const int row = (tile0 + t) * kTile + 32 * (warp & 3) + lane;
+    const uint32_t la = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+    const bool live = t < tiles && row < p.Sq;
+    if (t < tiles) {
+      int lo = 0, hi = p.Sk;
+      if (p.ranges && live) {
+        const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
+        lo = r.x;
+        hi = r.y;
+      }
+      const int lo_max = tab[t].z, hi_min = tab[t].w;
+      float m = -INFINITY;
+      float l0 = 0.f, l1 = 0.f;
+      bool ok = true;
+      for (int j = 0; j < steps; ++j) {
+        ok = mbar_wait(&ss.s_full[t], static_cast<uint32_t>(j & 1), abort_flag, err, 321);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(la + col_s(t) + 32 * c, r + 32 * c);
+        tmem_ld_wait();
+        const int key0 = (n0 + j) * kTile;
+        if constexpr (kCap) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            r[e] = __float_as_uint(p.cap_log2 * tanh_of(__uint_as_float(r[e]) * p.cap_in));
+        }
+        if (key0 < lo_max || key0 + kTile > hi_min) {
+          const uint32_t n = static_cast<uint32_t>(hi - lo);
+          const uint32_t d = static_cast<uint32_t>(key0 - lo);
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (d + e >= n) r[e] = 0xff800000u;
+        }
+        float mv[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mv[e] = __uint_as_float(r[e]);
+#pragma unroll
+        for (int c = 8; c < 128; c += 8)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mv[e] = fmaxf(mv[e], __uint_as_float(r[c + e]));
+        const float top = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])),
+                                fmaxf(fmaxf(mv[4], mv[5]), fmaxf(mv[6], mv[7])));
+        const float scale = kCap ? 1.f : p.scale_log2;
+        const float mx = top * scale;
+        float f = 1.f;
+        const bool raise = mx > m + kRescale || (m == -INFINITY && mx > m);
+        if (raise) {
+          f = ex2_approx(m - mx);  // 0 for the first maximum
+          m = mx;
+          l0 *= f;
+          l1 *= f;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(la + col_o(t) + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st32(la + col_o(t) + 32 * c, o);
+          }
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(nm, nm);
+        uint64_t l2 = f2_pack(l0, l1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int i = 64 * c + 2 * e;
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sc2, nm2), x0, x1);
+            x0 = ex2_approx(x0);
+            x1 = ex2_approx(x1);
+            l2 = f2_add(l2, f2_pack(x0, x1));
+            pk[e] = pack16<kBF16>(x0, x1);
+          }
+          tmem_st32(la + col_s(t) + 32 * c, pk);
+        }
+        f2_unpack(l2, l0, l1);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss.p_full[t]);
+      }
+      // ---- o / l and the row's log sum
+      if (ok && steps > 0) {
+        ok = mbar_wait(&ss.o_full[t], 0, abort_flag, err, 322);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      if (ok) {
+        const float l = l0 + l1;
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+        const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+        const long long flat = static_cast<long long>(bh) * p.Sq + row;
+        float* part = p.splits > 1 ? p.part + (split * p.rows + flat) * (p.D + 1) : nullptr;
+        const long long off = b * p.ob + h * p.oh + static_cast<long long>(row) * p.os;
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld32(la + col_o(t) + 32 * c, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          float v[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+          if (live) {
+#pragma unroll
+            for (int e8 = 0; e8 < 4; ++e8) {
+              const int d0 = 32 * c + 8 * e8;
+              if (d0 < p.D) {
+                if (part) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) part[d0 + e] = v[8 * e8 + e];
+                } else {
+                  store8<kBF16>(p.out, off + d0, v + 8 * e8);
+                }
+              }
+            }
+          }
+        }
+        if (live) {
+          if (part) part[p.D] = lse2;
+          else if (p.lse) p.lse[flat] = lse2 * 0.6931471805599453f;
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Joins the key splits of a row, always in their order: o = sum 2^(lse_s - m) o_s / sum 2^(lse_s - m).
+template <bool kBF16>
+__global__ void __launch_bounds__(128) dense_join_kernel(const Params p) {
+  constexpr int kLanes = 16;
+  const long long row = static_cast<long long>(blockIdx.x) * (128 / kLanes) + threadIdx.x / kLanes;
+  const int d0 = 8 * (threadIdx.x % kLanes);
+  if (row >= p.rows || d0 >= p.D) return;
+  const long long step = p.rows * (p.D + 1);
+  const float* src = p.part + row * (p.D + 1);
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, src[s * step + p.D]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const float f = exp2f(src[s * step + p.D] - base);
+    l += f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fmaf(f, src[s * step + d0 + e], v[e]);
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= inv;
+  const int i = static_cast<int>(row % p.Sq);
+  const long long bh = row / p.Sq;
+  const int h = static_cast<int>(bh % p.H);
+  store8<kBF16>(p.out, (bh / p.H) * p.ob + h * p.oh + static_cast<long long>(i) * p.os + d0, v);
+  if (p.lse && d0 == 0) p.lse[row] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int DP, bool kBF16, bool kCap>
+int launch(const CUtensorMap* maps, const Params& p, long long grid, cudaStream_t stream) {
+  auto* k = dense_fwd_kernel<DP, kBF16, kCap>;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<DP>()) != cudaSuccess)
+    return BSA_ERR_CUDA;
+  k<<<static_cast<int>(grid), kThreads, smem_bytes<DP>(), stream>>>(maps[0], maps[1], maps[2], p);
+  return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+}
+
+}  // namespace dense
+
+int make_map4(CUtensorMap* m, const Tensor4& t, int dtype, int B, int H, int S, int D, const char* name) {
+  auto enc = reinterpret_cast<CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                           const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                           CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                           CUtensorMapFloatOOBfill)>(tensor_map_encoder());
+  if (!enc) return set_error(BSA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  // an axis of one element may carry any stride: it is given one that every map accepts
+  const long long ss = S > 1 ? t.ss : D, sh = H > 1 ? t.sh : ss * S, sb = B > 1 ? t.sb : sh * H;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(H),
+                              static_cast<cuuint64_t>(B)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ss) * 2, static_cast<cuuint64_t>(sh) * 2,
+                                 static_cast<cuuint64_t>(sb) * 2};
+  const cuuint32_t box[4] = {64, dense::kTile, 1, 1}, es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, dtype == BSA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         4, t.p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(BSA_ERR_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", name, static_cast<int>(r));
+  return BSA_OK;
+}
+
+// Key splits of a call: 1 where the row tiles alone give every SM a CTA; else as many as fill them, with at
+// least 4 key tiles (512 keys) to a split, since each split costs a start and a partial output.
+int dense_pick_splits(int sms, int B, int H, int Sq, int Sk) {
+  const long long ctas = static_cast<long long>(B) * H * ((Sq + dense::kTile - 1) / dense::kTile);
+  if (ctas <= 0 || ctas * 2 > sms) return 1;
+  const int most = (Sk + 4 * dense::kTile - 1) / (4 * dense::kTile);
+  const int want = static_cast<int>(sms / ctas);
+  return want < most ? want : (most > 1 ? most : 1);
+}
+
+int launch_dense(const DenseArgs& a, int sms, cudaStream_t stream) {
+  using namespace dense;
+  CUtensorMap maps[3];
+  int rc;
+  if ((rc = make_map4(&maps[0], a.q, a.dtype, a.B, a.H, a.Sq, a.D, "q"))) return rc;
+  if ((rc = make_map4(&maps[1], a.k, a.dtype, a.B, a.Hk, a.Sk, a.D, "k"))) return rc;
+  if ((rc = make_map4(&maps[2], a.v, a.dtype, a.B, a.Hk, a.Sk, a.D, "v"))) return rc;
+  Params p = {};
+  p.ranges = a.ranges; p.table = a.table; p.Bm = a.Bm;
+  p.H = a.H; p.G = a.H / a.Hk; p.Sq = a.Sq; p.Sk = a.Sk; p.D = a.D;
+  p.q_tiles = (a.Sq + kTile - 1) / kTile;
+  // two query tiles to a CTA halve the key loads and overlap softmax and products; one each where two
+  // would leave SMs without a CTA
+  const long long bh = static_cast<long long>(a.B) * a.H;
+  p.per_cta = bh * ((p.q_tiles + 1) / 2) * a.splits >= sms ? 2 : 1;
+  p.groups = (p.q_tiles + p.per_cta - 1) / p.per_cta;
+  p.splits = a.splits;
+  p.scale_log2 = a.sm_scale * 1.4426950408889634f;
+  if (a.softcap > 0.f) {
+    p.cap_in = 2.f * p.scale_log2 / a.softcap;
+    p.cap_log2 = a.softcap * 1.4426950408889634f;
+  }
+  p.out = a.o.p; p.ob = a.o.sb; p.oh = a.o.sh; p.os = a.o.ss;
+  p.lse = a.lse;
+  p.part = a.part;
+  p.rows = bh * a.Sq;
+  const long long grid = bh * p.groups * p.splits;
+  if (grid > INT_MAX) return set_error(BSA_ERR_SHAPE, "too many row tiles for one launch");
+  const bool bf = a.dtype == BSA_DTYPE_BF16, cap = a.softcap > 0.f;
+  if (a.D > 64)
+    rc = bf ? (cap ? launch<128, true, true>(maps, p, grid, stream) : launch<128, true, false>(maps, p, grid, stream))
+            : (cap ? launch<128, false, true>(maps, p, grid, stream) : launch<128, false, false>(maps, p, grid, stream));
+  else
+    rc = bf ? (cap ? launch<64, true, true>(maps, p, grid, stream) : launch<64, true, false>(maps, p, grid, stream))
+            : (cap ? launch<64, false, true>(maps, p, grid, stream) : launch<64, false, false>(maps, p, grid, stream));
+  if (rc) return set_error(rc, "dense attention kernel launch: %s", cudaGetErrorString(cudaGetLastError()));
+  if (a.splits > 1) {
+    const int jg = static_cast<int>((p.rows + 7) / 8);
+    if (bf) dense_join_kernel<true><<<jg, 128, 0, stream>>>(p);
+    else dense_join_kernel<false><<<jg, 128, 0, stream>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return set_error(BSA_ERR_CUDA, "dense attention join launch");
+  }
+  return BSA_OK;
+}
+
+int dense_device_error(int clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, dense::g_dense_err, sizeof(int)) != cudaSuccess) return BSA_ERR_CUDA;
+  if (clear && v) {
+    const int z = 0;
+    cudaMemcpyToSymbol(dense::g_dense_err, &z, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace bsa

@@ -1,0 +1,87 @@
+// What the dense attention's forward and backward kernels share: tile geometry, tile loads, the tanh cap.
+#pragma once
+#include "bsa_dense.h"
+#include "bsa_ptx.cuh"
+
+namespace bsa {
+namespace dense {
+
+constexpr int kTile = 128;  // rows of a query tile and of a key tile
+
+// 4-D tiled load (d, token, head, batch), completion counted in bytes on `bar`.
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                            int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// A tile of 128 rows in shared memory: one 16 KB half for each 64 columns of d, rows of 128 bytes in the
+// 128-byte swizzle.  Rows past the tensor's end and columns past D arrive as zeros.
+template <int DP>
+__host__ __device__ constexpr int tile_bytes() { return kTile * DP * 2; }
+constexpr int kHalfBytes = kTile * 128;
+
+template <int DP>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int row, int h, int b) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * kHalfBytes, m, bar, 64 * c, row, h, b);
+}
+
+// Zeros in row r of a tile, by the 32 lanes of a warp: lanes split the row's 16-byte chunks.
+template <int DP>
+__device__ __forceinline__ void zero_row(uint8_t* tile, int r, int lane) {
+  constexpr int kChunks = DP / 8;
+  for (int c = lane; c < kChunks; c += 32)
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * kHalfBytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// Operand descriptors of a tile: k-step kk of 16 values along d (K-major), or of 16 rows (rows are K).
+__device__ __forceinline__ uint64_t desc_d(uint32_t tile, int kk) {
+  return sdesc_sw128(tile + (kk >> 2) * kHalfBytes + (kk & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int kk) {
+  return sdesc_sw128(tile + kk * 2048, kHalfBytes, 1024);
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh(a) for a2 = 2 a log2(e): 1 - 2 / (1 + e^(2a)); exact at both infinities, absolute error of an ulp of 1
+__device__ __forceinline__ float tanh_of(float a2) { return fmaf(-2.f, rcp_approx(1.f + ex2_approx(a2)), 1.f); }
+
+template <bool kBF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  return kBF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+}
+
+// 32 lanes x 32 columns store, counterpart of tmem_ld32
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Eight fp32 values as 16-bit ones in one 16-byte store
+template <bool kBF16>
+__device__ __forceinline__ void store8(void* out, long long off, const float* v) {
+  uint4 u;
+  u.x = pack16<kBF16>(v[0], v[1]);
+  u.y = pack16<kBF16>(v[2], v[3]);
+  u.z = pack16<kBF16>(v[4], v[5]);
+  u.w = pack16<kBF16>(v[6], v[7]);
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + off) = u;
+}
+
+}  // namespace dense
+}  // namespace bsa

@@ -1,0 +1,157 @@
+"""Key/value cache in 8 bits for the chunked continuation and for token-by-token decoding.
+
+Keys and values are held as e4m3 codes with one power-of-two scale for each 64 tokens of a head: half of the
+bf16 cache's memory and, where few rows attend, half of its traffic.  A floating-point code loses no precision
+by a power-of-two scale, and decoding a code to 16 bits is exact.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from .. import _dense, _native
+from .masked_attention import AttentionMask
+
+__all__ = ["KVCache8"]
+
+BLOCK = _dense.CACHE_BLOCK
+
+# Most rows (query heads of a key head x query tokens) that read the codes directly, 16 to a pass; above, the
+# cache is unpacked to 16 bits once and the tile kernel runs.
+FEW_ROWS = 64
+
+
+class KVCache8:
+    """Codes ``k_codes`` / ``v_codes`` [B, Hk, capacity, D] (e4m3), scales ``k_scale`` / ``v_scale``
+    [B, Hk, capacity / 64] (fp32) and ``lengths`` [B] (int32: tokens held), all on one CUDA device.
+
+    The lengths live on the device, so an append or a lookup can be captured into a CUDA graph and replayed.
+    Calls on one cache are ordered by their stream, like any in-place update of a tensor."""
+
+    def __init__(self, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
+                 lengths: torch.Tensor):
+        _dense._same_place(k_codes, k_scale, v_codes, v_scale, lengths)
+        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+            raise ValueError("codes must be [B, Hk, capacity, D]")
+        B, Hk, cap, D = k_codes.shape
+        if cap % BLOCK or cap == 0:
+            raise ValueError(f"capacity {cap} must be a positive multiple of {BLOCK}")
+        if D % 8 or not 0 < D <= 128:
+            raise ValueError(f"head_dim D={D} must be a multiple of 8 and <= 128")
+        for t in (k_codes, v_codes):
+            if t.dtype != torch.float8_e4m3fn or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError("codes must be contiguous, 16-byte aligned float8_e4m3fn")
+        for t in (k_scale, v_scale):
+            if t.dtype != torch.float32 or not t.is_contiguous() or tuple(t.shape) != (B, Hk, cap // BLOCK):
+                raise ValueError(f"scales must be contiguous fp32 [{B}, {Hk}, {cap // BLOCK}]")
+        if lengths.dtype != torch.int32 or not lengths.is_contiguous() or tuple(lengths.shape) != (B,):
+            raise ValueError(f"lengths must be contiguous int32 [{B}]")
+        self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.lengths = k_codes, k_scale, v_codes, v_scale, lengths
+
+    @classmethod
+    def allocate(cls, batch: int, heads: int, capacity: int, head_dim: int, device=None) -> "KVCache8":
+        """An empty cache; the capacity is rounded up to whole blocks of 64 tokens."""
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        cap = -(-int(capacity) // BLOCK) * BLOCK
+        codes = [torch.zeros((batch, heads, cap, head_dim), device=device, dtype=torch.uint8).view(torch.float8_e4m3fn)
+                 for _ in range(2)]
+        scale = [torch.zeros((batch, heads, cap // BLOCK), device=device, dtype=torch.float32) for _ in range(2)]
+        return cls(codes[0], scale[0], codes[1], scale[1], torch.zeros((batch,), device=device, dtype=torch.int32))
+
+    @classmethod
+    def from_kv(cls, k: torch.Tensor, v: torch.Tensor, capacity: Optional[int] = None) -> "KVCache8":
+        """A cache that holds k and v [B, Hk, S, D]."""
+        B, Hk, S, D = k.shape
+        cache = cls.allocate(B, Hk, max(S, 1) if capacity is None else capacity, D, k.device)
+        cache.append(k, v)
+        return cache
+
+    @property
+    def capacity(self) -> int:
+        return int(self.k_codes.shape[2])
+
+    def _check_kv(self, k, v) -> None:
+        B, Hk, cap, D = self.k_codes.shape
+        _dense._same_place(self.k_codes, k, v)
+        if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (B, Hk, D):
+            raise ValueError(f"k and v must be [{B}, {Hk}, n, {D}]")
+        if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("k and v must both be bf16 or fp16")
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
+        """Adds n tokens to every sequence (``counts`` int32 [B]: only the first counts[b] of them).
+
+        A block whose largest value grows takes a larger scale, and its codes are rounded again at it.  Tokens that
+        do not fit are dropped, and ``_native.device_error()`` then reports it; more tokens than the whole capacity
+        are refused here.  Infinities are held as the block's largest code, NaN as NaN; neither sets a scale."""
+        self._check_kv(k, v)
+        if k.shape[2] > self.capacity:
+            raise ValueError(f"{k.shape[2]} tokens for a capacity of {self.capacity}")
+        if counts is not None:
+            counts = _dense._i32(counts, "counts", (self.k_codes.shape[0],))
+            _dense._same_place(k, counts)
+        if k.numel():
+            _dense.cache_append(self, k, v, counts)
+
+    def truncate(self, lengths: Union[int, torch.Tensor]) -> None:
+        """Sets the lengths: a rejected draft, or the conditioning tokens before the next chunk.  Blocks keep their
+        scales; a block that ends up without tokens takes a new one at the next append."""
+        if isinstance(lengths, torch.Tensor):
+            _dense._same_place(self.lengths, lengths)
+            if tuple(lengths.shape) != tuple(self.lengths.shape):
+                raise ValueError(f"lengths must be {list(self.lengths.shape)}")
+            self.lengths.copy_(lengths)
+        else:
+            if not 0 <= int(lengths) <= self.capacity:
+                raise ValueError(f"length {lengths} is outside [0, {self.capacity}]")
+            self.lengths.fill_(int(lengths))
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(k, v) [B, Hk, capacity, D]: the held tokens, zeros behind them."""
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("dequantize to bf16 or fp16")
+        return _dense.cache_unpack(self, dtype)
+
+    def attend(self, q: torch.Tensor, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None, *,
+               causal: bool = False, sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of q [B, H, Sq, D] over the held tokens and, behind them, fresh keys and values k, v
+        [B, Hk, n, D] that are not cached (the frames being denoised); H is a multiple of Hk.
+
+        ``causal``: the last query sees every key (held, then fresh), the one before it one less, and so on.
+        sm_scale defaults to 1 / sqrt(D).  Sequences without a key give zeros.  Few rows read the codes as they are;
+        many rows, or fresh keys, unpack the cache into 16-bit scratch first."""
+        B, Hk, cap, D = self.k_codes.shape
+        _dense._same_place(self.k_codes, q, k, v, out)
+        if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
+            raise ValueError(f"q must be [{B}, H, Sq, {D}]")
+        if q.shape[1] % Hk:
+            raise ValueError(f"{q.shape[1]} query heads are no multiple of {Hk} key heads")
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"unsupported dtype {q.dtype} (bf16 or fp16)")
+        if (k is None) != (v is None):
+            raise ValueError("k and v come together")
+        if k is not None:
+            self._check_kv(k, v)
+            if k.dtype != q.dtype:
+                raise ValueError("q, k, v must share one dtype")
+        if any(t is not None and t.requires_grad for t in (q, k, v)) and torch.is_grad_enabled():
+            raise ValueError("attention over a cache has no gradient")
+        scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+        _dense.check_scale(scale)
+        if out is None:
+            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must have q's shape and dtype")
+        Sq = q.shape[2]
+        if q.numel() == 0:
+            return out
+        n = k.shape[2] if k is not None else 0
+        if n == 0 and q.shape[1] // Hk * Sq <= FEW_ROWS:
+            return _dense.cache_attention(self, q, causal, scale, out)
+        kd, vd = _dense.cache_unpack(self, q.dtype, k if n else None, v if n else None)
+        ranges, table = _dense.attention_ranges(B, Sq, cap + n, device=q.device, causal=causal, k_lengths=self.lengths,
+                                                k_add=n)
+        return _dense.masked_attention(q, kd, vd, ranges, table, scale, 0.0, out=out)[0]

@@ -8,17 +8,20 @@ positions (:79-82), every frequency drives one adjacent pair (:91-93), and
 On B200 the rotation is fused into the BSA routing kernel: ``RopeTables`` builds the per-axis
 fp32 angle tables once per grid and hands them to the engine (``bsa_attention(..., rope=...)``),
 which rotates Q and K on their single pass through HBM.  ``RotaryPositionalEmbedding.__call__``
-keeps the unfused torch form for the dense (non-BSA) attention path.
+keeps the unfused torch form; ``qk_norm_rope`` is the kernel of the dense (non-BSA) side, with gradients.
 """
 
 from __future__ import annotations
 
-from typing import Dict, Tuple
+from typing import Dict, Optional, Tuple
 
 import numpy as np
 import torch
 
-__all__ = ["rotate_half", "rope_axis_dims", "rope_axis_tables", "RopeTables", "RotaryPositionalEmbedding"]
+from .. import _dense
+
+__all__ = ["rotate_half", "rope_axis_dims", "rope_axis_tables", "RopeTables", "RotaryPositionalEmbedding",
+           "qk_norm_rope"]
 
 
 def rope_axis_dims(head_dim: int) -> Tuple[int, int, int]:
@@ -101,3 +104,53 @@ class RotaryPositionalEmbedding(torch.nn.Module):
         q_r = qf * cos + rotate_half(qf) * sin
         k_r = kf * cos + rotate_half(kf) * sin
         return q_r.to(out_dtype), k_r.to(out_dtype)
+
+
+class _NormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, eps, rope, start):
+        xs = [q] if k is None else [q, k]
+        ctx.save_for_backward(q, k, q_weight, k_weight)
+        ctx.rest = (eps, rope, start)
+        ctx.set_materialize_grads(False)
+        ys = _dense.norm_rope(xs, [q_weight, k_weight][:len(xs)], eps, rope, start)
+        return ys[0] if k is None else tuple(ys)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        q, k, q_weight, k_weight = ctx.saved_tensors
+        eps, rope, start = ctx.rest
+        need = ctx.needs_input_grad
+        sides = [(i, x, w) for i, (x, w) in enumerate(((q, q_weight), (k, k_weight)))
+                 if x is not None and grads[i] is not None and (need[i] or need[2 + i])]
+        res = [None] * 7
+        if sides:
+            gs = [grads[i].to(x.dtype) for i, x, _ in sides]
+            dxs, dws = _dense.norm_rope_backward([x for _, x, _ in sides], gs, [w for _, _, w in sides], eps, rope,
+                                                 start, [need[2 + i] for i, _, _ in sides])
+            for (i, _, w), dx, dw in zip(sides, dxs, dws):
+                res[i] = dx if need[i] else None
+                res[2 + i] = dw.to(w.dtype) if dw is not None else None
+        return tuple(res)
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, *, rope=None, start: int = 0):
+    """q/k RMSNorm (blocks.py:55-73) and 3-axis rotary positions (rope_3d.py:107-128) in one launch, differentiable.
+
+    q [B, H, S, D] and k [B, Hk, S, D] (k None: q alone): bf16, fp16 or fp32 CUDA tensors, D a multiple of 8 up to
+    128; strided views, such as the projection's ``qkv.reshape(B, N, 3, H, D).permute(2, 0, 3, 1, 4)``, are read in
+    place.  A weight [D] turns its tensor's norm on.  ``rope``: :class:`RopeTables` or (tables, axis dims, grid); the
+    tokens stand at places ``start`` .. ``start`` + S - 1 of the grid (t-major), so a continuation behind n cached
+    tokens passes ``start=n``.  Sums are fp32 and the result is rounded once (the unfused form rounds after each
+    step).  Returns contiguous tensors: (q, k), or q alone."""
+    if q_weight is None and k_weight is None and rope is None:
+        raise ValueError("nothing to do: give norm weights, rope tables or both")
+    if k is None and k_weight is not None:
+        raise ValueError("k_weight without k")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _NormRope.apply(q, k, q_weight, k_weight, float(eps), rope, int(start))
+    xs = [q] if k is None else [q, k]
+    ys = _dense.norm_rope(xs, [q_weight, k_weight][:len(xs)], float(eps), rope, int(start))
+    return ys[0] if k is None else tuple(ys)
