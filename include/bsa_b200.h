@@ -237,6 +237,18 @@ int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype,
                          const int32_t* ranges, const int32_t* table, int ranges_batch, float sm_scale, float softcap,
                          void* out, const int64_t* out_strides, float* lse, void* scratch, void* stream);
 
+/* bsa_masked_attention_backward: gradients of that call from its out and lse and the gradient of out (which is
+ * rounded to dtype, as out is).  dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may
+ * be NULL.  Shared key heads sum over their query heads; keys no row sees get zeros.  No atomics: the same bits
+ * every time.  scratch: bsa_masked_attention_backward_scratch_bytes() bytes (ranges_batch 0 without ranges). */
+int64_t bsa_masked_attention_backward_scratch_bytes(int B, int H, int Sq, int ranges_batch);
+int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* grad,
+                                  const float* lse, int dtype, int B, int H, int Hk, int Sq, int Sk, int D,
+                                  const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                  const int64_t* out_strides, const int64_t* grad_strides, const int32_t* ranges,
+                                  const int32_t* table, int ranges_batch, float sm_scale, float softcap, void* dq,
+                                  void* dk, void* dv, void* scratch, void* stream);
+
 /* 8-bit key/value cache: codes [B, Hk, capacity, D] e4m3, contiguous, 16-byte aligned; scales
  * [B, Hk, capacity / 64] fp32, each the smallest power of two that keeps the block's codes within 448 (0: a block
  * of zeros); lengths [B] int32: tokens held.  capacity is a multiple of 64.

@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "longcat_video", "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libbsa_b200.so")
 SOURCES = ["bsa_capi.cu", "bsa_attn.cu", "bsa_score.cu", "bsa_route.cu", "bsa_noalloc.cu", "bsa_xfer.cu",
-           "bsa_dense_capi.cu", "bsa_normrope.cu", "bsa_ranges.cu", "bsa_kv8.cu", "bsa_dense.cu"]
+           "bsa_dense_capi.cu", "bsa_normrope.cu", "bsa_ranges.cu", "bsa_kv8.cu", "bsa_dense.cu", "bsa_dense_bwd.cu"]
 HEADERS = ["bsa_ptx.cuh", "bsa_kernels.h", "bsa_select.cuh", "bsa_dense.h", "bsa_dense.cuh", "bsa_rows.cuh"]
 
 

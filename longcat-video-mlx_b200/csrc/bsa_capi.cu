@@ -286,8 +286,9 @@ int bsa_device_error(int clear) {
   const int r = bsa::route_device_error(clear);
   const int c = bsa::cache_device_error(clear);
   const int d = bsa::dense_device_error(clear);
+  const int w = bsa::dense_bwd_device_error(clear);
   const int first = a ? a : (s ? s : r);
-  return first ? first : (c ? c : d);
+  return first ? first : (c ? c : (d ? d : w));
 }
 
 int bsa_mean_pool(const void* x, int dtype, int B, int H, int S, int D, int64_t sb, int64_t sh, int64_t ss, int T,

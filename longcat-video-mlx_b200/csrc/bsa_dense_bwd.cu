@@ -1,0 +1,822 @@
+// Dense attention over key intervals, backward, on sm_100a (tcgen05 + TMA + TMEM).
+//
+// With s = sm_scale q.k, z = s or cap tanh(s / cap), p_ij = e^(z_ij - lse_i):
+//   delta_i = do_i . o_i,   dz_ij = p_ij (do_i . v_j - delta_i),   ds_ij = dz_ij (1 - (z_ij / cap)^2)
+//   dv_j = sum_i p_ij do_i,   dk_j = sm_scale sum_i ds_ij q_i,   dq_i = sm_scale sum_j ds_ij k_j
+// Nothing of size Sq x Sk is kept: the scores are computed again from q, k and lse.
+//
+// Two kernels of their own for (dk, dv) and for dq.  The scores and do.v are computed in both, 7 products where one
+// kernel would need 5, but neither adds into memory that another CTA adds into: no atomics, the same bits every
+// time, fp32 accumulators from the first product to the one rounding of the result.
+//   dkv_kernel: a CTA owns 128 keys of one key head and walks the query tiles that see them, over every query
+//               head that shares the key head.   S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//   dq_kernel : a CTA owns 128 queries and walks their key tiles.  S = Q K^T, dP = dO V^T, dQ += dS K
+// P^T and dS^T (dS) are rounded to 16 bits into tensor memory, over the scores they came from, as the A operands of
+// the second products.  TMEM: S, dP, dV, dK, or S, dP twice, dQ, 128 columns each.
+//
+// Roles (320 threads, one CTA to an SM): warps 0-7 compute, warps 0-3 on columns 0-63 of a score tile and 4-7 on
+// 64-127; warp 8 issues the products; warp 9 loads.  The products' order lets each phase of the arithmetic run beside
+// products that do not need it:
+//   dkv: S(0) dP(0) [P(i) ready] dV(i) S(i+1) [dS(i) ready] dK(i) dP(i+1) ...
+//   dq : S(0) dP(0) [S(j) read] S(j+1) dP(j+1) [dS(j) ready] dQ(j) ...
+//
+// Masked places: p and ds are set to 0 by comparison, whatever the scores hold; rows of empty queries (dkv) and keys
+// that no row of the tile sees (dq) are zeroed in shared memory, since 0 * NaN would be NaN.
+// Every wait is bounded (bsa_ptx.cuh).
+#include <climits>
+#include "bsa_dense.cuh"
+#include "bsa_rows.cuh"
+
+namespace bsa {
+namespace dense {
+
+__device__ int g_dense_bwd_err;
+
+constexpr int kBwdThreads = 320;
+constexpr uint32_t kColA = 0, kColB = 128, kColC = 256, kColD = 384;  // tensor memory, 128 columns each
+
+struct BwdParams {
+  const int2* ranges;   // [Bm][Sq], null: all keys
+  const int4* table;
+  int Bm, H, Hk, G, Sq, Sk, D;
+  int q_tiles, k_tiles, Sq_pad;
+  float scale_log2, sm_scale, cap_in, cap_log2;
+  float2* stats;        // [B * H][Sq_pad]: lse in log2 (+inf: no keys), delta
+  int2* rng;            // [Bm][Sq_pad]: ranges, padded with empty ones
+  const float* lse;
+  Tensor4 o, g;         // forward output, its gradient
+  Tensor4 d0, d1;       // dk, dv or dq
+};
+
+// ------------------------------------------------------------------------- row statistics
+// 8 or 16 lanes to a row; delta in fp32 from the stored o.
+template <typename T>
+__global__ void __launch_bounds__(256) stats_kernel(const BwdParams p) {
+  constexpr int kLanes = 16;
+  const int row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int bh = blockIdx.y;
+  const int b = bh / p.H, h = bh - b * p.H;
+  float dot = 0.f;
+  const bool on = row < p.Sq;
+  if (on && 8 * lane < p.D) {
+    Row8<T> o, g;
+    o.load(static_cast<const T*>(p.o.p) + b * p.o.sb + h * p.o.sh + row * p.o.ss + 8 * lane);
+    g.load(static_cast<const T*>(p.g.p) + b * p.g.sb + h * p.g.sh + row * p.g.ss + 8 * lane);
+    float a[8], c[8];
+    o.get(a);
+    g.get(c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dot = fmaf(a[e], c[e], dot);
+  }
+#pragma unroll
+  for (int s = kLanes / 2; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+  if (lane == 0 && row < p.Sq_pad) {
+    float l = INFINITY;
+    if (on) {
+      l = p.lse[static_cast<long long>(bh) * p.Sq + row] * 1.4426950408889634f;
+      if (l == -INFINITY) {
+        l = INFINITY;  // e^(z - lse) is 0 then
+        dot = 0.f;
+      }
+    }
+    p.stats[static_cast<long long>(bh) * p.Sq_pad + row] = make_float2(l, on ? dot : 0.f);
+    if (h == 0 && b < p.Bm && p.rng)
+      p.rng[static_cast<long long>(b) * p.Sq_pad + row] =
+          on ? p.ranges[static_cast<long long>(b) * p.Sq + row] : make_int2(0, 0);
+  }
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int N>
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// Waits that every load issued into a ring has landed (after an expired wait, before the CTA ends).
+__device__ __forceinline__ void drain_ring(uint64_t* full, int stages, int issued) {
+  const uint64_t t0 = globaltimer_ns();
+  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+    while (!mbar_try_wait(&full[i % stages], static_cast<uint32_t>((i / stages) & 1)) &&
+           globaltimer_ns() - t0 < kWaitLimitNs) {
+    }
+}
+
+// Products of a 128 x N accumulator: A and B along d (K-major both), or A in tensor memory (two runs of 32 columns at
+// `a` and `a` + 64, 64 values of K each) and B by rows.
+template <int DP>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t id) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) umma_ss(d, desc_d(a, kk), desc_d(b, kk), id, kk > 0);
+}
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool add) {
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    umma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, desc_rows(b, kk), id, add || kk > 0);
+}
+
+// One warp's 32 rows x (DP / 2) columns of an accumulator, times f, to 16-bit rows of a tensor.
+template <int DP, bool kBF16>
+__device__ __forceinline__ void store_acc(uint32_t addr, int col0, float f, void* out, long long off, int D, bool live,
+                                          bool some) {
+#pragma unroll 1
+  for (int c = 0; c < DP / 64; ++c) {
+    uint32_t r[32];
+    if (some) {
+      tmem_ld32(addr + col0 + 32 * c, r);
+      tmem_ld_wait();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) r[e] = 0u;
+    }
+    float v[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]) * f;
+    if (live) {
+#pragma unroll
+      for (int e8 = 0; e8 < 4; ++e8) {
+        const int d0 = col0 + 32 * c + 8 * e8;
+        if (d0 < D) store8<kBF16>(out, off + d0, v + 8 * e8);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------- dk, dv
+template <int DP>
+struct DkvSmem {
+  static constexpr int kQ = DP == 128 ? 2 : 4;   // query tiles in flight
+  static constexpr int kG = DP == 128 ? 2 : 4;   // tiles of do in flight
+  static constexpr int kTiles = (2 + kQ + kG) * tile_bytes<DP>();
+  alignas(16) float2 stats[kQ][kTile];
+  alignas(16) int2 rng[kQ][kTile];
+  uint64_t kv_full;
+  uint64_t q_full[kQ], q_empty[kQ], g_full[kG], g_empty[kG];
+  uint64_t fix;
+  uint64_t s_full, dp_full, p_full, ds_full, done, drain;
+  uint32_t tmem;
+  int abort_flag;
+  int first, last;
+};
+template <int DP>
+constexpr int dkv_smem_bytes() { return DkvSmem<DP>::kTiles + static_cast<int>(sizeof(DkvSmem<DP>)) + 1024; }
+
+template <int DP, bool kBF16, bool kCap>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g, const BwdParams p) {
+  using S = DkvSmem<DP>;
+  constexpr int kBytes = tile_bytes<DP>();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *sK = smem, *sV = smem + kBytes, *sQ = smem + 2 * kBytes, *sG = sQ + S::kQ * kBytes;
+  S& ss = *reinterpret_cast<S*>(smem + S::kTiles);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // key tiles ascending: under a causal mask the first are seen by the most queries
+  const int bhk = blockIdx.x / p.k_tiles;
+  const int kt = blockIdx.x - bhk * p.k_tiles;
+  const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
+  const int bm = p.Bm > 1 ? b : 0;
+  const int key0 = kt * kTile;
+  const int4* table = p.table ? p.table + static_cast<long long>(bm) * p.q_tiles : nullptr;
+  auto sees = [&](const int4& t) { return t.x < t.y && t.x < key0 + kTile && t.y > key0; };
+
+  if (tid == 0) {
+    mbar_init(&ss.kv_full, 1);
+    for (int i = 0; i < S::kQ; ++i) {
+      mbar_init(&ss.q_full[i], 1);
+      mbar_init(&ss.q_empty[i], 1);
+    }
+    for (int i = 0; i < S::kG; ++i) {
+      mbar_init(&ss.g_full[i], 1);
+      mbar_init(&ss.g_empty[i], 1);
+    }
+    mbar_init(&ss.fix, 1);
+    mbar_init(&ss.s_full, 1);
+    mbar_init(&ss.dp_full, 1);
+    mbar_init(&ss.p_full, 8);
+    mbar_init(&ss.ds_full, 8);
+    mbar_init(&ss.done, 1);
+    mbar_init(&ss.drain, 1);
+    ss.abort_flag = 0;
+    ss.first = table ? INT_MAX : 0;
+    ss.last = table ? -1 : p.q_tiles - 1;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&ss.tmem, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  if (table) {  // first and last query tile that sees a key of this tile
+    int lo = INT_MAX, hi = -1;
+    for (int i = tid; i < p.q_tiles; i += kBwdThreads)
+      if (sees(table[i])) {
+        lo = min(lo, i);
+        hi = i;
+      }
+    if (hi >= 0) {
+      atomicMin(&ss.first, lo);
+      atomicMax(&ss.last, hi);
+    }
+    __syncthreads();
+  }
+  tc_fence_after();
+  const uint32_t tmem = ss.tmem;
+  const int first = ss.first, last = ss.last;
+  const bool some = first <= last;
+  volatile int* abort_flag = &ss.abort_flag;
+  int* err = &g_dense_bwd_err;
+  // every role walks the same tiles: `step(g, i, tab)` returns false to stop
+  auto walk = [&](auto&& step) {
+    for (int g = 0; g < p.G; ++g)
+      for (int i = first; i <= last; ++i) {
+        const int4 t = table ? __ldg(table + i) : make_int4(0, p.Sk, 0, p.Sk);
+        if (!sees(t)) continue;
+        if (!step(g, i, t)) return false;
+      }
+    return true;
+  };
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------ loads
+    if (some) {
+      if (lane == 0) {
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_g);
+        mbar_arrive_expect_tx(&ss.kv_full, 2 * kBytes);
+        load_tile<DP>(sK, &tm_k, &ss.kv_full, key0, hk, b);
+        load_tile<DP>(sV, &tm_v, &ss.kv_full, key0, hk, b);
+      }
+      Ring<S::kQ> rq;
+      Ring<S::kG> rg;
+      int n = 0, fixes = 0;
+      const bool ok = walk([&](int g, int i, const int4& t) {
+        const int h = hk * p.G + g;
+        bool w = true;
+        if (n >= S::kQ) w = mbar_wait(&ss.q_empty[rq.slot], rq.phase ^ 1u, abort_flag, err, 401);
+        if (!__all_sync(0xffffffffu, w)) return false;
+        const bool fix = t.w <= 0;  // rows without keys, whose q and do may hold anything
+        uint8_t* q = sQ + rq.slot * kBytes;
+        const uint32_t extra = kTile * sizeof(float2) + (p.rng ? kTile * sizeof(int2) : 0);
+        if (lane == 0) {
+          uint64_t* bar = fix ? &ss.fix : &ss.q_full[rq.slot];
+          mbar_arrive_expect_tx(bar, kBytes + extra);
+          load_tile<DP>(q, &tm_q, bar, i * kTile, h, b);
+          bulk_load(ss.stats[rq.slot], p.stats + (static_cast<long long>(b) * p.H + h) * p.Sq_pad + i * kTile,
+                    kTile * sizeof(float2), bar);
+          if (p.rng)
+            bulk_load(ss.rng[rq.slot], p.rng + static_cast<long long>(bm) * p.Sq_pad + i * kTile, kTile * sizeof(int2),
+                      bar);
+        }
+        if (fix) {
+          __syncwarp();
+          w = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 402);
+          if (!__all_sync(0xffffffffu, w)) return false;
+          ++fixes;
+          for (int r = 0; r < kTile; ++r)
+            if (ss.rng[rq.slot][r].x >= ss.rng[rq.slot][r].y) zero_row<DP>(q, r, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss.q_full[rq.slot]);
+        }
+        if (n >= S::kG) w = mbar_wait(&ss.g_empty[rg.slot], rg.phase ^ 1u, abort_flag, err, 403);
+        if (!__all_sync(0xffffffffu, w)) return false;
+        uint8_t* go = sG + rg.slot * kBytes;
+        if (lane == 0) {
+          uint64_t* bar = fix ? &ss.fix : &ss.g_full[rg.slot];
+          mbar_arrive_expect_tx(bar, kBytes);
+          load_tile<DP>(go, &tm_g, bar, i * kTile, h, b);
+        }
+        if (fix) {
+          __syncwarp();
+          w = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 404);
+          if (!__all_sync(0xffffffffu, w)) return false;
+          ++fixes;
+          for (int r = 0; r < kTile; ++r)
+            if (ss.rng[rq.slot][r].x >= ss.rng[rq.slot][r].y) zero_row<DP>(go, r, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss.g_full[rg.slot]);
+        }
+        ++n;
+        rq.next();
+        rg.next();
+        return true;
+      });
+      if (!ok && lane == 0) {
+        drain_ring(&ss.kv_full, 1, 1);
+        drain_ring(ss.q_full, S::kQ, n + 1);
+        drain_ring(ss.g_full, S::kG, n);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ products
+    if (lane == 0 && some) {
+      constexpr uint32_t kIdS = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
+      constexpr uint32_t kIdR = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
+      const uint32_t kb = smem_u32(sK), vb = smem_u32(sV), qb = smem_u32(sQ), gb = smem_u32(sG);
+      Ring<S::kQ> rq;
+      Ring<S::kG> rg;
+      int n = 0;
+      int q_prev = 0;
+      // dK of the step before: its dS, then the step's own dP
+      auto finish = [&](int m) {
+        if (!mbar_wait(&ss.ds_full, static_cast<uint32_t>(m & 1), abort_flag, err, 411)) return false;
+        tc_fence_after();
+        mma_rows(tmem + kColD, tmem + kColB, qb + q_prev * kBytes, kIdR, m > 0);
+        umma_commit(&ss.q_empty[q_prev]);
+        return true;
+      };
+      bool ok = mbar_wait(&ss.kv_full, 0, abort_flag, err, 412);
+      int g_prev = 0;
+      if (ok)
+        ok = walk([&](int, int, const int4&) {
+          if (n > 0) {  // dV(n - 1)
+            if (!mbar_wait(&ss.p_full, static_cast<uint32_t>((n - 1) & 1), abort_flag, err, 413)) return false;
+            tc_fence_after();
+            mma_rows(tmem + kColC, tmem + kColA, gb + g_prev * kBytes, kIdR, n > 1);
+            umma_commit(&ss.g_empty[g_prev]);
+          }
+          if (!mbar_wait(&ss.q_full[rq.slot], rq.phase, abort_flag, err, 414)) return false;
+          tc_fence_after();
+          mma_scores<DP>(tmem + kColA, kb, qb + rq.slot * kBytes, kIdS);
+          umma_commit(&ss.s_full);
+          if (n > 0 && !finish(n - 1)) return false;
+          if (!mbar_wait(&ss.g_full[rg.slot], rg.phase, abort_flag, err, 415)) return false;
+          tc_fence_after();
+          mma_scores<DP>(tmem + kColB, vb, gb + rg.slot * kBytes, kIdS);
+          umma_commit(&ss.dp_full);
+          q_prev = rq.slot;
+          g_prev = rg.slot;
+          rq.next();
+          rg.next();
+          ++n;
+          return true;
+        });
+      if (ok) ok = mbar_wait(&ss.p_full, static_cast<uint32_t>((n - 1) & 1), abort_flag, err, 416);
+      if (ok) {
+        tc_fence_after();
+        mma_rows(tmem + kColC, tmem + kColA, gb + g_prev * kBytes, kIdR, n > 1);
+        ok = finish(n - 1);
+      }
+      if (ok) umma_commit(&ss.done);
+      umma_commit(&ss.drain);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(&ss.drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ p and ds
+    const int half = warp >> 2;
+    const uint32_t la = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+    const int key = key0 + 32 * (warp & 3) + lane;
+    bool ok = true;
+    if (some) {
+      Ring<S::kQ> rq;
+      int n = 0;
+      ok = walk([&](int, int, const int4& t) {
+        bool w = mbar_wait(&ss.q_full[rq.slot], rq.phase, abort_flag, err, 421);  // the tile's statistics
+        w = w && mbar_wait(&ss.s_full, static_cast<uint32_t>(n & 1), abort_flag, err, 422);
+        if (!__all_sync(0xffffffffu, w)) return false;
+        tc_fence_after();
+        uint32_t r[64];
+        tmem_ld32(la + kColA + 64 * half, r);
+        tmem_ld32(la + kColA + 64 * half + 32, r + 32);
+        tmem_ld_wait();
+        const float4* st = reinterpret_cast<const float4*>(ss.stats[rq.slot] + 64 * half);
+        const bool border = table && (t.z > key0 || t.w < key0 + kTile);
+        float pr[64];  // p, then p (1 - tanh^2)
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float4 s2 = st[e];  // lse, delta of two queries
+          float t0 = 0.f, t1 = 0.f, x0, x1;
+          if constexpr (kCap) {
+            t0 = tanh_of(__uint_as_float(r[2 * e]) * p.cap_in);
+            t1 = tanh_of(__uint_as_float(r[2 * e + 1]) * p.cap_in);
+            x0 = ex2_approx(fmaf(t0, p.cap_log2, -s2.x));
+            x1 = ex2_approx(fmaf(t1, p.cap_log2, -s2.z));
+          } else {
+            x0 = ex2_approx(fmaf(__uint_as_float(r[2 * e]), p.scale_log2, -s2.x));
+            x1 = ex2_approx(fmaf(__uint_as_float(r[2 * e + 1]), p.scale_log2, -s2.z));
+          }
+          if (border) {
+            const int4 b2 = reinterpret_cast<const int4*>(ss.rng[rq.slot] + 64 * half)[e];
+            if (key < b2.x || key >= b2.y) x0 = t0 = 0.f;
+            if (key < b2.z || key >= b2.w) x1 = t1 = 0.f;
+          }
+          pk[e] = pack16<kBF16>(x0, x1);
+          pr[2 * e] = kCap ? x0 * fmaf(-t0, t0, 1.f) : x0;
+          pr[2 * e + 1] = kCap ? x1 * fmaf(-t1, t1, 1.f) : x1;
+        }
+        tmem_st32(la + kColA + 64 * half, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss.p_full);
+        w = mbar_wait(&ss.dp_full, static_cast<uint32_t>(n & 1), abort_flag, err, 423);
+        if (!__all_sync(0xffffffffu, w)) return false;
+        tc_fence_after();
+        tmem_ld32(la + kColB + 64 * half, r);
+        tmem_ld32(la + kColB + 64 * half + 32, r + 32);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float4 s2 = st[e];
+          float y0 = pr[2 * e] * (__uint_as_float(r[2 * e]) - s2.y);
+          float y1 = pr[2 * e + 1] * (__uint_as_float(r[2 * e + 1]) - s2.w);
+          if (border) {  // 0 * NaN
+            if (pr[2 * e] == 0.f) y0 = 0.f;
+            if (pr[2 * e + 1] == 0.f) y1 = 0.f;
+          }
+          pk[e] = pack16<kBF16>(y0, y1);
+        }
+        tmem_st32(la + kColB + 64 * half, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss.ds_full);
+        rq.next();
+        ++n;
+        return true;
+      });
+      if (ok) {
+        ok = mbar_wait(&ss.done, 0, abort_flag, err, 424);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+    }
+    if (ok) {
+      const bool live = key < p.Sk;
+      const long long ok0 = b * p.d0.sb + hk * p.d0.sh + static_cast<long long>(key) * p.d0.ss;
+      const long long ov0 = b * p.d1.sb + hk * p.d1.sh + static_cast<long long>(key) * p.d1.ss;
+      store_acc<DP, kBF16>(la + kColD, half * (DP / 2), p.sm_scale, p.d0.p, ok0, p.D, live, some);
+      store_acc<DP, kBF16>(la + kColC, half * (DP / 2), 1.f, p.d1.p, ov0, p.D, live, some);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------- dq
+template <int DP>
+struct DqSmem {
+  static constexpr int kK = DP == 128 ? 3 : 5;
+  static constexpr int kV = DP == 128 ? 2 : 4;
+  static constexpr int kTiles = (2 + kK + kV) * tile_bytes<DP>();
+  uint64_t qg_full;
+  uint64_t k_full[kK], k_empty[kK], v_full[kV], v_empty[kV];
+  uint64_t fix;
+  uint64_t s_full, s_read, dp_full[2], ds_full, done, drain;
+  uint32_t tmem;
+  int abort_flag;
+};
+template <int DP>
+constexpr int dq_smem_bytes() { return DqSmem<DP>::kTiles + static_cast<int>(sizeof(DqSmem<DP>)) + 1024; }
+
+template <int DP, bool kBF16, bool kCap>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g, const BwdParams p) {
+  using S = DqSmem<DP>;
+  constexpr int kBytes = tile_bytes<DP>();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *sQ = smem, *sG = smem + kBytes, *sK = smem + 2 * kBytes, *sV = sK + S::kK * kBytes;
+  S& ss = *reinterpret_cast<S*>(smem + S::kTiles);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the last query tiles first: under a causal mask they see the most keys
+  const int bh = blockIdx.x / p.q_tiles;
+  const int qt = p.q_tiles - 1 - (blockIdx.x - bh * p.q_tiles);
+  const int b = bh / p.H, h = bh - b * p.H;
+  const int hk = h / p.G;
+  const int bm = p.Bm > 1 ? b : 0;
+  const int4 tab = p.table ? p.table[static_cast<long long>(bm) * p.q_tiles + qt] : make_int4(0, p.Sk, 0, p.Sk);
+  const int n0 = tab.x < tab.y ? tab.x / kTile : 0;
+  const int n1 = tab.x < tab.y ? (tab.y + kTile - 1) / kTile : 0;
+  const int steps = n1 - n0;
+
+  if (tid == 0) {
+    mbar_init(&ss.qg_full, 1);
+    for (int i = 0; i < S::kK; ++i) {
+      mbar_init(&ss.k_full[i], 1);
+      mbar_init(&ss.k_empty[i], 1);
+    }
+    for (int i = 0; i < S::kV; ++i) {
+      mbar_init(&ss.v_full[i], 1);
+      mbar_init(&ss.v_empty[i], 1);
+    }
+    mbar_init(&ss.fix, 1);
+    mbar_init(&ss.s_full, 1);
+    mbar_init(&ss.s_read, 8);
+    mbar_init(&ss.dp_full[0], 1);
+    mbar_init(&ss.dp_full[1], 1);
+    mbar_init(&ss.ds_full, 8);
+    mbar_init(&ss.done, 1);
+    mbar_init(&ss.drain, 1);
+    ss.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&ss.tmem, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ss.tmem;
+  volatile int* abort_flag = &ss.abort_flag;
+  int* err = &g_dense_bwd_err;
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------ loads
+    if (steps > 0) {
+      if (lane == 0) {
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        mbar_arrive_expect_tx(&ss.qg_full, 2 * kBytes);
+        load_tile<DP>(sQ, &tm_q, &ss.qg_full, qt * kTile, h, b);
+        load_tile<DP>(sG, &tm_g, &ss.qg_full, qt * kTile, h, b);
+      }
+      Ring<S::kK> rk;
+      Ring<S::kV> rv;
+      int n = 0, fixes = 0;
+      bool ok = true;
+      for (; n < steps; ++n) {
+        if (n >= S::kK) ok = mbar_wait(&ss.k_empty[rk.slot], rk.phase ^ 1u, abort_flag, err, 451);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int row = (n0 + n) * kTile;
+        uint8_t* dst = sK + rk.slot * kBytes;
+        const bool fix = row < tab.x || min(row + kTile, p.Sk) > tab.y;  // keys of the tile that no row sees
+        if (lane == 0) {
+          uint64_t* bar = fix ? &ss.fix : &ss.k_full[rk.slot];
+          mbar_arrive_expect_tx(bar, kBytes);
+          load_tile<DP>(dst, &tm_k, bar, row, hk, b);
+        }
+        if (fix) {
+          __syncwarp();
+          ok = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 452);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          ++fixes;
+          for (int r = 0; r < kTile; ++r)
+            if (row + r < tab.x || row + r >= tab.y) zero_row<DP>(dst, r, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss.k_full[rk.slot]);
+        }
+        if (n >= S::kV) ok = mbar_wait(&ss.v_empty[rv.slot], rv.phase ^ 1u, abort_flag, err, 453);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&ss.v_full[rv.slot], kBytes);
+          load_tile<DP>(sV + rv.slot * kBytes, &tm_v, &ss.v_full[rv.slot], row, hk, b);
+        }
+        rk.next();
+        rv.next();
+      }
+      if (!ok && lane == 0) {
+        drain_ring(&ss.qg_full, 1, 1);
+        drain_ring(ss.k_full, S::kK, n + 1);
+        drain_ring(ss.v_full, S::kV, n);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ products
+    if (lane == 0 && steps > 0) {
+      constexpr uint32_t kIdS = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
+      constexpr uint32_t kIdR = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
+      const uint32_t qb = smem_u32(sQ), gb = smem_u32(sG), kb = smem_u32(sK), vb = smem_u32(sV);
+      Ring<S::kK> rk;
+      Ring<S::kV> rv;
+      auto scores = [&](int n) {  // S(n) and dP(n)
+        if (!mbar_wait(&ss.k_full[rk.slot], rk.phase, abort_flag, err, 461)) return false;
+        tc_fence_after();
+        mma_scores<DP>(tmem + kColA, qb, kb + rk.slot * kBytes, kIdS);
+        umma_commit(&ss.s_full);
+        if (!mbar_wait(&ss.v_full[rv.slot], rv.phase, abort_flag, err, 462)) return false;
+        tc_fence_after();
+        mma_scores<DP>(tmem + ((n & 1) ? kColC : kColB), gb, vb + rv.slot * kBytes, kIdS);
+        umma_commit(&ss.dp_full[n & 1]);
+        umma_commit(&ss.v_empty[rv.slot]);
+        rk.next();
+        rv.next();
+        return true;
+      };
+      bool ok = mbar_wait(&ss.qg_full, 0, abort_flag, err, 463) && scores(0);
+      int k_used = 0;
+      for (int n = 0; n < steps && ok; ++n) {
+        if (n + 1 < steps) {
+          ok = mbar_wait(&ss.s_read, static_cast<uint32_t>(n & 1), abort_flag, err, 464);
+          if (!ok) break;
+          tc_fence_after();
+          ok = scores(n + 1);
+          if (!ok) break;
+        }
+        ok = mbar_wait(&ss.ds_full, static_cast<uint32_t>(n & 1), abort_flag, err, 465);
+        if (!ok) break;
+        tc_fence_after();
+        mma_rows(tmem + kColD, tmem + ((n & 1) ? kColC : kColB), kb + k_used * kBytes, kIdR, n > 0);
+        umma_commit(&ss.k_empty[k_used]);
+        if (++k_used == S::kK) k_used = 0;
+      }
+      if (ok) umma_commit(&ss.done);
+      umma_commit(&ss.drain);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(&ss.drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ ds
+    const int half = warp >> 2;
+    const uint32_t la = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+    const int row = qt * kTile + 32 * (warp & 3) + lane;
+    const bool live = row < p.Sq;
+    bool ok = true;
+    if (steps > 0) {
+      const float2 st = p.stats[static_cast<long long>(bh) * p.Sq_pad + row];
+      int lo = 0, hi = p.Sk;
+      if (p.ranges && live) {
+        const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
+        lo = r.x;
+        hi = r.y;
+      }
+      for (int n = 0; n < steps; ++n) {
+        ok = mbar_wait(&ss.s_full, static_cast<uint32_t>(n & 1), abort_flag, err, 471);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[64];
+        tmem_ld32(la + kColA + 64 * half, r);
+        tmem_ld32(la + kColA + 64 * half + 32, r + 32);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss.s_read);
+        const int key0 = (n0 + n) * kTile;
+        const bool border = key0 < tab.z || key0 + kTile > tab.w;
+        float pr[64];
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+          if constexpr (kCap) {
+            const float t = tanh_of(__uint_as_float(r[e]) * p.cap_in);
+            pr[e] = ex2_approx(fmaf(t, p.cap_log2, -st.x)) * fmaf(-t, t, 1.f);
+          } else {
+            pr[e] = ex2_approx(fmaf(__uint_as_float(r[e]), p.scale_log2, -st.x));
+          }
+        }
+        const uint32_t len = static_cast<uint32_t>(hi - lo);
+        const uint32_t d = static_cast<uint32_t>(key0 + 64 * half - lo);
+        const uint32_t col = (n & 1) ? kColC : kColB;
+        ok = mbar_wait(&ss.dp_full[n & 1], static_cast<uint32_t>((n >> 1) & 1), abort_flag, err, 472);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_ld32(la + col + 64 * half, r);
+        tmem_ld32(la + col + 64 * half + 32, r + 32);
+        tmem_ld_wait();
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float y0 = pr[2 * e] * (__uint_as_float(r[2 * e]) - st.y);
+          float y1 = pr[2 * e + 1] * (__uint_as_float(r[2 * e + 1]) - st.y);
+          if (border) {
+            if (d + 2 * e >= len) y0 = 0.f;
+            if (d + 2 * e + 1 >= len) y1 = 0.f;
+          }
+          pk[e] = pack16<kBF16>(y0, y1);
+        }
+        tmem_st32(la + col + 64 * half, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss.ds_full);
+      }
+      if (ok) {
+        ok = mbar_wait(&ss.done, 0, abort_flag, err, 473);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+    }
+    if (ok) {
+      const bool empty = p.ranges && live && [&] {
+        const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
+        return r.x >= r.y;
+      }();
+      const long long off = b * p.d0.sb + h * p.d0.sh + static_cast<long long>(row) * p.d0.ss;
+      store_acc<DP, kBF16>(la + kColD, half * (DP / 2), p.sm_scale, p.d0.p, off, p.D, live && !empty, steps > 0);
+      if (live && empty) {
+        const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int d0 = half * (DP / 2); d0 < min(p.D, (half + 1) * (DP / 2)); d0 += 8)
+          store8<kBF16>(p.d0.p, off + d0, z);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+template <int DP, bool kBF16, bool kCap>
+int launch_bwd(const CUtensorMap* m, BwdParams p, const DenseArgs& a, cudaStream_t stream) {
+  auto* kv = dkv_kernel<DP, kBF16, kCap>;
+  auto* qk = dq_kernel<DP, kBF16, kCap>;
+  if (cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, dkv_smem_bytes<DP>()) != cudaSuccess ||
+      cudaFuncSetAttribute(qk, cudaFuncAttributeMaxDynamicSharedMemorySize, dq_smem_bytes<DP>()) != cudaSuccess)
+    return BSA_ERR_CUDA;
+  if (a.dk.p) {
+    p.d0 = a.dk;
+    p.d1 = a.dv;
+    kv<<<a.B * a.Hk * p.k_tiles, kBwdThreads, dkv_smem_bytes<DP>(), stream>>>(m[0], m[1], m[2], m[3], p);
+    if (cudaGetLastError() != cudaSuccess) return BSA_ERR_CUDA;
+  }
+  if (!a.dq.p) return BSA_OK;
+  p.d0 = a.dq;
+  qk<<<a.B * a.H * p.q_tiles, kBwdThreads, dq_smem_bytes<DP>(), stream>>>(m[0], m[1], m[2], m[3], p);
+  return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+}
+
+}  // namespace dense
+
+long long dense_backward_stats_bytes(int B, int H, int Sq, int Bm) {
+  const long long rows = (static_cast<long long>(Sq) + dense::kTile - 1) / dense::kTile * dense::kTile;
+  return (static_cast<long long>(B) * H + Bm) * rows * 8;
+}
+
+int launch_dense_backward(const DenseArgs& a, cudaStream_t stream) {
+  using namespace dense;
+  CUtensorMap m[4];
+  int rc;
+  if ((rc = make_map4(&m[0], a.q, a.dtype, a.B, a.H, a.Sq, a.D, "q"))) return rc;
+  if ((rc = make_map4(&m[1], a.k, a.dtype, a.B, a.Hk, a.Sk, a.D, "k"))) return rc;
+  if ((rc = make_map4(&m[2], a.v, a.dtype, a.B, a.Hk, a.Sk, a.D, "v"))) return rc;
+  if ((rc = make_map4(&m[3], a.g, a.dtype, a.B, a.H, a.Sq, a.D, "gradient of out"))) return rc;
+  BwdParams p = {};
+  p.ranges = a.ranges; p.table = a.table; p.Bm = a.Bm;
+  p.H = a.H; p.Hk = a.Hk; p.G = a.H / a.Hk; p.Sq = a.Sq; p.Sk = a.Sk; p.D = a.D;
+  p.q_tiles = (a.Sq + kTile - 1) / kTile;
+  p.k_tiles = (a.Sk + kTile - 1) / kTile;
+  p.Sq_pad = p.q_tiles * kTile;
+  p.scale_log2 = a.sm_scale * 1.4426950408889634f;
+  p.sm_scale = a.sm_scale;
+  if (a.softcap > 0.f) {
+    p.cap_in = 2.f * p.scale_log2 / a.softcap;
+    p.cap_log2 = a.softcap * 1.4426950408889634f;
+  }
+  p.stats = reinterpret_cast<float2*>(a.stats);
+  p.rng = a.ranges ? reinterpret_cast<int2*>(a.stats + 2 * static_cast<long long>(a.B) * a.H * p.Sq_pad) : nullptr;
+  p.lse = a.lse;
+  p.o = a.o;
+  p.g = a.g;
+  if (static_cast<long long>(a.B) * a.H * p.q_tiles > INT_MAX || static_cast<long long>(a.B) * a.Hk * p.k_tiles > INT_MAX ||
+      static_cast<long long>(a.B) * a.H > 65535)
+    return set_error(BSA_ERR_SHAPE, "too many row tiles for one launch");
+  const dim3 sgrid(p.Sq_pad / 16, a.B * a.H);
+  const bool bf = a.dtype == BSA_DTYPE_BF16, cap = a.softcap > 0.f;
+  if (bf) stats_kernel<__nv_bfloat16><<<sgrid, 256, 0, stream>>>(p);
+  else stats_kernel<__half><<<sgrid, 256, 0, stream>>>(p);
+  rc = cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+  if (!rc) {
+    if (a.D > 64)
+      rc = bf ? (cap ? launch_bwd<128, true, true>(m, p, a, stream) : launch_bwd<128, true, false>(m, p, a, stream))
+              : (cap ? launch_bwd<128, false, true>(m, p, a, stream) : launch_bwd<128, false, false>(m, p, a, stream));
+    else
+      rc = bf ? (cap ? launch_bwd<64, true, true>(m, p, a, stream) : launch_bwd<64, true, false>(m, p, a, stream))
+              : (cap ? launch_bwd<64, false, true>(m, p, a, stream) : launch_bwd<64, false, false>(m, p, a, stream));
+  }
+  if (rc) return set_error(rc, "dense attention backward launch: %s", cudaGetErrorString(cudaGetLastError()));
+  return BSA_OK;
+}
+
+int dense_bwd_device_error(int clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, dense::g_dense_bwd_err, sizeof(int)) != cudaSuccess) return BSA_ERR_CUDA;
+  if (clear && v) {
+    const int z = 0;
+    cudaMemcpyToSymbol(dense::g_dense_bwd_err, &z, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace bsa

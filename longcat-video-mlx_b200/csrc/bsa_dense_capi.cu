@@ -252,6 +252,39 @@ int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype,
   return bsa::launch_dense(a, sms, static_cast<cudaStream_t>(stream));
 }
 
+int64_t bsa_masked_attention_backward_scratch_bytes(int B, int H, int Sq, int ranges_batch) {
+  if (B <= 0 || H <= 0 || Sq <= 0 || ranges_batch < 0) return 0;
+  return bsa::dense_backward_stats_bytes(B, H, Sq, ranges_batch);
+}
+
+int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* grad,
+                                  const float* lse, int dtype, int B, int H, int Hk, int Sq, int Sk, int D,
+                                  const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                                  const int64_t* out_strides, const int64_t* grad_strides, const int32_t* ranges,
+                                  const int32_t* table, int ranges_batch, float sm_scale, float softcap, void* dq,
+                                  void* dk, void* dv, void* scratch, void* stream) {
+  bsa::DenseArgs a;
+  int rc = dense_plan(a, q, k, v, dtype, B, H, Hk, Sq, Sk, D, q_strides, k_strides, v_strides, ranges, table,
+                      ranges_batch, sm_scale, softcap);
+  if (rc) return rc;
+  if (!out_strides || !grad_strides || !lse || !scratch || (dk == nullptr) != (dv == nullptr))
+    return set_error(BSA_ERR_ARG, "null pointer");
+  a.o = tensor(out, out_strides);
+  a.g = tensor(grad, grad_strides);
+  if ((rc = check_tensor(a.o, dtype, B, H, Sq, "out"))) return rc;
+  if ((rc = check_tensor(a.g, dtype, B, H, Sq, "gradient of out"))) return rc;
+  if (!aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) || !aligned(scratch, 16))
+    return set_error(BSA_ERR_ALIGN, "gradients and scratch must be 16-byte aligned");
+  const int64_t qs[3] = {static_cast<int64_t>(H) * Sq * D, static_cast<int64_t>(Sq) * D, D};
+  const int64_t ks[3] = {static_cast<int64_t>(Hk) * Sk * D, static_cast<int64_t>(Sk) * D, D};
+  a.dq = tensor(dq, qs);
+  a.dk = tensor(dk, ks);
+  a.dv = tensor(dv, ks);
+  a.lse = const_cast<float*>(lse);
+  a.stats = static_cast<float*>(scratch);
+  return bsa::launch_dense_backward(a, static_cast<cudaStream_t>(stream));
+}
+
 int bsa_kv8_append(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
                    int capacity, int D, const void* k, const void* v, int dtype, int n, const int64_t* k_strides,
                    const int64_t* v_strides, const int32_t* counts, void* stream) {

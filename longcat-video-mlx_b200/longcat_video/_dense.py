@@ -208,6 +208,31 @@ def masked_attention(q, k, v, ranges, table, sm_scale: float, softcap: float, ou
     return target, lse
 
 
+def masked_attention_backward(q, k, v, out, lse, grad, ranges, table, sm_scale: float, softcap: float, want_q: bool,
+                              want_kv: bool):
+    """(dq, dk, dv), contiguous; None where not wanted."""
+    B, H, Sq, D = q.shape
+    Hk, Sk = k.shape[1], k.shape[2]
+    empty = not (B and H and Sq and Sk)
+    new = torch.zeros if empty else torch.empty
+    dq = new((B, H, Sq, D), device=q.device, dtype=q.dtype) if want_q else None
+    dk, dv = (new((B, Hk, Sk, D), device=q.device, dtype=q.dtype) if want_kv else None for _ in range(2))
+    if empty:
+        return dq, dk, dv
+    q, k, v, out, grad = (_readable(t) for t in (q, k, v, out, grad))
+    bm = ranges.shape[0] if ranges is not None else 0
+    with _on(q):
+        n = int(_native.lib().bsa_masked_attention_backward_scratch_bytes(B, H, Sq, bm))
+        scratch = torch.empty((n,), device=q.device, dtype=torch.uint8)
+        rc = _native.lib().bsa_masked_attention_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), grad.data_ptr(), lse.data_ptr(),
+            _native._dtype_code(q), B, H, Hk, Sq, Sk, D, *(_native._strides(t) for t in (q, k, v, out, grad)),
+            _ptr(ranges), _ptr(table), max(bm, 1), float(sm_scale), float(softcap), _ptr(dq), _ptr(dk), _ptr(dv),
+            scratch.data_ptr(), _native._stream(q))
+    _native._check(rc, "bsa_masked_attention_backward")
+    return dq, dk, dv
+
+
 # ---------------------------------------------------------------------------------------------- 8-bit cache
 def _cache_args(c):
     B, Hk, cap, D = c.k_codes.shape

@@ -89,6 +89,28 @@ class AttentionMask:
         return cls(r, table, Sk)
 
 
+class _MaskedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, ranges, table, sm_scale, softcap):
+        out, lse = _dense.masked_attention(q, k, v, ranges, table, sm_scale, softcap, want_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, ranges, table)
+        ctx.rest = (sm_scale, softcap)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        q, k, v, out, lse, ranges, table = ctx.saved_tensors
+        if grad is None:
+            return (None,) * 7
+        need = ctx.needs_input_grad
+        dq, dk, dv = _dense.masked_attention_backward(q, k, v, out, lse, grad.to(q.dtype), ranges, table, *ctx.rest,
+                                                      need[0], need[1] or need[2])
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+
+
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[AttentionMask] = None, *,
                      sm_scale: Optional[float] = None, softcap: float = 0.0, return_lse: bool = False,
                      out: Optional[torch.Tensor] = None):
@@ -117,6 +139,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
             raise ValueError("out must have q's shape and dtype")
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if grad:
-        raise NotImplementedError
+        if out is not None:
+            raise ValueError("out= is for calls without gradients")
+        o, lse = _MaskedAttention.apply(q, k, v, ranges, table, scale, softcap)
+        return (o, lse) if return_lse else o
     o, lse = _dense.masked_attention(q, k, v, ranges, table, scale, softcap, out=out, want_lse=return_lse)
     return (o, lse) if return_lse else o

@@ -410,6 +410,166 @@ def test_attention_graph_replay(cuda):
         assert torch.equal(out, masked_attention(q, k, v, AttentionMask.build(3, 900, causal=True, k_lengths=lens)))
 
 
+def ref_gradients(q, k, v, g, lo, hi, scale, cap):
+    """(dq, dk, dv) in 64 bits, and for each the sum of the sizes of its terms."""
+    B, H, Sq, D = q.shape
+    G = H // k.shape[1]
+    o, lse, _, p = ref_attention(q, k, v, lo, hi, scale, cap)
+    qd, gd = q.double(), g.double()
+    kd, vd = k.double().repeat_interleave(G, 1), v.double().repeat_interleave(G, 1)
+    t = torch.tanh(qd @ kd.transpose(-1, -2) * scale / cap) if cap else torch.zeros((), device=q.device).double()
+    dp = gd @ vd.transpose(-1, -2)
+    delta = (gd * o).sum(-1, keepdim=True)
+    pt = p * (1 - t * t)
+    ds = pt * (dp - delta)
+    # what a rounding of p, ds or o can be relative to: ds itself, and delta's error by the rounding of o
+    loose = (gd.abs() * o.abs()).sum(-1, keepdim=True)
+    share = lambda x: x.view(B, H // G, G, *x.shape[2:]).sum(2)  # noqa: E731
+    grads = (ds @ kd * scale, share(ds.transpose(-1, -2) @ qd) * scale, share(p.transpose(-1, -2) @ gd))
+    sizes = lambda d: (d @ kd.abs() * scale, share(d.transpose(-1, -2) @ qd.abs()) * scale)  # noqa: E731
+    fine = pt * ((gd.abs() @ vd.abs().transpose(-1, -2)) + loose)  # fp32 error is relative to this
+    return grads, sizes(ds.abs()), sizes(pt * loose), sizes(fine), share(p.transpose(-1, -2) @ gd.abs())
+
+
+def check_gradients(got, q, k, v, g, lo, hi, scale, cap=0.0):
+    grads, ds, dl, fine, pg = ref_gradients(q, k, v, g, lo, hi, scale, cap)
+    u = unit(q.dtype)
+    tiny = 2.0 ** -24  # fp16 terms may be subnormal: p and ds are rounded to steps of 2^-24 there, over the row
+    for i in range(2):
+        n = q.shape[2] if i else k.shape[2]
+        x = (q if i else k).double().abs().amax() * scale * n * tiny * (q.dtype == torch.float16)
+        check(got[i], grads[i], u * grads[i].abs() + u * ds[i] + u * dl[i] + SLACK * fine[i] + x + tiny)
+    x = g.double().abs().amax() * q.shape[2] * (q.shape[1] // k.shape[1]) * tiny * (q.dtype == torch.float16)
+    check(got[2], grads[2], u * grads[2].abs() + (u + SLACK) * pg + x + tiny)
+
+
+def gradients(q, k, v, g, m, **kw):
+    from longcat_video.models.masked_attention import masked_attention
+
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = masked_attention(*leaves, m, **kw)
+    return out, torch.autograd.grad(out, leaves, g)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", SHAPES)
+def test_attention_gradients(cuda, dtype, B, H, Hk, Sq, Sk, D):
+    from longcat_video.models.masked_attention import AttentionMask, masked_attention
+
+    q, g = (rand((B, Sq, H, D), dtype, i, cuda).transpose(1, 2) for i in (1, 4))
+    k, v = rand((B, Hk, Sk, D), dtype, 2, cuda), rand((B, Hk, Sk, D), dtype, 3, cuda)
+    out, got = gradients(q, k, v, g, None)
+    assert torch.equal(out, masked_attention(q, k, v))
+    check_gradients(got, q, k, v, g, *full(Sq, Sk, cuda), 1 / math.sqrt(D))
+    m = AttentionMask.build(Sq, Sk, causal=True, prefix=5, device=cuda)
+    _, got = gradients(q, k, v, g, m, softcap=1.5, sm_scale=0.3)
+    check_gradients(got, q, k, v, g, *rows_of(m), 0.3, 1.5)
+
+
+@pytest.mark.parametrize("c", MASKS)
+@pytest.mark.parametrize("cap", [0.0, 4.0])
+def test_attention_mask_gradients(cuda, c, cap):
+    from longcat_video.models.masked_attention import AttentionMask
+
+    m = AttentionMask.from_ranges(torch.tensor([build_rows(**c)], dtype=torch.int32, device=cuda), c["Sk"])
+    q, k, v, g = (rand((2, n, s, 128), torch.bfloat16, i, cuda)
+                  for i, (n, s) in enumerate(((4, c["Sq"]), (2, c["Sk"]), (2, c["Sk"]), (4, c["Sq"]))))
+    _, got = gradients(q, k, v, g, m, softcap=cap)
+    check_gradients(got, q, k, v, g, *rows_of(m), 128 ** -0.5, cap)
+    _, again = gradients(q, k, v, g, m, softcap=cap)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("cap", [0.0, 4.0])
+def test_gradients_of_a_padded_batch(cuda, bad, cap):
+    """Padding of queries, keys and the gradient may hold anything; its own gradients are zeros."""
+    from longcat_video.models.masked_attention import AttentionMask
+
+    ql, kl = [200, 131, 0, 5], [130, 255, 300, 0]
+    q, k, v, g = (rand((4, n, s, 64), torch.float16, i, cuda)
+                  for i, (n, s) in enumerate(((4, 200), (2, 300), (2, 300), (4, 200))))
+    m = AttentionMask.build(200, 300, q_lengths=torch.tensor(ql, dtype=torch.int32, device=cuda),
+                            k_lengths=torch.tensor(kl, dtype=torch.int32, device=cuda))
+    out, want = gradients(q, k, v, g, m, softcap=cap)
+    check_gradients(want, q, k, v, g, *rows_of(m), 0.125, cap)
+    for b in range(4):
+        q[b, :, ql[b]:], g[b, :, ql[b]:], k[b, :, kl[b]:], v[b, :, kl[b]:] = bad, bad, bad, bad
+    out2, got = gradients(q, k, v, g, m, softcap=cap)
+    assert torch.equal(out, out2) and all(torch.equal(a, b) for a, b in zip(want, got))
+    for b in range(4):
+        assert (got[0][b, :, ql[b]:] == 0).all() and (got[1][b, :, kl[b]:] == 0).all() and (got[2][b, :, kl[b]:] == 0).all()
+
+
+def test_attention_gradient_against_differences(cuda):
+    from longcat_video.models.masked_attention import AttentionMask, masked_attention
+
+    q, k, v, g = (rand((1, 1, 9, 16), torch.float16, i, cuda) for i in range(4))
+    m = AttentionMask.build(9, 9, causal=True, device=cuda)
+    _, got = gradients(q, k, v, g, m, softcap=3.0)
+    f = lambda *a: (masked_attention(*a, m, softcap=3.0).double() * g.double()).sum().item()  # noqa: E731
+    for i, at in ((0, (0, 0, 5, 3)), (1, (0, 0, 2, 7)), (2, (0, 0, 0, 1))):
+        a, b = [[t.clone() for t in (q, k, v)] for _ in range(2)]
+        a[i][at] += 0.25
+        b[i][at] -= 0.25
+        h = (a[i][at] - b[i][at]).item()
+        # 9 rows of fp16 outputs below 4: 2^-11 * 4 * |g| each, twice over h; and h^2 of curvature
+        assert abs((f(*a) - f(*b)) / h - got[i][at].item()) < 0.05
+
+
+def test_attention_partial_gradients(cuda):
+    """Only some inputs want gradients; a broadcast key head; a gradient of another type and layout."""
+    from longcat_video.models.masked_attention import masked_attention
+
+    q, k, v = (rand((2, n, 140, 64), torch.bfloat16, n, cuda) for n in (4, 2, 2))
+    g = rand((2, 4, 140, 64), torch.bfloat16, 9, cuda)
+    full_g = gradients(q, k, v, g, None)[1]
+    for want in ((0,), (1,), (2,), (0, 2)):
+        leaves = [t.detach().requires_grad_(i in want) for i, t in enumerate((q, k, v))]
+        got = torch.autograd.grad(masked_attention(*leaves), [leaves[i] for i in want], g)
+        assert all(torch.equal(a, full_g[i]) for a, i in zip(got, want))
+    k1 = k[:, :1].detach().requires_grad_()
+    a = torch.autograd.grad(masked_attention(q, k1.expand(2, 2, 140, 64), v), k1, g)[0]
+    _, (_, dk, _) = gradients(q, k[:, :1].expand(2, 2, 140, 64), v, g, None)
+    assert torch.equal(a, dk.sum(1, keepdim=True))
+    leaf = q.detach().requires_grad_()
+    o = masked_attention(leaf, k, v).float().transpose(1, 2)
+    assert torch.equal(torch.autograd.grad(o, leaf, g.float().transpose(1, 2))[0], full_g[0])
+    one = torch.autograd.grad(masked_attention(leaf, k, v).sum(), leaf)[0]  # an expanded gradient
+    assert torch.equal(one, gradients(q, k, v, torch.ones_like(g), None)[1][0])
+
+
+def test_training_step_in_a_graph(cuda):
+    """Norm, rotation, attention and their gradients, captured on a side stream and replayed."""
+    from longcat_video.models.masked_attention import AttentionMask, masked_attention
+    from longcat_video.models.rope_3d import qk_norm_rope
+
+    rope = rope_of((2, 5, 14), 64, cuda)
+    x = [rand((1, n, 140, 64), torch.bfloat16, n, cuda) for n in (4, 2, 2)]
+    w = [torch.ones(64, device=cuda), torch.ones(64, device=cuda)]
+    g = rand((1, 4, 140, 64), torch.bfloat16, 9, cuda)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (*x, *w)]
+        q, k = qk_norm_rope(leaves[0], leaves[1], leaves[3], leaves[4], rope=rope)
+        out = masked_attention(q, k, leaves[2], AttentionMask.build(140, 140, prefix=70, device=cuda))
+        return (out.detach(), *torch.autograd.grad(out, leaves, g))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for i in range(3):
+        for t in (*x, g):
+            t.copy_(rand(t.shape, torch.bfloat16, 50 + i + t.shape[1], cuda))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(res, step()))
+
+
 def test_attention_refusals(cuda):
     from longcat_video.models.masked_attention import AttentionMask, masked_attention
 
