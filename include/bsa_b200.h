@@ -227,7 +227,8 @@ int bsa_attention_ranges(int32_t* ranges, int32_t* table, int batch, int Sq, int
 /* bsa_masked_attention: softmax attention of q [B, H, Sq, D] over k, v [B, Hk, Sk, D] (H a multiple of Hk: head
  * h reads key head h / (H / Hk)), fp16 or bf16.  ranges / table (both NULL: every key) hold ranges_batch (1 or B)
  * entries.  softcap > 0: scores are softcap * tanh(s / softcap).  A row without keys gives zeros, and -inf in lse
- * ([B, H, Sq] fp32, natural logarithm, NULL: not wanted).  scratch: bsa_masked_attention_scratch_bytes() bytes
+ * ([B, H, Sq] fp32, natural logarithm, NULL: not wanted).  out_rest ([B, H, Sq, D] in dtype, contiguous, NULL: not
+ * wanted) receives what the rounding of out left over; the backward needs it.  scratch: bsa_masked_attention_scratch_bytes() bytes
  * (0: none needed).  Scores of unseen keys never count, whatever they hold; so do values of keys that no row
  * of the same 256 rows sees.  A value that is infinite or NaN and seen by one row can reach another row of
  * the same tile. */
@@ -235,15 +236,15 @@ int64_t bsa_masked_attention_scratch_bytes(int B, int H, int Sq, int Sk, int D);
 int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype, int B, int H, int Hk, int Sq, int Sk,
                          int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                          const int32_t* ranges, const int32_t* table, int ranges_batch, float sm_scale, float softcap,
-                         void* out, const int64_t* out_strides, float* lse, void* scratch, void* stream);
+                         void* out, const int64_t* out_strides, void* out_rest, float* lse, void* scratch,
+                         void* stream);
 
-/* bsa_masked_attention_backward: gradients of that call from its out and lse and the gradient of out (which is
- * rounded to dtype, as out is).  dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may
+/* bsa_masked_attention_backward: gradients of that call from its out, out_rest and lse and the gradient of out.  dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may
  * be NULL.  Shared key heads sum over their query heads; keys no row sees get zeros.  No atomics: the same bits
  * every time.  scratch: bsa_masked_attention_backward_scratch_bytes() bytes (ranges_batch 0 without ranges). */
 int64_t bsa_masked_attention_backward_scratch_bytes(int B, int H, int Sq, int ranges_batch);
-int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* grad,
-                                  const float* lse, int dtype, int B, int H, int Hk, int Sq, int Sk, int D,
+int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
+                                  const void* grad, const float* lse, int dtype, int B, int H, int Hk, int Sq, int Sk, int D,
                                   const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                                   const int64_t* out_strides, const int64_t* grad_strides, const int32_t* ranges,
                                   const int32_t* table, int ranges_batch, float sm_scale, float softcap, void* dq,

@@ -42,6 +42,10 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   });
+  // The encoder is a driver call and needs a current context, which a host thread that has made no runtime
+  // call yet (an autograd worker, a fresh thread) does not have: this binds the current device's.
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
   return fn;
 }
 

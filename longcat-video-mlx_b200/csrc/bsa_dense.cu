@@ -67,6 +67,7 @@ struct Params {
   float cap_log2;      // cap log2(e)
   void* out;
   long long ob, oh, os;
+  void* out_lo;        // nullable: [B, H, Sq, D] contiguous, o - out in 16 bits
   float* lse;
   float* part;         // splits > 1: [splits][B * H * Sq][D + 1]: o, then lse in log2
   long long rows;      // B * H * Sq
@@ -399,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   for (int e = 0; e < 8; ++e) part[d0 + e] = v[8 * e8 + e];
                 } else {
                   store8<kBF16>(p.out, off + d0, v + 8 * e8);
+                  if (p.out_lo) store_rest8<kBF16>(p.out_lo, flat * p.D + d0, v + 8 * e8);
                 }
               }
             }
@@ -443,6 +445,7 @@ __global__ void __launch_bounds__(128) dense_join_kernel(const Params p) {
   const long long bh = row / p.Sq;
   const int h = static_cast<int>(bh % p.H);
   store8<kBF16>(p.out, (bh / p.H) * p.ob + h * p.oh + static_cast<long long>(i) * p.os + d0, v);
+  if (p.out_lo) store_rest8<kBF16>(p.out_lo, row * p.D + d0, v);
   if (p.lse && d0 == 0) p.lse[row] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
 }
 
@@ -511,6 +514,7 @@ int launch_dense(const DenseArgs& a, int sms, cudaStream_t stream) {
     p.cap_log2 = a.softcap * 1.4426950408889634f;
   }
   p.out = a.o.p; p.ob = a.o.sb; p.oh = a.o.sh; p.os = a.o.ss;
+  p.out_lo = a.o_lo;
   p.lse = a.lse;
   p.part = a.part;
   p.rows = bh * a.Sq;

@@ -83,5 +83,27 @@ __device__ __forceinline__ void store8(void* out, long long off, const float* v)
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + off) = u;
 }
 
+// What the rounding of store8 leaves over, in 16 bits: hi + lo holds a value to twice the bits
+template <bool kBF16>
+__device__ __forceinline__ void store_rest8(void* out, long long off, const float* v) {
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const uint32_t u = pack16<kBF16>(v[e], v[e + 1]);
+    float lo, hi;
+    if constexpr (kBF16) {
+      lo = __uint_as_float(u << 16);
+      hi = __uint_as_float(u & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+      lo = f.x;
+      hi = f.y;
+    }
+    r[e] = v[e] - lo;
+    r[e + 1] = v[e + 1] - hi;
+  }
+  store8<kBF16>(out, off, r);
+}
+
 }  // namespace dense
 }  // namespace bsa

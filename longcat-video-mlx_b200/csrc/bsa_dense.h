@@ -107,6 +107,7 @@ struct DenseArgs {
   int Bm = 1;                          // 1: one set of intervals for every batch entry
   float sm_scale = 1.f, softcap = 0.f;
   Tensor4 q, k, v, o, g;               // g: gradient of o
+  void* o_lo = nullptr;                // [B, H, Sq, D] contiguous: what o's rounding left over, nullable in the forward
   float* lse = nullptr;                // [B, H, Sq], nullable in the forward
   int splits = 1;
   float* part = nullptr;               // splits > 1: [splits][B * H * Sq][D + 1]

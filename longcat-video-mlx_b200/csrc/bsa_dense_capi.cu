@@ -234,7 +234,8 @@ int64_t bsa_masked_attention_scratch_bytes(int B, int H, int Sq, int Sk, int D) 
 int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype, int B, int H, int Hk, int Sq, int Sk,
                          int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                          const int32_t* ranges, const int32_t* table, int ranges_batch, float sm_scale, float softcap,
-                         void* out, const int64_t* out_strides, float* lse, void* scratch, void* stream) {
+                         void* out, const int64_t* out_strides, void* out_rest, float* lse, void* scratch,
+                         void* stream) {
   bsa::DenseArgs a;
   int rc = dense_plan(a, q, k, v, dtype, B, H, Hk, Sq, Sk, D, q_strides, k_strides, v_strides, ranges, table,
                       ranges_batch, sm_scale, softcap);
@@ -242,6 +243,8 @@ int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype,
   if (!out_strides) return set_error(BSA_ERR_ARG, "null pointer");
   a.o = tensor(out, out_strides);
   if ((rc = check_tensor(a.o, dtype, B, H, Sq, "out"))) return rc;
+  if (!aligned(out_rest, 16)) return set_error(BSA_ERR_ALIGN, "out_rest must be 16-byte aligned");
+  a.o_lo = out_rest;
   a.lse = lse;
   const int sms = sm_count();
   a.splits = bsa::dense_pick_splits(sms, B, H, Sq, Sk);
@@ -257,8 +260,8 @@ int64_t bsa_masked_attention_backward_scratch_bytes(int B, int H, int Sq, int ra
   return bsa::dense_backward_stats_bytes(B, H, Sq, ranges_batch);
 }
 
-int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* grad,
-                                  const float* lse, int dtype, int B, int H, int Hk, int Sq, int Sk, int D,
+int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
+                                  const void* grad, const float* lse, int dtype, int B, int H, int Hk, int Sq, int Sk, int D,
                                   const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                                   const int64_t* out_strides, const int64_t* grad_strides, const int32_t* ranges,
                                   const int32_t* table, int ranges_batch, float sm_scale, float softcap, void* dq,
@@ -267,14 +270,15 @@ int bsa_masked_attention_backward(const void* q, const void* k, const void* v, c
   int rc = dense_plan(a, q, k, v, dtype, B, H, Hk, Sq, Sk, D, q_strides, k_strides, v_strides, ranges, table,
                       ranges_batch, sm_scale, softcap);
   if (rc) return rc;
-  if (!out_strides || !grad_strides || !lse || !scratch || (dk == nullptr) != (dv == nullptr))
+  if (!out_strides || !grad_strides || !out_rest || !lse || !scratch || (dk == nullptr) != (dv == nullptr))
     return set_error(BSA_ERR_ARG, "null pointer");
   a.o = tensor(out, out_strides);
   a.g = tensor(grad, grad_strides);
   if ((rc = check_tensor(a.o, dtype, B, H, Sq, "out"))) return rc;
   if ((rc = check_tensor(a.g, dtype, B, H, Sq, "gradient of out"))) return rc;
-  if (!aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) || !aligned(scratch, 16))
-    return set_error(BSA_ERR_ALIGN, "gradients and scratch must be 16-byte aligned");
+  a.o_lo = const_cast<void*>(out_rest);
+  if (!aligned(out_rest, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) || !aligned(scratch, 16))
+    return set_error(BSA_ERR_ALIGN, "out_rest, gradients and scratch must be 16-byte aligned");
   const int64_t qs[3] = {static_cast<int64_t>(H) * Sq * D, static_cast<int64_t>(Sq) * D, D};
   const int64_t ks[3] = {static_cast<int64_t>(Hk) * Sk * D, static_cast<int64_t>(Sk) * D, D};
   a.dq = tensor(dq, qs);

@@ -179,8 +179,10 @@ def check_scale(sm_scale: float, softcap: float = 0.0) -> None:
         raise ValueError("softcap must be finite and >= 0")
 
 
-def masked_attention(q, k, v, ranges, table, sm_scale: float, softcap: float, out=None, want_lse: bool = False):
-    """(out, lse or None).  ranges / table: of attention_ranges, or None for every key."""
+def masked_attention(q, k, v, ranges, table, sm_scale: float, softcap: float, out=None, want_lse: bool = False,
+                     rest: Optional[torch.Tensor] = None):
+    """(out, lse or None).  ranges / table: of attention_ranges, or None for every key.  ``rest`` (contiguous, like
+    out) receives what out's rounding left over."""
     B, H, Sq, D = q.shape
     Hk, Sk = k.shape[1], k.shape[2]
     lse = torch.empty((B, H, Sq), device=q.device, dtype=torch.float32) if want_lse else None
@@ -196,7 +198,7 @@ def masked_attention(q, k, v, ranges, table, sm_scale: float, softcap: float, ou
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), _native._dtype_code(q), B, H, Hk, Sq, Sk, D,
                 _native._strides(q), _native._strides(k), _native._strides(v), _ptr(ranges), _ptr(table),
                 ranges.shape[0] if ranges is not None else 1, float(sm_scale), float(softcap), target.data_ptr(),
-                _native._strides(target), _ptr(lse), _ptr(scratch), _native._stream(q))
+                _native._strides(target), _ptr(rest), _ptr(lse), _ptr(scratch), _native._stream(q))
         _native._check(rc, "bsa_masked_attention")
     else:  # no rows, or no keys: zeros
         target.zero_()
@@ -208,7 +210,7 @@ def masked_attention(q, k, v, ranges, table, sm_scale: float, softcap: float, ou
     return target, lse
 
 
-def masked_attention_backward(q, k, v, out, lse, grad, ranges, table, sm_scale: float, softcap: float, want_q: bool,
+def masked_attention_backward(q, k, v, out, rest, lse, grad, ranges, table, sm_scale: float, softcap: float, want_q: bool,
                               want_kv: bool):
     """(dq, dk, dv), contiguous; None where not wanted."""
     B, H, Sq, D = q.shape
@@ -225,7 +227,7 @@ def masked_attention_backward(q, k, v, out, lse, grad, ranges, table, sm_scale: 
         n = int(_native.lib().bsa_masked_attention_backward_scratch_bytes(B, H, Sq, bm))
         scratch = torch.empty((n,), device=q.device, dtype=torch.uint8)
         rc = _native.lib().bsa_masked_attention_backward(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), grad.data_ptr(), lse.data_ptr(),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), grad.data_ptr(), lse.data_ptr(),
             _native._dtype_code(q), B, H, Hk, Sq, Sk, D, *(_native._strides(t) for t in (q, k, v, out, grad)),
             _ptr(ranges), _ptr(table), max(bm, 1), float(sm_scale), float(softcap), _ptr(dq), _ptr(dk), _ptr(dv),
             scratch.data_ptr(), _native._stream(q))

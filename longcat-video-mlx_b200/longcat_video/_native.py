@@ -80,10 +80,10 @@ _SIGNATURES = {
                                + [_vp, _vp], _i),
     "bsa_attention_ranges": ([_vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp], _i),
     "bsa_masked_attention_scratch_bytes": ([_i] * 5, ctypes.c_int64),
-    "bsa_masked_attention": ([_vp, _vp, _vp] + [_i] * 7 + [_c_i64p] * 3 + [_vp, _vp, _i, _f, _f, _vp, _c_i64p, _vp, _vp,
+    "bsa_masked_attention": ([_vp, _vp, _vp] + [_i] * 7 + [_c_i64p] * 3 + [_vp, _vp, _i, _f, _f, _vp, _c_i64p, _vp, _vp, _vp,
                                                                           _vp], _i),
     "bsa_masked_attention_backward_scratch_bytes": ([_i] * 4, ctypes.c_int64),
-    "bsa_masked_attention_backward": ([_vp] * 6 + [_i] * 7 + [_c_i64p] * 5 + [_vp, _vp, _i, _f, _f] + [_vp] * 5, _i),
+    "bsa_masked_attention_backward": ([_vp] * 7 + [_i] * 7 + [_c_i64p] * 5 + [_vp, _vp, _i, _f, _f] + [_vp] * 5, _i),
     "bsa_kv8_append": (_c_cache + [_vp, _vp, _i, _i, _c_i64p, _c_i64p, _vp, _vp], _i),
     "bsa_kv8_unpack": (_c_cache + [_vp, _vp, _i, _i, _c_i64p, _c_i64p, _vp, _vp, _i, _vp], _i),
     "bsa_kv8_attention_scratch_bytes": ([_i] * 6, ctypes.c_int64),

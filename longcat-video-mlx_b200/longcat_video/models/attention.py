@@ -9,18 +9,24 @@ name the reference accepts routes to the one CUDA engine; the hook's own fallbac
 shape that is not a multiple of chunk_thw falls back to dense attention (:174-179) -- is kept as
 the reference has it, and only for that error.  With BSA on, RoPE is fused into the routing
 kernel instead of being applied as a separate pass.
+
+With ``dense_kernels`` on, what is not block-sparse runs on the engine's own kernels too, with gradients:
+q/k norm and RoPE in one launch, dense attention, the conditioning branch as one call under a prefix
+mask, and the chunked continuation over a :class:`KVCache8`.
 """
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
 
 from .._native import BSAShapeError
 from .block_sparse_attention import bsa_attention
-from .rope_3d import RotaryPositionalEmbedding
+from .kv_cache import KVCache8
+from .masked_attention import AttentionMask, masked_attention
+from .rope_3d import RotaryPositionalEmbedding, qk_norm_rope
 
 BSA_BACKENDS = ("tier_a", "metal", "metal_v2", "metal_v3", "metal_v4", "cuda")
 
@@ -58,6 +64,7 @@ class Attention(torch.nn.Module):
         self.bsa_chunk_thw: Tuple[int, int, int] = (4, 4, 4)
         self.bsa_backend: str = "tier_a"
         self.bsa_topk: Optional[int] = None  # explicit k overrides the floor rule
+        self.dense_kernels: bool = False  # the engine's kernels for what is not block-sparse (bf16 / fp16 on CUDA)
 
     def _bsa_ok(self, q: torch.Tensor, k: torch.Tensor, shape) -> bool:
         return self.enable_bsa and shape is not None and q.shape[-2] == k.shape[-2]
@@ -85,11 +92,21 @@ class Attention(torch.nn.Module):
                 # FLOPs with no message.  Views the kernels cannot read in place are copied once by
                 # the engine's host layer, not refused.
                 pass
+        if self.dense_kernels:
+            if raw_qk or rope_grid is not None:
+                q, k = self._norm_rope(q, k, rope_grid, norm=raw_qk)
+            return masked_attention(q, k, v, sm_scale=self.scale)
         if raw_qk:
             q, k = self.q_norm(q), self.k_norm(k)
         if rope_grid is not None:
             q, k = self.rope_3d(q, k, rope_grid)
         return F.scaled_dot_product_attention(q, k, v, scale=self.scale)
+
+    def _norm_rope(self, q: torch.Tensor, k: torch.Tensor, grid=None, start: int = 0, norm: bool = True):
+        """q_norm / k_norm and the RoPE over ``grid`` (None: none) from place ``start`` on, in one launch."""
+        rope = self.rope_3d.tables(grid, q.device) if grid is not None else None
+        wq, wk = (self.q_norm.weight, self.k_norm.weight) if norm else (None, None)
+        return qk_norm_rope(q, k, wq, wk, self.q_norm.eps, rope=rope, start=start)
 
     def forward(self, x: torch.Tensor, shape: Tuple[int, int, int],
                 num_cond_latents: Optional[int] = None, return_kv: bool = False):
@@ -98,6 +115,8 @@ class Attention(torch.nn.Module):
         B, N, C = x.shape
         qkv = self.qkv(x).reshape(B, N, 3, self.num_heads, self.head_dim).permute(2, 0, 3, 1, 4)
         q, k, v = qkv[0], qkv[1], qkv[2]
+        if self.dense_kernels and not self.enable_bsa:
+            return self._forward_dense(q, k, v, shape, num_cond_latents, return_kv)
         # the q/k RMSNorm runs fused in the engine's routing kernel (one read of the raw q/k, one write of
         # the normalised, rotated q/k) when the call takes the BSA path on the GPU in bf16/fp16
         fuse_norm = (not return_kv and not (num_cond_latents is not None and num_cond_latents > 0)
@@ -129,15 +148,63 @@ class Attention(torch.nn.Module):
         out = self.proj(out.transpose(1, 2).reshape(B, N, C))
         return (out, kv) if return_kv else out
 
+    def _forward_dense(self, q, k, v, shape, num_cond_latents, return_kv):
+        """The block without BSA on the engine's dense kernels.  Conditioning frames attend to themselves and the
+        others to everything (attention.py:206-222), which is one call under a prefix mask."""
+        B, H, N, D = q.shape
+        mask = None
+        if num_cond_latents is not None and num_cond_latents > 0:
+            mask = AttentionMask.build(N, N, prefix=num_cond_latents * (N // shape[0]), device=q.device)
+        kv = None
+        if return_kv:  # the cache holds k after its norm, before RoPE
+            k = qk_norm_rope(k, q_weight=self.k_norm.weight, eps=self.k_norm.eps)
+            kv = (k, v)
+            rope = self.rope_3d.tables(shape, q.device)
+            q = qk_norm_rope(q, q_weight=self.q_norm.weight, eps=self.q_norm.eps, rope=rope)
+            k = qk_norm_rope(k, rope=rope)
+        else:
+            q, k = self._norm_rope(q, k, shape)
+        out = self._project(q, k, v, mask)
+        return (out, kv) if return_kv else out
+
+    def _project(self, q, k, v, mask=None):
+        """masked_attention and the output projection; without gradients the attention writes the projection's
+        [B, N, H, D] layout in place."""
+        B, H, N, D = q.shape
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+            out = masked_attention(q, k, v, mask, sm_scale=self.scale)
+            return self.proj(out.transpose(1, 2).reshape(B, N, H * D))
+        out = torch.empty((B, N, H, D), device=q.device, dtype=q.dtype)
+        masked_attention(q, k, v, mask, sm_scale=self.scale, out=out.permute(0, 2, 1, 3))
+        return self.proj(out.view(B, N, H * D))
+
+    def quantize_kv_cache(self, kv: Tuple[torch.Tensor, torch.Tensor], shape: Tuple[int, int, int],
+                          num_cond_latents: Optional[int]) -> KVCache8:
+        """The (k, v) of ``forward(..., return_kv=True)``, or their first tokens, as an 8-bit cache for
+        :meth:`forward_with_kv_cache` with the same ``num_cond_latents``: half of the memory in each of the
+        layers.  With conditioning latents the keys are rotated before they are held (their places are the first
+        of every grid with these frame sizes), so a lookup reads them as they are."""
+        k, v = kv
+        if num_cond_latents is not None and num_cond_latents > 0:
+            n = num_cond_latents * shape[1] * shape[2]
+            if k.shape[2] != n:
+                raise ValueError(f"{k.shape[2]} cached tokens are not {num_cond_latents} latents of {shape[1]} x {shape[2]}")
+            k = qk_norm_rope(k, rope=self.rope_3d.tables((num_cond_latents, shape[1], shape[2]), k.device))
+        return KVCache8.from_kv(k, v)
+
     def forward_with_kv_cache(self, x: torch.Tensor, shape: Tuple[int, int, int], num_cond_latents: Optional[int],
-                              kv_cache: Tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
+                              kv_cache: Union[Tuple[torch.Tensor, torch.Tensor], KVCache8]) -> torch.Tensor:
         """attention.py:235-275: chunked continuation.  The fresh K/V are appended to the cached ones
         (a cache stored at batch 1 is broadcast to B).  With conditioning latents, q is padded with zeros
         over the cache positions so that RoPE over the extended grid (T + num_cond_latents, H, W) gives
-        q and k their global positions.  Q and KV lengths differ, so the hook takes its dense path."""
+        q and k their global positions.  Q and KV lengths differ, so the hook takes its dense path.
+        A :class:`KVCache8` (:meth:`quantize_kv_cache`) is read by the engine's kernels, whatever
+        ``dense_kernels`` says."""
         B, N, C = x.shape
         qkv = self.qkv(x).reshape(B, N, 3, self.num_heads, self.head_dim).permute(2, 0, 3, 1, 4)
         q, k, v = qkv[0], qkv[1], qkv[2]
+        if isinstance(kv_cache, KVCache8) or self.dense_kernels:
+            return self._continue_dense(q, k, v, shape, num_cond_latents, kv_cache)
         q = self.q_norm(q)
         k = self.k_norm(k)
         T, Hl, Wl = shape
@@ -153,3 +220,23 @@ class Attention(torch.nn.Module):
             q = q_pad[:, :, -N:]
         out = self._process_attn(q, k_full, v_full, shape=None)
         return self.proj(out.transpose(1, 2).reshape(B, N, C))
+
+    def _continue_dense(self, q, k, v, shape, num_cond_latents, kv_cache):
+        """The continuation on the engine's dense kernels: the fresh tokens stand behind the cached ones in the
+        extended grid."""
+        B, H, N, D = q.shape
+        T, Hl, Wl = shape
+        rotated = num_cond_latents is not None and num_cond_latents > 0
+        grid = (T + num_cond_latents, Hl, Wl) if rotated else None
+        if isinstance(kv_cache, KVCache8):
+            cache = kv_cache.expand(B)
+            q, k = self._norm_rope(q, k, grid, start=num_cond_latents * Hl * Wl if rotated else 0)
+            out = torch.empty((B, N, H, D), device=q.device, dtype=q.dtype)
+            cache.attend(q.detach(), k.detach(), v.detach(), sm_scale=self.scale, out=out.permute(0, 2, 1, 3))
+            return self.proj(out.view(B, N, H * D))
+        k_cache, v_cache = (t.expand(B, *t.shape[1:]) if t.shape[0] == 1 else t for t in kv_cache)
+        n = k_cache.shape[2]
+        q, k = self._norm_rope(q, k, grid, start=n if rotated else 0)
+        if rotated:
+            k_cache = qk_norm_rope(k_cache, rope=self.rope_3d.tables(grid, q.device))
+        return self._project(q, torch.cat([k_cache, k], dim=2), torch.cat([v_cache, v], dim=2))

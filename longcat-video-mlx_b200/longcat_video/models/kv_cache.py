@@ -73,6 +73,17 @@ class KVCache8:
     def capacity(self) -> int:
         return int(self.k_codes.shape[2])
 
+    def expand(self, batch: int) -> "KVCache8":
+        """This cache, or a one-sequence cache repeated for a batch (a copy)."""
+        B = self.k_codes.shape[0]
+        if batch == B:
+            return self
+        if B != 1:
+            raise ValueError(f"a cache of {B} sequences for a batch of {batch}")
+        rep = lambda t: t.view(torch.uint8).repeat(batch, 1, 1, 1).view(t.dtype)  # noqa: E731
+        return KVCache8(rep(self.k_codes), self.k_scale.repeat(batch, 1, 1), rep(self.v_codes),
+                        self.v_scale.repeat(batch, 1, 1), self.lengths.repeat(batch))
+
     def _check_kv(self, k, v) -> None:
         B, Hk, cap, D = self.k_codes.shape
         _dense._same_place(self.k_codes, k, v)

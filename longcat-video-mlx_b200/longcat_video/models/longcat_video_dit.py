@@ -47,6 +47,8 @@ class LongCatVideoTransformer3DModel(torch.nn.Module):
         model._bsa_topk = int(topk) if topk is not None else None
         if config.get("enable_bsa", False):
             model.enable_bsa()
+        if config.get("enable_dense_kernels", False):
+            model.enable_dense_kernels()
         return model
 
     def enable_bsa(self, backend: str = "tier_a") -> None:
@@ -78,6 +80,16 @@ class LongCatVideoTransformer3DModel(torch.nn.Module):
         """longcat_video_dit.py:259-262."""
         for block in self.blocks:
             block.attn.enable_bsa = False
+
+    def enable_dense_kernels(self) -> None:
+        """What is not block-sparse (norm and RoPE, dense attention, the conditioning branch, the continuation) on
+        the engine's kernels, for bf16 / fp16 models on CUDA; BSA stays as it is set."""
+        for block in self.blocks:
+            block.attn.dense_kernels = True
+
+    def disable_dense_kernels(self) -> None:
+        for block in self.blocks:
+            block.attn.dense_kernels = False
 
     def attention_modules(self) -> List[Attention]:
         return [b.attn for b in self.blocks]

@@ -92,8 +92,9 @@ class AttentionMask:
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, ranges, table, sm_scale, softcap):
-        out, lse = _dense.masked_attention(q, k, v, ranges, table, sm_scale, softcap, want_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, ranges, table)
+        rest = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        out, lse = _dense.masked_attention(q, k, v, ranges, table, sm_scale, softcap, want_lse=True, rest=rest)
+        ctx.save_for_backward(q, k, v, out, rest, lse, ranges, table)
         ctx.rest = (sm_scale, softcap)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -102,11 +103,11 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
-        q, k, v, out, lse, ranges, table = ctx.saved_tensors
+        q, k, v, out, rest, lse, ranges, table = ctx.saved_tensors
         if grad is None:
             return (None,) * 7
         need = ctx.needs_input_grad
-        dq, dk, dv = _dense.masked_attention_backward(q, k, v, out, lse, grad.to(q.dtype), ranges, table, *ctx.rest,
+        dq, dk, dv = _dense.masked_attention_backward(q, k, v, out, rest, lse, grad.to(q.dtype), ranges, table, *ctx.rest,
                                                       need[0], need[1] or need[2])
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 

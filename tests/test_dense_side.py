@@ -393,6 +393,31 @@ def test_attention_views_streams_and_out(cuda):
     assert torch.equal(side, want)
 
 
+def test_attention_from_fresh_threads(cuda):
+    """A host thread whose first CUDA work is this call (an autograd worker is one)."""
+    import threading
+
+    from longcat_video.models.masked_attention import masked_attention
+
+    q = rand((1, 2, 130, 64), torch.bfloat16, 1, cuda)
+    g = rand(q.shape, torch.bfloat16, 2, cuda)
+    want = gradients(q, q, q, g, None)
+    res, outs = {}, [torch.empty_like(q) for _ in range(4)]
+
+    def work(i):
+        try:
+            res[i] = masked_attention(q, q, q, out=outs[i])
+        except Exception as e:  # noqa: BLE001
+            res[i] = e
+
+    for i in range(4):
+        t = threading.Thread(target=work, args=(i,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(res[i], want[0]) for i in range(4))
+
+
 def test_attention_graph_replay(cuda):
     """Captured with its mask: replays follow new lengths and inputs."""
     from longcat_video.models.masked_attention import AttentionMask, masked_attention
@@ -834,3 +859,96 @@ def test_cache_refusals(cuda):
             KVCache8(*[t if i == j else g for j, g in enumerate(good)])
     c.append(x[:, :, :0], x[:, :, :0])
     assert (c.attend(x) == 0).all() and c.attend(x[:, :, :0]).shape == (2, 2, 0, 64)
+
+
+# ------------------------------------------------------------------------------- the attention hook's dense side
+def hook(cuda, dtype=torch.bfloat16, dim=128, heads=2):
+    from longcat_video.models.attention import Attention
+
+    torch.manual_seed(3)
+    m = Attention(dim, heads).to(cuda, dtype)
+    with torch.no_grad():
+        for n in (m.q_norm, m.k_norm):
+            n.weight.add_(0.2 * torch.randn_like(n.weight))
+    return m
+
+
+def near(a, b, rel):
+    assert a.shape == b.shape and torch.isfinite(a).all()
+    assert ((a.double() - b.double()).norm() / b.double().norm()).item() <= rel
+
+
+# The torch path rounds after each step, the kernels once a stage: a handful of roundings each way, averaged over
+# the block's sums.  2^-8 of bf16 a rounding, two dozen of them in independent directions at most.
+HOOK_REL = 5 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("cond", [None, 0, 2])
+@pytest.mark.parametrize("B", [1, 2])
+def test_hook_forward(cuda, B, cond):
+    m = hook(cuda)
+    shape = (5, 6, 7)
+    x = rand((B, 210, 128), torch.bfloat16, 1, cuda)
+    with torch.no_grad():
+        want, kv = m(x, shape, cond, return_kv=True)
+        m.dense_kernels = True
+        got = m(x, shape, cond)
+        got2, kv2 = m(x, shape, cond, return_kv=True)
+    near(got, want, HOOK_REL)
+    near(got2, want, HOOK_REL)
+    near(kv2[0], kv[0], HOOK_REL)
+    assert torch.equal(kv2[1], kv[1])
+
+
+def test_hook_gradients(cuda):
+    m = hook(cuda)
+    x = rand((1, 210, 128), torch.bfloat16, 1, cuda).requires_grad_()
+    g = rand((1, 210, 128), torch.bfloat16, 2, cuda)
+    leaves = [x, m.q_norm.weight, m.k_norm.weight, m.qkv.weight]
+    want = torch.autograd.grad(m(x, (5, 6, 7), 2), leaves, g)
+    m.dense_kernels = True
+    got = torch.autograd.grad(m(x, (5, 6, 7), 2), leaves, g)
+    for a, b in zip(got, want):
+        near(a, b, 2 * HOOK_REL)
+
+
+@pytest.mark.parametrize("cond", [None, 2])
+@pytest.mark.parametrize("B", [1, 2])
+def test_hook_continuation(cuda, B, cond):
+    """Over the (k, v) of earlier tokens, as tensors and as an 8-bit cache."""
+    m = hook(cuda)
+    x0, x = rand((1, 84, 128), torch.bfloat16, 1, cuda), rand((B, 126, 128), torch.bfloat16, 2, cuda)
+    with torch.no_grad():
+        _, kv = m(x0, (2, 6, 7), None, return_kv=True)
+        want = m.forward_with_kv_cache(x, (3, 6, 7), cond, kv)
+        cache = m.quantize_kv_cache(kv, (2, 6, 7), cond)
+        eight = m.forward_with_kv_cache(x, (3, 6, 7), cond, cache)
+        m.dense_kernels = True
+        got = m.forward_with_kv_cache(x, (3, 6, 7), cond, kv)
+    assert cache.lengths.tolist() == [84]
+    near(got, want, HOOK_REL)
+    near(eight, want, HOOK_REL + 2 * 2.0 ** -4)  # keys and values in e4m3: half a step is 2^-4
+    with pytest.raises(ValueError):
+        m.quantize_kv_cache(kv, (2, 6, 7), 1)
+
+
+def test_hook_bsa_keeps_its_path(cuda):
+    """dense_kernels leaves block-sparse calls alone, and serves the hook's fallback for odd shapes."""
+    m = hook(cuda)
+    m.enable_bsa, m.bsa_sparsity = True, 0.5
+    x = rand((1, 512, 128), torch.bfloat16, 1, cuda)
+    odd = rand((1, 210, 128), torch.bfloat16, 2, cuda)
+    with torch.no_grad():
+        want, want_odd = m(x, (8, 8, 8)), m(odd, (5, 6, 7))
+        m.dense_kernels = True
+        assert torch.equal(m(x, (8, 8, 8)), want)
+        near(m(odd, (5, 6, 7)), want_odd, HOOK_REL)
+
+
+def test_dit_switch():
+    from longcat_video.models.longcat_video_dit import LongCatVideoTransformer3DModel
+
+    d = LongCatVideoTransformer3DModel.from_config(dict(hidden_size=64, depth=2, num_heads=2, enable_dense_kernels=True))
+    assert all(a.dense_kernels and not a.enable_bsa for a in d.attention_modules())
+    d.disable_dense_kernels()
+    assert not any(a.dense_kernels for a in d.attention_modules())
