@@ -10,15 +10,19 @@
 //     O_t[128 x D]  += P_t V           A = P_t in tensor memory, over the scores it came from; B = V
 // TMEM: S_0, S_1, O_0, O_1 of 128 columns each.
 //
-// Roles (320 threads, one CTA to an SM):
+// Roles (384 threads, one CTA to an SM):
 //   warps 0-3, 4-7 : softmax of tile 0, 1; a thread owns one row, so neither maximum nor sum leaves it
-//   warp 8         : issues every product, in the order S_0(0) S_1(0) [P_0 V, S_0(j+1), P_1 V, S_1(j+1)] ...;
-//                    products of one thread run in order, so S_t(j+1) may overwrite the P_t(j) that was read
-//                    before it, and its arrival also says that O_t holds all of P_t V up to j
-//   warp 9         : loads; one ring for K and V tiles in the order of their use
-// The maximum is raised, and O and l rescaled, only when a score exceeds it by more than 2^8: P stays within
+//   warps 8, 10    : issue the products of tile 0, 1: S(0), then P(j) V, S(j+1) for each j.  Products of one thread run in
+//                    order, so S(j+1) may overwrite the P(j) that was read before it, and its arrival also says that O
+//                    holds all of P V up to j.  A product adds to the same accumulator as the one before it and waits
+//                    for it, about 100 cycles where 64 would do (128 x 128 x 16); two issuing threads put the two tiles'
+//                    chains side by side, which one thread in a fixed order does not
+//   warp 9         : loads; one ring for K and V tiles in the order of their use (warp 11: idle, it makes the group
+//                    whole that gives its registers to the softmax warps)
+// The maximum is raised, and O and l rescaled, only when a score exceeds it by more than 2^8 (log2 8): P stays within
 // fp16's range and rounding is relative, so the result is as exact as with the true maximum.
-// P is rounded to the input type for the tensor cores; l is summed from the fp32 values.
+// P is rounded to the input type for the tensor cores, and o is divided by the sum of the rounded values: the weights
+// then sum to 1 and their rounding errors count against v_j - o_i instead of v_j.  lse comes from the fp32 values.
 //
 // Masked places never reach a result: scores are replaced by -inf whatever they hold, and V rows that no row
 // of the CTA sees are zeroed in shared memory (0 * NaN would be NaN).  Tiles outside the union of the rows'
@@ -33,8 +37,14 @@ namespace dense {
 
 __device__ int g_dense_err;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
 constexpr float kRescale = 8.f;  // log2
+#ifndef BSA_POLY_OF
+#define BSA_POLY_OF 4
+#endif
+// One pair of exponentials in kPolyOf is computed on the FMA pipe: the special-function unit's 16 a cycle are as
+// many cycles as the tensor cores need for both products, so what else waits for it shows at once.
+constexpr int kPolyOf = BSA_POLY_OF;
 constexpr uint32_t kTmemCols = 512;
 __host__ __device__ constexpr uint32_t col_s(int t) { return 128u * static_cast<uint32_t>(t); }
 __host__ __device__ constexpr uint32_t col_o(int t) { return 256u + 128u * static_cast<uint32_t>(t); }
@@ -46,8 +56,9 @@ struct Smem {
   uint64_t q_full;
   uint64_t full[kStages], empty[kStages];
   uint64_t fix;
-  uint64_t s_full[2], p_full[2], o_full[2];
-  uint64_t drain;
+  uint64_t s_full[2], p_full[2][2], o_full[2];
+  uint64_t turn[2];  // tile t's exponentials of a step are done: the other tile's turn
+  uint64_t drain[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -61,6 +72,7 @@ struct Params {
   int q_tiles;         // tiles of 128 rows
   int per_cta;         // 1 or 2 query tiles
   int groups;          // CTAs along the rows
+  int heads;           // B * H
   int splits;          // CTAs along the keys
   float scale_log2;    // sm_scale log2(e)
   float cap_in;        // 2 sm_scale log2(e) / cap
@@ -87,12 +99,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   S& ss = *reinterpret_cast<S*>(smem + S::kTiles);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // (b, h) outside, then the rows, the last tiles first (they see the most keys under a causal mask), then splits
+  // The last rows of every head first: under causal and prefix masks they see the most keys, and the CTAs that are
+  // left for the end are short (20,280 tokens, 6,240 of them a prefix: head by head left the SMs idle for a sixth
+  // of the time).  Heads side by side read K and V from L2 as long as they fit, and HBM has the rate for the rest.
   int item = blockIdx.x;
   const int split = item % p.splits;
   item /= p.splits;
-  const int grp = p.groups - 1 - item % p.groups;
-  const int bh = item / p.groups;
+  const int bh = item % p.heads;
+  const int grp = p.groups - 1 - item / p.heads;
   const int b = bh / p.H, h = bh - b * p.H;
   const int hk = h / p.G;
   const int tile0 = grp * p.per_cta;
@@ -121,15 +135,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&ss.q_full, 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&ss.full[i], 1);
-      mbar_init(&ss.empty[i], 1);
+      mbar_init(&ss.empty[i], tiles);  // both tiles' products have read it
     }
     mbar_init(&ss.fix, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&ss.s_full[t], 1);
-      mbar_init(&ss.p_full[t], 4);
+      mbar_init(&ss.p_full[t][0], 4);
+      mbar_init(&ss.p_full[t][1], 4);
       mbar_init(&ss.o_full[t], 1);
+      mbar_init(&ss.turn[t], 4);
     }
-    mbar_init(&ss.drain, 1);
+    mbar_init(&ss.drain[0], 1);
+    mbar_init(&ss.drain[1], 1);
     ss.abort_flag = 0;
     fence_mbar_init();
   }
@@ -143,6 +160,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &ss.abort_flag;
   int* err = &g_dense_err;
 
+  // registers: 384 x 168 at launch = 128 x 40 + 256 x 232; a softmax thread holds a row of 128 scores
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 9) {
     // ------------------------------------------------------------------ loads
     if (steps > 0) {
@@ -159,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int i = 0; i < 2 * steps && ok; ++i) {
         if (issued >= kStages) {
-          ok = mbar_wait(&ss.empty[slot], phase ^ 1u, abort_flag, err, 301);
+          ok = bar_wait(&ss.empty[slot], phase ^ 1u, abort_flag, err, 301);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
@@ -178,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             load_tile<DP>(dst, &tm_v, &ss.fix, row, hk, b);
           }
           __syncwarp();
-          ok = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 302);
+          ok = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 302);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           ++fixes;
@@ -206,18 +226,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 8) {
-    // ------------------------------------------------------------------ products
-    if (lane == 0 && steps > 0) {
+  } else if (warp != 11) {
+    // ------------------------------------------------------------------ products of tile t
+    const int t = (warp - 8) >> 1;
+    if (lane == 0 && steps > 0 && t < tiles) {
       constexpr uint32_t kIdQK = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t kIdPV = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
-      const uint32_t qb = smem_u32(sQ), kvb = smem_u32(sKV);
-      auto qk = [&](int t, int slot) {
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          umma_ss(tmem + col_s(t), desc_d(qb + t * kBytes, kk), desc_d(kvb + slot * kBytes, kk), kIdQK, kk > 0);
-        umma_commit(&ss.s_full[t]);
-      };
+      const uint32_t qb = smem_u32(sQ + t * kBytes), kvb = smem_u32(sKV);
+      const uint32_t s_col = tmem + col_s(t), o_col = tmem + col_o(t);
       int slot = 0;
       uint32_t phase = 0;
       auto next = [&] {
@@ -226,52 +242,45 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase ^= 1u;
         }
       };
-      bool ok = mbar_wait(&ss.q_full, 0, abort_flag, err, 311) && mbar_wait(&ss.full[0], 0, abort_flag, err, 312);
-      if (ok) {
+      auto qk = [&] {  // S of the ring's next tile
+        if (!bar_wait(&ss.full[slot], phase, abort_flag, err, 312)) return false;
         tc_fence_after();
-        for (int t = 0; t < tiles; ++t) qk(t, 0);
-        umma_commit(&ss.empty[0]);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+          umma_ss(s_col, desc_d(qb, kk), desc_d(kvb + slot * kBytes, kk), kIdQK, kk > 0);
+        umma_commit(&ss.s_full[t]);
+        umma_commit(&ss.empty[slot]);
         next();
-      }
+        return true;
+      };
+      bool ok = bar_wait(&ss.q_full, 0, abort_flag, err, 311) && qk();
       for (int j = 0; j < steps && ok; ++j) {
-        const int vs = slot;
-        ok = mbar_wait(&ss.full[vs], phase, abort_flag, err, 313);
-        if (!ok) break;
-        next();
-        const int ks = slot;
-        const uint32_t kphase = phase;
-        const bool more = j + 1 < steps;
-        for (int t = 0; t < tiles; ++t) {
-          ok = mbar_wait(&ss.p_full[t], static_cast<uint32_t>(j & 1), abort_flag, err, 314);
+        ok = bar_wait(&ss.full[slot], phase, abort_flag, err, 313);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // the first 64 keys' products run while the others' weights are computed
+          if (ok) ok = bar_wait(&ss.p_full[t][x], static_cast<uint32_t>(j & 1), abort_flag, err, 314);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_ts(tmem + col_o(t), tmem + col_s(t) + 8 * kk, desc_rows(kvb + vs * kBytes, kk), kIdPV, j > 0 || kk > 0);
-          if (more) {
-            if (t == 0) ok = mbar_wait(&ss.full[ks], kphase, abort_flag, err, 315);
-            if (!ok) break;
-            tc_fence_after();
-            qk(t, ks);
-          } else {
-            umma_commit(&ss.o_full[t]);
-          }
+          for (int kk = 4 * x; kk < 4 * x + 4; ++kk)
+            umma_ts(o_col, s_col + 8 * kk, desc_rows(kvb + slot * kBytes, kk), kIdPV, j > 0 || kk > 0);
         }
         if (!ok) break;
-        umma_commit(&ss.empty[vs]);
-        if (more) {
-          umma_commit(&ss.empty[ks]);
-          next();
-        }
+        umma_commit(&ss.empty[slot]);
+        next();
+        if (j + 1 < steps) ok = qk();
+        else umma_commit(&ss.o_full[t]);
       }
       // teardown: this thread's products complete before the tensor memory is released
-      umma_commit(&ss.drain);
+      umma_commit(&ss.drain[t]);
       const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(&ss.drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+      while (!mbar_try_wait(&ss.drain[t], 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
       }
     }
     __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ------------------------------------------------------------------ softmax
     const int t = warp >> 2;
     const int row = (tile0 + t) * kTile + 32 * (warp & 3) + lane;
@@ -286,48 +295,68 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int lo_max = tab[t].z, hi_min = tab[t].w;
       float m = -INFINITY;
-      float l0 = 0.f, l1 = 0.f;
+      uint64_t l2 = f2_pack(0.f, 0.f);  // sum of the rounded weights, two partial sums
+      uint64_t t2 = l2;                 // of the fp32 ones
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
-        ok = mbar_wait(&ss.s_full[t], static_cast<uint32_t>(j & 1), abort_flag, err, 321);
+        ok = bar_wait(&ss.s_full[t], static_cast<uint32_t>(j & 1), abort_flag, err, 321);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         uint32_t r[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(la + col_s(t) + 32 * c, r + 32 * c);
-        tmem_ld_wait();
+        tmem_read128(la + col_s(t), r);
         const int key0 = (n0 + j) * kTile;
+        const bool border = key0 < lo_max || key0 + kTile > hi_min;
+        const uint32_t seen = static_cast<uint32_t>(hi - lo), first = static_cast<uint32_t>(key0 - lo);
         if constexpr (kCap) {
+          float top = 0.f;
+          if (border) {  // what a masked place holds must not choose the form of tanh below
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if (first + e >= seen) r[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 128; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+          if (__all_sync(0xffffffffu, top * p.cap_in <= 2.f * 1.44269504f)) {  // |s| <= cap in all of the warp's rows
+            const float ci = p.cap_in * 0.34657359f;  // cap_in = 2 log2(e) sm_scale / cap
+            const uint64_t in2 = f2_pack(ci, ci), out2 = f2_pack(p.cap_log2, p.cap_log2);
+#pragma unroll
+            for (int e = 0; e < 128; e += 2) {
+              float a, c;
+              f2_unpack(f2_mul(tanh_poly2(f2_mul(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), in2)), out2), a, c);
+              r[e] = __float_as_uint(a);
+              r[e + 1] = __float_as_uint(c);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              r[e] = __float_as_uint(p.cap_log2 * tanh_of(__uint_as_float(r[e]) * p.cap_in));
+          }
+        }
+        if (border) {
 #pragma unroll
           for (int e = 0; e < 128; ++e)
-            r[e] = __float_as_uint(p.cap_log2 * tanh_of(__uint_as_float(r[e]) * p.cap_in));
+            if (first + e >= seen) r[e] = 0xff800000u;
         }
-        if (key0 < lo_max || key0 + kTile > hi_min) {
-          const uint32_t n = static_cast<uint32_t>(hi - lo);
-          const uint32_t d = static_cast<uint32_t>(key0 - lo);
+        float mv[4];
 #pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (d + e >= n) r[e] = 0xff800000u;
-        }
-        float mv[8];
+        for (int e = 0; e < 4; ++e) mv[e] = __uint_as_float(r[e]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mv[e] = __uint_as_float(r[e]);
+        for (int c = 4; c + 8 <= 128; c += 8)
 #pragma unroll
-        for (int c = 8; c < 128; c += 8)
+          for (int e = 0; e < 4; ++e) mv[e] = max3(mv[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mv[e] = fmaxf(mv[e], __uint_as_float(r[c + e]));
-        const float top = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])),
-                                fmaxf(fmaxf(mv[4], mv[5]), fmaxf(mv[6], mv[7])));
+        for (int e = 0; e < 4; ++e) mv[e] = max3(mv[e], __uint_as_float(r[124 + e]), __uint_as_float(r[124 + e]));
+        const float top = max3(max3(mv[0], mv[1], mv[2]), mv[3], mv[3]);
         const float scale = kCap ? 1.f : p.scale_log2;
         const float mx = top * scale;
         float f = 1.f;
-        const bool raise = mx > m + kRescale || (m == -INFINITY && mx > m);
+        const bool raise = !(mx <= m + kRescale);  // a NaN raises too, and stays
         if (raise) {
           f = ex2_approx(m - mx);  // 0 for the first maximum
           m = mx;
-          l0 *= f;
-          l1 *= f;
+          l2 = f2_mul(l2, f2_pack(f, f));
+          t2 = f2_mul(t2, f2_pack(f, f));
         }
         if (j > 0 && __any_sync(0xffffffffu, raise)) {
 #pragma unroll 1
@@ -340,40 +369,61 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st32(la + col_o(t) + 32 * c, o);
           }
         }
+        // The tiles take turns: side by side they would share the special-function unit, finish together, and leave it
+        // idle while both wait for their products.
+        if (tiles > 1 && (t == 1 || j > 0)) {
+          ok = bar_wait(&ss.turn[t ^ 1], static_cast<uint32_t>((t ? j : j - 1) & 1), abort_flag, err, 323);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
         const float nm = m == -INFINITY ? 0.f : -m;
         const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(nm, nm);
-        uint64_t l2 = f2_pack(l0, l1);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int i = 64 * c + 2 * e;
+          for (int e = 0; e < 16; ++e) {
+            const int i = 32 * c + 2 * e;
             float x0, x1;
             f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sc2, nm2), x0, x1);
-            x0 = ex2_approx(x0);
-            x1 = ex2_approx(x1);
-            l2 = f2_add(l2, f2_pack(x0, x1));
+            if (e % kPolyOf == kPolyOf - 1) {
+              ex2_poly2(x0, x1);
+            } else {
+              x0 = ex2_approx(x0);
+              x1 = ex2_approx(x1);
+            }
+            t2 = f2_add(t2, f2_pack(x0, x1));
             pk[e] = pack16<kBF16>(x0, x1);
+            unpack16<kBF16>(pk[e], x0, x1);
+            l2 = f2_add(l2, f2_pack(x0, x1));
           }
-          tmem_st32(la + col_s(t) + 32 * c, pk);
+          if (c == 3 && tiles > 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ss.turn[t]);
+          }
+          tmem_st16(la + col_s(t) + 16 * c, pk);
+          if (c & 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ss.p_full[t][c >> 1]);
+          }
         }
-        f2_unpack(l2, l0, l1);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ss.p_full[t]);
       }
       // ---- o / l and the row's log sum
       if (ok && steps > 0) {
-        ok = mbar_wait(&ss.o_full[t], 0, abort_flag, err, 322);
+        ok = bar_wait(&ss.o_full[t], 0, abort_flag, err, 322);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
       if (ok) {
-        const float l = l0 + l1;
+        float l, lt, half;
+        f2_unpack(l2, l, half);
+        l += half;
+        f2_unpack(t2, lt, half);
+        lt += half;
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
-        const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+        const float lse2 = lt == 0.f ? -INFINITY : m + log2f(lt);
         const long long flat = static_cast<long long>(bh) * p.Sq + row;
         float* part = p.splits > 1 ? p.part + (split * p.rows + flat) * (p.D + 1) : nullptr;
         const long long off = b * p.ob + h * p.oh + static_cast<long long>(row) * p.os;
@@ -508,6 +558,7 @@ int launch_dense(const DenseArgs& a, int sms, cudaStream_t stream) {
   p.per_cta = bh * ((p.q_tiles + 1) / 2) * a.splits >= sms ? 2 : 1;
   p.groups = (p.q_tiles + p.per_cta - 1) / p.per_cta;
   p.splits = a.splits;
+  p.heads = static_cast<int>(bh);
   p.scale_log2 = a.sm_scale * 1.4426950408889634f;
   if (a.softcap > 0.f) {
     p.cap_in = 2.f * p.scale_log2 / a.softcap;

@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const bool ok = walk([&](int g, int i, const int4& t) {
         const int h = hk * p.G + g;
         bool w = true;
-        if (n >= S::kQ) w = mbar_wait(&ss.q_empty[rq.slot], rq.phase ^ 1u, abort_flag, err, 401);
+        if (n >= S::kQ) w = bar_wait(&ss.q_empty[rq.slot], rq.phase ^ 1u, abort_flag, err, 401);
         if (!__all_sync(0xffffffffu, w)) return false;
         const bool fix = t.w <= 0;  // rows without keys, whose q and do may hold anything
         uint8_t* q = sQ + rq.slot * kBytes;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (fix) {
           __syncwarp();
-          w = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 402);
+          w = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 402);
           if (!__all_sync(0xffffffffu, w)) return false;
           ++fixes;
           for (int r = 0; r < kTile; ++r)
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&ss.q_full[rq.slot]);
         }
-        if (n >= S::kG) w = mbar_wait(&ss.g_empty[rg.slot], rg.phase ^ 1u, abort_flag, err, 403);
+        if (n >= S::kG) w = bar_wait(&ss.g_empty[rg.slot], rg.phase ^ 1u, abort_flag, err, 403);
         if (!__all_sync(0xffffffffu, w)) return false;
         uint8_t* go = sG + rg.slot * kBytes;
         if (lane == 0) {
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (fix) {
           __syncwarp();
-          w = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 404);
+          w = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 404);
           if (!__all_sync(0xffffffffu, w)) return false;
           ++fixes;
           for (int r = 0; r < kTile; ++r)
@@ -341,28 +341,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int q_prev = 0;
       // dK of the step before: its dS, then the step's own dP
       auto finish = [&](int m) {
-        if (!mbar_wait(&ss.ds_full, static_cast<uint32_t>(m & 1), abort_flag, err, 411)) return false;
+        if (!bar_wait(&ss.ds_full, static_cast<uint32_t>(m & 1), abort_flag, err, 411)) return false;
         tc_fence_after();
         mma_rows(tmem + kColD, tmem + kColB, qb + q_prev * kBytes, kIdR, m > 0);
         umma_commit(&ss.q_empty[q_prev]);
         return true;
       };
-      bool ok = mbar_wait(&ss.kv_full, 0, abort_flag, err, 412);
+      bool ok = bar_wait(&ss.kv_full, 0, abort_flag, err, 412);
       int g_prev = 0;
       if (ok)
         ok = walk([&](int, int, const int4&) {
           if (n > 0) {  // dV(n - 1)
-            if (!mbar_wait(&ss.p_full, static_cast<uint32_t>((n - 1) & 1), abort_flag, err, 413)) return false;
+            if (!bar_wait(&ss.p_full, static_cast<uint32_t>((n - 1) & 1), abort_flag, err, 413)) return false;
             tc_fence_after();
             mma_rows(tmem + kColC, tmem + kColA, gb + g_prev * kBytes, kIdR, n > 1);
             umma_commit(&ss.g_empty[g_prev]);
           }
-          if (!mbar_wait(&ss.q_full[rq.slot], rq.phase, abort_flag, err, 414)) return false;
+          if (!bar_wait(&ss.q_full[rq.slot], rq.phase, abort_flag, err, 414)) return false;
           tc_fence_after();
           mma_scores<DP>(tmem + kColA, kb, qb + rq.slot * kBytes, kIdS);
           umma_commit(&ss.s_full);
           if (n > 0 && !finish(n - 1)) return false;
-          if (!mbar_wait(&ss.g_full[rg.slot], rg.phase, abort_flag, err, 415)) return false;
+          if (!bar_wait(&ss.g_full[rg.slot], rg.phase, abort_flag, err, 415)) return false;
           tc_fence_after();
           mma_scores<DP>(tmem + kColB, vb, gb + rg.slot * kBytes, kIdS);
           umma_commit(&ss.dp_full);
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           ++n;
           return true;
         });
-      if (ok) ok = mbar_wait(&ss.p_full, static_cast<uint32_t>((n - 1) & 1), abort_flag, err, 416);
+      if (ok) ok = bar_wait(&ss.p_full, static_cast<uint32_t>((n - 1) & 1), abort_flag, err, 416);
       if (ok) {
         tc_fence_after();
         mma_rows(tmem + kColC, tmem + kColA, gb + g_prev * kBytes, kIdR, n > 1);
@@ -396,8 +396,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       Ring<S::kQ> rq;
       int n = 0;
       ok = walk([&](int, int, const int4& t) {
-        bool w = mbar_wait(&ss.q_full[rq.slot], rq.phase, abort_flag, err, 421);  // the tile's statistics
-        w = w && mbar_wait(&ss.s_full, static_cast<uint32_t>(n & 1), abort_flag, err, 422);
+        bool w = bar_wait(&ss.q_full[rq.slot], rq.phase, abort_flag, err, 421);  // the tile's statistics
+        w = w && bar_wait(&ss.s_full, static_cast<uint32_t>(n & 1), abort_flag, err, 422);
         if (!__all_sync(0xffffffffu, w)) return false;
         tc_fence_after();
         uint32_t r[64];
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ss.p_full);
-        w = mbar_wait(&ss.dp_full, static_cast<uint32_t>(n & 1), abort_flag, err, 423);
+        w = bar_wait(&ss.dp_full, static_cast<uint32_t>(n & 1), abort_flag, err, 423);
         if (!__all_sync(0xffffffffu, w)) return false;
         tc_fence_after();
         tmem_ld32(la + kColB + 64 * half, r);
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         return true;
       });
       if (ok) {
-        ok = mbar_wait(&ss.done, 0, abort_flag, err, 424);
+        ok = bar_wait(&ss.done, 0, abort_flag, err, 424);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int n = 0, fixes = 0;
       bool ok = true;
       for (; n < steps; ++n) {
-        if (n >= S::kK) ok = mbar_wait(&ss.k_empty[rk.slot], rk.phase ^ 1u, abort_flag, err, 451);
+        if (n >= S::kK) ok = bar_wait(&ss.k_empty[rk.slot], rk.phase ^ 1u, abort_flag, err, 451);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const int row = (n0 + n) * kTile;
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (fix) {
           __syncwarp();
-          ok = mbar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 452);
+          ok = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 452);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           ++fixes;
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&ss.k_full[rk.slot]);
         }
-        if (n >= S::kV) ok = mbar_wait(&ss.v_empty[rv.slot], rv.phase ^ 1u, abort_flag, err, 453);
+        if (n >= S::kV) ok = bar_wait(&ss.v_empty[rv.slot], rv.phase ^ 1u, abort_flag, err, 453);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) {
@@ -614,11 +614,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       Ring<S::kK> rk;
       Ring<S::kV> rv;
       auto scores = [&](int n) {  // S(n) and dP(n)
-        if (!mbar_wait(&ss.k_full[rk.slot], rk.phase, abort_flag, err, 461)) return false;
+        if (!bar_wait(&ss.k_full[rk.slot], rk.phase, abort_flag, err, 461)) return false;
         tc_fence_after();
         mma_scores<DP>(tmem + kColA, qb, kb + rk.slot * kBytes, kIdS);
         umma_commit(&ss.s_full);
-        if (!mbar_wait(&ss.v_full[rv.slot], rv.phase, abort_flag, err, 462)) return false;
+        if (!bar_wait(&ss.v_full[rv.slot], rv.phase, abort_flag, err, 462)) return false;
         tc_fence_after();
         mma_scores<DP>(tmem + ((n & 1) ? kColC : kColB), gb, vb + rv.slot * kBytes, kIdS);
         umma_commit(&ss.dp_full[n & 1]);
@@ -627,17 +627,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         rv.next();
         return true;
       };
-      bool ok = mbar_wait(&ss.qg_full, 0, abort_flag, err, 463) && scores(0);
+      bool ok = bar_wait(&ss.qg_full, 0, abort_flag, err, 463) && scores(0);
       int k_used = 0;
       for (int n = 0; n < steps && ok; ++n) {
         if (n + 1 < steps) {
-          ok = mbar_wait(&ss.s_read, static_cast<uint32_t>(n & 1), abort_flag, err, 464);
+          ok = bar_wait(&ss.s_read, static_cast<uint32_t>(n & 1), abort_flag, err, 464);
           if (!ok) break;
           tc_fence_after();
           ok = scores(n + 1);
           if (!ok) break;
         }
-        ok = mbar_wait(&ss.ds_full, static_cast<uint32_t>(n & 1), abort_flag, err, 465);
+        ok = bar_wait(&ss.ds_full, static_cast<uint32_t>(n & 1), abort_flag, err, 465);
         if (!ok) break;
         tc_fence_after();
         mma_rows(tmem + kColD, tmem + ((n & 1) ? kColC : kColB), kb + k_used * kBytes, kIdR, n > 0);
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         hi = r.y;
       }
       for (int n = 0; n < steps; ++n) {
-        ok = mbar_wait(&ss.s_full, static_cast<uint32_t>(n & 1), abort_flag, err, 471);
+        ok = bar_wait(&ss.s_full, static_cast<uint32_t>(n & 1), abort_flag, err, 471);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint32_t len = static_cast<uint32_t>(hi - lo);
         const uint32_t d = static_cast<uint32_t>(key0 + 64 * half - lo);
         const uint32_t col = (n & 1) ? kColC : kColB;
-        ok = mbar_wait(&ss.dp_full[n & 1], static_cast<uint32_t>((n >> 1) & 1), abort_flag, err, 472);
+        ok = bar_wait(&ss.dp_full[n & 1], static_cast<uint32_t>((n >> 1) & 1), abort_flag, err, 472);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (lane == 0) mbar_arrive(&ss.ds_full);
       }
       if (ok) {
-        ok = mbar_wait(&ss.done, 0, abort_flag, err, 473);
+        ok = bar_wait(&ss.done, 0, abort_flag, err, 473);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }

@@ -4,8 +4,9 @@ launch on the tensors' device and its current stream; the public functions are i
 
 from __future__ import annotations
 
-import contextlib
-from typing import Optional, Sequence, Tuple
+import functools
+import struct
+from typing import Optional, Tuple
 
 import torch
 
@@ -14,30 +15,67 @@ from . import _native
 CACHE_BLOCK = 64  # tokens of a head that share a scale
 
 
-def _on(t: torch.Tensor):
-    """The tensor's device as the current one for a launch."""
-    if torch.cuda.current_device() == t.device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+_pack3 = struct.Struct("3q").pack  # the strides of one tensor, as the C ABI reads them
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _call(name: str, device: int, *args) -> None:
+    """One C entry on ``device`` and its current stream (the entry's last argument)."""
+    fn = getattr(_native.lib(), name)
+    if _current_device() == device:
+        rc = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc:
+        _native._check(rc, name)
 
 
 def _same_place(*tensors: Optional[torch.Tensor]) -> None:
-    given = [t for t in tensors if t is not None]
-    _native._require_cuda(*given)
-    if any(t.device != given[0].device for t in given):
-        raise ValueError("all tensors must be on one device")
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("expected torch tensors")
+        d = t.get_device()
+        if d < 0:
+            raise ValueError("BSA engine inputs must be CUDA tensors (there is no CPU path)")
+        if device is None:
+            device = d
+        elif d != device:
+            raise ValueError("all tensors must be on one device")
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    """A view the kernels read in place, else a contiguous copy.  In place: d contiguous, base and strides in
-    multiples of 16 bytes; any order and gaps of batch, heads and tokens otherwise."""
-    if t.stride(-1) != 1 or _native._misaligned(t) or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+def _view(t: torch.Tensor) -> Tuple[torch.Tensor, int, bytes]:
+    """(tensor to keep alive, address, strides) of a [B, H, S, D] tensor that the kernels can read in place, else of a
+    contiguous copy.  In place: d contiguous, base and strides in multiples of 16 bytes, nothing broadcast; any
+    order and gaps of batch, heads and tokens otherwise."""
+    sb, sh, ss, sd = t.stride()
+    p = t.data_ptr()
+    if sd != 1 or p & 15 or (sb | sh | ss) & (16 // t.element_size() - 1) or not (sb and sh and ss):
+        # an axis of one element may have any stride, which the kernels do not use
+        sizes = t.shape
+        sb, sh, ss = (st if n > 1 else 8 * sizes[3] for st, n in zip((sb, sh, ss), sizes))
+        if sd != 1 or p & 15 or (sb | sh | ss) & (16 // t.element_size() - 1) or not (sb and sh and ss):
+            t = t.clone(memory_format=torch.contiguous_format)
+            sb, sh, ss, _ = t.stride()
+            p = t.data_ptr()
+    return t, p, _pack3(sb, sh, ss)
+
+
+def _out_view(t: torch.Tensor) -> Optional[Tuple[int, bytes]]:
+    """(address, strides) of an output that the kernels can write in place, else None."""
+    sb, sh, ss, sd = t.stride()
+    p = t.data_ptr()
+    if sd != 1 or p & 15 or (sb | sh | ss) & (16 // t.element_size() - 1):
+        return None
+    return p, _pack3(sb, sh, ss)
 
 
 def _i32(t: Optional[torch.Tensor], name: str, shape: Optional[Tuple[int, ...]] = None) -> Optional[torch.Tensor]:
@@ -51,125 +89,131 @@ def _i32(t: Optional[torch.Tensor], name: str, shape: Optional[Tuple[int, ...]] 
 
 
 # ------------------------------------------------------------------------------- q/k norm + rotary positions
+@functools.lru_cache(maxsize=1024)
+def _scratch(name: str, device: int, *sizes: int) -> int:
+    """Scratch bytes of a call of these sizes (a function of them and of the device's SM count)."""
+    with torch.cuda.device(device):
+        return int(getattr(_native.lib(), name)(*sizes))
+
+
 def _rope_args(rope, start: int):
     if rope is None:
         return (None, 0, 0, 0, 0, 0, 0, 0)
-    tables, dims, grid = rope.native_args() if hasattr(rope, "native_args") else rope
-    if tables.dtype != torch.float32 or not tables.is_contiguous():
+    tables, (dt, dh, dw), (T, H, W) = rope
+    if tables.dtype is not torch.float32 or not tables.is_contiguous():
         raise ValueError("rope tables must be contiguous fp32")
-    if tables.numel() != sum(int(n) * int(d) for n, d in zip(grid, dims)):
-        raise ValueError(f"rope tables of {tables.numel()} values do not match grid {tuple(grid)} and dims {tuple(dims)}")
-    return (tables.data_ptr(), *(int(d) for d in dims), *(int(g) for g in grid), int(start))
+    if tables.numel() != T * dt + H * dh + W * dw:
+        raise ValueError(f"rope tables of {tables.numel()} values do not match grid {(T, H, W)} and dims {(dt, dh, dw)}")
+    return (tables.data_ptr(), dt, dh, dw, T, H, W, start)
 
 
-def _norm_rope_check(xs: Sequence[torch.Tensor], ws, rope):
-    tables = (rope.native_args() if hasattr(rope, "native_args") else rope)[0] if rope is not None else None
-    _same_place(*xs, *ws, tables)
+def _norm_rope_check(xs, ws, rope):
+    _same_place(*xs, *ws, rope[0] if rope is not None else None)
     x = xs[0]
-    for t in xs:
-        if t.dim() != 4:
-            raise ValueError("expected tensors of shape [B, H, S, D]")
-        if t.dtype != x.dtype or t.shape[0] != x.shape[0] or t.shape[2:] != x.shape[2:]:
+    shape, dt = x.shape, x.dtype
+    if dt not in _native.DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {dt}")
+    if len(shape) != 4:
+        raise ValueError("expected tensors of shape [B, H, S, D]")
+    for t in xs[1:]:
+        st = t.shape
+        if t.dtype is not dt or len(st) != 4 or st[0] != shape[0] or st[2] != shape[2] or st[3] != shape[3]:
             raise ValueError("q and k must share dtype, batch, length and head_dim")
-    _native._dtype_code(x)
     for w in ws:
-        if w is not None and tuple(w.shape) != (x.shape[-1],):
-            raise ValueError(f"norm weight must be [{x.shape[-1]}]")
+        if w is not None and (w.dim() != 1 or w.shape[0] != shape[3]):
+            raise ValueError(f"norm weight must be [{shape[3]}]")
 
 
 def _weights(ws, x: torch.Tensor):
     """Contiguous weights of one type: fp32 or the input's are read as they are, others as fp32."""
-    kinds = {w.dtype for w in ws if w is not None}
-    if len(kinds) == 1 and kinds <= {torch.float32, x.dtype}:
-        kind = kinds.pop()
-        return [w.contiguous() if w is not None else None for w in ws], _native.DTYPE_CODES[kind]
-    return [w.float().contiguous() if w is not None else None for w in ws], 0
+    kind = None
+    for w in ws:
+        if w is not None:
+            if not w.is_contiguous() or (w.dtype is not torch.float32 and w.dtype is not x.dtype) or \
+                    (kind is not None and w.dtype is not kind):
+                return [u.float().contiguous() if u is not None else None for u in ws], 0
+            kind = w.dtype
+    return ws, _native.DTYPE_CODES[kind] if kind is not None else 0
 
 
 def norm_rope(xs, ws, eps: float, rope, start: int):
     _norm_rope_check(xs, ws, rope)
-    ra = _rope_args(rope, start)
     x = xs[0]
     B, _, S, D = x.shape
-    ys = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in xs]
-    if any(t.numel() == 0 for t in xs):
-        return ys
-    xs = [_readable(t) for t in xs]
+    ys = [t.new_empty(t.shape) for t in xs]
+    for t in xs:
+        if t.numel() == 0:
+            return ys
+    views = [_view(t) for t in xs]
     ws, wcode = _weights(ws, x)
     sides = []
-    for t, w, y in zip(xs, ws, ys):
-        sides += [t.data_ptr(), _native._strides(t), t.shape[1], _ptr(w), y.data_ptr()]
+    for (t, p, st), w, y in zip(views, ws, ys):
+        sides += (p, st, t.shape[1], _ptr(w), y.data_ptr())
     if len(xs) == 1:
-        sides += [None, None, 0, None, None]
-    with _on(x):
-        rc = _native.lib().bsa_norm_rope(*sides, _native._dtype_code(x), wcode, B, S, D, float(eps), *ra,
-                                         _native._stream(x))
-    _native._check(rc, "bsa_norm_rope")
+        sides += (None, None, 0, None, None)
+    _call("bsa_norm_rope", x.get_device(), *sides, _native.DTYPE_CODES[x.dtype], wcode, B, S, D, eps,
+          *_rope_args(rope, start))
     return ys
 
 
 def norm_rope_backward(xs, gs, ws, eps: float, rope, start: int, want_dw):
     x = xs[0]
     B, _, S, D = x.shape
-    dxs = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in xs]
-    dws = [torch.zeros((D,), device=x.device, dtype=torch.float32) if want else None for want in want_dw]
+    dxs = [t.new_empty(t.shape) for t in xs]
     if any(t.numel() == 0 for t in xs):
-        return dxs, dws
-    xs, gs = [_readable(t) for t in xs], [_readable(g) for g in gs]
+        return dxs, [torch.zeros((D,), device=x.device) if want else None for want in want_dw]
+    dws = [x.new_empty((D,), dtype=torch.float32) if want else None for want in want_dw]
+    xv, gv = [_view(t) for t in xs], [_view(g) for g in gs]
     ws, wcode = _weights(ws, x)
     sides = []
-    for t, g, w, dx, dw in zip(xs, gs, ws, dxs, dws):
-        sides += [t.data_ptr(), _native._strides(t), g.data_ptr(), _native._strides(g), t.shape[1], _ptr(w),
-                  dx.data_ptr(), _ptr(dw)]
+    for (t, p, st), (_, gp, gst), w, dx, dw in zip(xv, gv, ws, dxs, dws):
+        sides += (p, st, gp, gst, t.shape[1], _ptr(w), dx.data_ptr(), _ptr(dw))
     if len(xs) == 1:
-        sides += [None, None, None, None, 0, None, None, None]
-    with _on(x):
-        scratch = None
-        if any(want_dw):
-            n = int(_native.lib().bsa_norm_rope_backward_scratch_bytes(D))
-            scratch = torch.empty((n,), device=x.device, dtype=torch.uint8)
-        rc = _native.lib().bsa_norm_rope_backward(*sides, _native._dtype_code(x), wcode, B, S, D, float(eps),
-                                                  *_rope_args(rope, start), _ptr(scratch), _native._stream(x))
-    _native._check(rc, "bsa_norm_rope_backward")
+        sides += (None, None, None, None, 0, None, None, None)
+    scratch = None
+    if any(want_dw):
+        scratch = x.new_empty((_scratch("bsa_norm_rope_backward_scratch_bytes", x.get_device(), D),), dtype=torch.uint8)
+    _call("bsa_norm_rope_backward", x.get_device(), *sides, _native.DTYPE_CODES[x.dtype], wcode, B, S, D, eps,
+          *_rope_args(rope, start), _ptr(scratch))
     return dxs, dws
 
 
 # ------------------------------------------------------------------------------------------- key intervals
 def attention_ranges(batch: int, Sq: int, Sk: int, *, device, given=None, causal=False, prefix=0, prefixes=None,
                      q_offsets=None, k_offsets=None, q_lengths=None, k_lengths=None, k_add: int = 0):
-    ranges = torch.empty((batch, Sq, 2), device=device, dtype=torch.int32)
-    table = torch.empty((batch, (Sq + 127) // 128, 4), device=device, dtype=torch.int32)
-    _same_place(ranges, given, prefixes, q_offsets, k_offsets, q_lengths, k_lengths)
-    if Sq == 0 or batch == 0:
-        return ranges, table
-    with _on(ranges):
-        rc = _native.lib().bsa_attention_ranges(
-            ranges.data_ptr(), table.data_ptr(), batch, Sq, Sk, _ptr(given), int(bool(causal)), int(prefix),
-            _ptr(prefixes), _ptr(q_offsets), _ptr(k_offsets), q_offsets.numel() - 1 if q_offsets is not None else 0,
-            _ptr(q_lengths), _ptr(k_lengths), int(k_add), _native._stream(ranges))
-    _native._check(rc, "bsa_attention_ranges")
-    return ranges, table
+    """The intervals and their tile table in one allocation: (buffer, address of ranges, address of table)."""
+    n = batch * Sq * 2
+    at = (n + 3) & ~3  # the table starts on 16 bytes
+    buf = torch.empty((at + batch * ((Sq + 127) // 128) * 4,), device=device, dtype=torch.int32)
+    _same_place(buf, given, prefixes, q_offsets, k_offsets, q_lengths, k_lengths)
+    ranges = buf.data_ptr()
+    table = ranges + 4 * at
+    if n:
+        _call("bsa_attention_ranges", buf.get_device(), ranges, table, batch, Sq, Sk, _ptr(given), 1 if causal else 0,
+              prefix, _ptr(prefixes), _ptr(q_offsets), _ptr(k_offsets),
+              q_offsets.numel() - 1 if q_offsets is not None else 0, _ptr(q_lengths), _ptr(k_lengths), k_add)
+    return buf, ranges, table
 
 
 # ------------------------------------------------------------------------------------------ dense attention
-def check_qkv(q, k, v, names=("q", "k", "v")) -> None:
+def check_qkv(q, k, v) -> None:
     _same_place(q, k, v)
-    for t, n in zip((q, k, v), names):
-        if t.dim() != 4:
-            raise ValueError(f"{n} must be [B, H, S, D]")
-    if k.shape != v.shape:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4:
+        raise ValueError("q, k and v must be [B, H, S, D]")
+    if ks != v.shape:
         raise ValueError("k and v must have the same shape")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
+    dt = q.dtype
+    if dt != k.dtype or dt != v.dtype:
         raise ValueError("q, k, v must share one dtype")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"unsupported dtype {q.dtype} (bf16 or fp16)")
-    if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise ValueError(f"unsupported dtype {dt} (bf16 or fp16)")
+    if qs[0] != ks[0] or qs[3] != ks[3]:
         raise ValueError("q and k must share batch and head_dim")
-    D = q.shape[3]
-    if D % 8 or not 0 < D <= 128:
-        raise ValueError(f"head_dim D={D} must be a multiple of 8 and <= 128")
-    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{q.shape[1]} query heads are no multiple of {k.shape[1]} key heads")
+    if qs[3] % 8 or not 0 < qs[3] <= 128:
+        raise ValueError(f"head_dim D={qs[3]} must be a multiple of 8 and <= 128")
+    if ks[1] == 0 or qs[1] % ks[1]:
+        raise ValueError(f"{qs[1]} query heads are no multiple of {ks[1]} key heads")
 
 
 def check_scale(sm_scale: float, softcap: float = 0.0) -> None:
@@ -179,27 +223,26 @@ def check_scale(sm_scale: float, softcap: float = 0.0) -> None:
         raise ValueError("softcap must be finite and >= 0")
 
 
-def masked_attention(q, k, v, ranges, table, sm_scale: float, softcap: float, out=None, want_lse: bool = False,
-                     rest: Optional[torch.Tensor] = None):
-    """(out, lse or None).  ranges / table: of attention_ranges, or None for every key.  ``rest`` (contiguous, like
-    out) receives what out's rounding left over."""
+def masked_attention(q, k, v, ranges, table, batch: int, sm_scale: float, softcap: float, out=None,
+                     want_lse: bool = False, rest: Optional[torch.Tensor] = None):
+    """(out, lse or None).  ranges / table: addresses of attention_ranges with ``batch`` entries, or None for every key.
+    ``rest`` (contiguous, like out) receives what out's rounding left over."""
     B, H, Sq, D = q.shape
     Hk, Sk = k.shape[1], k.shape[2]
-    lse = torch.empty((B, H, Sq), device=q.device, dtype=torch.float32) if want_lse else None
-    target = out
-    if out is None or _native._misaligned(out) or out.stride(-1) != 1:
-        target = torch.empty((B, H, Sq, D), device=q.device, dtype=q.dtype)
+    lse = q.new_empty((B, H, Sq), dtype=torch.float32) if want_lse else None
+    target, tv = out, None
+    if out is not None:
+        tv = _out_view(out)
+    if tv is None:
+        target = q.new_empty((B, H, Sq, D))
+        tv = target.data_ptr(), _pack3(H * Sq * D, Sq * D, D)
     if B and H and Sq and Sk:
-        q, k, v = _readable(q), _readable(k), _readable(v)
-        with _on(q):
-            n = int(_native.lib().bsa_masked_attention_scratch_bytes(B, H, Sq, Sk, D))
-            scratch = torch.empty((n,), device=q.device, dtype=torch.uint8) if n else None
-            rc = _native.lib().bsa_masked_attention(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), _native._dtype_code(q), B, H, Hk, Sq, Sk, D,
-                _native._strides(q), _native._strides(k), _native._strides(v), _ptr(ranges), _ptr(table),
-                ranges.shape[0] if ranges is not None else 1, float(sm_scale), float(softcap), target.data_ptr(),
-                _native._strides(target), _ptr(rest), _ptr(lse), _ptr(scratch), _native._stream(q))
-        _native._check(rc, "bsa_masked_attention")
+        (q, qp, qst), (k, kp, kst), (v, vp, vst) = _view(q), _view(k), _view(v)
+        device = q.get_device()
+        n = _scratch("bsa_masked_attention_scratch_bytes", device, B, H, Sq, Sk, D)
+        scratch = q.new_empty((n,), dtype=torch.uint8) if n else None
+        _call("bsa_masked_attention", device, qp, kp, vp, _native.DTYPE_CODES[q.dtype], B, H, Hk, Sq, Sk, D, qst, kst,
+              vst, ranges, table, batch, sm_scale, softcap, tv[0], tv[1], _ptr(rest), _ptr(lse), _ptr(scratch))
     else:  # no rows, or no keys: zeros
         target.zero_()
         if lse is not None:
@@ -210,80 +253,67 @@ def masked_attention(q, k, v, ranges, table, sm_scale: float, softcap: float, ou
     return target, lse
 
 
-def masked_attention_backward(q, k, v, out, rest, lse, grad, ranges, table, sm_scale: float, softcap: float, want_q: bool,
-                              want_kv: bool):
+def masked_attention_backward(q, k, v, out, rest, lse, grad, ranges, table, batch: int, sm_scale: float,
+                              softcap: float, want_q: bool, want_kv: bool):
     """(dq, dk, dv), contiguous; None where not wanted."""
     B, H, Sq, D = q.shape
     Hk, Sk = k.shape[1], k.shape[2]
     empty = not (B and H and Sq and Sk)
-    new = torch.zeros if empty else torch.empty
-    dq = new((B, H, Sq, D), device=q.device, dtype=q.dtype) if want_q else None
-    dk, dv = (new((B, Hk, Sk, D), device=q.device, dtype=q.dtype) if want_kv else None for _ in range(2))
+    new = q.new_zeros if empty else q.new_empty
+    dq = new((B, H, Sq, D)) if want_q else None
+    dk, dv = (new((B, Hk, Sk, D)) if want_kv else None for _ in range(2))
     if empty:
         return dq, dk, dv
-    q, k, v, out, grad = (_readable(t) for t in (q, k, v, out, grad))
-    bm = ranges.shape[0] if ranges is not None else 0
-    with _on(q):
-        n = int(_native.lib().bsa_masked_attention_backward_scratch_bytes(B, H, Sq, bm))
-        scratch = torch.empty((n,), device=q.device, dtype=torch.uint8)
-        rc = _native.lib().bsa_masked_attention_backward(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), grad.data_ptr(), lse.data_ptr(),
-            _native._dtype_code(q), B, H, Hk, Sq, Sk, D, *(_native._strides(t) for t in (q, k, v, out, grad)),
-            _ptr(ranges), _ptr(table), max(bm, 1), float(sm_scale), float(softcap), _ptr(dq), _ptr(dk), _ptr(dv),
-            scratch.data_ptr(), _native._stream(q))
-    _native._check(rc, "bsa_masked_attention_backward")
+    (q, qp, qst), (k, kp, kst), (v, vp, vst) = _view(q), _view(k), _view(v)
+    (out, op, ost), (grad, gp, gst) = _view(out), _view(grad)
+    device = q.get_device()
+    n = _scratch("bsa_masked_attention_backward_scratch_bytes", device, B, H, Sq, batch if ranges else 0)
+    scratch = q.new_empty((n,), dtype=torch.uint8)
+    _call("bsa_masked_attention_backward", device, qp, kp, vp, op, rest.data_ptr(), gp, lse.data_ptr(),
+          _native.DTYPE_CODES[q.dtype], B, H, Hk, Sq, Sk, D, qst, kst, vst, ost, gst, ranges, table, batch, sm_scale,
+          softcap, _ptr(dq), _ptr(dk), _ptr(dv), scratch.data_ptr())
     return dq, dk, dv
 
 
 # ---------------------------------------------------------------------------------------------- 8-bit cache
 def _cache_args(c):
-    B, Hk, cap, D = c.k_codes.shape
     return (c.k_codes.data_ptr(), c.k_scale.data_ptr(), c.v_codes.data_ptr(), c.v_scale.data_ptr(),
-            c.lengths.data_ptr(), B, Hk, cap, D)
+            c.lengths.data_ptr(), *c.k_codes.shape)
 
 
 def cache_append(c, k, v, counts) -> None:
-    k, v = _readable(k), _readable(v)
-    with _on(k):
-        rc = _native.lib().bsa_kv8_append(*_cache_args(c), k.data_ptr(), v.data_ptr(), _native._dtype_code(k),
-                                          k.shape[2], _native._strides(k), _native._strides(v), _ptr(counts),
-                                          _native._stream(k))
-    _native._check(rc, "bsa_kv8_append")
+    (k, kp, kst), (v, vp, vst) = _view(k), _view(v)
+    _call("bsa_kv8_append", k.get_device(), *_cache_args(c), kp, vp, _native.DTYPE_CODES[k.dtype], k.shape[2], kst, vst,
+          _ptr(counts))
 
 
-def cache_unpack(c, dtype, k=None, v=None, rows: Optional[int] = None):
+def cache_unpack(c, dtype, k=None, v=None):
+    """(k, v) in 16 bits: the held tokens, the fresh ones k, v, zeros up to capacity + fresh."""
     B, Hk, cap, D = c.k_codes.shape
-    n = k.shape[2] if k is not None else 0
-    rows = cap + n if rows is None else rows
-    ko, vo = (torch.empty((B, Hk, rows, D), device=c.k_codes.device, dtype=dtype) for _ in range(2))
-    ks = vs = None
-    if n:
-        k, v = _readable(k), _readable(v)
-        ks, vs = _native._strides(k), _native._strides(v)
-    with _on(ko):
-        rc = _native.lib().bsa_kv8_unpack(*_cache_args(c), _ptr(k) if n else None, _ptr(v) if n else None,
-                                          _native.DTYPE_CODES[dtype], n, ks, vs, ko.data_ptr(), vo.data_ptr(), rows,
-                                          _native._stream(ko))
-    _native._check(rc, "bsa_kv8_unpack")
+    n, kp, vp, kst, vst = 0, None, None, None, None
+    if k is not None:
+        n = k.shape[2]
+        (k, kp, kst), (v, vp, vst) = _view(k), _view(v)
+    ko, vo = (c.k_codes.new_empty((B, Hk, cap + n, D), dtype=dtype) for _ in range(2))
+    _call("bsa_kv8_unpack", ko.get_device(), *_cache_args(c), kp, vp, _native.DTYPE_CODES[dtype], n, kst, vst,
+          ko.data_ptr(), vo.data_ptr(), cap + n)
     return ko, vo
 
 
 def cache_attention(c, q, causal: bool, sm_scale: float, out: torch.Tensor) -> torch.Tensor:
     B, H, Sq, D = q.shape
-    Hk, cap = c.k_codes.shape[1], c.k_codes.shape[2]
-    q = _readable(q)
-    target = out
-    if _native._misaligned(out) or out.stride(-1) != 1:
-        target = torch.empty((B, H, Sq, D), device=q.device, dtype=q.dtype)
-    with _on(q):
-        n = int(_native.lib().bsa_kv8_attention_scratch_bytes(B, H, Hk, Sq, cap, D))
-        scratch = torch.empty((n,), device=q.device, dtype=torch.uint8) if n else None
-        rc = _native.lib().bsa_kv8_attention(
-            q.data_ptr(), _native._dtype_code(q), B, H, Sq, _native._strides(q), c.k_codes.data_ptr(),
-            c.k_scale.data_ptr(), c.v_codes.data_ptr(), c.v_scale.data_ptr(), c.lengths.data_ptr(), Hk, cap, D,
-            int(bool(causal)), float(sm_scale), target.data_ptr(), _native._strides(target), _ptr(scratch),
-            _native._stream(q))
-    _native._check(rc, "bsa_kv8_attention")
+    _, Hk, cap, _ = c.k_codes.shape
+    q, qp, qst = _view(q)
+    target, tv = out, _out_view(out)
+    if tv is None:
+        target = q.new_empty((B, H, Sq, D))
+        tv = target.data_ptr(), _pack3(H * Sq * D, Sq * D, D)
+    device = q.get_device()
+    n = _scratch("bsa_kv8_attention_scratch_bytes", device, B, H, Hk, Sq, cap, D)
+    scratch = q.new_empty((n,), dtype=torch.uint8) if n else None
+    _call("bsa_kv8_attention", device, qp, _native.DTYPE_CODES[q.dtype], B, H, Sq, qst, c.k_codes.data_ptr(),
+          c.k_scale.data_ptr(), c.v_codes.data_ptr(), c.v_scale.data_ptr(), c.lengths.data_ptr(), Hk, cap, D,
+          1 if causal else 0, sm_scale, tv[0], tv[1], _ptr(scratch))
     if target is not out:
         out.copy_(target)
     return out

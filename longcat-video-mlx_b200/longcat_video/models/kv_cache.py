@@ -12,8 +12,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from .. import _dense, _native
-from .masked_attention import AttentionMask
+from .. import _dense
 
 __all__ = ["KVCache8"]
 
@@ -34,20 +33,21 @@ class KVCache8:
     def __init__(self, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
                  lengths: torch.Tensor):
         _dense._same_place(k_codes, k_scale, v_codes, v_scale, lengths)
-        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+        shape = k_codes.shape
+        if len(shape) != 4 or shape != v_codes.shape:
             raise ValueError("codes must be [B, Hk, capacity, D]")
-        B, Hk, cap, D = k_codes.shape
+        B, Hk, cap, D = shape
         if cap % BLOCK or cap == 0:
             raise ValueError(f"capacity {cap} must be a positive multiple of {BLOCK}")
         if D % 8 or not 0 < D <= 128:
             raise ValueError(f"head_dim D={D} must be a multiple of 8 and <= 128")
         for t in (k_codes, v_codes):
-            if t.dtype != torch.float8_e4m3fn or not t.is_contiguous() or t.data_ptr() % 16:
+            if t.dtype is not torch.float8_e4m3fn or not t.is_contiguous() or t.data_ptr() & 15:
                 raise ValueError("codes must be contiguous, 16-byte aligned float8_e4m3fn")
         for t in (k_scale, v_scale):
-            if t.dtype != torch.float32 or not t.is_contiguous() or tuple(t.shape) != (B, Hk, cap // BLOCK):
+            if t.dtype is not torch.float32 or not t.is_contiguous() or t.shape != (B, Hk, cap // BLOCK):
                 raise ValueError(f"scales must be contiguous fp32 [{B}, {Hk}, {cap // BLOCK}]")
-        if lengths.dtype != torch.int32 or not lengths.is_contiguous() or tuple(lengths.shape) != (B,):
+        if lengths.dtype is not torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous():
             raise ValueError(f"lengths must be contiguous int32 [{B}]")
         self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.lengths = k_codes, k_scale, v_codes, v_scale, lengths
 
@@ -148,12 +148,12 @@ class KVCache8:
             self._check_kv(k, v)
             if k.dtype != q.dtype:
                 raise ValueError("q, k, v must share one dtype")
-        if any(t is not None and t.requires_grad for t in (q, k, v)) and torch.is_grad_enabled():
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v)):
             raise ValueError("attention over a cache has no gradient")
         scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
         _dense.check_scale(scale)
         if out is None:
-            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+            out = q.new_empty(q.shape)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out must have q's shape and dtype")
         Sq = q.shape[2]
@@ -163,6 +163,6 @@ class KVCache8:
         if n == 0 and q.shape[1] // Hk * Sq <= FEW_ROWS:
             return _dense.cache_attention(self, q, causal, scale, out)
         kd, vd = _dense.cache_unpack(self, q.dtype, k if n else None, v if n else None)
-        ranges, table = _dense.attention_ranges(B, Sq, cap + n, device=q.device, causal=causal, k_lengths=self.lengths,
-                                                k_add=n)
-        return _dense.masked_attention(q, kd, vd, ranges, table, scale, 0.0, out=out)[0]
+        mask, ranges, table = _dense.attention_ranges(B, Sq, cap + n, device=q.device, causal=causal,
+                                                      k_lengths=self.lengths, k_add=n)
+        return _dense.masked_attention(q, kd, vd, ranges, table, B, scale, 0.0, out=out)[0]

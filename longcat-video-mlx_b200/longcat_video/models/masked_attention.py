@@ -19,16 +19,25 @@ __all__ = ["AttentionMask", "masked_attention"]
 
 
 class AttentionMask:
-    """Which keys each query row sees: ``ranges`` [batch or 1, Sq, 2] int32 and the kernels' tile table.
+    """Which keys each query row sees: ``ranges`` [batch or 1, Sq, 2] int32 and the kernels' tile ``table``.
 
     Build one with :meth:`build` or, from intervals of one's own, with :meth:`from_ranges`."""
 
-    def __init__(self, ranges: torch.Tensor, table: torch.Tensor, Sk: int):
-        self.ranges, self.table, self.Sk = ranges, table, int(Sk)
+    def __init__(self, buffer, ranges: int, table: int, batch: int, Sq: int, Sk: int):
+        # one device buffer, the addresses of its two parts, and their sizes (see _dense.attention_ranges)
+        self._buffer, self._ranges, self._table = buffer, ranges, table
+        self.batch, self.Sq, self.Sk = batch, Sq, Sk
 
     @property
-    def Sq(self) -> int:
-        return int(self.ranges.shape[1])
+    def ranges(self) -> torch.Tensor:
+        return self._buffer[:self.batch * self.Sq * 2].view(self.batch, self.Sq, 2)
+
+    @property
+    def table(self) -> torch.Tensor:
+        """[batch, tiles of 128 rows, 4]: lowest lo and highest hi of the rows that see a key, highest lo and lowest hi of
+        all rows."""
+        tiles = (self.Sq + 127) // 128
+        return self._buffer[self._buffer.numel() - self.batch * tiles * 4:].view(self.batch, tiles, 4)
 
     @classmethod
     def build(cls, Sq: int, Sk: int, *, causal: bool = False, prefix: Union[int, torch.Tensor, None] = None,
@@ -71,11 +80,11 @@ class AttentionMask:
         prefix = 0 if prefix is None else int(prefix)
         if prefix < 0:
             raise ValueError("prefix must be >= 0")
-        ranges, table = _dense.attention_ranges(
+        parts = _dense.attention_ranges(
             batch, Sq, Sk, device=device, causal=causal, prefix=prefix, prefixes=prefixes,
             q_offsets=_dense._i32(q_offsets, "q_offsets"), k_offsets=_dense._i32(k_offsets, "k_offsets"),
             q_lengths=_dense._i32(q_lengths, "q_lengths"), k_lengths=_dense._i32(k_lengths, "k_lengths"))
-        return cls(ranges, table, Sk)
+        return cls(*parts, batch, Sq, Sk)
 
     @classmethod
     def from_ranges(cls, ranges: torch.Tensor, Sk: int) -> "AttentionMask":
@@ -85,16 +94,17 @@ class AttentionMask:
         given = _dense._i32(ranges, "ranges")
         if given.data_ptr() % 8:
             given = given.clone()
-        r, table = _dense.attention_ranges(given.shape[0], given.shape[1], Sk, device=given.device, given=given)
-        return cls(r, table, Sk)
+        batch, Sq = int(given.shape[0]), int(given.shape[1])
+        return cls(*_dense.attention_ranges(batch, Sq, Sk, device=given.device, given=given), batch, Sq, int(Sk))
 
 
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, ranges, table, sm_scale, softcap):
+    def forward(ctx, q, k, v, mask, sm_scale, softcap):
         rest = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        out, lse = _dense.masked_attention(q, k, v, ranges, table, sm_scale, softcap, want_lse=True, rest=rest)
-        ctx.save_for_backward(q, k, v, out, rest, lse, ranges, table)
+        out, lse = _dense.masked_attention(q, k, v, *_mask_args(mask), sm_scale, softcap, want_lse=True, rest=rest)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
+        ctx.mask = mask
         ctx.rest = (sm_scale, softcap)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -103,13 +113,17 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
-        q, k, v, out, rest, lse, ranges, table = ctx.saved_tensors
         if grad is None:
-            return (None,) * 7
+            return (None,) * 6
+        q, k, v, out, rest, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = _dense.masked_attention_backward(q, k, v, out, rest, lse, grad.to(q.dtype), ranges, table, *ctx.rest,
-                                                      need[0], need[1] or need[2])
-        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+        dq, dk, dv = _dense.masked_attention_backward(q, k, v, out, rest, lse, grad.to(q.dtype), *_mask_args(ctx.mask),
+                                                      *ctx.rest, need[0], need[1] or need[2])
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
+
+
+def _mask_args(mask):
+    return (mask._ranges, mask._table, mask.batch) if mask is not None else (None, None, 1)
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[AttentionMask] = None, *,
@@ -126,14 +140,12 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
     softcap = float(softcap)
     _dense.check_scale(scale, softcap)
-    ranges = table = None
     if mask is not None:
         if mask.Sq != q.shape[2] or mask.Sk != k.shape[2]:
             raise ValueError(f"the mask is for {mask.Sq} queries and {mask.Sk} keys, got {q.shape[2]} and {k.shape[2]}")
-        if mask.ranges.shape[0] not in (1, q.shape[0]):
-            raise ValueError(f"the mask has {mask.ranges.shape[0]} batch entries, q has {q.shape[0]}")
-        _dense._same_place(q, mask.ranges)
-        ranges, table = mask.ranges, mask.table
+        if mask.batch != 1 and mask.batch != q.shape[0]:
+            raise ValueError(f"the mask has {mask.batch} batch entries, q has {q.shape[0]}")
+        _dense._same_place(q, mask._buffer)
     if out is not None:
         _dense._same_place(q, out)
         if out.shape != q.shape or out.dtype != q.dtype:
@@ -142,7 +154,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     if grad:
         if out is not None:
             raise ValueError("out= is for calls without gradients")
-        o, lse = _MaskedAttention.apply(q, k, v, ranges, table, scale, softcap)
+        o, lse = _MaskedAttention.apply(q, k, v, mask, scale, softcap)
         return (o, lse) if return_lse else o
-    o, lse = _dense.masked_attention(q, k, v, ranges, table, scale, softcap, out=out, want_lse=return_lse)
+    o, lse = _dense.masked_attention(q, k, v, *_mask_args(mask), scale, softcap, out=out, want_lse=return_lse)
     return (o, lse) if return_lse else o

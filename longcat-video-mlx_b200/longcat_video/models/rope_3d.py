@@ -149,6 +149,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Op
         raise ValueError("nothing to do: give norm weights, rope tables or both")
     if k is None and k_weight is not None:
         raise ValueError("k_weight without k")
+    if rope is not None:
+        tables, dims, grid = rope.native_args() if hasattr(rope, "native_args") else rope
+        rope = (tables, dims, grid)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _NormRope.apply(q, k, q_weight, k_weight, float(eps), rope, int(start))
     xs = [q] if k is None else [q, k]
