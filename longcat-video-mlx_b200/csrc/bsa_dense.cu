@@ -3,22 +3,22 @@
 //   z_ij = s_ij = sm_scale q_i . k_j, or cap tanh(s_ij / cap);   p_ij = 2^(z_ij log2(e) - m_i) for j in [lo_i, hi_i)
 //   o_i = sum_j p_ij v_j / l_i,  l_i = sum_j p_ij,  lse_i = ln sum_j e^z_ij        (0 and -inf for an empty row)
 //
-// One pass over the keys with a running maximum and sum, scores and output accumulators in tensor memory.
-// A CTA takes up to two query tiles of 128 rows of one head: while the softmax warps of one tile work on its
-// scores, the tensor cores run the other tile's products, and each key and value tile is loaded once for both.
-//     S_t[128 x 128] = Q_t K^T         A = Q_t, B = K, both in shared memory
-//     O_t[128 x D]  += P_t V           A = P_t in tensor memory, over the scores it came from; B = V
-// TMEM: S_0, S_1, O_0, O_1 of 128 columns each.
+// One pass over the keys with a running maximum and sum, scores and output accumulator in tensor memory.  A CTA takes one
+// query tile of 128 rows of one head:
+//     S(j)[128 x 128] = Q K_j^T        A = Q in tensor memory, B = K in shared memory
+//     O[128 x D]     += P(j) V_j       A = P in tensor memory, B = V in shared memory
+// TMEM: two S buffers and O of 128 columns each, Q and P of 64 (16-bit pairs).  With Q in shared memory too, the operands
+// of both products and the loads of K and V move 160 KB a step through it, 1,250 cycles, and a product of
+// 128 x 128 x 16 was seen to take 97 cycles instead of 64; with Q in tensor memory it is 128 KB.  S(j+3) is issued
+// when S(j+1) has been read, behind P(j) V, two steps before it is needed.
 //
 // Roles (384 threads, one CTA to an SM):
-//   warps 0-3, 4-7 : softmax of tile 0, 1; a thread owns one row, so neither maximum nor sum leaves it
-//   warps 8, 10    : issue the products of tile 0, 1: S(0), then P(j) V, S(j+1) for each j.  Products of one thread run in
-//                    order, so S(j+1) may overwrite the P(j) that was read before it, and its arrival also says that O
-//                    holds all of P V up to j.  A product adds to the same accumulator as the one before it and waits
-//                    for it, about 100 cycles where 64 would do (128 x 128 x 16); two issuing threads put the two tiles'
-//                    chains side by side, which one thread in a fixed order does not
-//   warp 9         : loads; one ring for K and V tiles in the order of their use (warp 11: idle, it makes the group
-//                    whole that gives its registers to the softmax warps)
+//   warps 0-7 : softmax, warps 0-3 on the keys 0-63 of a step, 4-7 on 64-127, a thread on half a row.  The two threads
+//               of a row need one maximum only when one of them finds it exceeded (below), which a barrier with a vote
+//               tells; their sums join at the end.  Of its 64 scores a thread reads the next step's first 32 before
+//               it computes the exponentials of this step's last 32, so their maximum is found beside those
+//   warp 8    : issues the products: P(j) V first, which the next step's P waits for, then S(j+3)
+//   warp 9    : loads; one ring for K and V tiles in the order of their use (warps 10, 11: idle)
 // The maximum is raised, and O and l rescaled, only when a score exceeds it by more than 2^8 (log2 8): P stays within
 // fp16's range and rounding is relative, so the result is as exact as with the true maximum.
 // P is rounded to the input type for the tensor cores, and o is divided by the sum of the rounded values: the weights
@@ -38,29 +38,28 @@ namespace dense {
 __device__ int g_dense_err;
 
 constexpr int kThreads = 384;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kIssue = kSoftmaxWarps, kLoad = kSoftmaxWarps + 1;  // warps
 constexpr float kRescale = 8.f;  // log2
-#ifndef BSA_POLY_OF
-#define BSA_POLY_OF 4
-#endif
-// One pair of exponentials in kPolyOf is computed on the FMA pipe: the special-function unit's 16 a cycle are as
-// many cycles as the tensor cores need for both products, so what else waits for it shows at once.
-constexpr int kPolyOf = BSA_POLY_OF;
 constexpr uint32_t kTmemCols = 512;
-__host__ __device__ constexpr uint32_t col_s(int t) { return 128u * static_cast<uint32_t>(t); }
-__host__ __device__ constexpr uint32_t col_o(int t) { return 256u + 128u * static_cast<uint32_t>(t); }
-
+__host__ __device__ constexpr uint32_t col_s(int b) { return 128u * static_cast<uint32_t>(b); }
+constexpr uint32_t kColO = 256, kColQ = 384, kColP = 448;
 template <int DP>
 struct Smem {
   static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr int kTiles = (2 + kStages) * tile_bytes<DP>();
+  static constexpr int kTiles = (1 + kStages) * tile_bytes<DP>();
   uint64_t q_full;
   uint64_t full[kStages], empty[kStages];
   uint64_t fix;
-  uint64_t s_full[2], p_full[2][2], o_full[2];
-  uint64_t turn[2];  // tile t's exponentials of a step are done: the other tile's turn
-  uint64_t drain[2];
+  uint64_t q_ready;              // Q copied into tensor memory
+  uint64_t s_full[2], s_read[2];  // S(j) in buffer j % 2
+  // of step j in [j % 2]; a waiter may be one step behind or ahead of the others, so one barrier each would not tell
+  uint64_t p_full[2];  // P(j) written, O rescaled where it had to be (one arrival for each softmax warp)
+  uint64_t o_full[2];  // P(j) V done
+  uint64_t drain;
   uint32_t tmem;
   int abort_flag;
+  float join[2][2][kTile];  // [half][maximum or sum, fp32 sum][row]
 };
 template <int DP>
 constexpr int smem_bytes() { return Smem<DP>::kTiles + static_cast<int>(sizeof(Smem<DP>)) + 1024; }
@@ -70,9 +69,8 @@ struct Params {
   const int4* table;   // [Bm][q_tiles]
   int Bm, H, G, Sq, Sk, D;
   int q_tiles;         // tiles of 128 rows
-  int per_cta;         // 1 or 2 query tiles
-  int groups;          // CTAs along the rows
   int heads;           // B * H
+  int group;           // heads that run side by side
   int splits;          // CTAs along the keys
   float scale_log2;    // sm_scale log2(e)
   float cap_in;        // 2 sm_scale log2(e) / cap
@@ -95,30 +93,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* sQ = smem;
-  uint8_t* sKV = smem + 2 * kBytes;
+  uint8_t* sKV = smem + kBytes;
   S& ss = *reinterpret_cast<S*>(smem + S::kTiles);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // The last rows of every head first: under causal and prefix masks they see the most keys, and the CTAs that are
-  // left for the end are short (20,280 tokens, 6,240 of them a prefix: head by head left the SMs idle for a sixth
-  // of the time).  Heads side by side read K and V from L2 as long as they fit, and HBM has the rate for the rest.
+  // Heads in groups whose K and V fit in L2 together; within a group the last rows of every head first: under causal
+  // and prefix masks they see the most keys, and what is left for the end is short.  (4,096 rows of 7 documents,
+  // 12 heads: 80 us head by head, 60 like this; 14,040 rows x 8 heads, 10 MB of K and V a head, all
+  // heads as one group: 1.33 ms, head by head 1.27.)
   int item = blockIdx.x;
   const int split = item % p.splits;
   item /= p.splits;
-  const int bh = item % p.heads;
-  const int grp = p.groups - 1 - item / p.heads;
+  const int grp = item / (p.group * p.q_tiles);
+  item -= grp * p.group * p.q_tiles;
+  const int in_grp = min(p.group, p.heads - grp * p.group);
+  const int bh = grp * p.group + item % in_grp;
+  const int tile = p.q_tiles - 1 - item / in_grp;
   const int b = bh / p.H, h = bh - b * p.H;
   const int hk = h / p.G;
-  const int tile0 = grp * p.per_cta;
-  const int tiles = min(p.per_cta, p.q_tiles - tile0);
   const int bm = p.Bm > 1 ? b : 0;
-  int4 tab[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    tab[t] = make_int4(INT_MAX, 0, 0, 0);
-    if (t < tiles) tab[t] = p.table ? p.table[bm * p.q_tiles + tile0 + t] : make_int4(0, p.Sk, 0, p.Sk);
-  }
-  const int lo_u = min(tab[0].x, tab[1].x), hi_u = max(tab[0].y, tab[1].y);
+  const int4 tab = p.table ? p.table[static_cast<long long>(bm) * p.q_tiles + tile] : make_int4(0, p.Sk, 0, p.Sk);
+  const int lo_u = tab.x, hi_u = tab.y;
   int n0 = 0, n1 = 0;
   if (lo_u < hi_u) {
     n0 = lo_u / kTile;
@@ -135,22 +130,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&ss.q_full, 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&ss.full[i], 1);
-      mbar_init(&ss.empty[i], tiles);  // both tiles' products have read it
+      mbar_init(&ss.empty[i], 1);
     }
     mbar_init(&ss.fix, 1);
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&ss.s_full[t], 1);
-      mbar_init(&ss.p_full[t][0], 4);
-      mbar_init(&ss.p_full[t][1], 4);
-      mbar_init(&ss.o_full[t], 1);
-      mbar_init(&ss.turn[t], 4);
+    mbar_init(&ss.q_ready, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ss.s_full[i], 1);
+      mbar_init(&ss.s_read[i], kSoftmaxWarps);
+      mbar_init(&ss.p_full[i], kSoftmaxWarps);
+      mbar_init(&ss.o_full[i], 1);
     }
-    mbar_init(&ss.drain[0], 1);
-    mbar_init(&ss.drain[1], 1);
+    mbar_init(&ss.drain, 1);
     ss.abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == kIssue) {
     tmem_alloc(&ss.tmem, kTmemCols);
     tmem_relinquish();
   }
@@ -160,37 +154,37 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &ss.abort_flag;
   int* err = &g_dense_err;
 
-  // registers: 384 x 168 at launch = 128 x 40 + 256 x 232; a softmax thread holds a row of 128 scores
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  if (warp == 9) {
+  if (warp == kLoad) {
     // ------------------------------------------------------------------ loads
     if (steps > 0) {
       if (lane == 0) {
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
-        mbar_arrive_expect_tx(&ss.q_full, static_cast<uint32_t>(tiles * kBytes));
-        for (int t = 0; t < tiles; ++t)
-          load_tile<DP>(sQ + t * kBytes, &tm_q, &ss.q_full, (tile0 + t) * kTile, h, b);
+        mbar_arrive_expect_tx(&ss.q_full, kBytes);
+        load_tile<DP>(sQ, &tm_q, &ss.q_full, tile * kTile, h, b);
       }
       int slot = 0, issued = 0, fixes = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // in the order of use: K(0) K(1) K(2), then V(j) K(j+3)
+      int ik = 0, iv = 0;
       for (int i = 0; i < 2 * steps && ok; ++i) {
+        const bool is_v = ik == steps || ik > iv + 2;
+        const int step = is_v ? iv++ : ik++;
         if (issued >= kStages) {
           ok = bar_wait(&ss.empty[slot], phase ^ 1u, abort_flag, err, 301);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
-        const int row = (n0 + (i >> 1)) * kTile;
+        const int row = (n0 + step) * kTile;
         uint8_t* dst = sKV + slot * kBytes;
         // V rows of this tile that no row of the CTA sees, but the tensor holds
-        const bool fix = (i & 1) && (row < lo_u || min(row + kTile, p.Sk) > hi_u);
+        const bool fix = is_v && (row < lo_u || min(row + kTile, p.Sk) > hi_u);
         if (!fix) {
           if (lane == 0) {
             mbar_arrive_expect_tx(&ss.full[slot], kBytes);
-            load_tile<DP>(dst, (i & 1) ? &tm_v : &tm_k, &ss.full[slot], row, hk, b);
+            load_tile<DP>(dst, is_v ? &tm_v : &tm_k, &ss.full[slot], row, hk, b);
           }
         } else {
           if (lane == 0) {
@@ -226,14 +220,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp != 11) {
-    // ------------------------------------------------------------------ products of tile t
-    const int t = (warp - 8) >> 1;
-    if (lane == 0 && steps > 0 && t < tiles) {
+  } else if (warp == kIssue) {
+    // ------------------------------------------------------------------ products
+    if (lane == 0 && steps > 0) {
       constexpr uint32_t kIdQK = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t kIdPV = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
-      const uint32_t qb = smem_u32(sQ + t * kBytes), kvb = smem_u32(sKV);
-      const uint32_t s_col = tmem + col_s(t), o_col = tmem + col_o(t);
+      const uint32_t kvb = smem_u32(sKV);
       int slot = 0;
       uint32_t phase = 0;
       auto next = [&] {
@@ -242,86 +234,82 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase ^= 1u;
         }
       };
-      auto qk = [&] {  // S of the ring's next tile
+      auto qk = [&](int j) {  // S(j) of the ring's next tile, once S(j - 2) has been read
+        if (j >= 2 &&
+            !bar_wait(&ss.s_read[j & 1], static_cast<uint32_t>(((j - 2) >> 1) & 1), abort_flag, err, 314))
+          return false;
         if (!bar_wait(&ss.full[slot], phase, abort_flag, err, 312)) return false;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
-          umma_ss(s_col, desc_d(qb, kk), desc_d(kvb + slot * kBytes, kk), kIdQK, kk > 0);
-        umma_commit(&ss.s_full[t]);
+          umma_ts(tmem + col_s(j & 1), tmem + kColQ + 8 * kk, desc_d(kvb + slot * kBytes, kk), kIdQK, kk > 0);
+        umma_commit(&ss.s_full[j & 1]);
         umma_commit(&ss.empty[slot]);
         next();
         return true;
       };
-      bool ok = bar_wait(&ss.q_full, 0, abort_flag, err, 311) && qk();
+      bool ok = bar_wait(&ss.q_ready, 0, abort_flag, err, 311);
+      for (int j = 0; j < 3 && j < steps && ok; ++j) ok = qk(j);
       for (int j = 0; j < steps && ok; ++j) {
-        ok = bar_wait(&ss.full[slot], phase, abort_flag, err, 313);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {  // the first 64 keys' products run while the others' weights are computed
-          if (ok) ok = bar_wait(&ss.p_full[t][x], static_cast<uint32_t>(j & 1), abort_flag, err, 314);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 4 * x; kk < 4 * x + 4; ++kk)
-            umma_ts(o_col, s_col + 8 * kk, desc_rows(kvb + slot * kBytes, kk), kIdPV, j > 0 || kk > 0);
-        }
+        ok = bar_wait(&ss.full[slot], phase, abort_flag, err, 313) &&
+             bar_wait(&ss.p_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag, err, 315);
         if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_ts(tmem + kColO, tmem + kColP + 8 * kk, desc_rows(kvb + slot * kBytes, kk), kIdPV, j > 0 || kk > 0);
+        umma_commit(&ss.o_full[j & 1]);
         umma_commit(&ss.empty[slot]);
         next();
-        if (j + 1 < steps) ok = qk();
-        else umma_commit(&ss.o_full[t]);
+        if (j + 3 < steps) ok = qk(j + 3);
       }
       // teardown: this thread's products complete before the tensor memory is released
-      umma_commit(&ss.drain[t]);
+      umma_commit(&ss.drain);
       const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(&ss.drain[t], 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+      while (!mbar_try_wait(&ss.drain, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
       }
     }
     __syncwarp();
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+  } else if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------------ softmax
-    const int t = warp >> 2;
-    const int row = (tile0 + t) * kTile + 32 * (warp & 3) + lane;
+    const int half = warp >> 2;
+    const int r_tile = 32 * (warp & 3) + lane;
+    const int row = tile * kTile + r_tile;
     const uint32_t la = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-    const bool live = t < tiles && row < p.Sq;
-    if (t < tiles) {
+    const int pair = 1 + (warp & 3);  // named barrier of the two warps that share 32 rows
+    const bool live = row < p.Sq;
+    {
       int lo = 0, hi = p.Sk;
       if (p.ranges && live) {
         const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
         lo = r.x;
         hi = r.y;
       }
-      const int lo_max = tab[t].z, hi_min = tab[t].w;
+      const uint32_t seen = static_cast<uint32_t>(hi - lo);
+      const int lo_max = tab.z, hi_min = tab.w;
+      const float scale = kCap ? 1.f : p.scale_log2;
       float m = -INFINITY;
       uint64_t l2 = f2_pack(0.f, 0.f);  // sum of the rounded weights, two partial sums
       uint64_t t2 = l2;                 // of the fp32 ones
       bool ok = true;
-      for (int j = 0; j < steps; ++j) {
-        ok = bar_wait(&ss.s_full[t], static_cast<uint32_t>(j & 1), abort_flag, err, 321);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t r[128];
-        tmem_read128(la + col_s(t), r);
-        const int key0 = (n0 + j) * kTile;
-        const bool border = key0 < lo_max || key0 + kTile > hi_min;
-        const uint32_t seen = static_cast<uint32_t>(hi - lo), first = static_cast<uint32_t>(key0 - lo);
+      uint32_t rx[32], ry[32];  // scores of this step's first and last 32 keys
+      // the cap and the mask on 32 scores of keys from `key` on
+      auto prepare = [&](uint32_t* r, int key, bool border) {
+        const uint32_t first = static_cast<uint32_t>(key - lo);
         if constexpr (kCap) {
           float top = 0.f;
           if (border) {  // what a masked place holds must not choose the form of tanh below
 #pragma unroll
-            for (int e = 0; e < 128; ++e)
+            for (int e = 0; e < 32; ++e)
               if (first + e >= seen) r[e] = 0u;
           }
 #pragma unroll
-          for (int e = 0; e < 128; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+          for (int e = 0; e < 32; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
           if (__all_sync(0xffffffffu, top * p.cap_in <= 2.f * 1.44269504f)) {  // |s| <= cap in all of the warp's rows
             const float ci = p.cap_in * 0.34657359f;  // cap_in = 2 log2(e) sm_scale / cap
             const uint64_t in2 = f2_pack(ci, ci), out2 = f2_pack(p.cap_log2, p.cap_log2);
 #pragma unroll
-            for (int e = 0; e < 128; e += 2) {
+            for (int e = 0; e < 32; e += 2) {
               float a, c;
               f2_unpack(f2_mul(tanh_poly2(f2_mul(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), in2)), out2), a, c);
               r[e] = __float_as_uint(a);
@@ -329,99 +317,171 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 128; ++e)
-              r[e] = __float_as_uint(p.cap_log2 * tanh_of(__uint_as_float(r[e]) * p.cap_in));
+            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(p.cap_log2 * tanh_of(__uint_as_float(r[e]) * p.cap_in));
           }
         }
         if (border) {
 #pragma unroll
-          for (int e = 0; e < 128; ++e)
+          for (int e = 0; e < 32; ++e)
             if (first + e >= seen) r[e] = 0xff800000u;
         }
+      };
+      auto top_of = [&](const uint32_t* r) {
         float mv[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mv[e] = __uint_as_float(r[e]);
+        for (int e = 0; e < 4; ++e) mv[e] = max3(__uint_as_float(r[e]), __uint_as_float(r[e + 4]), __uint_as_float(r[e + 8]));
 #pragma unroll
-        for (int c = 4; c + 8 <= 128; c += 8)
+        for (int c = 12; c < 28; c += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) mv[e] = max3(mv[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mv[e] = max3(mv[e], __uint_as_float(r[124 + e]), __uint_as_float(r[124 + e]));
-        const float top = max3(max3(mv[0], mv[1], mv[2]), mv[3], mv[3]);
-        const float scale = kCap ? 1.f : p.scale_log2;
-        const float mx = top * scale;
-        float f = 1.f;
-        const bool raise = !(mx <= m + kRescale);  // a NaN raises too, and stays
-        if (raise) {
-          f = ex2_approx(m - mx);  // 0 for the first maximum
-          m = mx;
-          l2 = f2_mul(l2, f2_pack(f, f));
-          t2 = f2_mul(t2, f2_pack(f, f));
-        }
-        if (j > 0 && __any_sync(0xffffffffu, raise)) {
-#pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(la + col_o(t) + 32 * c, o);
-            tmem_ld_wait();
+        for (int e = 0; e < 4; ++e) mv[e] = max3(mv[e], mv[e], __uint_as_float(r[28 + e]));
+        return max3(max3(mv[0], mv[1], mv[2]), mv[3], mv[3]);
+      };
+      // exponentials of 32 scores: their sums and, in pairs, their 16-bit roundings
+      auto weights = [&](const uint32_t* r, uint64_t sc2, uint64_t nm2, uint32_t* pk) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(la + col_o(t) + 32 * c, o);
-          }
+        for (int e = 0; e < 16; ++e) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), sc2, nm2), x0, x1);
+          x0 = ex2_approx(x0);
+          x1 = ex2_approx(x1);
+          t2 = f2_add(t2, f2_pack(x0, x1));
+          pk[e] = pack16<kBF16>(x0, x1);
+          unpack16<kBF16>(pk[e], x0, x1);
+          l2 = f2_add(l2, f2_pack(x0, x1));
         }
-        // The tiles take turns: side by side they would share the special-function unit, finish together, and leave it
-        // idle while both wait for their products.
-        if (tiles > 1 && (t == 1 || j > 0)) {
-          ok = bar_wait(&ss.turn[t ^ 1], static_cast<uint32_t>((t ? j : j - 1) & 1), abort_flag, err, 323);
+      };
+      float mx = -INFINITY;
+      if (steps > 0) {
+        if (half == 0) {  // Q into tensor memory: row r_tile, 16-bit pairs along d
+          ok = bar_wait(&ss.q_full, 0, abort_flag, err, 324);
           ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-        const float nm = m == -INFINITY ? 0.f : -m;
-        const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(nm, nm);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int i = 32 * c + 2 * e;
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sc2, nm2), x0, x1);
-            if (e % kPolyOf == kPolyOf - 1) {
-              ex2_poly2(x0, x1);
-            } else {
-              x0 = ex2_approx(x0);
-              x1 = ex2_approx(x1);
+            for (int x = 0; x < 4; ++x) {
+              const uint4 u = *reinterpret_cast<const uint4*>(sQ + (c >> 1) * kHalfBytes +
+                                                              sw128_offset(static_cast<uint32_t>(r_tile), 4 * (c & 1) + x));
+              w[4 * x] = u.x;
+              w[4 * x + 1] = u.y;
+              w[4 * x + 2] = u.z;
+              w[4 * x + 3] = u.w;
             }
-            t2 = f2_add(t2, f2_pack(x0, x1));
-            pk[e] = pack16<kBF16>(x0, x1);
-            unpack16<kBF16>(pk[e], x0, x1);
-            l2 = f2_add(l2, f2_pack(x0, x1));
+            tmem_st16(la + kColQ + 16 * c, w);
           }
-          if (c == 3 && tiles > 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ss.turn[t]);
-          }
-          tmem_st16(la + col_s(t) + 16 * c, pk);
-          if (c & 1) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ss.p_full[t][c >> 1]);
-          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss.q_ready);
+        }
+        if (ok) ok = bar_wait(&ss.s_full[0], 0, abort_flag, err, 321);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          tc_fence_after();
+          tmem_read32(la + col_s(0) + 64 * half, rx);
+          tmem_read32(la + col_s(0) + 64 * half + 32, ry);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss.s_read[0]);
+          const int key = n0 * kTile;
+          const bool border = key < lo_max || key + kTile > hi_min;
+          prepare(rx, key + 64 * half, border);
+          prepare(ry, key + 64 * half + 32, border);
+          mx = max3(top_of(rx), top_of(ry), -INFINITY) * scale;
         }
       }
-      // ---- o / l and the row's log sum
+      // After an expired wait the loop goes on without work: both warps of a pair pass the same barriers.
+      for (int j = 0; j < steps; ++j) {
+        if (pair_any(pair, !(mx <= m + kRescale))) {  // a NaN raises too, and stays
+          ss.join[half][0][r_tile] = mx;
+          pair_sync(pair);
+          mx = max3(mx, ss.join[half ^ 1][0][r_tile], mx);
+          float f = 1.f;
+          if (!(mx <= m + kRescale)) {
+            f = ex2_approx(m - mx);  // 0 for the first maximum
+            m = mx;
+            l2 = f2_mul(l2, f2_pack(f, f));
+            t2 = f2_mul(t2, f2_pack(f, f));
+          }
+          if (j > 0 && ok) {
+            // O holds P V up to step j - 1 once that step's products are done; the next ones wait for this step's P
+            ok = bar_wait(&ss.o_full[(j - 1) & 1], static_cast<uint32_t>(((j - 1) >> 1) & 1), abort_flag, err, 323);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+          }
+          if (j > 0 && ok) {
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[16];
+              const uint32_t at = la + kColO + half * (DP / 2) + 16 * c;
+              tmem_read16(at, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(at, o);
+            }
+          }
+        }
+        if (!ok) continue;
+        const float nm = m == -INFINITY ? 0.f : -m;
+        const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(nm, nm);
+        const bool more = j + 1 < steps;
+        uint32_t pk[16];
+        weights(rx, sc2, nm2, pk);
+        if (j > 0) {  // P(j - 1) has been read
+          ok = bar_wait(&ss.o_full[(j - 1) & 1], static_cast<uint32_t>(((j - 1) >> 1) & 1), abort_flag, err, 325);
+          tc_fence_after();
+        }
+        if (ok && more) ok = bar_wait(&ss.s_full[(j + 1) & 1], static_cast<uint32_t>(((j + 1) >> 1) & 1), abort_flag, err, 326);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) continue;
+        tmem_st16(la + kColP + 32 * half, pk);
+        const uint32_t s_next = la + col_s((j + 1) & 1) + 64 * half;
+        const int key = (n0 + j + 1) * kTile;
+        const bool border = key < lo_max || key + kTile > hi_min;
+        float top = -INFINITY;
+        if (more) {
+          tc_fence_after();
+          tmem_read32(s_next, rx);
+          if (kCap || border) prepare(rx, key + 64 * half, border);
+          weights(ry, sc2, nm2, pk);
+          top = top_of(rx);
+        } else {
+          weights(ry, sc2, nm2, pk);
+        }
+        tmem_st16(la + kColP + 32 * half + 16, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ss.p_full[j & 1]);
+        if (more) {
+          tmem_read32(s_next + 32, ry);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ss.s_read[(j + 1) & 1]);
+          if (kCap || border) prepare(ry, key + 64 * half + 32, border);
+          mx = max3(top, top_of(ry), top) * scale;
+        }
+      }
+      // ---- join the halves' sums; o / l and the row's log sum, half of the columns to a thread
+      float l, lt, other;
+      f2_unpack(l2, l, other);
+      l += other;
+      f2_unpack(t2, lt, other);
+      lt += other;
+      pair_sync(pair);  // the last maximum has been read
+      ss.join[half][0][r_tile] = l;
+      ss.join[half][1][r_tile] = lt;
+      pair_sync(pair);
+      l += ss.join[half ^ 1][0][r_tile];
+      lt += ss.join[half ^ 1][1][r_tile];
       if (ok && steps > 0) {
-        ok = bar_wait(&ss.o_full[t], 0, abort_flag, err, 322);
+        ok = bar_wait(&ss.o_full[(steps - 1) & 1], static_cast<uint32_t>(((steps - 1) >> 1) & 1), abort_flag, err, 322);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
       if (ok) {
-        float l, lt, half;
-        f2_unpack(l2, l, half);
-        l += half;
-        f2_unpack(t2, lt, half);
-        lt += half;
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
         const float lse2 = lt == 0.f ? -INFINITY : m + log2f(lt);
         const long long flat = static_cast<long long>(bh) * p.Sq + row;
@@ -429,21 +489,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         const long long off = b * p.ob + h * p.oh + static_cast<long long>(row) * p.os;
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
+          const int c0 = half * (DP / 2) + 16 * c;
+          uint32_t o[16];
           if (steps > 0) {
-            tmem_ld32(la + col_o(t) + 32 * c, o);
-            tmem_ld_wait();
+            tmem_read16(la + kColO + c0, o);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int e = 0; e < 16; ++e) o[e] = 0u;
           }
-          float v[32];
+          float v[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+          for (int e = 0; e < 16; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
           if (live) {
 #pragma unroll
-            for (int e8 = 0; e8 < 4; ++e8) {
-              const int d0 = 32 * c + 8 * e8;
+            for (int e8 = 0; e8 < 2; ++e8) {
+              const int d0 = c0 + 8 * e8;
               if (d0 < p.D) {
                 if (part) {
 #pragma unroll
@@ -456,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (live) {
+        if (live && half == 0) {
           if (part) part[p.D] = lse2;
           else if (p.lse) p.lse[flat] = lse2 * 0.6931471805599453f;
         }
@@ -466,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, kTmemCols);
+  if (warp == kIssue) tmem_dealloc(tmem, kTmemCols);
 }
 
 // Joins the key splits of a row, always in their order: o = sum 2^(lse_s - m) o_s / sum 2^(lse_s - m).
@@ -552,13 +612,13 @@ int launch_dense(const DenseArgs& a, int sms, cudaStream_t stream) {
   p.ranges = a.ranges; p.table = a.table; p.Bm = a.Bm;
   p.H = a.H; p.G = a.H / a.Hk; p.Sq = a.Sq; p.Sk = a.Sk; p.D = a.D;
   p.q_tiles = (a.Sq + kTile - 1) / kTile;
-  // two query tiles to a CTA halve the key loads and overlap softmax and products; one each where two
-  // would leave SMs without a CTA
   const long long bh = static_cast<long long>(a.B) * a.H;
-  p.per_cta = bh * ((p.q_tiles + 1) / 2) * a.splits >= sms ? 2 : 1;
-  p.groups = (p.q_tiles + p.per_cta - 1) / p.per_cta;
   p.splits = a.splits;
   p.heads = static_cast<int>(bh);
+  // a third of the 126 MB of L2 for K and V of a group: each of the two dies keeps its own copy of what both read
+  const long long kv_bytes = 4ll * a.Sk * a.D;
+  const long long group = (40ll << 20) / kv_bytes * p.G;
+  p.group = static_cast<int>(group < 1 ? 1 : (group < bh ? group : bh));
   p.scale_log2 = a.sm_scale * 1.4426950408889634f;
   if (a.softcap > 0.f) {
     p.cap_in = 2.f * p.scale_log2 / a.softcap;
@@ -569,7 +629,7 @@ int launch_dense(const DenseArgs& a, int sms, cudaStream_t stream) {
   p.lse = a.lse;
   p.part = a.part;
   p.rows = bh * a.Sq;
-  const long long grid = bh * p.groups * p.splits;
+  const long long grid = bh * p.q_tiles * p.splits;
   if (grid > INT_MAX) return set_error(BSA_ERR_SHAPE, "too many row tiles for one launch");
   const bool bf = a.dtype == BSA_DTYPE_BF16, cap = a.softcap > 0.f;
   if (a.D > 64)
