@@ -41,7 +41,9 @@ struct BwdParams {
   int Bm, H, Hk, G, Sq, Sk, D;
   int q_tiles, k_tiles, Sq_pad;
   float scale_log2, sm_scale, cap_in, cap_log2;
-  float2* stats;        // [B * H][Sq_pad]: lse in log2 (+inf: no keys), delta
+  float* lse2;          // [B * H][Sq_pad]: lse in log2 (+inf: no keys)
+  float* delta;         // [B * H][Sq_pad]
+  float cap_inv, cap_mask;  // 1 / cap_log2, and a score below every capped one by 2^300
   int2* rng;            // [Bm][Sq_pad]: ranges, padded with empty ones
   const float* lse;
   Tensor4 o, g;         // forward output, its gradient
@@ -85,7 +87,8 @@ __global__ void __launch_bounds__(256) stats_kernel(const BwdParams p) {
         dot = 0.f;
       }
     }
-    p.stats[static_cast<long long>(bh) * p.Sq_pad + row] = make_float2(l, on ? dot : 0.f);
+    p.lse2[static_cast<long long>(bh) * p.Sq_pad + row] = l;
+    p.delta[static_cast<long long>(bh) * p.Sq_pad + row] = on ? dot : 0.f;
     if (h == 0 && b < p.Bm && p.rng)
       p.rng[static_cast<long long>(b) * p.Sq_pad + row] =
           on ? p.ranges[static_cast<long long>(b) * p.Sq + row] : make_int2(0, 0);
@@ -97,6 +100,33 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                    smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
+}
+
+// 64 scores q.k through the cap, in log2 units; |s| <= cap in the whole warp: the polynomial form
+__device__ __forceinline__ void capped64(uint32_t* r, float cap_in, float cap_log2) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 64; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+  if (__all_sync(0xffffffffu, top * cap_in <= 2.f * 1.44269504f)) {
+    const float ci = cap_in * 0.34657359f;  // cap_in = 2 log2(e) sm_scale / cap
+    const uint64_t in2 = f2_pack(ci, ci), out2 = f2_pack(cap_log2, cap_log2);
+#pragma unroll
+    for (int e = 0; e < 64; e += 2) {
+      float a, c;
+      f2_unpack(f2_mul(tanh_poly2(f2_mul(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), in2)), out2), a, c);
+      r[e] = __float_as_uint(a);
+      r[e + 1] = __float_as_uint(c);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 64; ++e) r[e] = __float_as_uint(cap_log2 * tanh_of(__uint_as_float(r[e]) * cap_in));
+  }
+}
+
+__device__ __forceinline__ void put_masked(uint32_t* r, const uint32_t* seen, uint32_t v) {
+#pragma unroll
+  for (int e = 0; e < 64; ++e)
+    if (!(seen[e >> 5] & (1u << (e & 31)))) r[e] = v;
 }
 
 template <int N>
@@ -166,7 +196,7 @@ struct DkvSmem {
   static constexpr int kQ = DP == 128 ? 2 : 4;   // query tiles in flight
   static constexpr int kG = DP == 128 ? 2 : 4;   // tiles of do in flight
   static constexpr int kTiles = (2 + kQ + kG) * tile_bytes<DP>();
-  alignas(16) float2 stats[kQ][kTile];
+  alignas(16) float lse2[kQ][kTile], delta[kQ][kTile];
   alignas(16) int2 rng[kQ][kTile];
   uint64_t kv_full;
   uint64_t q_full[kQ], q_empty[kQ], g_full[kG], g_empty[kG];
@@ -276,13 +306,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!__all_sync(0xffffffffu, w)) return false;
         const bool fix = t.w <= 0;  // rows without keys, whose q and do may hold anything
         uint8_t* q = sQ + rq.slot * kBytes;
-        const uint32_t extra = kTile * sizeof(float2) + (p.rng ? kTile * sizeof(int2) : 0);
+        const uint32_t extra = 2 * kTile * sizeof(float) + (p.rng ? kTile * sizeof(int2) : 0);
         if (lane == 0) {
           uint64_t* bar = fix ? &ss.fix : &ss.q_full[rq.slot];
           mbar_arrive_expect_tx(bar, kBytes + extra);
           load_tile<DP>(q, &tm_q, bar, i * kTile, h, b);
-          bulk_load(ss.stats[rq.slot], p.stats + (static_cast<long long>(b) * p.H + h) * p.Sq_pad + i * kTile,
-                    kTile * sizeof(float2), bar);
+          const long long at = (static_cast<long long>(b) * p.H + h) * p.Sq_pad + i * kTile;
+          bulk_load(ss.lse2[rq.slot], p.lse2 + at, kTile * sizeof(float), bar);
+          bulk_load(ss.delta[rq.slot], p.delta + at, kTile * sizeof(float), bar);
           if (p.rng)
             bulk_load(ss.rng[rq.slot], p.rng + static_cast<long long>(bm) * p.Sq_pad + i * kTile, kTile * sizeof(int2),
                       bar);
@@ -401,34 +432,42 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!__all_sync(0xffffffffu, w)) return false;
         tc_fence_after();
         uint32_t r[64];
-        tmem_ld32(la + kColA + 64 * half, r);
-        tmem_ld32(la + kColA + 64 * half + 32, r + 32);
-        tmem_ld_wait();
-        const float4* st = reinterpret_cast<const float4*>(ss.stats[rq.slot] + 64 * half);
+        tmem_read32(la + kColA + 64 * half, r);
+        tmem_read32(la + kColA + 64 * half + 32, r + 32);
+        // p = 2^(z - lse), in pairs of 16 bits for the product and as r = p (1 - tanh^2) for ds.  The queries' statistics
+        // come four to a load: what a load returns to 32 lanes passes the same port as the tiles.
+        const float4* ls = reinterpret_cast<const float4*>(ss.lse2[rq.slot] + 64 * half);
         const bool border = table && (t.z > key0 || t.w < key0 + kTile);
-        float pr[64];  // p, then p (1 - tanh^2)
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};  // one bit for each of the thread's 64 queries
+        if (border) {
+          const int4* rg = reinterpret_cast<const int4*>(ss.rng[rq.slot] + 64 * half);
+          seen[0] = seen[1] = 0u;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int4 b2 = rg[e];
+            if (key >= b2.x && key < b2.y) seen[e >> 4] |= 1u << (2 * (e & 15));
+            if (key >= b2.z && key < b2.w) seen[e >> 4] |= 2u << (2 * (e & 15));
+          }
+          // what a masked place holds must not choose the form of tanh, nor reach anything else
+          if constexpr (kCap) put_masked(r, seen, 0u);
+        }
+        if constexpr (kCap) capped64(r, p.cap_in, p.cap_log2);
+        if (border) put_masked(r, seen, __float_as_uint(kCap ? p.cap_mask : -INFINITY));
         uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float4 s2 = st[e];  // lse, delta of two queries
-          float t0 = 0.f, t1 = 0.f, x0, x1;
-          if constexpr (kCap) {
-            t0 = tanh_of(__uint_as_float(r[2 * e]) * p.cap_in);
-            t1 = tanh_of(__uint_as_float(r[2 * e + 1]) * p.cap_in);
-            x0 = ex2_approx(fmaf(t0, p.cap_log2, -s2.x));
-            x1 = ex2_approx(fmaf(t1, p.cap_log2, -s2.z));
-          } else {
-            x0 = ex2_approx(fmaf(__uint_as_float(r[2 * e]), p.scale_log2, -s2.x));
-            x1 = ex2_approx(fmaf(__uint_as_float(r[2 * e + 1]), p.scale_log2, -s2.z));
+        for (int e = 0; e < 16; ++e) {
+          const float4 l4 = ls[e];
+          const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+          float x[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float s = __uint_as_float(r[4 * e + c]);
+            x[c] = ex2_approx(kCap ? s - lv[c] : fmaf(s, p.scale_log2, -lv[c]));
+            const float u = s * p.cap_inv;  // tanh
+            r[4 * e + c] = __float_as_uint(kCap ? x[c] * fmaf(-u, u, 1.f) : x[c]);
           }
-          if (border) {
-            const int4 b2 = reinterpret_cast<const int4*>(ss.rng[rq.slot] + 64 * half)[e];
-            if (key < b2.x || key >= b2.y) x0 = t0 = 0.f;
-            if (key < b2.z || key >= b2.w) x1 = t1 = 0.f;
-          }
-          pk[e] = pack16<kBF16>(x0, x1);
-          pr[2 * e] = kCap ? x0 * fmaf(-t0, t0, 1.f) : x0;
-          pr[2 * e + 1] = kCap ? x1 * fmaf(-t1, t1, 1.f) : x1;
+          pk[2 * e] = pack16<kBF16>(x[0], x[1]);
+          pk[2 * e + 1] = pack16<kBF16>(x[2], x[3]);
         }
         tmem_st32(la + kColA + 64 * half, pk);
         tmem_st_wait();
@@ -438,19 +477,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         w = bar_wait(&ss.dp_full, static_cast<uint32_t>(n & 1), abort_flag, err, 423);
         if (!__all_sync(0xffffffffu, w)) return false;
         tc_fence_after();
-        tmem_ld32(la + kColB + 64 * half, r);
-        tmem_ld32(la + kColB + 64 * half + 32, r + 32);
-        tmem_ld_wait();
+        const float4* dl = reinterpret_cast<const float4*>(ss.delta[rq.slot] + 64 * half);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float4 s2 = st[e];
-          float y0 = pr[2 * e] * (__uint_as_float(r[2 * e]) - s2.y);
-          float y1 = pr[2 * e + 1] * (__uint_as_float(r[2 * e + 1]) - s2.w);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t g[32];
+          tmem_read32(la + kColB + 64 * half + 32 * c, g);
           if (border) {  // 0 * NaN
-            if (pr[2 * e] == 0.f) y0 = 0.f;
-            if (pr[2 * e + 1] == 0.f) y1 = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (__uint_as_float(r[32 * c + e]) == 0.f) g[e] = 0u;
           }
-          pk[e] = pack16<kBF16>(y0, y1);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 d4 = dl[8 * c + e];
+            const uint32_t* rr = r + 32 * c + 4 * e;
+            pk[16 * c + 2 * e] = pack16<kBF16>(__uint_as_float(rr[0]) * (__uint_as_float(g[4 * e]) - d4.x),
+                                               __uint_as_float(rr[1]) * (__uint_as_float(g[4 * e + 1]) - d4.y));
+            pk[16 * c + 2 * e + 1] = pack16<kBF16>(__uint_as_float(rr[2]) * (__uint_as_float(g[4 * e + 2]) - d4.z),
+                                                   __uint_as_float(rr[3]) * (__uint_as_float(g[4 * e + 3]) - d4.w));
+          }
         }
         tmem_st32(la + kColB + 64 * half, pk);
         tmem_st_wait();
@@ -659,57 +704,69 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const bool live = row < p.Sq;
     bool ok = true;
     if (steps > 0) {
-      const float2 st = p.stats[static_cast<long long>(bh) * p.Sq_pad + row];
+      const float lse2 = p.lse2[static_cast<long long>(bh) * p.Sq_pad + row];
+      const float delta = p.delta[static_cast<long long>(bh) * p.Sq_pad + row];
       int lo = 0, hi = p.Sk;
       if (p.ranges && live) {
         const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
         lo = r.x;
         hi = r.y;
       }
+      const uint32_t len = static_cast<uint32_t>(hi - lo);
       for (int n = 0; n < steps; ++n) {
         ok = bar_wait(&ss.s_full, static_cast<uint32_t>(n & 1), abort_flag, err, 471);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         uint32_t r[64];
-        tmem_ld32(la + kColA + 64 * half, r);
-        tmem_ld32(la + kColA + 64 * half + 32, r + 32);
-        tmem_ld_wait();
+        tmem_read32(la + kColA + 64 * half, r);
+        tmem_read32(la + kColA + 64 * half + 32, r + 32);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ss.s_read);
         const int key0 = (n0 + n) * kTile;
         const bool border = key0 < tab.z || key0 + kTile > tab.w;
-        float pr[64];
+        const uint32_t d = static_cast<uint32_t>(key0 + 64 * half - lo);
+        if constexpr (kCap) {
+          if (border) {  // what a masked place holds must not choose the form of tanh
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (d + e >= len) r[e] = 0u;
+          }
+          capped64(r, p.cap_in, p.cap_log2);
+        }
+        if (border) {
+          const uint32_t out = __float_as_uint(kCap ? p.cap_mask : -INFINITY);
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (d + e >= len) r[e] = out;
+        }
 #pragma unroll
         for (int e = 0; e < 64; ++e) {
-          if constexpr (kCap) {
-            const float t = tanh_of(__uint_as_float(r[e]) * p.cap_in);
-            pr[e] = ex2_approx(fmaf(t, p.cap_log2, -st.x)) * fmaf(-t, t, 1.f);
-          } else {
-            pr[e] = ex2_approx(fmaf(__uint_as_float(r[e]), p.scale_log2, -st.x));
-          }
+          const float s = __uint_as_float(r[e]);
+          const float x = ex2_approx(kCap ? s - lse2 : fmaf(s, p.scale_log2, -lse2));
+          const float u = s * p.cap_inv;  // tanh
+          r[e] = __float_as_uint(kCap ? x * fmaf(-u, u, 1.f) : x);
         }
-        const uint32_t len = static_cast<uint32_t>(hi - lo);
-        const uint32_t d = static_cast<uint32_t>(key0 + 64 * half - lo);
         const uint32_t col = (n & 1) ? kColC : kColB;
         ok = bar_wait(&ss.dp_full[n & 1], static_cast<uint32_t>((n >> 1) & 1), abort_flag, err, 472);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        tmem_ld32(la + col + 64 * half, r);
-        tmem_ld32(la + col + 64 * half + 32, r + 32);
-        tmem_ld_wait();
         uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float y0 = pr[2 * e] * (__uint_as_float(r[2 * e]) - st.y);
-          float y1 = pr[2 * e + 1] * (__uint_as_float(r[2 * e + 1]) - st.y);
-          if (border) {
-            if (d + 2 * e >= len) y0 = 0.f;
-            if (d + 2 * e + 1 >= len) y1 = 0.f;
+        for (int c = 0; c < 2; ++c) {
+          uint32_t g[32];
+          tmem_read32(la + col + 64 * half + 32 * c, g);
+          if (border) {  // 0 * NaN
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (__uint_as_float(r[32 * c + e]) == 0.f) g[e] = 0u;
           }
-          pk[e] = pack16<kBF16>(y0, y1);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            pk[16 * c + e] = pack16<kBF16>(__uint_as_float(r[32 * c + 2 * e]) * (__uint_as_float(g[2 * e]) - delta),
+                                           __uint_as_float(r[32 * c + 2 * e + 1]) * (__uint_as_float(g[2 * e + 1]) - delta));
         }
         tmem_st32(la + col + 64 * half, pk);
         tmem_st_wait();
@@ -788,8 +845,11 @@ int launch_dense_backward(const DenseArgs& a, cudaStream_t stream) {
   if (a.softcap > 0.f) {
     p.cap_in = 2.f * p.scale_log2 / a.softcap;
     p.cap_log2 = a.softcap * 1.4426950408889634f;
+    p.cap_inv = 1.f / p.cap_log2;
+    p.cap_mask = -p.cap_log2 - 300.f;
   }
-  p.stats = reinterpret_cast<float2*>(a.stats);
+  p.lse2 = a.stats;
+  p.delta = a.stats + static_cast<long long>(a.B) * a.H * p.Sq_pad;
   p.rng = a.ranges ? reinterpret_cast<int2*>(a.stats + 2 * static_cast<long long>(a.B) * a.H * p.Sq_pad) : nullptr;
   p.lse = a.lse;
   p.o = a.o;
