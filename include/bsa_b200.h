@@ -198,13 +198,13 @@ int bsa_forward_noalloc(const void* q, const void* k, const void* v, int dtype, 
  * w0 / w1 (w_dtype, [D]; NULL: no norm), rope (NULL: no rotation) as in bsa_mean_pool; the tokens of x stand at
  * places start .. start + S - 1 of the rope grid.  x1 NULL: one tensor.  Outputs are contiguous.
  * bsa_norm_rope_backward: gradients dx (contiguous) of the inputs and dw ([D] fp32, NULL: none) of the weights
- * from the outputs' gradients g; scratch (bsa_norm_rope_backward_scratch_bytes(D)) is needed for the weights'.
+ * from the outputs' gradients g; scratch (bsa_norm_rope_backward_scratch_bytes(), H1 0 for one tensor) is needed for the weights'.
  * Sums are taken in a fixed order. */
 int bsa_norm_rope(const void* x0, const int64_t* x0_strides, int H0, const void* w0, void* y0, const void* x1,
                   const int64_t* x1_strides, int H1, const void* w1, void* y1, int dtype, int w_dtype, int B, int S,
                   int D, float eps, const float* rope, int rope_dt, int rope_dh, int rope_dw, int rope_T, int rope_H,
                   int rope_W, int start, void* stream);
-int64_t bsa_norm_rope_backward_scratch_bytes(int D);
+int64_t bsa_norm_rope_backward_scratch_bytes(int H0, int H1, int D);
 int bsa_norm_rope_backward(const void* x0, const int64_t* x0_strides, const void* g0, const int64_t* g0_strides, int H0,
                            const void* w0, void* dx0, float* dw0, const void* x1, const int64_t* x1_strides,
                            const void* g1, const int64_t* g1_strides, int H1, const void* w1, void* dx1, float* dw1,

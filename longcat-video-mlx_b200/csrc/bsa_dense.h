@@ -35,10 +35,10 @@ struct NormRopeArgs {
   float eps = 0.f;
   const float* rope = nullptr;  // nullable: [cos_t | sin_t | cos_h | sin_h | cos_w | sin_w]
   int dt = 0, dh = 0, dw = 0, gT = 0, gH = 0, gW = 0, start = 0;
-  float* partial = nullptr;     // backward: norm_rope_partials() rows of [sides][D]
+  float* partial = nullptr;     // backward: norm_rope_partials() rows of D
 };
 int launch_norm_rope(const NormRopeArgs& a, cudaStream_t stream);
-int norm_rope_partials();       // most rows of `partial` on the current device
+int norm_rope_partials(int head_groups);  // most rows of `partial` on the current device
 int launch_norm_rope_backward(const NormRopeArgs& a, cudaStream_t stream);
 
 // ------------------------------------------------------------------ key intervals

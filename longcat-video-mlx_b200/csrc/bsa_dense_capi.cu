@@ -65,6 +65,7 @@ int norm_rope_plan(bsa::NormRopeArgs& a, int dtype, int w_dtype, int B, int S, i
   if (w_dtype != BSA_DTYPE_F32 && w_dtype != BSA_DTYPE_F16 && w_dtype != BSA_DTYPE_BF16)
     return set_error(BSA_ERR_DTYPE, "unsupported weight dtype code %d", w_dtype);
   if (B <= 0 || S <= 0) return set_error(BSA_ERR_SHAPE, "empty tensor");
+  if (static_cast<long long>(B) * (S / 16 + 1) >= INT_MAX) return set_error(BSA_ERR_SHAPE, "too many tokens for one launch");
   int rc = check_head_dim(D);
   if (rc) return rc;
   if (!(eps >= 0.f)) return set_error(BSA_ERR_ARG, "norm eps must be >= 0");
@@ -73,6 +74,7 @@ int norm_rope_plan(bsa::NormRopeArgs& a, int dtype, int w_dtype, int B, int S, i
         rope_dw < 0)
       return set_error(BSA_ERR_SHAPE, "rope dims (%d, %d, %d) must be even and sum to D=%d", rope_dt, rope_dh, rope_dw, D);
     if (rope_T <= 0 || rope_H <= 0 || rope_W <= 0 || start < 0 ||
+        static_cast<long long>(rope_H) * rope_W > INT_MAX ||
         static_cast<long long>(start) + S > static_cast<long long>(rope_T) * rope_H * rope_W)
       return set_error(BSA_ERR_SHAPE, "rope grid (%d, %d, %d) does not cover tokens %d to %lld", rope_T, rope_H, rope_W,
                        start, static_cast<long long>(start) + S);
@@ -168,8 +170,10 @@ int bsa_norm_rope(const void* x0, const int64_t* x0_strides, int H0, const void*
   return launched(bsa::launch_norm_rope(a, static_cast<cudaStream_t>(stream)), "norm + rope");
 }
 
-int64_t bsa_norm_rope_backward_scratch_bytes(int D) {
-  return static_cast<int64_t>(bsa::norm_rope_partials()) * 2 * D * static_cast<int64_t>(sizeof(float));
+int64_t bsa_norm_rope_backward_scratch_bytes(int H0, int H1, int D) {
+  if (H0 <= 0 || H1 < 0 || D <= 0) return 0;
+  return static_cast<int64_t>(bsa::norm_rope_partials((H0 + 7) / 8 + (H1 + 7) / 8)) * D *
+         static_cast<int64_t>(sizeof(float));
 }
 
 int bsa_norm_rope_backward(const void* x0, const int64_t* x0_strides, const void* g0, const int64_t* g0_strides, int H0,

@@ -37,6 +37,19 @@ struct Row8 {
     unpack_pair(u.z, f[4], f[5], T());
     unpack_pair(u.w, f[6], f[7], T());
   }
+  // as four packed pairs
+  __device__ __forceinline__ void get2(uint64_t* v) const {
+    float f[8];
+    get(f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm("mov.b64 %0, {%1, %2};" : "=l"(v[e]) : "f"(f[2 * e]), "f"(f[2 * e + 1]));
+  }
+  static __device__ __forceinline__ void store2(T* p, const uint64_t* v) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm("mov.b64 {%0, %1}, %2;" : "=f"(f[2 * e]), "=f"(f[2 * e + 1]) : "l"(v[e]));
+    store(p, f);
+  }
   static __device__ __forceinline__ void store(T* p, const float* f) {
     uint4 o;
     o.x = pack_pair(f[0], f[1], T());
@@ -58,6 +71,18 @@ struct Row8<float> {
   __device__ __forceinline__ void get(float* f) const {
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+  __device__ __forceinline__ void get2(uint64_t* v) const {
+    float f[8];
+    get(f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm("mov.b64 %0, {%1, %2};" : "=l"(v[e]) : "f"(f[2 * e]), "f"(f[2 * e + 1]));
+  }
+  static __device__ __forceinline__ void store2(float* p, const uint64_t* v) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm("mov.b64 {%0, %1}, %2;" : "=f"(f[2 * e]), "=f"(f[2 * e + 1]) : "l"(v[e]));
+    store(p, f);
   }
   static __device__ __forceinline__ void store(float* p, const float* f) {
     reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);

@@ -172,7 +172,8 @@ def norm_rope_backward(xs, gs, ws, eps: float, rope, start: int, want_dw):
         sides += (None, None, None, None, 0, None, None, None)
     scratch = None
     if any(want_dw):
-        scratch = x.new_empty((_scratch("bsa_norm_rope_backward_scratch_bytes", x.get_device(), D),), dtype=torch.uint8)
+        scratch = x.new_empty((_scratch("bsa_norm_rope_backward_scratch_bytes", x.get_device(), x.shape[1],
+                                       xs[1].shape[1] if len(xs) > 1 else 0, D),), dtype=torch.uint8)
     _call("bsa_norm_rope_backward", x.get_device(), *sides, _native.DTYPE_CODES[x.dtype], wcode, B, S, D, eps,
           *_rope_args(rope, start), _ptr(scratch))
     return dxs, dws

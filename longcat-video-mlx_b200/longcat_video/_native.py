@@ -75,7 +75,7 @@ _SIGNATURES = {
                             _f, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp, _c_i64p, _i, _vp],
                            _i),
     "bsa_norm_rope": ([_vp, _vp, _i, _vp, _vp] * 2 + [_i, _i, _i, _i, _i, _f] + _c_rope + [_vp], _i),
-    "bsa_norm_rope_backward_scratch_bytes": ([_i], ctypes.c_int64),
+    "bsa_norm_rope_backward_scratch_bytes": ([_i, _i, _i], ctypes.c_int64),
     "bsa_norm_rope_backward": ([_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp] * 2 + [_i, _i, _i, _i, _i, _f] + _c_rope
                                + [_vp, _vp], _i),
     "bsa_attention_ranges": ([_vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp], _i),
