@@ -258,7 +258,7 @@ int bsa_masked_attention_backward(const void* q, const void* k, const void* v, c
  * Rows behind the last token keep what they hold.
  * bsa_kv8_unpack: held tokens, then n fresh ones, then zeros, as [B, Hk, rows, D] in dtype.
  * bsa_kv8_attention: q [B, H, Sq, D] over the held tokens, straight from the codes; causal: query i sees
- * lengths[b] - Sq + i + 1 tokens.  Meant for few rows (H / Hk * Sq up to about 64): 16 rows are one pass over the
+ * lengths[b] - Sq + i + 1 tokens.  Meant for few rows (H / Hk * Sq up to about 128): 16 rows are one pass over the
  * codes.  scratch: bsa_kv8_attention_scratch_bytes() bytes (0: none needed). */
 int bsa_kv8_append(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
                    int capacity, int D, const void* k, const void* v, int dtype, int n, const int64_t* k_strides,

@@ -63,6 +63,7 @@ int launch_ranges(const RangesArgs& a, cudaStream_t stream);
 
 // ------------------------------------------------------------------ 8-bit cache
 constexpr int kCacheBlock = 64;        // tokens that share a scale
+constexpr int kMostSplits = 256;       // of the few-row attention along the tokens
 struct CacheView {
   uint8_t* k = nullptr;                // [B, Hk, cap, D] e4m3 codes, contiguous
   uint8_t* v = nullptr;
@@ -93,7 +94,7 @@ struct CacheAttnArgs {
   Tensor4 o;
   int dtype = 0, H = 0, Sq = 0, causal = 0, splits = 1;
   float sm_scale = 1.f;
-  float* part = nullptr;               // splits > 1: [splits][B * H * Sq][D + 2]
+  float* part = nullptr;               // splits > 1: [splits][B * H * Sq] rows of D + 2
 };
 int launch_cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
 int cache_device_error(int clear);

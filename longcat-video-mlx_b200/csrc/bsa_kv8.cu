@@ -218,6 +218,9 @@ constexpr int kSlotBytes = kCacheBlock * kRowBytes;  // K or V of one block
 constexpr int kSlots = 3;
 constexpr int kAttnSmem = kWarps * kSlots * kSlotBytes;
 
+__device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
 struct AttnParams {
   CacheView c;
   const void* q;
@@ -226,7 +229,8 @@ struct AttnParams {
   long long ob, oh, os;
   int H, G, Sq, rows, row_tiles, splits, causal;
   float scale_log2;
-  float* part;  // [splits][B * H * Sq][D + 2]
+  long long total;  // B * H * Sq
+  float* part;      // splits > 1: [splits][total][D] sums, then [splits][total][2] of (maximum, sum)
 };
 
 // 16-byte chunk `chunk` of token row `r`, exchanged by the row's low bits: the fragments below read one
@@ -235,25 +239,60 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int chunk) {
   return static_cast<uint32_t>(r * kRowBytes + ((chunk ^ (r & 7)) << 4));
 }
 
-// The codes of block `blk` (64 token rows of D bytes) into a slot; rows from `held` on arrive as zeros.
-template <int kPiece>
-__device__ __forceinline__ void load_block(uint8_t* slot, const uint8_t* src, int D, int first, int held, int lane) {
-  const int pieces = D / kPiece;
+// The codes of a block (64 token rows of D bytes, `held` of them of tokens) into a slot; the rows behind arrive as
+// zeros.  kPieces: D / kPiece where it is known (D = 128: a lane keeps its column and steps 4 rows), 0: as it comes.
+template <int kPiece, int kPieces>
+__device__ __forceinline__ void load_block(uint8_t* slot, const uint8_t* src, int D, int held, int lane) {
   const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
-  for (int j = lane; j < kCacheBlock * pieces; j += 32) {
-    const int r = j / pieces, c = j - r * pieces;
-    const int byte = c * kPiece;
-    const uint32_t dst = base + chunk_at(r, byte >> 4) + (byte & 15);
-    const int bytes = first + r < held ? kPiece : 0;
-    const uint8_t* from = src + (bytes ? static_cast<long long>(r) * D + byte : 0);
+  auto copy = [&](uint32_t dst, const uint8_t* from, bool token) {
+    const int bytes = token ? kPiece : 0;
     if constexpr (kPiece == 16)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
     else
       asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+  };
+  if constexpr (kPieces == 8) {
+    const int r = lane >> 3, c = lane & 7;
+    const uint8_t* from = src + lane * 16;
+    const uint32_t even = base + chunk_at(r, c), odd = base + chunk_at(r + 4, c);
+    if (held >= kCacheBlock) {
+#pragma unroll
+      for (int i = 0; i < kCacheBlock / 8; ++i) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(even + i * 8 * kRowBytes), "l"(from + i * 1024)
+                     : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(odd + i * 8 * kRowBytes), "l"(from + i * 1024 + 512)
+                     : "memory");
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCacheBlock / 8; ++i) {
+        copy(even + i * 8 * kRowBytes, from + i * 1024, 8 * i + r < held);
+        copy(odd + i * 8 * kRowBytes, from + i * 1024 + 512, 8 * i + 4 + r < held);
+      }
+    }
+  } else {
+    const int pieces = D / kPiece;
+    int r = lane / pieces, c = lane - r * pieces;
+    const int dr = 32 / pieces, dc = 32 - dr * pieces;
+    for (; r < kCacheBlock;) {
+      const int byte = c * kPiece;
+      copy(base + chunk_at(r, byte >> 4) + (byte & 15), src + r * D + byte, r < held);
+      r += dr;
+      c += dc;
+      if (c >= pieces) {
+        c -= pieces;
+        ++r;
+      }
+    }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -262,7 +301,7 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
 }
 __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int sel) { return __byte_perm(a, b, sel); }
 
-template <typename T>
+template <typename T, bool kFull>  // kFull: D = 128
 __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float st_m[kWarps][16], st_l[kWarps][16];
@@ -272,9 +311,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
   const int r0 = (blockIdx.y - bh * p.row_tiles) * 16;
   const int b = bh / p.c.Hk, hk = bh - b * p.c.Hk;
   const int held = min(max(p.c.lengths[b], 0), p.c.cap);
-  const int D = p.c.D;
+  const int D = kFull ? 128 : p.c.D;
   uint8_t* ring = smem + warp * kSlots * kSlotBytes;
-  if (D < 128) {  // columns behind D stay zero: the copies never write them
+  if (!kFull) {  // columns behind D stay zero: the copies never write them
     for (int i = threadIdx.x * 16; i < kAttnSmem; i += kAttnThreads * 16)
       *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
@@ -302,8 +341,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
     uint8_t* slot = ring + slot_load * kSlotBytes;
     if (k < blk_end) {
       const uint8_t* src = codes + static_cast<long long>(k) * kCacheBlock * D;
-      if (wide) load_block<16>(slot, src, D, k * kCacheBlock, held, lane);
-      else load_block<8>(slot, src, D, k * kCacheBlock, held, lane);
+      const int n = held - k * kCacheBlock;
+      if (kFull) load_block<16, 8>(slot, src, D, n, lane);
+      else if (wide) load_block<16, 0>(slot, src, D, n, lane);
+      else load_block<8, 0>(slot, src, D, n, lane);
     } else {
       asm volatile("cp.async.commit_group;" ::: "memory");  // empty: the group count stays in step
     }
@@ -356,6 +397,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   int slot = 0;
   for (; blk < blk_end; blk += kWarps) {
+    const float kscale = ksc[blk], vscale = vsc[blk];
     fetch(kc, blk + kWarps);  // into the slot of the last V read
     asm volatile("cp.async.wait_group 2;" ::: "memory");
     __syncwarp();
@@ -376,7 +418,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
                   e4m3x2_to_f16x2(static_cast<uint16_t>(w[x] >> 16)));
       }
     }
-    const float kscale = ksc[blk], vscale = vsc[blk];
     const int key0 = blk * kCacheBlock + 2 * c;
     float alpha[2];
 #pragma unroll
@@ -395,7 +436,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float mn = fmaxf(m[hf], mx);
       const float base = mn == -INFINITY ? 0.f : mn;
-      alpha[hf] = exp2f(m[hf] - base);
+      alpha[hf] = ex2(m[hf] - base);
       m[hf] = mn;
       float sum = 0.f;
 #pragma unroll
@@ -403,7 +444,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& v = s[t][2 * hf + e];
-          v = exp2f(v - base);
+          v = ex2(v - base);
           sum += v;
         }
       l[hf] = l[hf] * alpha[hf] + sum;
@@ -487,7 +528,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
   float f[kWarps], ll = 0.f;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    f[w] = exp2f(st_m[w][r] - base);
+    f[w] = ex2(st_m[w][r] - base);
     ll += f[w] * st_l[w][r];
   }
   const int head = (r0 + r) / p.Sq, tok = (r0 + r) - head * p.Sq;
@@ -495,12 +536,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
   const float inv = p.splits > 1 ? 1.f : (ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll));
   float* part = nullptr;
   if (p.splits > 1) {
-    const long long row = (static_cast<long long>(b) * p.H + h) * p.Sq + tok;
-    part = p.part + (static_cast<long long>(blockIdx.x) * p.c.B * p.H * p.Sq + row) * (D + 2);
-    if (threadIdx.x % tpr == 0) {
-      part[0] = mm;
-      part[1] = ll;
-    }
+    const long long row = blockIdx.x * p.total + (static_cast<long long>(b) * p.H + h) * p.Sq + tok;
+    part = p.part + row * D;
+    if (threadIdx.x % tpr == 0)
+      reinterpret_cast<float2*>(p.part + p.splits * p.total * D)[row] = make_float2(mm, ll);
   }
   T* out = static_cast<T*>(p.o) + b * p.ob + h * p.oh + tok * p.os;
   for (int d0 = 8 * (threadIdx.x % tpr); d0 < D; d0 += 8 * tpr) {
@@ -514,43 +553,50 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
       v[e] *= inv;
     }
     if (part) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) part[2 + d0 + e] = v[e];
+      reinterpret_cast<float4*>(part + d0)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(part + d0)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
       Row8<T>::store(out + d0, v);
     }
   }
 }
 
-// Joins the splits of a row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, always in the splits' order.
+// Joins the splits of a row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, always in the splits' order.  A CTA a row: a
+// thread holds a column, and the splits' weights are worked out once.
 template <typename T>
 __global__ void __launch_bounds__(128) cache_join_kernel(const AttnParams p) {
-  const int lanes = 16;
-  const long long rows = static_cast<long long>(p.c.B) * p.H * p.Sq;
-  const long long row = static_cast<long long>(blockIdx.x) * (128 / lanes) + threadIdx.x / lanes;
-  const int d0 = 8 * (threadIdx.x % lanes);
-  const int D = p.c.D;
-  if (row >= rows || d0 >= D) return;
-  const long long step = rows * (D + 2);
-  const float* src = p.part + row * (D + 2);
-  float mm = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, src[s * step]);
-  const float base = mm == -INFINITY ? 0.f : mm;
-  float l = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = exp2f(src[s * step] - base);
-    l = fmaf(f, src[s * step + 1], l);
+  __shared__ float weight[kMostSplits];
+  const long long row = blockIdx.x;
+  const int D = p.c.D, d = threadIdx.x;
+  if (threadIdx.x < 32) {
+    const float2* ml = reinterpret_cast<const float2*>(p.part + p.splits * p.total * D) + row;
+    float m = -INFINITY;
+    for (int s = threadIdx.x; s < p.splits; s += 32) m = fmaxf(m, ml[s * p.total].x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fmaf(f, src[s * step + 2 + d0 + e], v[e]);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int s = threadIdx.x; s < p.splits; s += 32) {
+      const float2 v = ml[s * p.total];
+      const float f = ex2(v.x - base);
+      weight[s] = f;
+      l = fmaf(f, v.y, l);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    for (int s = threadIdx.x; s < p.splits; s += 32) weight[s] *= inv;
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] *= inv;
+  __syncthreads();
+  if (d >= D) return;
+  const float* src = p.part + row * D + d;
+  float v = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < p.splits; ++s) v = fmaf(weight[s], src[s * p.total * D], v);
   const int tok = static_cast<int>(row % p.Sq);
   const long long bh = row / p.Sq;
   const int h = static_cast<int>(bh % p.H);
-  const long long b = bh / p.H;
-  Row8<T>::store(static_cast<T*>(p.o) + b * p.ob + h * p.oh + tok * p.os + d0, v);
+  store1(static_cast<T*>(p.o) + (bh / p.H) * p.ob + h * p.oh + tok * p.os + d, v);
 }
 
 template <typename T>
@@ -568,14 +614,13 @@ int attention(const CacheAttnArgs& a, cudaStream_t stream) {
   p.causal = a.causal;
   p.scale_log2 = a.sm_scale * 1.4426950408889634f;
   p.part = a.part;
-  if (cudaFuncSetAttribute(cache_attn_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem) != cudaSuccess)
+  p.total = static_cast<long long>(a.c.B) * a.H * a.Sq;
+  auto* kernel = a.c.D == 128 ? cache_attn_kernel<T, true> : cache_attn_kernel<T, false>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem) != cudaSuccess)
     return BSA_ERR_CUDA;
-  cache_attn_kernel<T><<<dim3(a.splits, a.c.B * a.c.Hk * p.row_tiles), kAttnThreads, kAttnSmem, stream>>>(p);
+  kernel<<<dim3(a.splits, a.c.B * a.c.Hk * p.row_tiles), kAttnThreads, kAttnSmem, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return BSA_ERR_CUDA;
-  if (a.splits > 1) {
-    const long long rows = static_cast<long long>(a.c.B) * a.H * a.Sq;
-    cache_join_kernel<T><<<static_cast<int>((rows + 7) / 8), 128, 0, stream>>>(p);
-  }
+  if (a.splits > 1) cache_join_kernel<T><<<static_cast<int>(p.total), 128, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
 }
 

@@ -19,8 +19,9 @@ __all__ = ["KVCache8"]
 BLOCK = _dense.CACHE_BLOCK
 
 # Most rows (query heads of a key head x query tokens) that read the codes directly, 16 to a pass; above, the
-# cache is unpacked to 16 bits once and the tile kernel runs.
-FEW_ROWS = 64
+# cache is unpacked to 16 bits once and the tile kernel runs.  On one B200, codes against unpacked: 1 x 8 heads x
+# 4,096 tokens, 128 rows 29 and 46 us, 256 rows 48 and 45; 8 x 8 x 8,192, 128 rows 169 and 255, 256 rows 285 and 255.
+FEW_ROWS = 128
 
 
 class KVCache8:
