@@ -82,6 +82,8 @@ struct AppendParams {
 
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+  after_previous();
+  let_next_start();
   const int bh = blockIdx.y;
   const int b = bh / p.c.Hk, h = bh - b * p.c.Hk;
   const int which = blockIdx.z;
@@ -105,31 +107,47 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   float* sp = (which ? p.c.vs : p.c.ks) + static_cast<long long>(bh) * nblk + blk;
   const T* x = static_cast<const T*>(p.x[which]) + b * p.sb[which] + h * p.sh[which] + 8 * col;
   Row8<T> v[kCacheBlock / per];
-  float amax = 0.f;
+  uint32_t top = 0u;  // largest magnitude bits of the low and the high halves: their order is the values' order
 #pragma unroll
   for (int i = 0; i < kCacheBlock / per; ++i) {
     const int t = t0 + row0 + i * per - held;  // place among the new tokens
     if (live && t >= 0 && t < n) {
       v[i].load(x + static_cast<long long>(t) * p.ss[which]);
-      float f[8];
-      v[i].get(f);
+      const uint32_t w[4] = {v[i].u.x, v[i].u.y, v[i].u.z, v[i].u.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(f[e]);
-        if (a <= 3.4028235e38f) amax = fmaxf(amax, a);  // neither infinity nor NaN sets a scale
-      }
+      for (int e = 0; e < 4; ++e) top = __vmaxu2(top, w[e] & 0x7fff7fffu);
     } else {
       v[i].zero();
     }
   }
-  __shared__ float red[kAppendThreads / 32];
+  __shared__ uint32_t red[2][kAppendThreads / 32];
+  constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  auto block_max = [&](uint32_t m, int k) {
+    uint32_t one = max(m & 0xffffu, m >> 16);
+    one = __reduce_max_sync(0xffffffffu, one);
+    if ((threadIdx.x & 31) == 0) red[k][threadIdx.x >> 5] = one;
+    __syncthreads();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    for (int i = 0; i < kAppendThreads / 32; ++i) one = max(one, red[k][i]);
+    return one;
+  };
   const float was = *sp;
-  __syncthreads();
+  uint32_t largest = block_max(top, 0);
+  if (largest >= kInf) {  // neither infinity nor NaN sets a scale: once more without them
+    top = 0u;
 #pragma unroll
-  for (int k = 0; k < kAppendThreads / 32; ++k) amax = fmaxf(amax, red[k]);
+    for (int i = 0; i < kCacheBlock / per; ++i) {
+      const uint32_t w[4] = {v[i].u.x, v[i].u.y, v[i].u.z, v[i].u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
+        top = max(top, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+      }
+    }
+    largest = block_max(top, 1);
+  }
+  float amax, none;
+  unpack_pair(largest, amax, none, T());
   const float old = t0 < held ? was : 0.f;     // a block without tokens has no scale to keep
   const float s = fmaxf(old, scale_of(amax));
   const float inv = inverse_of(s);
@@ -155,6 +173,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 
 // lengths[b] += what append_kernel wrote; a launch of its own, since every CTA above reads the old lengths
 __global__ void advance_kernel(int32_t* lengths, const int32_t* counts, int n, int cap, int B) {
+  after_previous();
   for (int b = threadIdx.x; b < B; b += blockDim.x) {
     const int held = lengths[b];
     const int add = counts ? min(max(counts[b], 0), n) : n;
@@ -303,6 +322,8 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int sel) {
 
 template <typename T, bool kFull>  // kFull: D = 128
 __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnParams p) {
+  after_previous();
+  let_next_start();
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float st_m[kWarps][16], st_l[kWarps][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -566,6 +587,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
 template <typename T>
 __global__ void __launch_bounds__(128) cache_join_kernel(const AttnParams p) {
   __shared__ float weight[kMostSplits];
+  after_previous();
   const long long row = blockIdx.x;
   const int D = p.c.D, d = threadIdx.x;
   if (threadIdx.x < 32) {
@@ -618,10 +640,13 @@ int attention(const CacheAttnArgs& a, cudaStream_t stream) {
   auto* kernel = a.c.D == 128 ? cache_attn_kernel<T, true> : cache_attn_kernel<T, false>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem) != cudaSuccess)
     return BSA_ERR_CUDA;
-  kernel<<<dim3(a.splits, a.c.B * a.c.Hk * p.row_tiles), kAttnThreads, kAttnSmem, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return BSA_ERR_CUDA;
-  if (a.splits > 1) cache_join_kernel<T><<<static_cast<int>(p.total), 128, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+  if (launch_behind(kernel, dim3(a.splits, a.c.B * a.c.Hk * p.row_tiles), dim3(kAttnThreads), kAttnSmem, stream, p) !=
+      cudaSuccess)
+    return BSA_ERR_CUDA;
+  if (a.splits > 1 && launch_behind(cache_join_kernel<T>, dim3(static_cast<unsigned>(p.total)), dim3(128), 0, stream, p) !=
+                          cudaSuccess)
+    return BSA_ERR_CUDA;
+  return BSA_OK;
 }
 
 template <typename P>
@@ -640,13 +665,12 @@ int launch_cache_append(const AppendArgs& a, cudaStream_t stream) {
   p.n = a.n;
   // n tokens from any place in a block touch at most this many blocks
   const dim3 grid((a.n + kCacheBlock - 2) / kCacheBlock + 1, a.c.B * a.c.Hk, 2);
-  if (a.dtype == BSA_DTYPE_F16)
-    kv8::append_kernel<__half><<<grid, kv8::kAppendThreads, 0, stream>>>(p);
-  else
-    kv8::append_kernel<__nv_bfloat16><<<grid, kv8::kAppendThreads, 0, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return BSA_ERR_CUDA;
-  kv8::advance_kernel<<<1, 128, 0, stream>>>(a.c.lengths, a.counts, a.n, a.c.cap, a.c.B);
-  return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+  auto* kernel = a.dtype == BSA_DTYPE_F16 ? kv8::append_kernel<__half> : kv8::append_kernel<__nv_bfloat16>;
+  if (launch_behind(kernel, grid, dim3(kv8::kAppendThreads), 0, stream, p) != cudaSuccess ||
+      launch_behind(kv8::advance_kernel, dim3(1), dim3(128), 0, stream, a.c.lengths, a.counts, a.n, a.c.cap, a.c.B) !=
+          cudaSuccess)
+    return BSA_ERR_CUDA;
+  return BSA_OK;
 }
 
 int launch_cache_unpack(const UnpackArgs& a, cudaStream_t stream) {

@@ -24,6 +24,7 @@ struct Params {
 };
 
 __global__ void __launch_bounds__(kTile) ranges_kernel(const Params p) {
+  let_next_start();
   const int b = blockIdx.x / p.tiles;
   const int tile = blockIdx.x - b * p.tiles;
   const int i = tile * kTile + threadIdx.x;

@@ -1,0 +1,545 @@
+// Python binding of the C ABI's dense side: q/k norm with rotary positions, attention over key intervals, and the
+// 8-bit key/value cache.  Checks of tensors, allocation of outputs and scratch, and the call on the tensors' device
+// and its current stream, in C++: at a few tokens these calls are shorter than the same steps in Python
+// (norm and rope of 390 tokens 20 us, a lookup 16 us of host time there).
+//
+// The entries are looked up in the engine's library, which Python has loaded; errors of the C ABI come back as
+// ValueError (arguments) or BSAError, with its message.
+#include <dlfcn.h>
+#include <cmath>
+#include <mutex>
+#include <optional>
+#include <string>
+#include <torch/extension.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include "../../include/bsa_b200.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+namespace py = pybind11;
+
+struct Api {
+#define ENTRY(name) decltype(&::name) name = nullptr
+  ENTRY(bsa_last_error);
+  ENTRY(bsa_norm_rope);
+  ENTRY(bsa_norm_rope_backward_scratch_bytes);
+  ENTRY(bsa_norm_rope_backward);
+  ENTRY(bsa_attention_ranges);
+  ENTRY(bsa_masked_attention_scratch_bytes);
+  ENTRY(bsa_masked_attention);
+  ENTRY(bsa_masked_attention_backward_scratch_bytes);
+  ENTRY(bsa_masked_attention_backward);
+  ENTRY(bsa_kv8_append);
+  ENTRY(bsa_kv8_unpack);
+  ENTRY(bsa_kv8_attention_scratch_bytes);
+  ENTRY(bsa_kv8_attention);
+#undef ENTRY
+} api;
+
+PyObject* cuda_error = nullptr;  // BSAError, kept for the life of the process
+
+void load(const std::string& path, const py::object& error) {
+  cuda_error = py::object(error).release().ptr();
+  void* lib = dlopen(path.c_str(), RTLD_NOW);
+  if (!lib) throw std::runtime_error("cannot load " + path + ": " + dlerror());
+#define ENTRY(name)                                                                        \
+  api.name = reinterpret_cast<decltype(api.name)>(dlsym(lib, #name));                       \
+  if (!api.name) throw std::runtime_error(std::string("missing entry ") + #name)
+  ENTRY(bsa_last_error);
+  ENTRY(bsa_norm_rope);
+  ENTRY(bsa_norm_rope_backward_scratch_bytes);
+  ENTRY(bsa_norm_rope_backward);
+  ENTRY(bsa_attention_ranges);
+  ENTRY(bsa_masked_attention_scratch_bytes);
+  ENTRY(bsa_masked_attention);
+  ENTRY(bsa_masked_attention_backward_scratch_bytes);
+  ENTRY(bsa_masked_attention_backward);
+  ENTRY(bsa_kv8_append);
+  ENTRY(bsa_kv8_unpack);
+  ENTRY(bsa_kv8_attention_scratch_bytes);
+  ENTRY(bsa_kv8_attention);
+#undef ENTRY
+}
+
+[[noreturn]] void refuse(const std::string& what) { throw py::value_error(what); }
+
+void check(int rc, const char* what) {
+  if (rc == BSA_OK) return;
+  char buf[512] = {0};
+  api.bsa_last_error(buf, sizeof(buf));
+  const std::string msg = buf[0] ? buf : std::string(what) + " failed";
+  if (rc == BSA_ERR_SHAPE || rc == BSA_ERR_DTYPE || rc == BSA_ERR_ALIGN || rc == BSA_ERR_ARG) refuse(msg);
+  PyErr_SetString(cuda_error, (std::string(what) + " failed (code " + std::to_string(rc) + "): " + msg).c_str());
+  throw py::error_already_set();
+}
+
+int dtype_code(at::ScalarType t) {
+  if (t == at::kBFloat16) return BSA_DTYPE_BF16;
+  if (t == at::kHalf) return BSA_DTYPE_F16;
+  if (t == at::kFloat) return BSA_DTYPE_F32;
+  refuse(std::string("unsupported dtype ") + c10::toString(t));
+}
+
+void on_cuda(const Tensor& t) {
+  if (!t.is_cuda()) refuse("BSA engine inputs must be CUDA tensors (there is no CPU path)");
+}
+void same_place(const Tensor& a, const Tensor& t) {
+  on_cuda(t);
+  if (t.device() != a.device()) refuse("all tensors must be on one device");
+}
+void same_place(const Tensor& a, const OptTensor& t) {
+  if (t) same_place(a, *t);
+}
+
+void* ptr(const Tensor& t) { return t.data_ptr(); }
+void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
+
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+std::string shape_text(at::IntArrayRef s) {
+  std::string r = "[";
+  for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
+  return r + "]";
+}
+
+bool readable(const Tensor& t) {
+  const int64_t unit = 16 / t.element_size();
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) return false;
+  if (t.stride(3) != 1 && t.size(3) > 1) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && (t.stride(i) % unit || t.stride(i) <= 0)) return false;
+  return true;
+}
+
+// A [B, H, S, D] tensor that the kernels read in place, else a contiguous copy.  In place: d contiguous, base and strides
+// in multiples of 16 bytes, nothing broadcast; any order and gaps of batch, heads and tokens otherwise.
+struct View {
+  Tensor t;
+  int64_t strides[3];
+  explicit View(const Tensor& given) : t(readable(given) ? given : given.clone(at::MemoryFormat::Contiguous)) {
+    for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
+  }
+  void* p() const { return t.data_ptr(); }
+};
+
+Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
+Tensor bytes(const Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
+
+// ------------------------------------------------------------------------------- q/k norm + rotary positions
+struct Rope {
+  OptTensor tables;
+  int dt, dh, dw, T, H, W, start;
+  const float* p() const { return tables ? static_cast<const float*>(tables->data_ptr()) : nullptr; }
+  void check(const Tensor& x) const {
+    if (!tables) return;
+    same_place(x, tables);
+    if (tables->scalar_type() != at::kFloat || !tables->is_contiguous()) refuse("rope tables must be contiguous fp32");
+    if (tables->numel() != int64_t(T) * dt + int64_t(H) * dh + int64_t(W) * dw)
+      refuse("rope tables of " + std::to_string(tables->numel()) + " values do not match their grid and dims");
+  }
+};
+
+void check_pair(const Tensor& q, const OptTensor& k) {
+  on_cuda(q);
+  dtype_code(q.scalar_type());
+  if (q.dim() != 4) refuse("expected tensors of shape [B, H, S, D]");
+  if (k) {
+    same_place(q, *k);
+    if (k->scalar_type() != q.scalar_type() || k->dim() != 4 || k->size(0) != q.size(0) || k->size(2) != q.size(2) ||
+        k->size(3) != q.size(3))
+      refuse("q and k must share dtype, batch, length and head_dim");
+  }
+}
+
+// Contiguous weights of one type: fp32 or the input's are read as they are, others as fp32.
+int weights(const Tensor& q, OptTensor& wq, OptTensor& wk) {
+  at::ScalarType kind = at::kFloat;
+  bool one = true, any = false;
+  for (OptTensor* w : {&wq, &wk})
+    if (*w) {
+      same_place(q, **w);
+      if ((*w)->dim() != 1 || (*w)->size(0) != q.size(3)) refuse("norm weight must be [" + std::to_string(q.size(3)) + "]");
+      const at::ScalarType t = (*w)->scalar_type();
+      one = one && (t == at::kFloat || t == q.scalar_type()) && (!any || t == kind) && (*w)->is_contiguous();
+      kind = t;
+      any = true;
+    }
+  if (!one) {
+    for (OptTensor* w : {&wq, &wk})
+      if (*w) *w = (*w)->to(at::kFloat).contiguous();
+    kind = at::kFloat;
+  }
+  return dtype_code(kind);
+}
+
+py::object norm_rope(const Tensor& q, const OptTensor& k, OptTensor wq, OptTensor wk, double eps, OptTensor tables, int dt,
+                     int dh, int dw, int T, int H, int W, int start) {
+  check_pair(q, k);
+  const Rope rope{std::move(tables), dt, dh, dw, T, H, W, start};
+  rope.check(q);
+  const int wcode = weights(q, wq, wk);
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor y0 = like(q);
+  OptTensor y1;
+  if (k) y1 = like(*k);
+  if (q.numel() && (!k || k->numel())) {
+    const View x0(q);
+    std::optional<View> x1;
+    if (k) x1.emplace(*k);
+    check(api.bsa_norm_rope(x0.p(), x0.strides, q.size(1), ptr(wq), ptr(y0), x1 ? x1->p() : nullptr,
+                            x1 ? x1->strides : nullptr, k ? k->size(1) : 0, ptr(wk), ptr(y1), dtype_code(q.scalar_type()),
+                            wcode, q.size(0), q.size(2), q.size(3), static_cast<float>(eps), rope.p(), dt, dh, dw, T, H, W,
+                            start, stream_of(q)),
+          "bsa_norm_rope");
+  }
+  return k ? py::object(py::make_tuple(y0, *y1)) : py::cast(y0);
+}
+
+// One or two sides (x, gradient, weight, whether its weight's gradient is wanted): [dx0, dw0, dx1, dw1]
+std::vector<OptTensor> norm_rope_backward(const Tensor& x0, const Tensor& g0, OptTensor w0, bool want0, const OptTensor& x1,
+                                          const OptTensor& g1, OptTensor w1, bool want1, double eps, OptTensor tables,
+                                          int dt, int dh, int dw, int T, int H, int W, int start) {
+  const Rope rope{std::move(tables), dt, dh, dw, T, H, W, start};
+  const int wcode = weights(x0, w0, w1);
+  const c10::cuda::CUDAGuard guard(x0.device());
+  const int64_t D = x0.size(3);
+  Tensor dx0 = like(x0);
+  OptTensor dx1, dw0, dw1, scratch;
+  if (x1) dx1 = like(*x1);
+  const bool empty = !x0.numel() || (x1 && !x1->numel());
+  auto grad = [&] {
+    return empty ? at::zeros({D}, x0.options().dtype(at::kFloat)) : at::empty({D}, x0.options().dtype(at::kFloat));
+  };
+  if (want0) dw0 = grad();
+  if (want1) dw1 = grad();
+  if (!empty) {
+    if (want0 || want1)
+      scratch = bytes(x0, api.bsa_norm_rope_backward_scratch_bytes(x0.size(1), x1 ? x1->size(1) : 0, D));
+    const View a(x0), ga(g0);
+    std::optional<View> b, gb;
+    if (x1) {
+      b.emplace(*x1);
+      gb.emplace(*g1);
+    }
+    check(api.bsa_norm_rope_backward(
+              a.p(), a.strides, ga.p(), ga.strides, x0.size(1), ptr(w0), ptr(dx0), static_cast<float*>(ptr(dw0)),
+              b ? b->p() : nullptr, b ? b->strides : nullptr, gb ? gb->p() : nullptr, gb ? gb->strides : nullptr,
+              x1 ? x1->size(1) : 0, ptr(w1), ptr(dx1), static_cast<float*>(ptr(dw1)), dtype_code(x0.scalar_type()), wcode,
+              x0.size(0), x0.size(2), D, static_cast<float>(eps), rope.p(), dt, dh, dw, T, H, W, start, ptr(scratch),
+              stream_of(x0)),
+          "bsa_norm_rope_backward");
+  }
+  return {dx0, dw0, dx1, dw1};
+}
+
+// ------------------------------------------------------------------------------------------- key intervals
+const int32_t* i32(const Tensor& place, OptTensor& t, const char* name, int64_t n) {
+  if (!t) return nullptr;
+  same_place(place, *t);
+  if (t->scalar_type() != at::kInt) refuse(std::string(name) + " must be int32");
+  if (n >= 0 && t->numel() != n) refuse(std::string(name) + " must have " + std::to_string(n) + " values");
+  t = t->contiguous();
+  return static_cast<const int32_t*>(t->data_ptr());
+}
+
+// (buffer, batch entries, places of the table in the buffer): the intervals and, on 16 bytes, their tile table
+py::tuple attention_ranges(const py::object& device, int64_t Sq, int64_t Sk, int64_t batch, OptTensor given, bool causal,
+                           int64_t prefix, OptTensor prefixes, OptTensor q_offsets, OptTensor k_offsets,
+                           OptTensor q_lengths, OptTensor k_lengths, int64_t k_add) {
+  if (Sq < 0 || Sk < 0 || Sq > INT32_MAX || Sk > INT32_MAX) refuse("lengths must be >= 0 and fit 32 bits");
+  if (prefix < 0) refuse("prefix must be >= 0");
+  if (q_offsets.has_value() != k_offsets.has_value()) refuse("q_offsets and k_offsets come together");
+  if (q_offsets && (q_lengths || k_lengths)) refuse("give documents or lengths, not both");
+  int64_t n = -1;
+  if (q_offsets) {
+    if (q_offsets->dim() != 1 || k_offsets->dim() != 1 || q_offsets->numel() != k_offsets->numel() || q_offsets->numel() < 2)
+      refuse("q_offsets and k_offsets must be [documents + 1]");
+    n = q_offsets->numel() - 1;
+  }
+  for (const OptTensor* t : {&q_lengths, &k_lengths})
+    if (*t) {
+      if ((*t)->dim() != 1 || (n >= 0 && (*t)->numel() != n)) refuse("lengths must be [B]");
+      batch = n = (*t)->numel();
+    }
+  if (prefixes && n < 0) batch = n = prefixes->numel();
+  if (prefixes && prefixes->dim() != 1) refuse("prefix must be one number or one for each document or entry");
+  c10::Device dev(c10::kCUDA, -1);
+  for (const OptTensor* t : {&given, &prefixes, &q_offsets, &q_lengths, &k_lengths})
+    if (*t && device.is_none()) {
+      on_cuda(**t);
+      dev = (*t)->device();
+    }
+  if (!device.is_none()) dev = py::cast<c10::Device>(device);
+  if (!dev.is_cuda()) refuse("BSA engine inputs must be CUDA tensors (there is no CPU path)");
+  if (!dev.has_index()) dev.set_index(c10::cuda::current_device());
+  const c10::cuda::CUDAGuard guard(dev);
+  const int64_t at0 = (batch * Sq * 2 + 3) & ~int64_t(3);
+  const Tensor buf = at::empty({at0 + batch * ((Sq + 127) / 128) * 4}, at::TensorOptions().device(dev).dtype(at::kInt));
+  const int32_t* g = i32(buf, given, "ranges", -1);
+  if (g && reinterpret_cast<uintptr_t>(g) & 7) {
+    given = given->clone();
+    g = static_cast<const int32_t*>(given->data_ptr());
+  }
+  const int32_t* pre = i32(buf, prefixes, "prefix", n);
+  const int32_t* qo = i32(buf, q_offsets, "q_offsets", -1);
+  const int32_t* ko = i32(buf, k_offsets, "k_offsets", -1);
+  const int32_t* ql = i32(buf, q_lengths, "q_lengths", -1);
+  const int32_t* kl = i32(buf, k_lengths, "k_lengths", -1);
+  if (batch * Sq) {
+    int32_t* r = static_cast<int32_t*>(buf.data_ptr());
+    check(api.bsa_attention_ranges(r, r + at0, batch, Sq, Sk, g, causal, prefix, pre, qo, ko, qo ? n : 0, ql, kl, k_add,
+                                   stream_of(buf)),
+          "bsa_attention_ranges");
+  }
+  return py::make_tuple(buf, batch, at0);
+}
+
+struct Mask {
+  const int32_t *ranges = nullptr, *table = nullptr;
+  int64_t batch = 1;
+  Mask(const Tensor& q, const OptTensor& buf, int64_t batch_, int64_t at0) {
+    if (!buf) return;
+    same_place(q, *buf);
+    if (batch_ != 1 && batch_ != q.size(0))
+      refuse("the mask has " + std::to_string(batch_) + " batch entries, q has " + std::to_string(q.size(0)));
+    ranges = static_cast<const int32_t*>(buf->data_ptr());
+    table = ranges + at0;
+    batch = batch_;
+  }
+};
+
+// ------------------------------------------------------------------------------------------ dense attention
+void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
+  on_cuda(q);
+  same_place(q, k);
+  same_place(q, v);
+  if (q.dim() != 4 || k.dim() != 4) refuse("q, k and v must be [B, H, S, D]");
+  if (k.sizes() != v.sizes()) refuse("k and v must have the same shape");
+  const at::ScalarType t = q.scalar_type();
+  if (k.scalar_type() != t || v.scalar_type() != t) refuse("q, k, v must share one dtype");
+  if (t != at::kBFloat16 && t != at::kHalf) refuse(std::string("unsupported dtype ") + c10::toString(t) + " (bf16 or fp16)");
+  const int64_t D = q.size(3);
+  if (q.size(0) != k.size(0) || k.size(3) != D) refuse("q and k must share batch and head_dim");
+  if (D % 8 || D <= 0 || D > 128) refuse("head_dim D=" + std::to_string(D) + " must be a multiple of 8 and <= 128");
+  if (k.size(1) == 0 || q.size(1) % k.size(1))
+    refuse(std::to_string(q.size(1)) + " query heads are no multiple of " + std::to_string(k.size(1)) + " key heads");
+}
+
+void check_scale(double sm_scale, double softcap) {
+  if (!(sm_scale > 0) || std::isinf(sm_scale)) refuse("sm_scale must be positive and finite");
+  if (!(softcap >= 0) || std::isinf(softcap)) refuse("softcap must be finite and >= 0");
+}
+
+void check_out(const Tensor& q, const OptTensor& out) {
+  if (!out) return;
+  same_place(q, *out);
+  if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type()) refuse("out must have q's shape and dtype");
+}
+
+// The caller's output where the kernels can write it, else a new tensor that is copied there at the end.
+struct Output {
+  Tensor t;
+  bool copy;
+  int64_t strides[3];
+  Output(const Tensor& q, const OptTensor& out) : copy(out && !readable(*out)) {
+    t = out && !copy ? *out : like(q);
+    for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
+  }
+  Tensor done(const OptTensor& out) {
+    if (copy) out->copy_(t);
+    return out ? *out : t;
+  }
+};
+
+// (out, lse or None, rest or None)
+py::tuple masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, int64_t mask_batch,
+                           int64_t mask_table, int64_t mask_q, int64_t mask_k, double sm_scale, double softcap,
+                           const OptTensor& out, bool want_lse, bool want_rest) {
+  check_qkv(q, k, v);
+  check_scale(sm_scale, softcap);
+  const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
+  if (mask && (mask_q != Sq || mask_k != Sk))
+    refuse("the mask is for " + std::to_string(mask_q) + " queries and " + std::to_string(mask_k) + " keys, got " +
+           std::to_string(Sq) + " and " + std::to_string(Sk));
+  const Mask m(q, mask, mask_batch, mask_table);
+  check_out(q, out);
+  const c10::cuda::CUDAGuard guard(q.device());
+  Output o(q, out);
+  OptTensor lse, rest;
+  if (want_lse) lse = at::empty({B, H, Sq}, q.options().dtype(at::kFloat));
+  if (want_rest) rest = like(q);
+  if (q.numel() && Sk) {
+    const View a(q), b(k), c(v);
+    OptTensor scratch;
+    const int64_t n = api.bsa_masked_attention_scratch_bytes(B, H, Sq, Sk, D);
+    if (n) scratch = bytes(q, n);
+    check(api.bsa_masked_attention(a.p(), b.p(), c.p(), dtype_code(q.scalar_type()), B, H, Hk, Sq, Sk, D, a.strides,
+                                   b.strides, c.strides, m.ranges, m.table, m.batch, static_cast<float>(sm_scale),
+                                   static_cast<float>(softcap), ptr(o.t), o.strides, ptr(rest),
+                                   static_cast<float*>(ptr(lse)), ptr(scratch), stream_of(q)),
+          "bsa_masked_attention");
+  } else {  // no rows, or no keys: zeros
+    o.t.zero_();
+    if (rest) rest->zero_();
+    if (lse) lse->fill_(-INFINITY);
+  }
+  return py::make_tuple(o.done(out), lse, rest);
+}
+
+std::vector<OptTensor> masked_attention_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                                                 const Tensor& rest, const Tensor& lse, const Tensor& grad,
+                                                 const OptTensor& mask, int64_t mask_batch, int64_t mask_table,
+                                                 double sm_scale, double softcap, bool want_q, bool want_kv) {
+  const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
+  const Mask m(q, mask, mask_batch, mask_table);
+  const c10::cuda::CUDAGuard guard(q.device());
+  const bool empty = !q.numel() || !Sk;
+  auto grad_of = [&](const Tensor& t) { return empty ? at::zeros(t.sizes(), t.options()) : like(t); };
+  OptTensor dq, dk, dv;
+  if (want_q) dq = grad_of(q);
+  if (want_kv) {
+    dk = grad_of(k);
+    dv = grad_of(v);
+  }
+  if (!empty) {
+    const View a(q), b(k), c(v), o(out), g(grad);
+    const Tensor scratch = bytes(q, api.bsa_masked_attention_backward_scratch_bytes(B, H, Sq, m.ranges ? m.batch : 0));
+    check(api.bsa_masked_attention_backward(
+              a.p(), b.p(), c.p(), o.p(), ptr(rest), g.p(), static_cast<const float*>(ptr(lse)),
+              dtype_code(q.scalar_type()), B, H, Hk, Sq, Sk, D, a.strides, b.strides, c.strides, o.strides, g.strides,
+              m.ranges, m.table, m.batch, static_cast<float>(sm_scale), static_cast<float>(softcap), ptr(dq), ptr(dk),
+              ptr(dv), ptr(scratch), stream_of(q)),
+          "bsa_masked_attention_backward");
+  }
+  return {dq, dk, dv};
+}
+
+// ---------------------------------------------------------------------------------------------- 8-bit cache
+struct Cache {
+  Tensor kc, ks, vc, vs, len;
+  int64_t B, Hk, cap, D;
+
+  Cache(Tensor k_codes, Tensor k_scale, Tensor v_codes, Tensor v_scale, Tensor lengths)
+      : kc(std::move(k_codes)), ks(std::move(k_scale)), vc(std::move(v_codes)), vs(std::move(v_scale)),
+        len(std::move(lengths)) {
+    on_cuda(kc);
+    for (const Tensor* t : {&ks, &vc, &vs, &len}) same_place(kc, *t);
+    if (kc.dim() != 4 || kc.sizes() != vc.sizes()) refuse("codes must be [B, Hk, capacity, D]");
+    B = kc.size(0), Hk = kc.size(1), cap = kc.size(2), D = kc.size(3);
+    if (cap % 64 || cap == 0) refuse("capacity " + std::to_string(cap) + " must be a positive multiple of 64");
+    if (D % 8 || D <= 0 || D > 128) refuse("head_dim D=" + std::to_string(D) + " must be a multiple of 8 and <= 128");
+    for (const Tensor* t : {&kc, &vc})
+      if (t->scalar_type() != at::kFloat8_e4m3fn || !t->is_contiguous() || reinterpret_cast<uintptr_t>(t->data_ptr()) & 15)
+        refuse("codes must be contiguous, 16-byte aligned float8_e4m3fn");
+    for (const Tensor* t : {&ks, &vs})
+      if (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->dim() != 3 || t->size(0) != B || t->size(1) != Hk ||
+          t->size(2) != cap / 64)
+        refuse("scales must be contiguous fp32 " + shape_text({B, Hk, cap / 64}));
+    if (len.scalar_type() != at::kInt || !len.is_contiguous() || len.dim() != 1 || len.size(0) != B)
+      refuse("lengths must be contiguous int32 " + shape_text({B}));
+  }
+
+  float* scale(const Tensor& t) const { return static_cast<float*>(t.data_ptr()); }
+  int32_t* lengths() const { return static_cast<int32_t*>(len.data_ptr()); }
+
+  void check_kv(const Tensor& k, const Tensor& v) const {
+    same_place(kc, k);
+    same_place(kc, v);
+    if (k.dim() != 4 || k.sizes() != v.sizes() || k.size(0) != B || k.size(1) != Hk || k.size(3) != D)
+      refuse("k and v must be [" + std::to_string(B) + ", " + std::to_string(Hk) + ", n, " + std::to_string(D) + "]");
+    const at::ScalarType t = k.scalar_type();
+    if (t != v.scalar_type() || (t != at::kBFloat16 && t != at::kHalf)) refuse("k and v must both be bf16 or fp16");
+  }
+
+  void append(const Tensor& k, const Tensor& v, OptTensor counts) {
+    check_kv(k, v);
+    if (k.size(2) > cap) refuse(std::to_string(k.size(2)) + " tokens for a capacity of " + std::to_string(cap));
+    const int32_t* n = i32(kc, counts, "counts", B);
+    if (!k.numel()) return;
+    const c10::cuda::CUDAGuard guard(kc.device());
+    const View a(k), b(v);
+    check(api.bsa_kv8_append(ptr(kc), scale(ks), ptr(vc), scale(vs), lengths(), B, Hk, cap, D, a.p(), b.p(),
+                             dtype_code(k.scalar_type()), k.size(2), a.strides, b.strides, n, stream_of(kc)),
+          "bsa_kv8_append");
+  }
+
+  // (k, v) in 16 bits: the held tokens, the fresh ones, zeros up to capacity + fresh
+  std::pair<Tensor, Tensor> unpack(at::ScalarType dtype, const OptTensor& k, const OptTensor& v) {
+    if (dtype != at::kBFloat16 && dtype != at::kHalf) refuse("dequantize to bf16 or fp16");
+    const c10::cuda::CUDAGuard guard(kc.device());
+    const int64_t n = k ? k->size(2) : 0;
+    const auto opt = kc.options().dtype(dtype);
+    Tensor ko = at::empty({B, Hk, cap + n, D}, opt), vo = at::empty({B, Hk, cap + n, D}, opt);
+    std::optional<View> a, b;
+    if (n) {
+      a.emplace(*k);
+      b.emplace(*v);
+    }
+    check(api.bsa_kv8_unpack(ptr(kc), scale(ks), ptr(vc), scale(vs), lengths(), B, Hk, cap, D, a ? a->p() : nullptr,
+                             b ? b->p() : nullptr, dtype_code(dtype), n, a ? a->strides : nullptr,
+                             b ? b->strides : nullptr, ptr(ko), ptr(vo), cap + n, stream_of(kc)),
+          "bsa_kv8_unpack");
+    return {ko, vo};
+  }
+
+  Tensor attend(const Tensor& q, const OptTensor& k, const OptTensor& v, bool causal, std::optional<double> sm_scale,
+                const OptTensor& out, int64_t few_rows) {
+    same_place(kc, q);
+    if (q.dim() != 4 || q.size(0) != B || q.size(3) != D)
+      refuse("q must be [" + std::to_string(B) + ", H, Sq, " + std::to_string(D) + "]");
+    const int64_t H = q.size(1), Sq = q.size(2);
+    if (H % Hk) refuse(std::to_string(H) + " query heads are no multiple of " + std::to_string(Hk) + " key heads");
+    const at::ScalarType t = q.scalar_type();
+    if (t != at::kBFloat16 && t != at::kHalf) refuse(std::string("unsupported dtype ") + c10::toString(t) + " (bf16 or fp16)");
+    if (k.has_value() != v.has_value()) refuse("k and v come together");
+    if (k) {
+      check_kv(*k, *v);
+      if (k->scalar_type() != t) refuse("q, k, v must share one dtype");
+    }
+    if (at::GradMode::is_enabled() && (q.requires_grad() || (k && (k->requires_grad() || v->requires_grad()))))
+      refuse("attention over a cache has no gradient");
+    const double s = sm_scale ? *sm_scale : 1.0 / std::sqrt(static_cast<double>(D));
+    check_scale(s, 0.0);
+    check_out(q, out);
+    const c10::cuda::CUDAGuard guard(kc.device());
+    if (!q.numel()) return out ? *out : like(q);
+    const int64_t n = k ? k->size(2) : 0;
+    if (n == 0 && H / Hk * Sq <= few_rows) {
+      Output o(q, out);
+      const View a(q);
+      OptTensor scratch;
+      const int64_t need = api.bsa_kv8_attention_scratch_bytes(B, H, Hk, Sq, cap, D);
+      if (need) scratch = bytes(q, need);
+      check(api.bsa_kv8_attention(a.p(), dtype_code(t), B, H, Sq, a.strides, ptr(kc), scale(ks), ptr(vc), scale(vs),
+                                  lengths(), Hk, cap, D, causal, static_cast<float>(s), ptr(o.t), o.strides, ptr(scratch),
+                                  stream_of(q)),
+            "bsa_kv8_attention");
+      return o.done(out);
+    }
+    const auto kv = n ? unpack(t, k, v) : unpack(t, std::nullopt, std::nullopt);
+    const py::tuple m = attention_ranges(py::cast(kc.device()), Sq, cap + n, B, std::nullopt, causal, 0, std::nullopt,
+                                         std::nullopt, std::nullopt, std::nullopt, len, n);
+    const py::tuple r = masked_attention(q, kv.first, kv.second, py::cast<Tensor>(m[0]), B, py::cast<int64_t>(m[2]), Sq,
+                                         cap + n, s, 0.0, out, false, false);
+    return py::cast<Tensor>(r[0]);
+  }
+};
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("load", &load, "The engine's library, and the exception of its CUDA errors");
+  m.def("norm_rope", &norm_rope);
+  m.def("norm_rope_backward", &norm_rope_backward);
+  m.def("attention_ranges", &attention_ranges);
+  m.def("masked_attention", &masked_attention);
+  m.def("masked_attention_backward", &masked_attention_backward);
+  py::class_<Cache>(m, "Cache")
+      .def(py::init<Tensor, Tensor, Tensor, Tensor, Tensor>())
+      .def("append", &Cache::append)
+      .def("unpack", &Cache::unpack)
+      .def("attend", &Cache::attend);
+}

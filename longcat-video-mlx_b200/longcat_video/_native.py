@@ -37,8 +37,6 @@ _c_i64p = ctypes.POINTER(ctypes.c_int64)
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
-_c_rope = [_vp, _i, _i, _i, _i, _i, _i, _i]  # tables, axis dims, grid, start
-_c_cache = [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i]  # codes and scales of K and V, lengths, sizes
 
 _SIGNATURES = {
     "bsa_version": ([], _i),
@@ -74,21 +72,6 @@ _SIGNATURES = {
     "bsa_forward_qknorm": ([_vp, _vp, _vp, _i, _i, _i, _i, _i, _c_i64p, _c_i64p, _c_i64p, _i, _i, _i, _i, _i, _i, _i,
                             _f, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp, _c_i64p, _i, _vp],
                            _i),
-    "bsa_norm_rope": ([_vp, _vp, _i, _vp, _vp] * 2 + [_i, _i, _i, _i, _i, _f] + _c_rope + [_vp], _i),
-    "bsa_norm_rope_backward_scratch_bytes": ([_i, _i, _i], ctypes.c_int64),
-    "bsa_norm_rope_backward": ([_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp] * 2 + [_i, _i, _i, _i, _i, _f] + _c_rope
-                               + [_vp, _vp], _i),
-    "bsa_attention_ranges": ([_vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp], _i),
-    "bsa_masked_attention_scratch_bytes": ([_i] * 5, ctypes.c_int64),
-    "bsa_masked_attention": ([_vp, _vp, _vp] + [_i] * 7 + [_vp] * 3 + [_vp, _vp, _i, _f, _f, _vp, _vp, _vp, _vp, _vp,
-                                                                          _vp], _i),
-    "bsa_masked_attention_backward_scratch_bytes": ([_i] * 4, ctypes.c_int64),
-    "bsa_masked_attention_backward": ([_vp] * 7 + [_i] * 7 + [_vp] * 5 + [_vp, _vp, _i, _f, _f] + [_vp] * 5, _i),
-    "bsa_kv8_append": (_c_cache + [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp], _i),
-    "bsa_kv8_unpack": (_c_cache + [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp], _i),
-    "bsa_kv8_attention_scratch_bytes": ([_i] * 6, ctypes.c_int64),
-    "bsa_kv8_attention": ([_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp, _vp,
-                           _vp], _i),
 }
 
 

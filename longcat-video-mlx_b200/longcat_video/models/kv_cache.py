@@ -7,7 +7,6 @@ by a power-of-two scale, and decoding a code to 16 bits is exact.
 
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -33,23 +32,7 @@ class KVCache8:
 
     def __init__(self, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
                  lengths: torch.Tensor):
-        _dense._same_place(k_codes, k_scale, v_codes, v_scale, lengths)
-        shape = k_codes.shape
-        if len(shape) != 4 or shape != v_codes.shape:
-            raise ValueError("codes must be [B, Hk, capacity, D]")
-        B, Hk, cap, D = shape
-        if cap % BLOCK or cap == 0:
-            raise ValueError(f"capacity {cap} must be a positive multiple of {BLOCK}")
-        if D % 8 or not 0 < D <= 128:
-            raise ValueError(f"head_dim D={D} must be a multiple of 8 and <= 128")
-        for t in (k_codes, v_codes):
-            if t.dtype is not torch.float8_e4m3fn or not t.is_contiguous() or t.data_ptr() & 15:
-                raise ValueError("codes must be contiguous, 16-byte aligned float8_e4m3fn")
-        for t in (k_scale, v_scale):
-            if t.dtype is not torch.float32 or not t.is_contiguous() or t.shape != (B, Hk, cap // BLOCK):
-                raise ValueError(f"scales must be contiguous fp32 [{B}, {Hk}, {cap // BLOCK}]")
-        if lengths.dtype is not torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous():
-            raise ValueError(f"lengths must be contiguous int32 [{B}]")
+        self._cache = _dense.ops().Cache(k_codes, k_scale, v_codes, v_scale, lengths)
         self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.lengths = k_codes, k_scale, v_codes, v_scale, lengths
 
     @classmethod
@@ -85,35 +68,19 @@ class KVCache8:
         return KVCache8(rep(self.k_codes), self.k_scale.repeat(batch, 1, 1), rep(self.v_codes),
                         self.v_scale.repeat(batch, 1, 1), self.lengths.repeat(batch))
 
-    def _check_kv(self, k, v) -> None:
-        B, Hk, cap, D = self.k_codes.shape
-        _dense._same_place(self.k_codes, k, v)
-        if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (B, Hk, D):
-            raise ValueError(f"k and v must be [{B}, {Hk}, n, {D}]")
-        if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError("k and v must both be bf16 or fp16")
-
     def append(self, k: torch.Tensor, v: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
         """Adds n tokens to every sequence (``counts`` int32 [B]: only the first counts[b] of them).
 
         A block whose largest value grows takes a larger scale, and its codes are rounded again at it.  Tokens that
         do not fit are dropped, and ``_native.device_error()`` then reports it; more tokens than the whole capacity
         are refused here.  Infinities are held as the block's largest code, NaN as NaN; neither sets a scale."""
-        self._check_kv(k, v)
-        if k.shape[2] > self.capacity:
-            raise ValueError(f"{k.shape[2]} tokens for a capacity of {self.capacity}")
-        if counts is not None:
-            counts = _dense._i32(counts, "counts", (self.k_codes.shape[0],))
-            _dense._same_place(k, counts)
-        if k.numel():
-            _dense.cache_append(self, k, v, counts)
+        self._cache.append(k, v, counts)
 
     def truncate(self, lengths: Union[int, torch.Tensor]) -> None:
         """Sets the lengths: a rejected draft, or the conditioning tokens before the next chunk.  Blocks keep their
         scales; a block that ends up without tokens takes a new one at the next append."""
         if isinstance(lengths, torch.Tensor):
-            _dense._same_place(self.lengths, lengths)
-            if tuple(lengths.shape) != tuple(self.lengths.shape):
+            if lengths.shape != self.lengths.shape:
                 raise ValueError(f"lengths must be {list(self.lengths.shape)}")
             self.lengths.copy_(lengths)
         else:
@@ -123,9 +90,7 @@ class KVCache8:
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
         """(k, v) [B, Hk, capacity, D]: the held tokens, zeros behind them."""
-        if dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError("dequantize to bf16 or fp16")
-        return _dense.cache_unpack(self, dtype)
+        return self._cache.unpack(dtype, None, None)
 
     def attend(self, q: torch.Tensor, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None, *,
                causal: bool = False, sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -135,35 +100,4 @@ class KVCache8:
         ``causal``: the last query sees every key (held, then fresh), the one before it one less, and so on.
         sm_scale defaults to 1 / sqrt(D).  Sequences without a key give zeros.  Few rows read the codes as they are;
         many rows, or fresh keys, unpack the cache into 16-bit scratch first."""
-        B, Hk, cap, D = self.k_codes.shape
-        _dense._same_place(self.k_codes, q, k, v, out)
-        if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
-            raise ValueError(f"q must be [{B}, H, Sq, {D}]")
-        if q.shape[1] % Hk:
-            raise ValueError(f"{q.shape[1]} query heads are no multiple of {Hk} key heads")
-        if q.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"unsupported dtype {q.dtype} (bf16 or fp16)")
-        if (k is None) != (v is None):
-            raise ValueError("k and v come together")
-        if k is not None:
-            self._check_kv(k, v)
-            if k.dtype != q.dtype:
-                raise ValueError("q, k, v must share one dtype")
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v)):
-            raise ValueError("attention over a cache has no gradient")
-        scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-        _dense.check_scale(scale)
-        if out is None:
-            out = q.new_empty(q.shape)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out must have q's shape and dtype")
-        Sq = q.shape[2]
-        if q.numel() == 0:
-            return out
-        n = k.shape[2] if k is not None else 0
-        if n == 0 and q.shape[1] // Hk * Sq <= FEW_ROWS:
-            return _dense.cache_attention(self, q, causal, scale, out)
-        kd, vd = _dense.cache_unpack(self, q.dtype, k if n else None, v if n else None)
-        mask, ranges, table = _dense.attention_ranges(B, Sq, cap + n, device=q.device, causal=causal,
-                                                      k_lengths=self.lengths, k_add=n)
-        return _dense.masked_attention(q, kd, vd, ranges, table, B, scale, 0.0, out=out)[0]
+        return self._cache.attend(q, k, v, causal, sm_scale, out, FEW_ROWS)

@@ -23,9 +23,9 @@ class AttentionMask:
 
     Build one with :meth:`build` or, from intervals of one's own, with :meth:`from_ranges`."""
 
-    def __init__(self, buffer, ranges: int, table: int, batch: int, Sq: int, Sk: int):
-        # one device buffer, the addresses of its two parts, and their sizes (see _dense.attention_ranges)
-        self._buffer, self._ranges, self._table = buffer, ranges, table
+    def __init__(self, buffer: torch.Tensor, batch: int, table_at: int, Sq: int, Sk: int):
+        # one device buffer: the intervals, and the table from `table_at` on
+        self._buffer, self._table_at = buffer, table_at
         self.batch, self.Sq, self.Sk = batch, Sq, Sk
 
     @property
@@ -36,8 +36,7 @@ class AttentionMask:
     def table(self) -> torch.Tensor:
         """[batch, tiles of 128 rows, 4]: lowest lo and highest hi of the rows that see a key, highest lo and lowest hi of
         all rows."""
-        tiles = (self.Sq + 127) // 128
-        return self._buffer[self._buffer.numel() - self.batch * tiles * 4:].view(self.batch, tiles, 4)
+        return self._buffer[self._table_at:].view(self.batch, (self.Sq + 127) // 128, 4)
 
     @classmethod
     def build(cls, Sq: int, Sk: int, *, causal: bool = False, prefix: Union[int, torch.Tensor, None] = None,
@@ -52,60 +51,34 @@ class AttentionMask:
         at a < prefix see exactly the first ``prefix`` keys: conditioning tokens that attend to themselves, or a
         prompt in both directions in front of a causal continuation.  Rows outside every document or behind their
         length see nothing and come out as zeros."""
-        if Sq < 0 or Sk < 0:
-            raise ValueError("lengths must be >= 0")
-        given = [t for t in (q_offsets, k_offsets, q_lengths, k_lengths) if t is not None]
-        given += [prefix] if isinstance(prefix, torch.Tensor) else []
-        if device is None:
-            device = given[0].device if given else torch.device("cuda", torch.cuda.current_device())
-        if (q_offsets is None) != (k_offsets is None):
-            raise ValueError("q_offsets and k_offsets come together")
-        if q_offsets is not None and (q_lengths is not None or k_lengths is not None):
-            raise ValueError("give documents or lengths, not both")
-        batch, n = 1, None
-        if q_offsets is not None:
-            if q_offsets.dim() != 1 or q_offsets.shape != k_offsets.shape or q_offsets.numel() < 2:
-                raise ValueError("q_offsets and k_offsets must be [documents + 1]")
-            n = q_offsets.numel() - 1
-        for t, name in ((q_lengths, "q_lengths"), (k_lengths, "k_lengths")):
-            if t is not None:
-                if t.dim() != 1 or (n is not None and t.numel() != n):
-                    raise ValueError(f"{name} must be [B]")
-                batch = n = t.numel()
-        prefixes = None
-        if isinstance(prefix, torch.Tensor):
-            if n is None:
-                batch = n = prefix.numel()
-            prefixes, prefix = _dense._i32(prefix, "prefix", (n,)), 0
-        prefix = 0 if prefix is None else int(prefix)
-        if prefix < 0:
-            raise ValueError("prefix must be >= 0")
-        parts = _dense.attention_ranges(
-            batch, Sq, Sk, device=device, causal=causal, prefix=prefix, prefixes=prefixes,
-            q_offsets=_dense._i32(q_offsets, "q_offsets"), k_offsets=_dense._i32(k_offsets, "k_offsets"),
-            q_lengths=_dense._i32(q_lengths, "q_lengths"), k_lengths=_dense._i32(k_lengths, "k_lengths"))
-        return cls(*parts, batch, Sq, Sk)
+        many = isinstance(prefix, torch.Tensor)
+        parts = _dense.ops().attention_ranges(
+            None if device is None else torch.device(device), Sq, Sk, 1, None, causal, 0 if many or prefix is None else prefix,
+            prefix if many else None, q_offsets, k_offsets, q_lengths, k_lengths, 0)
+        return cls(*parts, Sq, Sk)
 
     @classmethod
     def from_ranges(cls, ranges: torch.Tensor, Sk: int) -> "AttentionMask":
         """From [batch or 1, Sq, 2] int32 intervals [lo, hi); they are clamped to [0, Sk]."""
         if ranges.dim() != 3 or ranges.shape[-1] != 2:
             raise ValueError("ranges must be [batch, Sq, 2]")
-        given = _dense._i32(ranges, "ranges")
-        if given.data_ptr() % 8:
-            given = given.clone()
-        batch, Sq = int(given.shape[0]), int(given.shape[1])
-        return cls(*_dense.attention_ranges(batch, Sq, Sk, device=given.device, given=given), batch, Sq, int(Sk))
+        batch, Sq = int(ranges.shape[0]), int(ranges.shape[1])
+        parts = _dense.ops().attention_ranges(ranges.device, Sq, Sk, batch, ranges, False, 0, None, None, None, None, None, 0)
+        return cls(*parts, Sq, int(Sk))
+
+    def _args(self):
+        return self._buffer, self.batch, self._table_at, self.Sq, self.Sk
+
+
+_NO_MASK = (None, 1, 0, 0, 0)
 
 
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, sm_scale, softcap):
-        rest = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        out, lse = _dense.masked_attention(q, k, v, *_mask_args(mask), sm_scale, softcap, want_lse=True, rest=rest)
+        out, lse, rest = _dense.ops().masked_attention(q, k, v, *mask, sm_scale, softcap, None, True, True)
         ctx.save_for_backward(q, k, v, out, rest, lse)
-        ctx.mask = mask
-        ctx.rest = (sm_scale, softcap)
+        ctx.rest = (*mask[:3], sm_scale, softcap)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -117,13 +90,9 @@ class _MaskedAttention(torch.autograd.Function):
             return (None,) * 6
         q, k, v, out, rest, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv = _dense.masked_attention_backward(q, k, v, out, rest, lse, grad.to(q.dtype), *_mask_args(ctx.mask),
-                                                      *ctx.rest, need[0], need[1] or need[2])
+        dq, dk, dv = _dense.ops().masked_attention_backward(q, k, v, out, rest, lse, grad.to(q.dtype), *ctx.rest, need[0],
+                                                            need[1] or need[2])
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
-
-
-def _mask_args(mask):
-    return (mask._ranges, mask._table, mask.batch) if mask is not None else (None, None, 1)
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[AttentionMask] = None, *,
@@ -136,25 +105,12 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     are copied once).  sm_scale defaults to 1 / sqrt(D).  Rows that see no key give zeros, and -inf in the
     log-sum-exp [B, H, Sq] (fp32, natural) that ``return_lse`` adds; it carries no gradient.  ``out``: a
     preallocated [B, H, Sq, D] result (not with gradients)."""
-    _dense.check_qkv(q, k, v)
-    scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
-    softcap = float(softcap)
-    _dense.check_scale(scale, softcap)
-    if mask is not None:
-        if mask.Sq != q.shape[2] or mask.Sk != k.shape[2]:
-            raise ValueError(f"the mask is for {mask.Sq} queries and {mask.Sk} keys, got {q.shape[2]} and {k.shape[2]}")
-        if mask.batch != 1 and mask.batch != q.shape[0]:
-            raise ValueError(f"the mask has {mask.batch} batch entries, q has {q.shape[0]}")
-        _dense._same_place(q, mask._buffer)
-    if out is not None:
-        _dense._same_place(q, out)
-        if out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out must have q's shape and dtype")
-    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    if grad:
+    scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale
+    args = _NO_MASK if mask is None else mask._args()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None:
             raise ValueError("out= is for calls without gradients")
-        o, lse = _MaskedAttention.apply(q, k, v, mask, scale, softcap)
-        return (o, lse) if return_lse else o
-    o, lse = _dense.masked_attention(q, k, v, *_mask_args(mask), scale, softcap, out=out, want_lse=return_lse)
+        o, lse = _MaskedAttention.apply(q, k, v, args, scale, softcap)
+    else:
+        o, lse, _ = _dense.ops().masked_attention(q, k, v, *args, scale, softcap, out, return_lse, False)
     return (o, lse) if return_lse else o

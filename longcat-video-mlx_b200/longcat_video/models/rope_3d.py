@@ -108,31 +108,35 @@ class RotaryPositionalEmbedding(torch.nn.Module):
 
 class _NormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, eps, rope, start):
-        xs = [q] if k is None else [q, k]
+    def forward(ctx, q, k, q_weight, k_weight, eps, rope):
         ctx.save_for_backward(q, k, q_weight, k_weight)
-        ctx.rest = (eps, rope, start)
+        ctx.rest = (eps, rope)
         ctx.set_materialize_grads(False)
-        ys = _dense.norm_rope(xs, [q_weight, k_weight][:len(xs)], eps, rope, start)
-        return ys[0] if k is None else tuple(ys)
+        return _dense.ops().norm_rope(q, k, q_weight, k_weight, eps, *rope)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         q, k, q_weight, k_weight = ctx.saved_tensors
-        eps, rope, start = ctx.rest
+        eps, rope = ctx.rest
         need = ctx.needs_input_grad
         sides = [(i, x, w) for i, (x, w) in enumerate(((q, q_weight), (k, k_weight)))
                  if x is not None and grads[i] is not None and (need[i] or need[2 + i])]
-        res = [None] * 7
+        res = [None] * 6
         if sides:
-            gs = [grads[i].to(x.dtype) for i, x, _ in sides]
-            dxs, dws = _dense.norm_rope_backward([x for _, x, _ in sides], gs, [w for _, _, w in sides], eps, rope,
-                                                 start, [need[2 + i] for i, _, _ in sides])
-            for (i, _, w), dx, dw in zip(sides, dxs, dws):
+            args = []
+            for i, x, w in sides:
+                args += [x, grads[i].to(x.dtype), w, need[2 + i]]
+            if len(sides) == 1:
+                args += [None, None, None, False]
+            got = _dense.ops().norm_rope_backward(*args, eps, *rope)
+            for (i, _, w), dx, dw in zip(sides, got[::2], got[1::2]):
                 res[i] = dx if need[i] else None
                 res[2 + i] = dw.to(w.dtype) if dw is not None else None
         return tuple(res)
+
+
+_NO_ROPE = (None, 0, 0, 0, 0, 0, 0, 0)
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
@@ -149,11 +153,11 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Op
         raise ValueError("nothing to do: give norm weights, rope tables or both")
     if k is None and k_weight is not None:
         raise ValueError("k_weight without k")
-    if rope is not None:
+    if rope is None:
+        args = _NO_ROPE
+    else:
         tables, dims, grid = rope.native_args() if hasattr(rope, "native_args") else rope
-        rope = (tables, dims, grid)
+        args = (tables, *dims, *grid, start)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _NormRope.apply(q, k, q_weight, k_weight, float(eps), rope, int(start))
-    xs = [q] if k is None else [q, k]
-    ys = _dense.norm_rope(xs, [q_weight, k_weight][:len(xs)], float(eps), rope, int(start))
-    return ys[0] if k is None else tuple(ys)
+        return _NormRope.apply(q, k, q_weight, k_weight, eps, args)
+    return _dense.ops().norm_rope(q, k, q_weight, k_weight, eps, *args)
