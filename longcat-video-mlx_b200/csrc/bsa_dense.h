@@ -141,7 +141,7 @@ int dense_pick_splits(int sms, int B, int H, int Sq, int Sk);
 int launch_dense(const DenseArgs& a, int sms, cudaStream_t stream);
 int make_map4(CUtensorMap* m, const Tensor4& t, int dtype, int B, int H, int S, int D, const char* name);
 long long dense_backward_stats_bytes(int B, int H, int Sq, int Bm);
-int launch_dense_backward(const DenseArgs& a, cudaStream_t stream);
+int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream);
 int dense_bwd_device_error(int clear);
 int dense_device_error(int clear);
 

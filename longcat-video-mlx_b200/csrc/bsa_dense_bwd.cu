@@ -40,6 +40,7 @@ struct BwdParams {
   const int4* table;
   int Bm, H, Hk, G, Sq, Sk, D;
   int q_tiles, k_tiles, Sq_pad;
+  int cluster;          // CTAs that share the query heads of a key tile (dkv)
   float scale_log2, sm_scale, cap_in, cap_log2;
   float* lse2;          // [B * H][Sq_pad]: lse in log2 (+inf: no keys)
   float* delta;         // [B * H][Sq_pad]
@@ -190,6 +191,42 @@ __device__ __forceinline__ void store_acc(uint32_t addr, int col0, float f, void
   }
 }
 
+// One warp's 32 rows x (DP / 2) columns of an accumulator to shared memory as fp32, [4 columns][row][4], so that lanes
+// write side by side.
+template <int DP>
+__device__ __forceinline__ void to_shared(uint32_t addr, int half, int row, uint8_t* dst, bool some) {
+#pragma unroll 1
+  for (int c = 0; c < DP / 64; ++c) {
+    const int c0 = half * (DP / 2) + 32 * c;
+    uint32_t r[32];
+    if (some) {
+      tmem_read32(addr + c0, r);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) r[e] = 0u;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<uint4*>(dst + ((c0 / 4 + e) * kTile + row) * 16) =
+          make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+  }
+}
+
+// All threads of all CTAs of the cluster; every CTA comes here whatever happened before.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 load_peer(uint32_t addr, int rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
 // ------------------------------------------------------------------------- dk, dv
 template <int DP>
 struct DkvSmem {
@@ -221,8 +258,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   S& ss = *reinterpret_cast<S*>(smem + S::kTiles);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // key tiles ascending: under a causal mask the first are seen by the most queries
-  const int bhk = blockIdx.x / p.k_tiles;
-  const int kt = blockIdx.x - bhk * p.k_tiles;
+  const int item = blockIdx.x / p.cluster, rank = blockIdx.x - item * p.cluster;
+  const int bhk = item / p.k_tiles;
+  const int kt = item - bhk * p.k_tiles;
+  const int g_count = p.G / p.cluster, g_first = rank * g_count;
   const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
   const int bm = p.Bm > 1 ? b : 0;
   const int key0 = kt * kTile;
@@ -277,7 +316,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   int* err = &g_dense_bwd_err;
   // every role walks the same tiles: `step(g, i, tab)` returns false to stop
   auto walk = [&](auto&& step) {
-    for (int g = 0; g < p.G; ++g)
+    for (int g = g_first; g < g_first + g_count; ++g)
       for (int i = first; i <= last; ++i) {
         const int4 t = table ? __ldg(table + i) : make_int4(0, p.Sk, 0, p.Sk);
         if (!sees(t)) continue;
@@ -512,7 +551,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
       }
     }
-    if (ok) {
+    if (p.cluster > 1) {  // this CTA's sums to shared memory: its tiles are done with
+      to_shared<DP>(la + kColD, half, 32 * (warp & 3) + lane, smem, ok && some);
+      to_shared<DP>(la + kColC, half, 32 * (warp & 3) + lane, smem + kTile * DP * 4, ok && some);
+    } else if (ok) {
       const bool live = key < p.Sk;
       const long long ok0 = b * p.d0.sb + hk * p.d0.sh + static_cast<long long>(key) * p.d0.ss;
       const long long ov0 = b * p.d1.sb + hk * p.d1.sh + static_cast<long long>(key) * p.d1.ss;
@@ -524,6 +566,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 8) tmem_dealloc(tmem, 512);
+  if (p.cluster > 1) {
+    // The CTAs of a cluster took a part of the query heads each.  Each now adds up a share of the columns, in the order of
+    // the CTAs, from everybody's shared memory.
+    cluster_sync();
+    constexpr int kEights = DP / 8;  // runs of 8 columns of dk, then of dv
+    for (int t = tid; t < 2 * kEights * kTile; t += kBwdThreads) {
+      const int run = t / kTile, row = t - run * kTile;
+      if (run % p.cluster != rank) continue;
+      const int which = run / kEights, d = 8 * (run - which * kEights);
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      const uint32_t at = smem_u32(smem) + which * kTile * DP * 4 + ((d >> 2) * kTile + row) * 16;
+      for (int c = 0; c < p.cluster; ++c) {
+        const float4 a = load_peer(at, c), e = load_peer(at + kTile * 16, c);
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += e.x; v[5] += e.y; v[6] += e.z; v[7] += e.w;
+      }
+      if (key0 + row >= p.Sk || d >= p.D) continue;
+      const Tensor4& o = which ? p.d1 : p.d0;
+      const float f = which ? 1.f : p.sm_scale;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= f;
+      store8<kBF16>(o.p, b * o.sb + hk * o.sh + static_cast<long long>(key0 + row) * o.ss + d, v);
+    }
+    cluster_sync();  // nobody leaves while its sums are read
+  }
 }
 
 // ------------------------------------------------------------------------- dq
@@ -810,8 +877,18 @@ int launch_bwd(const CUtensorMap* m, BwdParams p, const DenseArgs& a, cudaStream
   if (a.dk.p) {
     p.d0 = a.dk;
     p.d1 = a.dv;
-    kv<<<a.B * a.Hk * p.k_tiles, kBwdThreads, dkv_smem_bytes<DP>(), stream>>>(m[0], m[1], m[2], m[3], p);
-    if (cudaGetLastError() != cudaSuccess) return BSA_ERR_CUDA;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = p.cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.B * a.Hk * p.k_tiles * p.cluster);
+    cfg.blockDim = dim3(kBwdThreads);
+    cfg.dynamicSmemBytes = dkv_smem_bytes<DP>();
+    cfg.stream = stream;
+    cfg.attrs = at;
+    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kv, m[0], m[1], m[2], m[3], p) != cudaSuccess) return BSA_ERR_CUDA;
   }
   if (!a.dq.p) return BSA_OK;
   p.d0 = a.dq;
@@ -826,7 +903,7 @@ long long dense_backward_stats_bytes(int B, int H, int Sq, int Bm) {
   return (static_cast<long long>(B) * H + Bm) * rows * 8;
 }
 
-int launch_dense_backward(const DenseArgs& a, cudaStream_t stream) {
+int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
   using namespace dense;
   CUtensorMap m[4];
   int rc;
@@ -840,6 +917,12 @@ int launch_dense_backward(const DenseArgs& a, cudaStream_t stream) {
   p.q_tiles = (a.Sq + kTile - 1) / kTile;
   p.k_tiles = (a.Sk + kTile - 1) / kTile;
   p.Sq_pad = p.q_tiles * kTile;
+  // Key tiles alone may be few and uneven (4,680 rows of 9 documents, 4 key heads: 148 tiles that see 8 to 44 query
+  // tiles): then the query heads of a key head are shared among the CTAs of a cluster, 8 at most.
+  p.cluster = 1;
+  if (static_cast<long long>(a.B) * a.Hk * p.k_tiles < 4ll * sms)
+    for (int c = 2; c <= 8; ++c)
+      if (p.G % c == 0) p.cluster = c;
   p.scale_log2 = a.sm_scale * 1.4426950408889634f;
   p.sm_scale = a.sm_scale;
   if (a.softcap > 0.f) {
@@ -855,7 +938,7 @@ int launch_dense_backward(const DenseArgs& a, cudaStream_t stream) {
   p.o = a.o;
   p.o_lo = a.o_lo;
   p.g = a.g;
-  if (static_cast<long long>(a.B) * a.H * p.q_tiles > INT_MAX || static_cast<long long>(a.B) * a.Hk * p.k_tiles > INT_MAX ||
+  if (static_cast<long long>(a.B) * a.H * p.q_tiles > INT_MAX || static_cast<long long>(a.B) * a.Hk * p.k_tiles > INT_MAX / 8 ||
       static_cast<long long>(a.B) * a.H > 65535)
     return set_error(BSA_ERR_SHAPE, "too many row tiles for one launch");
   const dim3 sgrid(p.Sq_pad / 16, a.B * a.H);

@@ -292,7 +292,7 @@ int bsa_masked_attention_backward(const void* q, const void* k, const void* v, c
   a.dv = tensor(dv, ks);
   a.lse = const_cast<float*>(lse);
   a.stats = static_cast<float*>(scratch);
-  return bsa::launch_dense_backward(a, static_cast<cudaStream_t>(stream));
+  return bsa::launch_dense_backward(a, sm_count(), static_cast<cudaStream_t>(stream));
 }
 
 int bsa_kv8_append(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
