@@ -313,7 +313,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -426,18 +426,23 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
     if (++slot == kSlots) slot = 0;
     float s[8][4];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
+    for (int t = 0; t < 8; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+    // the eight token groups' products side by side: one after the other each would wait for the one before
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 u = *reinterpret_cast<const uint4*>(ks + chunk_at(8 * t + g, 2 * c + i));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int i = 0; i < 2; ++i) {
+      uint4 u[8];
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          mma_f16(s[t], qa[4 * i + x], e4m3x2_to_f16x2(static_cast<uint16_t>(w[x])),
-                  e4m3x2_to_f16x2(static_cast<uint16_t>(w[x] >> 16)));
-      }
+      for (int t = 0; t < 8; ++t) u[t] = *reinterpret_cast<const uint4*>(ks + chunk_at(8 * t + g, 2 * c + i));
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const uint32_t w = (&u[t].x)[x];
+          mma_f16(s[t], qa[4 * i + x], e4m3x2_to_f16x2(static_cast<uint16_t>(w)),
+                  e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16)));
+        }
     }
     const int key0 = blk * kCacheBlock + 2 * c;
     float alpha[2];

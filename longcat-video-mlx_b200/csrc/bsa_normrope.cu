@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* partial,
   const int first = blockIdx.y ? rows0 : 0, rows = blockIdx.y ? rows1 : rows0;
   float v = 0.f;
   if (col < D)
+#pragma unroll 8
     for (int r = part; r < rows; r += 32) v += partial[static_cast<long long>(first + r) * D + col];
   red[part][c] = v;
   __syncthreads();
@@ -348,9 +349,9 @@ int launch(const NormRopeArgs& a, int most, cudaStream_t stream, int* rows_out) 
 
 }  // namespace nrope
 
-// CTAs: several waves forward, so that the last ones are short; backward each leaves a row of weight gradients, and a
-// head group may have one even where there are more groups than CTAs were asked for
-constexpr int kForwardCtas = 64, kBackwardCtas = 16;  // for each SM
+// CTAs: several waves forward, so that the last ones are short; one wave backward, where each leaves a row of weight
+// gradients to add up (a head group has one at least)
+constexpr int kForwardCtas = 64, kBackwardCtas = 4;  // for each SM
 
 int norm_rope_partials(int groups) {
   const int most = kBackwardCtas * nrope::sm_count();
