@@ -7,10 +7,9 @@
 // query tile of 128 rows of one head:
 //     S(j)[128 x 128] = Q K_j^T        A = Q in tensor memory, B = K in shared memory
 //     O[128 x D]     += P(j) V_j       A = P in tensor memory, B = V in shared memory
-// TMEM: two S buffers and O of 128 columns each, Q and P of 64 (16-bit pairs).  With Q in shared memory too, the operands
-// of both products and the loads of K and V move 160 KB a step through it, 1,250 cycles, and a product of
-// 128 x 128 x 16 was seen to take 97 cycles instead of 64; with Q in tensor memory it is 128 KB.  S(j+3) is issued
-// when S(j+1) has been read, behind P(j) V, two steps before it is needed.
+// TMEM: two S buffers and O of 128 columns each, Q and P of 64 (16-bit pairs).  With Q in tensor memory the operands of
+// both products and the loads of K and V move 128 KB a step through shared memory, 160 KB with Q there too.  S(j+3)
+// is issued when S(j+1) has been read, behind P(j) V, two steps before it is needed.
 //
 // Roles (384 threads, one CTA to an SM):
 //   warps 0-7 : softmax, warps 0-3 on the keys 0-63 of a step, 4-7 on 64-127, a thread on half a row.  The two threads
@@ -160,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kLoad) {
     // ------------------------------------------------------------------ loads
     if (steps > 0) {
-      if (lane == 0) {
+      if (elect_one()) {
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // V rows of this tile that no row of the CTA sees, but the tensor holds
         const bool fix = is_v && (row < lo_u || min(row + kTile, p.Sk) > hi_u);
         if (!fix) {
-          if (lane == 0) {
+          if (elect_one()) {
             mbar_arrive_expect_tx(&ss.full[slot], kBytes);
             load_tile<DP>(dst, is_v ? &tm_v : &tm_k, &ss.full[slot], row, hk, b);
           }
@@ -225,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kIssue) {
     // ------------------------------------------------------------------ products
-    if (lane == 0 && steps > 0) {
+    if (steps > 0 && elect_one()) {
       constexpr uint32_t kIdQK = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t kIdPV = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
       const uint32_t kvb = smem_u32(sKV);

@@ -55,12 +55,22 @@ __device__ __forceinline__ void zero_row(uint8_t* tile, int r, int lane) {
     *reinterpret_cast<uint4*>(tile + (c >> 3) * kHalfBytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// Operand descriptors of a tile: k-step kk of 16 values along d (K-major), or of 16 rows (rows are K).
+// Operand descriptors of a tile for k-step kk: 16 values along d (K-major), or 16 rows (rows are K).  The step adds to
+// the address field, which a tile in shared memory cannot carry out of.
 __device__ __forceinline__ uint64_t desc_d(uint32_t tile, int kk) {
-  return sdesc_sw128(tile + (kk >> 2) * kHalfBytes + (kk & 3) * 32, 16, 1024);
+  return sdesc_sw128(tile, 16, 1024) + static_cast<uint64_t>(((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4);
 }
 __device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int kk) {
-  return sdesc_sw128(tile + kk * 2048, kHalfBytes, 1024);
+  return sdesc_sw128(tile, kHalfBytes, 1024) + static_cast<uint64_t>((kk * 2048) >> 4);
+}
+
+// One lane of a whole warp, as a predicate the compiler knows to be one lane: issuing a product takes 14 to 26 cycles
+// then, behind `lane == 0` 46 to 56 (its operands go through registers that a whole warp shares), where the tensor
+// cores take 64 for it.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 __device__ __forceinline__ float rcp_approx(float x) {

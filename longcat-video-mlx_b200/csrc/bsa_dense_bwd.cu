@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (warp == 9) {
     // ------------------------------------------------------------------ loads
     if (some) {
-      if (lane == 0) {
+      if (elect_one()) {
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_g);
         mbar_arrive_expect_tx(&ss.kv_full, 2 * kBytes);
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const bool fix = t.w <= 0;  // rows without keys, whose q and do may hold anything
         uint8_t* q = sQ + rq.slot * kBytes;
         const uint32_t extra = 2 * kTile * sizeof(float) + (p.rng ? kTile * sizeof(int2) : 0);
-        if (lane == 0) {
+        if (elect_one()) {
           uint64_t* bar = fix ? &ss.fix : &ss.q_full[rq.slot];
           mbar_arrive_expect_tx(bar, kBytes + extra);
           load_tile<DP>(q, &tm_q, bar, i * kTile, h, b);
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (n >= S::kG) w = bar_wait(&ss.g_empty[rg.slot], rg.phase ^ 1u, abort_flag, err, 403);
         if (!__all_sync(0xffffffffu, w)) return false;
         uint8_t* go = sG + rg.slot * kBytes;
-        if (lane == 0) {
+        if (elect_one()) {
           uint64_t* bar = fix ? &ss.fix : &ss.g_full[rg.slot];
           mbar_arrive_expect_tx(bar, kBytes);
           load_tile<DP>(go, &tm_g, bar, i * kTile, h, b);
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     __syncwarp();
   } else if (warp == 8) {
     // ------------------------------------------------------------------ products
-    if (lane == 0 && some) {
+    if (some && elect_one()) {
       constexpr uint32_t kIdS = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t kIdR = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
       const uint32_t kb = smem_u32(sK), vb = smem_u32(sV), qb = smem_u32(sQ), gb = smem_u32(sG);
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (warp == 9) {
     // ------------------------------------------------------------------ loads
     if (steps > 0) {
-      if (lane == 0) {
+      if (elect_one()) {
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
         mbar_arrive_expect_tx(&ss.qg_full, 2 * kBytes);
@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int row = (n0 + n) * kTile;
         uint8_t* dst = sK + rk.slot * kBytes;
         const bool fix = row < tab.x || min(row + kTile, p.Sk) > tab.y;  // keys of the tile that no row sees
-        if (lane == 0) {
+        if (elect_one()) {
           uint64_t* bar = fix ? &ss.fix : &ss.k_full[rk.slot];
           mbar_arrive_expect_tx(bar, kBytes);
           load_tile<DP>(dst, &tm_k, bar, row, hk, b);
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (n >= S::kV) ok = bar_wait(&ss.v_empty[rv.slot], rv.phase ^ 1u, abort_flag, err, 453);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) {
+        if (elect_one()) {
           mbar_arrive_expect_tx(&ss.v_full[rv.slot], kBytes);
           load_tile<DP>(sV + rv.slot * kBytes, &tm_v, &ss.v_full[rv.slot], row, hk, b);
         }
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     __syncwarp();
   } else if (warp == 8) {
     // ------------------------------------------------------------------ products
-    if (lane == 0 && steps > 0) {
+    if (steps > 0 && elect_one()) {
       constexpr uint32_t kIdS = idesc_f16(128, 128, kBF16 ? 1 : 0, 0, 0);
       constexpr uint32_t kIdR = idesc_f16(128, DP, kBF16 ? 1 : 0, 0, 1);
       const uint32_t qb = smem_u32(sQ), gb = smem_u32(sG), kb = smem_u32(sK), vb = smem_u32(sV);
