@@ -430,38 +430,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(nm, nm);
         const bool more = j + 1 < steps;
         uint32_t pk[16];
+        const uint32_t o_phase = static_cast<uint32_t>(((j - 1) >> 1) & 1), s_phase = static_cast<uint32_t>(((j + 1) >> 1) & 1);
+        uint64_t *o_bar = &ss.o_full[(j - 1) & 1], *s_bar = &ss.s_full[(j + 1) & 1];
+        const bool o_done = j == 0 || bar_test(o_bar, o_phase);
+        const bool s_done = !more || bar_test(s_bar, s_phase);
         weights(rx, sc2, nm2, pk);
-        if (j > 0) {  // P(j - 1) has been read
-          ok = bar_wait(&ss.o_full[(j - 1) & 1], static_cast<uint32_t>(((j - 1) >> 1) & 1), abort_flag, err, 325);
-          tc_fence_after();
-        }
-        if (ok && more) ok = bar_wait(&ss.s_full[(j + 1) & 1], static_cast<uint32_t>(((j + 1) >> 1) & 1), abort_flag, err, 326);
+        if (!o_done) ok = bar_wait(o_bar, o_phase, abort_flag, err, 325);  // P(j - 1) has been read
+        if (ok && !s_done) ok = bar_wait(s_bar, s_phase, abort_flag, err, 326);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) continue;
+        tc_fence_after();
         tmem_st16(la + kColP + 32 * half, pk);
         const uint32_t s_next = la + col_s((j + 1) & 1) + 64 * half;
         const int key = (n0 + j + 1) * kTile;
         const bool border = key < lo_max || key + kTile > hi_min;
         float top = -INFINITY;
         if (more) {
-          tc_fence_after();
           tmem_read32(s_next, rx);
           if (kCap || border) prepare(rx, key + 64 * half, border);
           weights(ry, sc2, nm2, pk);
+          tmem_st16(la + kColP + 32 * half + 16, pk);
+          tmem_read32(s_next + 32, ry);  // beside the store
           top = top_of(rx);
         } else {
           weights(ry, sc2, nm2, pk);
+          tmem_st16(la + kColP + 32 * half + 16, pk);
         }
-        tmem_st16(la + kColP + 32 * half + 16, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ss.p_full[j & 1]);
+        if (lane == 0) {
+          mbar_arrive(&ss.p_full[j & 1]);
+          if (more) mbar_arrive(&ss.s_read[(j + 1) & 1]);
+        }
         if (more) {
-          tmem_read32(s_next + 32, ry);
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ss.s_read[(j + 1) & 1]);
           if (kCap || border) prepare(ry, key + 64 * half + 32, border);
           mx = max3(top, top_of(ry), top) * scale;
         }
