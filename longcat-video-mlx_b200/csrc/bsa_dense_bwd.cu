@@ -602,7 +602,9 @@ struct DqSmem {
   uint64_t qg_full;
   uint64_t k_full[kK], k_empty[kK], v_full[kV], v_empty[kV];
   uint64_t fix;
-  uint64_t s_full, s_read, dp_full[2], ds_full, done, drain;
+  uint64_t s_full, s_read;
+  uint64_t dp_full[2], ds_full[2];  // of step n in [n % 2]: the arithmetic may be a step ahead of who issues the products
+  uint64_t done, drain;
   uint32_t tmem;
   int abort_flag;
 };
@@ -646,7 +648,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(&ss.s_read, 8);
     mbar_init(&ss.dp_full[0], 1);
     mbar_init(&ss.dp_full[1], 1);
-    mbar_init(&ss.ds_full, 8);
+    mbar_init(&ss.ds_full[0], 8);
+    mbar_init(&ss.ds_full[1], 8);
     mbar_init(&ss.done, 1);
     mbar_init(&ss.drain, 1);
     ss.abort_flag = 0;
@@ -749,7 +752,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           ok = scores(n + 1);
           if (!ok) break;
         }
-        ok = bar_wait(&ss.ds_full, static_cast<uint32_t>(n & 1), abort_flag, err, 465);
+        ok = bar_wait(&ss.ds_full[n & 1], static_cast<uint32_t>((n >> 1) & 1), abort_flag, err, 465);
         if (!ok) break;
         tc_fence_after();
         mma_rows(tmem + kColD, tmem + ((n & 1) ? kColC : kColB), kb + k_used * kBytes, kIdR, n > 0);
@@ -839,7 +842,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ss.ds_full);
+        if (lane == 0) mbar_arrive(&ss.ds_full[n & 1]);
       }
       if (ok) {
         ok = bar_wait(&ss.done, 0, abort_flag, err, 473);

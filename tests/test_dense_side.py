@@ -946,10 +946,57 @@ def test_hook_bsa_keeps_its_path(cuda):
         near(m(odd, (5, 6, 7)), want_odd, HOOK_REL)
 
 
-def test_dit_switch():
-    from longcat_video.models.longcat_video_dit import LongCatVideoTransformer3DModel
+def test_hook_bsa_conditioning(cuda):
+    """With BSA on, the noise tokens' dense part of the conditioning branch runs on the engine's kernel."""
+    m = hook(cuda)
+    m.enable_bsa, m.bsa_sparsity = True, 0.5
+    x = rand((1, 512, 128), torch.bfloat16, 1, cuda)
+    with torch.no_grad():
+        want = m(x, (8, 8, 8), 4)
+        m.dense_kernels = True
+        near(m(x, (8, 8, 8), 4), want, HOOK_REL)
 
-    d = LongCatVideoTransformer3DModel.from_config(dict(hidden_size=64, depth=2, num_heads=2, enable_dense_kernels=True))
-    assert all(a.dense_kernels and not a.enable_bsa for a in d.attention_modules())
-    d.disable_dense_kernels()
-    assert not any(a.dense_kernels for a in d.attention_modules())
+
+# ------------------------------------------------------------------------------- large sizes
+def test_cache_beyond_32_bits(cuda):
+    """Codes of the last head start behind 2^31 bytes: all keys weigh the same, values are ones in the last 100 tokens."""
+    from longcat_video.models.kv_cache import KVCache8
+
+    Hk, cap = 9, 1 << 21
+    c = KVCache8.allocate(1, Hk, cap, 128, cuda)
+    c.truncate(cap - 100)
+    ones = torch.ones((1, Hk, 100, 128), dtype=torch.bfloat16, device=cuda)
+    ones[:, :8] = 0
+    c.append(ones * 0, ones)
+    assert c.lengths.tolist() == [cap]
+    out = c.attend(rand((1, Hk, 1, 128), torch.bfloat16, 1, cuda)).float()
+    assert (out[:, :8] == 0).all()
+    want = 100 / cap  # one rounding, and sums of 2^21 equal weights in 32 bits, block by block: 2^-24 of it for each join
+    assert ((out[:, 8] - want).abs() <= want * (2.0 ** -8 + 2.0 ** -12)).all()
+
+
+def test_norm_rope_beyond_32_bits(cuda):
+    from longcat_video.models.rope_3d import qk_norm_rope
+
+    grid, H, D = (33, 64, 64), 126, 128  # 2.2e9 values
+    S = grid[0] * grid[1] * grid[2]
+    rope = rope_of(grid, D, cuda)
+    x = torch.empty((1, H, S, D), dtype=torch.bfloat16, device=cuda).normal_()
+    w = torch.ones(D, device=cuda)
+    y = qk_norm_rope(x, q_weight=w, rope=rope)
+    for rows in (slice(0, 3), slice(S - 3, S)):
+        turn = turns(rope, rows.start, 3)
+        ref = ref_norm_rope(x[:, -2:, rows].double(), w.double(), 1e-6, turn)
+        check(y[:, -2:, rows], ref, unit(torch.bfloat16) * ref.abs() + 2.0 ** -20 * ref.abs().amax(-1, keepdim=True))
+
+
+def test_attention_over_many_keys(cuda):
+    """A query tile over 300,000 keys in splits, and a long ragged mask of a few rows."""
+    from longcat_video.models.masked_attention import AttentionMask, masked_attention
+
+    Sk = 300001
+    q, k, v = (rand((1, 2, s, 64), torch.bfloat16, i, cuda) for i, s in enumerate((5, Sk, Sk)))
+    m = AttentionMask.from_ranges(torch.tensor([[[0, Sk], [Sk - 1, Sk], [7, 7], [100, 250000], [299990, Sk]]],
+                                               dtype=torch.int32, device=cuda), Sk)
+    out, lse = masked_attention(q, k, v, m, return_lse=True)
+    check_attention(out, lse, ref_attention(q, k, v, *rows_of(m), 0.125), torch.bfloat16)
