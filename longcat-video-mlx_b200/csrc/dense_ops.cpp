@@ -6,11 +6,12 @@
 // The entries are looked up in the engine's library, which Python has loaded; errors of the C ABI come back as
 // ValueError (arguments) or BSAError, with its message.
 #include <dlfcn.h>
+#include <array>
 #include <cmath>
-#include <mutex>
 #include <optional>
 #include <string>
 #include <torch/extension.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include "../../include/bsa_b200.h"
@@ -19,6 +20,8 @@ namespace {
 
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 namespace py = pybind11;
 
 struct Api {
@@ -66,14 +69,19 @@ void load(const std::string& path, const py::object& error) {
 
 [[noreturn]] void refuse(const std::string& what) { throw py::value_error(what); }
 
+// A CUDA-side failure; becomes BSAError where it reaches Python (autograd's own threads, which hold
+// no interpreter lock, turn what a backward pass throws into RuntimeError).
+struct CudaFailure : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
 void check(int rc, const char* what) {
   if (rc == BSA_OK) return;
   char buf[512] = {0};
   api.bsa_last_error(buf, sizeof(buf));
   const std::string msg = buf[0] ? buf : std::string(what) + " failed";
   if (rc == BSA_ERR_SHAPE || rc == BSA_ERR_DTYPE || rc == BSA_ERR_ALIGN || rc == BSA_ERR_ARG) refuse(msg);
-  PyErr_SetString(cuda_error, (std::string(what) + " failed (code " + std::to_string(rc) + "): " + msg).c_str());
-  throw py::error_already_set();
+  throw CudaFailure(std::string(what) + " failed (code " + std::to_string(rc) + "): " + msg);
 }
 
 int dtype_code(at::ScalarType t) {
@@ -175,11 +183,8 @@ int weights(const Tensor& q, OptTensor& wq, OptTensor& wk) {
   return dtype_code(kind);
 }
 
-py::object norm_rope(const Tensor& q, const OptTensor& k, OptTensor wq, OptTensor wk, double eps, OptTensor tables, int dt,
-                     int dh, int dw, int T, int H, int W, int start) {
-  check_pair(q, k);
-  const Rope rope{std::move(tables), dt, dh, dw, T, H, W, start};
-  rope.check(q);
+std::pair<Tensor, OptTensor> norm_rope_forward(const Tensor& q, const OptTensor& k, OptTensor wq, OptTensor wk, double eps,
+                                               const Rope& rope) {
   const int wcode = weights(q, wq, wk);
   const c10::cuda::CUDAGuard guard(q.device());
   Tensor y0 = like(q);
@@ -191,18 +196,16 @@ py::object norm_rope(const Tensor& q, const OptTensor& k, OptTensor wq, OptTenso
     if (k) x1.emplace(*k);
     check(api.bsa_norm_rope(x0.p(), x0.strides, q.size(1), ptr(wq), ptr(y0), x1 ? x1->p() : nullptr,
                             x1 ? x1->strides : nullptr, k ? k->size(1) : 0, ptr(wk), ptr(y1), dtype_code(q.scalar_type()),
-                            wcode, q.size(0), q.size(2), q.size(3), static_cast<float>(eps), rope.p(), dt, dh, dw, T, H, W,
-                            start, stream_of(q)),
+                            wcode, q.size(0), q.size(2), q.size(3), static_cast<float>(eps), rope.p(), rope.dt, rope.dh,
+                            rope.dw, rope.T, rope.H, rope.W, rope.start, stream_of(q)),
           "bsa_norm_rope");
   }
-  return k ? py::object(py::make_tuple(y0, *y1)) : py::cast(y0);
+  return {y0, y1};
 }
 
 // One or two sides (x, gradient, weight, whether its weight's gradient is wanted): [dx0, dw0, dx1, dw1]
-std::vector<OptTensor> norm_rope_backward(const Tensor& x0, const Tensor& g0, OptTensor w0, bool want0, const OptTensor& x1,
-                                          const OptTensor& g1, OptTensor w1, bool want1, double eps, OptTensor tables,
-                                          int dt, int dh, int dw, int T, int H, int W, int start) {
-  const Rope rope{std::move(tables), dt, dh, dw, T, H, W, start};
+std::array<Tensor, 4> norm_rope_backward(const Tensor& x0, const Tensor& g0, OptTensor w0, bool want0, const OptTensor& x1,
+                                         const OptTensor& g1, OptTensor w1, bool want1, double eps, const Rope& rope) {
   const int wcode = weights(x0, w0, w1);
   const c10::cuda::CUDAGuard guard(x0.device());
   const int64_t D = x0.size(3);
@@ -228,11 +231,92 @@ std::vector<OptTensor> norm_rope_backward(const Tensor& x0, const Tensor& g0, Op
               a.p(), a.strides, ga.p(), ga.strides, x0.size(1), ptr(w0), ptr(dx0), static_cast<float*>(ptr(dw0)),
               b ? b->p() : nullptr, b ? b->strides : nullptr, gb ? gb->p() : nullptr, gb ? gb->strides : nullptr,
               x1 ? x1->size(1) : 0, ptr(w1), ptr(dx1), static_cast<float*>(ptr(dw1)), dtype_code(x0.scalar_type()), wcode,
-              x0.size(0), x0.size(2), D, static_cast<float>(eps), rope.p(), dt, dh, dw, T, H, W, start, ptr(scratch),
-              stream_of(x0)),
+              x0.size(0), x0.size(2), D, static_cast<float>(eps), rope.p(), rope.dt, rope.dh, rope.dw, rope.T, rope.H, rope.W,
+              rope.start, ptr(scratch), stream_of(x0)),
           "bsa_norm_rope_backward");
   }
-  return {dx0, dw0, dx1, dw1};
+  const Tensor none;
+  return {dx0, dw0.value_or(none), dx1.value_or(none), dw1.value_or(none)};
+}
+
+// Whether a graph has to be recorded.  Refused in a capture: a leaf whose gradient node an eager graph still holds.  Its
+// gradient is added up on that graph's stream, which the capture cannot reach; autograd then ends the process.
+bool any_grad(std::initializer_list<const OptTensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  bool any = false;
+  for (const OptTensor* t : ts) any = any || (*t && (*t)->requires_grad());
+  if (!any || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return any;
+  for (const OptTensor* t : ts)
+    if (*t && (*t)->requires_grad() && (*t)->is_leaf())
+      if (const auto node = torch::autograd::impl::try_get_grad_accumulator(**t))
+        if (const auto s = node->stream(); s && *s != c10::cuda::getCurrentCUDAStream(s->device_index()).unwrap())
+          refuse("an eager graph of this leaf is alive on another stream: drop its outputs before the capture");
+  return any;
+}
+
+// Called in a backward pass: autograd records it only for create_graph.
+void first_order() {
+  if (at::GradMode::is_enabled()) throw std::runtime_error("these gradients cannot be differentiated again (create_graph=True)");
+}
+
+OptTensor some(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+class NormRope : public torch::autograd::Function<NormRope> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& wq,
+                               const OptTensor& wk, const OptTensor& tables, double eps, std::array<int, 7> r) {
+    const Rope rope{tables, r[0], r[1], r[2], r[3], r[4], r[5], r[6]};
+    const auto y = norm_rope_forward(q, k, wq, wk, eps, rope);
+    const Tensor none;
+    ctx->save_for_backward({q, k.value_or(none), wq.value_or(none), wk.value_or(none), tables.value_or(none)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["rope"] = std::vector<int64_t>(r.begin(), r.end());
+    ctx->set_materialize_grads(false);
+    return y.second ? variable_list{y.first, *y.second} : variable_list{y.first};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order();
+    const variable_list saved = ctx->get_saved_variables();
+    const auto r = ctx->saved_data["rope"].toIntVector();
+    const Rope rope{some(saved[4]),          static_cast<int>(r[0]), static_cast<int>(r[1]), static_cast<int>(r[2]),
+                    static_cast<int>(r[3]), static_cast<int>(r[4]), static_cast<int>(r[5]), static_cast<int>(r[6])};
+    // the edges count the tensors that were given: q, k, wq, wk, tables
+    bool need[4];
+    for (int i = 0, edge = 0; i < 4; ++i) need[i] = saved[i].defined() && ctx->needs_input_grad(edge++);
+    int sides[2], n = 0;
+    for (int i = 0; i < 2; ++i)
+      if (saved[i].defined() && grads[i].defined() && (need[i] || need[2 + i])) sides[n++] = i;
+    variable_list res(7);
+    if (n) {
+      auto grad = [&](int i) { return grads[i].to(saved[i].scalar_type()); };
+      const int a = sides[0], b = sides[n - 1];
+      const auto got = norm_rope_backward(saved[a], grad(a), some(saved[2 + a]), need[2 + a], n > 1 ? some(saved[b]) : std::nullopt,
+                                          n > 1 ? OptTensor(grad(b)) : std::nullopt,
+                                          n > 1 ? some(saved[2 + b]) : std::nullopt, n > 1 && need[2 + b],
+                                          ctx->saved_data["eps"].toDouble(), rope);
+      for (int s = 0; s < n; ++s) {
+        const int i = sides[s];
+        if (need[i]) res[i] = got[2 * s];
+        if (need[2 + i]) res[2 + i] = got[2 * s + 1].to(saved[2 + i].scalar_type());
+      }
+    }
+    return res;
+  }
+};
+
+py::object norm_rope(const Tensor& q, const OptTensor& k, const OptTensor& wq, const OptTensor& wk, double eps,
+                     const OptTensor& tables, int dt, int dh, int dw, int T, int H, int W, int start) {
+  check_pair(q, k);
+  const Rope rope{tables, dt, dh, dw, T, H, W, start};
+  rope.check(q);
+  const OptTensor q0(q);
+  if (any_grad({&q0, &k, &wq, &wk})) {
+    const variable_list y = NormRope::apply(q, k, wq, wk, tables, eps, std::array<int, 7>{dt, dh, dw, T, H, W, start});
+    return k ? py::object(py::make_tuple(y[0], y[1])) : py::cast(y[0]);
+  }
+  const auto y = norm_rope_forward(q, k, wq, wk, eps, rope);
+  return k ? py::object(py::make_tuple(y.first, *y.second)) : py::cast(y.first);
 }
 
 // ------------------------------------------------------------------------------------------- key intervals
@@ -354,18 +438,14 @@ struct Output {
   }
 };
 
-// (out, lse or None, rest or None)
-py::tuple masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, int64_t mask_batch,
-                           int64_t mask_table, int64_t mask_q, int64_t mask_k, double sm_scale, double softcap,
+struct Attended {
+  Tensor out;
+  OptTensor lse, rest;
+};
+
+Attended attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Mask& m, double sm_scale, double softcap,
                            const OptTensor& out, bool want_lse, bool want_rest) {
-  check_qkv(q, k, v);
-  check_scale(sm_scale, softcap);
   const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
-  if (mask && (mask_q != Sq || mask_k != Sk))
-    refuse("the mask is for " + std::to_string(mask_q) + " queries and " + std::to_string(mask_k) + " keys, got " +
-           std::to_string(Sq) + " and " + std::to_string(Sk));
-  const Mask m(q, mask, mask_batch, mask_table);
-  check_out(q, out);
   const c10::cuda::CUDAGuard guard(q.device());
   Output o(q, out);
   OptTensor lse, rest;
@@ -386,19 +466,18 @@ py::tuple masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     if (rest) rest->zero_();
     if (lse) lse->fill_(-INFINITY);
   }
-  return py::make_tuple(o.done(out), lse, rest);
+  return {o.done(out), lse, rest};
 }
 
-std::vector<OptTensor> masked_attention_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-                                                 const Tensor& rest, const Tensor& lse, const Tensor& grad,
-                                                 const OptTensor& mask, int64_t mask_batch, int64_t mask_table,
-                                                 double sm_scale, double softcap, bool want_q, bool want_kv) {
+std::array<Tensor, 3> attention_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                                         const Tensor& rest, const Tensor& lse, const Tensor& grad, const Mask& m,
+                                         double sm_scale, double softcap, bool want_q, bool want_kv) {
   const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
-  const Mask m(q, mask, mask_batch, mask_table);
   const c10::cuda::CUDAGuard guard(q.device());
   const bool empty = !q.numel() || !Sk;
   auto grad_of = [&](const Tensor& t) { return empty ? at::zeros(t.sizes(), t.options()) : like(t); };
-  OptTensor dq, dk, dv;
+  Tensor dq, dk, dv;
+  auto to = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
   if (want_q) dq = grad_of(q);
   if (want_kv) {
     dk = grad_of(k);
@@ -410,11 +489,64 @@ std::vector<OptTensor> masked_attention_backward(const Tensor& q, const Tensor& 
     check(api.bsa_masked_attention_backward(
               a.p(), b.p(), c.p(), o.p(), ptr(rest), g.p(), static_cast<const float*>(ptr(lse)),
               dtype_code(q.scalar_type()), B, H, Hk, Sq, Sk, D, a.strides, b.strides, c.strides, o.strides, g.strides,
-              m.ranges, m.table, m.batch, static_cast<float>(sm_scale), static_cast<float>(softcap), ptr(dq), ptr(dk),
-              ptr(dv), ptr(scratch), stream_of(q)),
+              m.ranges, m.table, m.batch, static_cast<float>(sm_scale), static_cast<float>(softcap), to(dq), to(dk), to(dv),
+              ptr(scratch), stream_of(q)),
           "bsa_masked_attention_backward");
   }
   return {dq, dk, dv};
+}
+
+class MaskedAttention : public torch::autograd::Function<MaskedAttention> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const OptTensor& mask, int64_t mask_batch, int64_t mask_table, double sm_scale,
+                               double softcap) {
+    const Attended a = attention_forward(q, k, v, Mask(q, mask, mask_batch, mask_table), sm_scale, softcap, std::nullopt,
+                                         true, true);
+    ctx->save_for_backward({q, k, v, a.out, *a.rest, *a.lse, mask.value_or(Tensor())});
+    ctx->saved_data["mask"] = std::vector<int64_t>{mask_batch, mask_table};
+    ctx->saved_data["scale"] = std::vector<double>{sm_scale, softcap};
+    ctx->mark_non_differentiable({*a.lse});
+    ctx->set_materialize_grads(false);
+    return {a.out, *a.lse};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order();
+    variable_list res(8);
+    if (!grads[0].defined()) return res;
+    const variable_list s = ctx->get_saved_variables();
+    const auto at = ctx->saved_data["mask"].toIntVector();
+    const auto scale = ctx->saved_data["scale"].toDoubleVector();
+    const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
+    const auto d = attention_backward(s[0], s[1], s[2], s[3], s[4], s[5], grads[0].to(s[0].scalar_type()),
+                                      Mask(s[0], some(s[6]), at[0], at[1]), scale[0], scale[1], need[0],
+                                      need[1] || need[2]);
+    for (int i = 0; i < 3; ++i)
+      if (need[i]) res[i] = d[i];
+    return res;
+  }
+};
+
+// (out, lse or None)
+py::tuple masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, int64_t mask_batch,
+                           int64_t mask_table, int64_t mask_q, int64_t mask_k, double sm_scale, double softcap,
+                           const OptTensor& out, bool want_lse) {
+  check_qkv(q, k, v);
+  check_scale(sm_scale, softcap);
+  if (mask && (mask_q != q.size(2) || mask_k != k.size(2)))
+    refuse("the mask is for " + std::to_string(mask_q) + " queries and " + std::to_string(mask_k) + " keys, got " +
+           std::to_string(q.size(2)) + " and " + std::to_string(k.size(2)));
+  const Mask m(q, mask, mask_batch, mask_table);
+  check_out(q, out);
+  const OptTensor q0(q), k0(k), v0(v);
+  if (any_grad({&q0, &k0, &v0})) {
+    if (out) refuse("out= is for calls without gradients");
+    const variable_list r = MaskedAttention::apply(q, k, v, mask, mask_batch, mask_table, sm_scale, softcap);
+    return py::make_tuple(r[0], r[1]);
+  }
+  const Attended a = attention_forward(q, k, v, m, sm_scale, softcap, out, want_lse, false);
+  return py::make_tuple(a.out, a.lse);
 }
 
 // ---------------------------------------------------------------------------------------------- 8-bit cache
@@ -522,21 +654,25 @@ struct Cache {
     const auto kv = n ? unpack(t, k, v) : unpack(t, std::nullopt, std::nullopt);
     const py::tuple m = attention_ranges(py::cast(kc.device()), Sq, cap + n, B, std::nullopt, causal, 0, std::nullopt,
                                          std::nullopt, std::nullopt, std::nullopt, len, n);
-    const py::tuple r = masked_attention(q, kv.first, kv.second, py::cast<Tensor>(m[0]), B, py::cast<int64_t>(m[2]), Sq,
-                                         cap + n, s, 0.0, out, false, false);
-    return py::cast<Tensor>(r[0]);
+    const OptTensor buf = py::cast<Tensor>(m[0]);
+    return attention_forward(q, kv.first, kv.second, Mask(q, buf, B, py::cast<int64_t>(m[2])), s, 0.0, out, false, false).out;
   }
 };
 
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const CudaFailure& e) {
+      PyErr_SetString(cuda_error, e.what());
+    }
+  });
   m.def("load", &load, "The engine's library, and the exception of its CUDA errors");
   m.def("norm_rope", &norm_rope);
-  m.def("norm_rope_backward", &norm_rope_backward);
   m.def("attention_ranges", &attention_ranges);
   m.def("masked_attention", &masked_attention);
-  m.def("masked_attention_backward", &masked_attention_backward);
   py::class_<Cache>(m, "Cache")
       .def(py::init<Tensor, Tensor, Tensor, Tensor, Tensor>())
       .def("append", &Cache::append)

@@ -2,8 +2,8 @@
 
 The dense side of the attention hook on the engine's own kernels.  A mask is a key interval [lo, hi) for each
 query row (:class:`AttentionMask`), built once for a batch and used by every layer; no Sq x Sk tensor exists.
-``masked_attention`` is differentiable; its gradients are computed without atomics, so two runs give the same
-bits.
+``masked_attention`` is differentiable, once (``create_graph=True`` is refused); its gradients are computed without
+atomics, so two runs give the same bits.
 """
 
 from __future__ import annotations
@@ -73,28 +73,6 @@ class AttentionMask:
 _NO_MASK = (None, 1, 0, 0, 0)
 
 
-class _MaskedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, mask, sm_scale, softcap):
-        out, lse, rest = _dense.ops().masked_attention(q, k, v, *mask, sm_scale, softcap, None, True, True)
-        ctx.save_for_backward(q, k, v, out, rest, lse)
-        ctx.rest = (*mask[:3], sm_scale, softcap)
-        ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
-        return out, lse
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad, _):
-        if grad is None:
-            return (None,) * 6
-        q, k, v, out, rest, lse = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, dv = _dense.ops().masked_attention_backward(q, k, v, out, rest, lse, grad.to(q.dtype), *ctx.rest, need[0],
-                                                            need[1] or need[2])
-        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None
-
-
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[AttentionMask] = None, *,
                      sm_scale: Optional[float] = None, softcap: float = 0.0, return_lse: bool = False,
                      out: Optional[torch.Tensor] = None):
@@ -107,10 +85,5 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     preallocated [B, H, Sq, D] result (not with gradients)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale
     args = _NO_MASK if mask is None else mask._args()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        if out is not None:
-            raise ValueError("out= is for calls without gradients")
-        o, lse = _MaskedAttention.apply(q, k, v, args, scale, softcap)
-    else:
-        o, lse, _ = _dense.ops().masked_attention(q, k, v, *args, scale, softcap, out, return_lse, False)
+    o, lse = _dense.ops().masked_attention(q, k, v, *args, scale, softcap, out, return_lse)
     return (o, lse) if return_lse else o

@@ -106,36 +106,6 @@ class RotaryPositionalEmbedding(torch.nn.Module):
         return q_r.to(out_dtype), k_r.to(out_dtype)
 
 
-class _NormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, eps, rope):
-        ctx.save_for_backward(q, k, q_weight, k_weight)
-        ctx.rest = (eps, rope)
-        ctx.set_materialize_grads(False)
-        return _dense.ops().norm_rope(q, k, q_weight, k_weight, eps, *rope)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        q, k, q_weight, k_weight = ctx.saved_tensors
-        eps, rope = ctx.rest
-        need = ctx.needs_input_grad
-        sides = [(i, x, w) for i, (x, w) in enumerate(((q, q_weight), (k, k_weight)))
-                 if x is not None and grads[i] is not None and (need[i] or need[2 + i])]
-        res = [None] * 6
-        if sides:
-            args = []
-            for i, x, w in sides:
-                args += [x, grads[i].to(x.dtype), w, need[2 + i]]
-            if len(sides) == 1:
-                args += [None, None, None, False]
-            got = _dense.ops().norm_rope_backward(*args, eps, *rope)
-            for (i, _, w), dx, dw in zip(sides, got[::2], got[1::2]):
-                res[i] = dx if need[i] else None
-                res[2 + i] = dw.to(w.dtype) if dw is not None else None
-        return tuple(res)
-
-
 _NO_ROPE = (None, 0, 0, 0, 0, 0, 0, 0)
 
 
@@ -148,7 +118,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Op
     place.  A weight [D] turns its tensor's norm on.  ``rope``: :class:`RopeTables` or (tables, axis dims, grid); the
     tokens stand at places ``start`` .. ``start`` + S - 1 of the grid (t-major), so a continuation behind n cached
     tokens passes ``start=n``.  Sums are fp32 and the result is rounded once (the unfused form rounds after each
-    step).  Returns contiguous tensors: (q, k), or q alone."""
+    step).  Gradients are first-order (``create_graph=True`` is refused).  Returns contiguous tensors: (q, k), or q alone."""
     if q_weight is None and k_weight is None and rope is None:
         raise ValueError("nothing to do: give norm weights, rope tables or both")
     if k is None and k_weight is not None:
@@ -158,6 +128,4 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Op
     else:
         tables, dims, grid = rope.native_args() if hasattr(rope, "native_args") else rope
         args = (tables, *dims, *grid, start)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _NormRope.apply(q, k, q_weight, k_weight, eps, args)
     return _dense.ops().norm_rope(q, k, q_weight, k_weight, eps, *args)

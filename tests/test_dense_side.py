@@ -595,6 +595,52 @@ def test_training_step_in_a_graph(cuda):
         assert all(torch.equal(a, b) for a, b in zip(res, step()))
 
 
+def test_gradient_refusals(cuda):
+    """Second derivatives; a capture while an eager graph of the same leaf lives on another stream."""
+    from longcat_video.models.masked_attention import masked_attention
+    from longcat_video.models.rope_3d import qk_norm_rope
+
+    x = rand((1, 2, 20, 64), torch.bfloat16, 1, cuda).requires_grad_()
+    w = torch.ones(64, device=cuda, requires_grad=True)
+    for f in (lambda: masked_attention(x, x, x), lambda: qk_norm_rope(x, q_weight=w)):
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(f().sum(), x, create_graph=True)
+        eager = f()
+        with pytest.raises(ValueError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                f()
+        del eager
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = torch.autograd.grad(f(), x, torch.ones_like(x))[0]
+        graph.replay()
+        assert torch.equal(res, torch.autograd.grad(f(), x, torch.ones_like(x))[0])
+
+
+@pytest.mark.parametrize("want", [(0,), (1,), (2,), (3,), (0, 3), (1, 2), (2, 3)])
+def test_norm_rope_some_gradients(cuda, want):
+    """Any part of q, k and their weights, with and without rotation: as when all four are asked for."""
+    from longcat_video.models.rope_3d import qk_norm_rope
+
+    x = [rand((2, n, 30, 64), torch.bfloat16, n, cuda) for n in (4, 2)]
+    x += [rand((64,), torch.bfloat16, 5 + i, cuda) for i in range(2)]
+    g = [rand((2, n, 30, 64), torch.bfloat16, 7 + n, cuda) for n in (4, 2)]
+    for rope in (None, rope_of((1, 5, 6), 64, cuda)):
+        def grads(want):
+            leaves = [t.detach().requires_grad_(i in want) for i, t in enumerate(x)]
+            out = qk_norm_rope(*leaves, rope=rope)
+            at = [i for i in range(2) if out[i].requires_grad]
+            return torch.autograd.grad([out[i] for i in at], [leaves[i] for i in want], [g[i] for i in at])
+
+        full = grads((0, 1, 2, 3))
+        for a, i in zip(grads(want), want):
+            assert a.dtype == torch.bfloat16
+            if i < 2:
+                assert torch.equal(a, full[i])
+            else:  # rows added up in another order (fp32, 240 terms of at most 16), then one rounding: a bf16 step
+                torch.testing.assert_close(a, full[i], rtol=2.0**-7, atol=240 * 240 * 16 * 2.0**-24)
+
+
 def test_attention_refusals(cuda):
     from longcat_video.models.masked_attention import AttentionMask, masked_attention
 
