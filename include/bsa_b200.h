@@ -198,8 +198,8 @@ int bsa_forward_noalloc(const void* q, const void* k, const void* v, int dtype, 
  * w0 / w1 (w_dtype, [D]; NULL: no norm), rope (NULL: no rotation) as in bsa_mean_pool; the tokens of x stand at
  * places start .. start + S - 1 of the rope grid.  x1 NULL: one tensor.  Outputs are contiguous.
  * bsa_norm_rope_backward: gradients dx (contiguous) of the inputs and dw ([D] fp32, NULL: none) of the weights
- * from the outputs' gradients g; scratch (bsa_norm_rope_backward_scratch_bytes(), H1 0 for one tensor) is needed for the weights'.
- * Sums are taken in a fixed order. */
+ * from the outputs' gradients g; scratch (bsa_norm_rope_backward_scratch_bytes() bytes, H1 0 for one tensor) is needed
+ * for the weights'.  Sums are taken in a fixed order. */
 int bsa_norm_rope(const void* x0, const int64_t* x0_strides, int H0, const void* w0, void* y0, const void* x1,
                   const int64_t* x1_strides, int H1, const void* w1, void* y1, int dtype, int w_dtype, int B, int S,
                   int D, float eps, const float* rope, int rope_dt, int rope_dh, int rope_dw, int rope_T, int rope_H,
@@ -228,10 +228,10 @@ int bsa_attention_ranges(int32_t* ranges, int32_t* table, int batch, int Sq, int
  * h reads key head h / (H / Hk)), fp16 or bf16.  ranges / table (both NULL: every key) hold ranges_batch (1 or B)
  * entries.  softcap > 0: scores are softcap * tanh(s / softcap).  A row without keys gives zeros, and -inf in lse
  * ([B, H, Sq] fp32, natural logarithm, NULL: not wanted).  out_rest ([B, H, Sq, D] in dtype, contiguous, NULL: not
- * wanted) receives what the rounding of out left over; the backward needs it.  scratch: bsa_masked_attention_scratch_bytes() bytes
- * (0: none needed).  Scores of unseen keys never count, whatever they hold; so do values of keys that no row
- * of the same 256 rows sees.  A value that is infinite or NaN and seen by one row can reach another row of
- * the same tile. */
+ * wanted) receives what the rounding of out left over; the backward needs it.  scratch:
+ * bsa_masked_attention_scratch_bytes() bytes (0: none needed).  Scores of unseen keys never count, whatever they
+ * hold; nor do values of keys that no row of the same 128 rows sees.  A value that is infinite or NaN and seen by
+ * one row can reach another row of the same 128. */
 int64_t bsa_masked_attention_scratch_bytes(int B, int H, int Sq, int Sk, int D);
 int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype, int B, int H, int Hk, int Sq, int Sk,
                          int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
@@ -239,8 +239,8 @@ int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype,
                          void* out, const int64_t* out_strides, void* out_rest, float* lse, void* scratch,
                          void* stream);
 
-/* bsa_masked_attention_backward: gradients of that call from its out, out_rest and lse and the gradient of out.  dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may
- * be NULL.  Shared key heads sum over their query heads; keys no row sees get zeros.  No atomics: the same bits
+/* bsa_masked_attention_backward: gradients of that call from its out, out_rest and lse and the gradient of out.
+ * dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may be NULL.  Shared key heads sum over their query heads; keys no row sees get zeros.  No atomics: the same bits
  * every time.  scratch: bsa_masked_attention_backward_scratch_bytes() bytes (ranges_batch 0 without ranges). */
 int64_t bsa_masked_attention_backward_scratch_bytes(int B, int H, int Sq, int ranges_batch);
 int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* out_rest,

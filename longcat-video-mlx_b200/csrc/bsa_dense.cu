@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int pair = 1 + (warp & 3);  // named barrier of the two warps that share 32 rows
     const bool live = row < p.Sq;
     {
-      int lo = 0, hi = p.Sk;
+      int lo = 0, hi = live ? p.Sk : 0;  // rows behind the last see nothing, and choose nothing
       if (p.ranges && live) {
         const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
         lo = r.x;

@@ -24,6 +24,7 @@
 // that no row of the tile sees (dq) are zeroed in shared memory, since 0 * NaN would be NaN.
 // Every wait is bounded (bsa_ptx.cuh).
 #include <climits>
+#include <type_traits>
 #include "bsa_dense.cuh"
 #include "bsa_rows.cuh"
 
@@ -34,6 +35,10 @@ __device__ int g_dense_bwd_err;
 
 constexpr int kBwdThreads = 320;
 constexpr uint32_t kColA = 0, kColB = 128, kColC = 256, kColD = 384;  // tensor memory, 128 columns each
+// Up to this many steps of a CTA, p and ds go through the second products as their rounding and what it left over, so
+// that a gradient carries no error but its own rounding's.  Beyond, the one rounding of p and ds to the tensors' type adds
+// as much again (1.4 times the error).
+constexpr int kFineSteps = 4;
 
 struct BwdParams {
   const int2* ranges;   // [Bm][Sq], null: all keys
@@ -44,6 +49,8 @@ struct BwdParams {
   float scale_log2, sm_scale, cap_in, cap_log2;
   float* lse2;          // [B * H][Sq_pad]: lse in log2 (+inf: no keys)
   float* delta;         // [B * H][Sq_pad]
+  float* up;            // fp16: [B * H][Sq_pad], what dq's row of ds is raised by (log2), then its least of 16 rows each
+  int heads;            // B * H
   float cap_inv, cap_mask;  // 1 / cap_log2, and a score below every capped one by 2^300
   int2* rng;            // [Bm][Sq_pad]: ranges, padded with empty ones
   const float* lse;
@@ -56,43 +63,72 @@ struct BwdParams {
 // 16 lanes to a row.  delta in fp32 from o to twice its type's bits: do.v - delta is a difference of near values where
 // few keys share a row, and with the rounded o alone dq and dk came out with twice the error of their own rounding
 // (0.0034 against 0.0017 on causal documents in bf16).
+//
+// fp16 keeps 11 bits only above 2^-14, and ds is a product of p, which falls with the number of keys, and of do, which may
+// be small altogether.  So p and ds are raised by powers of two, which their sums are lowered by again: p by 2^kUp, ds of
+// a row by the 2^n, 0 <= n <= kUp, that brings |do_i| below 2^3 (dkv: the least of a CTA's rows).  |ds_ij| is at
+// most 2 |do_i| |v_j|, so it stays below 65504 with |v_j| up to 4,000.
+constexpr int kUp = 15;
 template <typename T>
 __global__ void __launch_bounds__(256) stats_kernel(const BwdParams p) {
   constexpr int kLanes = 16;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   const int row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const int bh = blockIdx.y;
-  const int b = bh / p.H, h = bh - b * p.H;
-  float dot = 0.f;
   const bool on = row < p.Sq;
-  if (on && 8 * lane < p.D) {
-    Row8<T> o, g, r;
-    r.load(static_cast<const T*>(p.o_lo) + (static_cast<long long>(bh) * p.Sq + row) * p.D + 8 * lane);
-    o.load(static_cast<const T*>(p.o.p) + b * p.o.sb + h * p.o.sh + row * p.o.ss + 8 * lane);
-    g.load(static_cast<const T*>(p.g.p) + b * p.g.sb + h * p.g.sh + row * p.g.ss + 8 * lane);
-    float a[8], c[8], d[8];
-    o.get(a);
-    g.get(c);
-    r.get(d);
+  __shared__ int least[8];
+  for (int bh = blockIdx.y; bh < p.heads; bh += gridDim.y) {
+    const int b = bh / p.H, h = bh - b * p.H;
+    const long long at = static_cast<long long>(bh) * p.Sq_pad + row;
+    float dot = 0.f, norm2 = 0.f;
+    if (on && 8 * lane < p.D) {
+      Row8<T> o, g, r;
+      r.load(static_cast<const T*>(p.o_lo) + (static_cast<long long>(bh) * p.Sq + row) * p.D + 8 * lane);
+      o.load(static_cast<const T*>(p.o.p) + b * p.o.sb + h * p.o.sh + row * p.o.ss + 8 * lane);
+      g.load(static_cast<const T*>(p.g.p) + b * p.g.sb + h * p.g.sh + row * p.g.ss + 8 * lane);
+      float a[8], c[8], d[8];
+      o.get(a);
+      g.get(c);
+      r.get(d);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dot = fmaf(a[e] + d[e], c[e], dot);
-  }
-#pragma unroll
-  for (int s = kLanes / 2; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-  if (lane == 0 && row < p.Sq_pad) {
-    float l = INFINITY;
-    if (on) {
-      l = p.lse[static_cast<long long>(bh) * p.Sq + row] * 1.4426950408889634f;
-      if (l == -INFINITY) {
-        l = INFINITY;  // e^(z - lse) is 0 then
-        dot = 0.f;
+      for (int e = 0; e < 8; ++e) {
+        dot = fmaf(a[e] + d[e], c[e], dot);
+        norm2 = fmaf(c[e], c[e], norm2);
       }
     }
-    p.lse2[static_cast<long long>(bh) * p.Sq_pad + row] = l;
-    p.delta[static_cast<long long>(bh) * p.Sq_pad + row] = on ? dot : 0.f;
-    if (h == 0 && b < p.Bm && p.rng)
-      p.rng[static_cast<long long>(b) * p.Sq_pad + row] =
-          on ? p.ranges[static_cast<long long>(b) * p.Sq + row] : make_int2(0, 0);
+#pragma unroll
+    for (int s = kLanes / 2; s > 0; s >>= 1) {
+      dot += __shfl_xor_sync(0xffffffffu, dot, s);
+      if constexpr (kHalf) norm2 += __shfl_xor_sync(0xffffffffu, norm2, s);
+    }
+    float l = INFINITY;
+    if (on) l = p.lse[static_cast<long long>(bh) * p.Sq + row] * 1.4426950408889634f;
+    const bool keys = on && l != -INFINITY;
+    if (!keys) l = INFINITY;  // e^(z - lse) is 0 then
+    if (lane == 0) {
+      p.lse2[at] = kHalf ? l - kUp : l;
+      p.delta[at] = keys ? dot : 0.f;
+      if (h == 0 && b < p.Bm && p.rng)
+        p.rng[static_cast<long long>(b) * p.Sq_pad + row] =
+            on ? p.ranges[static_cast<long long>(b) * p.Sq + row] : make_int2(0, 0);
+    }
+    if constexpr (kHalf) {
+      // |do|^2 < 2^(e + 1): n = floor(3 - (e + 1) / 2)
+      const int e = static_cast<int>(__float_as_uint(norm2) >> 23) - 127;
+      const int n = keys ? min(max((5 - e) >> 1, 0), kUp) : kUp;
+      if (lane == 0) p.up[at] = static_cast<float>(n);
+      const int both = __reduce_min_sync(0xffffffffu, n);
+      if ((threadIdx.x & 31) == 0) least[threadIdx.x >> 5] = both;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int m = least[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) m = min(m, least[w]);
+        (p.up + static_cast<long long>(p.heads) * p.Sq_pad)[static_cast<long long>(bh) * (p.Sq_pad / 16) + blockIdx.x] =
+            static_cast<float>(m);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -164,6 +200,14 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uin
     umma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, desc_rows(b, kk), id, add || kk > 0);
 }
 
+// What the 16-bit roundings of two values leave over, as a pair
+template <bool kBF16>
+__device__ __forceinline__ uint32_t rest16(uint32_t pair, float x0, float x1) {
+  float lo, hi;
+  unpack16<kBF16>(pair, lo, hi);
+  return pack16<kBF16>(x0 - lo, x1 - hi);
+}
+
 // One warp's 32 rows x (DP / 2) columns of an accumulator, times f, to 16-bit rows of a tensor.
 template <int DP, bool kBF16>
 __device__ __forceinline__ void store_acc(uint32_t addr, int col0, float f, void* out, long long off, int D, bool live,
@@ -194,13 +238,15 @@ __device__ __forceinline__ void store_acc(uint32_t addr, int col0, float f, void
 // One warp's 32 rows x (DP / 2) columns of an accumulator to shared memory as fp32, [4 columns][row][4], so that lanes
 // write side by side.
 template <int DP>
-__device__ __forceinline__ void to_shared(uint32_t addr, int half, int row, uint8_t* dst, bool some) {
+__device__ __forceinline__ void to_shared(uint32_t addr, int half, int row, float f, uint8_t* dst, bool some) {
 #pragma unroll 1
   for (int c = 0; c < DP / 64; ++c) {
     const int c0 = half * (DP / 2) + 32 * c;
     uint32_t r[32];
     if (some) {
       tmem_read32(addr + c0, r);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
     } else {
 #pragma unroll
       for (int e = 0; e < 32; ++e) r[e] = 0u;
@@ -242,6 +288,7 @@ struct DkvSmem {
   uint32_t tmem;
   int abort_flag;
   int first, last;
+  int up;  // fp16: what ds is raised by (log2)
 };
 template <int DP>
 constexpr int dkv_smem_bytes() { return DkvSmem<DP>::kTiles + static_cast<int>(sizeof(DkvSmem<DP>)) + 1024; }
@@ -288,6 +335,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     ss.abort_flag = 0;
     ss.first = table ? INT_MAX : 0;
     ss.last = table ? -1 : p.q_tiles - 1;
+    ss.up = kUp;
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -312,6 +360,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t tmem = ss.tmem;
   const int first = ss.first, last = ss.last;
   const bool some = first <= last;
+  if constexpr (!kBF16) {
+    if (some) {
+      const int runs = 8 * (last - first + 1);
+      const float* from = p.up + static_cast<long long>(p.heads) * p.Sq_pad +
+                          (static_cast<long long>(b) * p.H + hk * p.G + g_first) * (p.Sq_pad / 16) + 8 * first;
+      float least = kUp;
+      for (int g = 0; g < g_count; ++g)
+        for (int i = tid; i < runs; i += kBwdThreads) least = fminf(least, from[g * static_cast<long long>(p.Sq_pad / 16) + i]);
+      atomicMin(&ss.up, static_cast<int>(least));
+    }
+    __syncthreads();
+  }
+  const bool fine = some && static_cast<long long>(g_count) * (last - first + 1) <= kFineSteps;
   volatile int* abort_flag = &ss.abort_flag;
   int* err = &g_dense_bwd_err;
   // every role walks the same tiles: `step(g, i, tab)` returns false to stop
@@ -414,6 +475,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!bar_wait(&ss.ds_full, static_cast<uint32_t>(m & 1), abort_flag, err, 411)) return false;
         tc_fence_after();
         mma_rows(tmem + kColD, tmem + kColB, qb + q_prev * kBytes, kIdR, m > 0);
+        if (fine) mma_rows(tmem + kColD, tmem + kColB + 32, qb + q_prev * kBytes, kIdR, true);
         umma_commit(&ss.q_empty[q_prev]);
         return true;
       };
@@ -425,6 +487,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             if (!bar_wait(&ss.p_full, static_cast<uint32_t>((n - 1) & 1), abort_flag, err, 413)) return false;
             tc_fence_after();
             mma_rows(tmem + kColC, tmem + kColA, gb + g_prev * kBytes, kIdR, n > 1);
+            if (fine) mma_rows(tmem + kColC, tmem + kColA + 32, gb + g_prev * kBytes, kIdR, true);
             umma_commit(&ss.g_empty[g_prev]);
           }
           if (!bar_wait(&ss.q_full[rq.slot], rq.phase, abort_flag, err, 414)) return false;
@@ -447,6 +510,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (ok) {
         tc_fence_after();
         mma_rows(tmem + kColC, tmem + kColA, gb + g_prev * kBytes, kIdR, n > 1);
+        if (fine) mma_rows(tmem + kColC, tmem + kColA + 32, gb + g_prev * kBytes, kIdR, true);
         ok = finish(n - 1);
       }
       if (ok) umma_commit(&ss.done);
@@ -461,6 +525,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int half = warp >> 2;
     const uint32_t la = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     const int key = key0 + 32 * (warp & 3) + lane;
+    const float raise = kBF16 ? 1.f : __uint_as_float(static_cast<uint32_t>(127 + ss.up - kUp) << 23);  // of ds over p's
     bool ok = true;
     if (some) {
       Ring<S::kQ> rq;
@@ -493,21 +558,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if constexpr (kCap) capped64(r, p.cap_in, p.cap_log2);
         if (border) put_masked(r, seen, __float_as_uint(kCap ? p.cap_mask : -INFINITY));
         uint32_t pk[32];
+        auto weights = [&](auto split) {
+          uint32_t lo[32];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float4 l4 = ls[e];
-          const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-          float x[4];
+          for (int e = 0; e < 16; ++e) {
+            const float4 l4 = ls[e];
+            const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+            float x[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float s = __uint_as_float(r[4 * e + c]);
-            x[c] = ex2_approx(kCap ? s - lv[c] : fmaf(s, p.scale_log2, -lv[c]));
-            const float u = s * p.cap_inv;  // tanh
-            r[4 * e + c] = __float_as_uint(kCap ? x[c] * fmaf(-u, u, 1.f) : x[c]);
+            for (int c = 0; c < 4; ++c) {
+              const float s = __uint_as_float(r[4 * e + c]);
+              x[c] = ex2_approx(kCap ? s - lv[c] : fmaf(s, p.scale_log2, -lv[c]));
+              const float u = s * p.cap_inv;  // tanh
+              r[4 * e + c] = __float_as_uint(kCap ? x[c] * fmaf(-u, u, 1.f) : x[c]);
+            }
+            pk[2 * e] = pack16<kBF16>(x[0], x[1]);
+            pk[2 * e + 1] = pack16<kBF16>(x[2], x[3]);
+            if constexpr (split.value) {
+              lo[2 * e] = rest16<kBF16>(pk[2 * e], x[0], x[1]);
+              lo[2 * e + 1] = rest16<kBF16>(pk[2 * e + 1], x[2], x[3]);
+            }
           }
-          pk[2 * e] = pack16<kBF16>(x[0], x[1]);
-          pk[2 * e + 1] = pack16<kBF16>(x[2], x[3]);
-        }
+          if constexpr (split.value) tmem_st32(la + kColA + 64 * half + 32, lo);
+        };
+        if (fine) weights(std::true_type()); else weights(std::false_type());
         tmem_st32(la + kColA + 64 * half, pk);
         tmem_st_wait();
         tc_fence_before();
@@ -517,25 +591,40 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!__all_sync(0xffffffffu, w)) return false;
         tc_fence_after();
         const float4* dl = reinterpret_cast<const float4*>(ss.delta[rq.slot] + 64 * half);
+        auto slopes = [&](auto split) {
+          uint32_t lo[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t g[32];
-          tmem_read32(la + kColB + 64 * half + 32 * c, g);
-          if (border) {  // 0 * NaN
+          for (int c = 0; c < 2; ++c) {
+            uint32_t g[32];
+            tmem_read32(la + kColB + 64 * half + 32 * c, g);
+            if (border) {  // 0 * NaN
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (__uint_as_float(r[32 * c + e]) == 0.f) g[e] = 0u;
+              for (int e = 0; e < 32; ++e)
+                if (__uint_as_float(r[32 * c + e]) == 0.f) g[e] = 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 d4 = dl[8 * c + e];
+              const float dv[4] = {d4.x, d4.y, d4.z, d4.w};
+              float x[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                float f = __uint_as_float(r[32 * c + 4 * e + y]);
+                if constexpr (!kBF16) f *= raise;
+                x[y] = f * (__uint_as_float(g[4 * e + y]) - dv[y]);
+              }
+              const int at = 16 * c + 2 * e;
+              pk[at] = pack16<kBF16>(x[0], x[1]);
+              pk[at + 1] = pack16<kBF16>(x[2], x[3]);
+              if constexpr (split.value) {
+                lo[at] = rest16<kBF16>(pk[at], x[0], x[1]);
+                lo[at + 1] = rest16<kBF16>(pk[at + 1], x[2], x[3]);
+              }
+            }
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 d4 = dl[8 * c + e];
-            const uint32_t* rr = r + 32 * c + 4 * e;
-            pk[16 * c + 2 * e] = pack16<kBF16>(__uint_as_float(rr[0]) * (__uint_as_float(g[4 * e]) - d4.x),
-                                               __uint_as_float(rr[1]) * (__uint_as_float(g[4 * e + 1]) - d4.y));
-            pk[16 * c + 2 * e + 1] = pack16<kBF16>(__uint_as_float(rr[2]) * (__uint_as_float(g[4 * e + 2]) - d4.z),
-                                                   __uint_as_float(rr[3]) * (__uint_as_float(g[4 * e + 3]) - d4.w));
-          }
-        }
+          if constexpr (split.value) tmem_st32(la + kColB + 64 * half + 32, lo);
+        };
+        if (fine) slopes(std::true_type()); else slopes(std::false_type());
         tmem_st32(la + kColB + 64 * half, pk);
         tmem_st_wait();
         tc_fence_before();
@@ -551,15 +640,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
       }
     }
+    // what p and ds were raised by
+    const float lower_p = kBF16 ? 1.f : __uint_as_float((127u - kUp) << 23);
+    const float lower_ds = kBF16 ? 1.f : __uint_as_float(static_cast<uint32_t>(127 - ss.up) << 23);
     if (p.cluster > 1) {  // this CTA's sums to shared memory: its tiles are done with
-      to_shared<DP>(la + kColD, half, 32 * (warp & 3) + lane, smem, ok && some);
-      to_shared<DP>(la + kColC, half, 32 * (warp & 3) + lane, smem + kTile * DP * 4, ok && some);
+      to_shared<DP>(la + kColD, half, 32 * (warp & 3) + lane, lower_ds, smem, ok && some);
+      to_shared<DP>(la + kColC, half, 32 * (warp & 3) + lane, lower_p, smem + kTile * DP * 4, ok && some);
     } else if (ok) {
       const bool live = key < p.Sk;
       const long long ok0 = b * p.d0.sb + hk * p.d0.sh + static_cast<long long>(key) * p.d0.ss;
       const long long ov0 = b * p.d1.sb + hk * p.d1.sh + static_cast<long long>(key) * p.d1.ss;
-      store_acc<DP, kBF16>(la + kColD, half * (DP / 2), p.sm_scale, p.d0.p, ok0, p.D, live, some);
-      store_acc<DP, kBF16>(la + kColC, half * (DP / 2), 1.f, p.d1.p, ov0, p.D, live, some);
+      store_acc<DP, kBF16>(la + kColD, half * (DP / 2), p.sm_scale * lower_ds, p.d0.p, ok0, p.D, live, some);
+      store_acc<DP, kBF16>(la + kColC, half * (DP / 2), lower_p, p.d1.p, ov0, p.D, live, some);
     }
     tc_fence_before();
   }
@@ -632,6 +724,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int n0 = tab.x < tab.y ? tab.x / kTile : 0;
   const int n1 = tab.x < tab.y ? (tab.y + kTile - 1) / kTile : 0;
   const int steps = n1 - n0;
+  const bool fine = steps <= kFineSteps;
 
   if (tid == 0) {
     mbar_init(&ss.qg_full, 1);
@@ -756,6 +849,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         mma_rows(tmem + kColD, tmem + ((n & 1) ? kColC : kColB), kb + k_used * kBytes, kIdR, n > 0);
+        if (fine) mma_rows(tmem + kColD, tmem + ((n & 1) ? kColC : kColB) + 32, kb + k_used * kBytes, kIdR, true);
         umma_commit(&ss.k_empty[k_used]);
         if (++k_used == S::kK) k_used = 0;
       }
@@ -773,10 +867,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int row = qt * kTile + 32 * (warp & 3) + lane;
     const bool live = row < p.Sq;
     bool ok = true;
+    float lower = 1.f;
     if (steps > 0) {
-      const float lse2 = p.lse2[static_cast<long long>(bh) * p.Sq_pad + row];
+      float lse2 = p.lse2[static_cast<long long>(bh) * p.Sq_pad + row];
+      if constexpr (!kBF16) {  // p raised by 2^kUp there; here p, and so ds, by what the row's do allows
+        const float n = p.up[static_cast<long long>(bh) * p.Sq_pad + row];
+        lse2 += kUp - n;
+        lower = __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(n)) << 23);
+      }
       const float delta = p.delta[static_cast<long long>(bh) * p.Sq_pad + row];
-      int lo = 0, hi = p.Sk;
+      int lo = 0, hi = live ? p.Sk : 0;  // rows behind the last see nothing, and choose nothing
       if (p.ranges && live) {
         const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
         lo = r.x;
@@ -824,20 +924,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         uint32_t pk[32];
+        auto slopes = [&](auto split) {
+          uint32_t lo[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t g[32];
-          tmem_read32(la + col + 64 * half + 32 * c, g);
-          if (border) {  // 0 * NaN
+          for (int c = 0; c < 2; ++c) {
+            uint32_t g[32];
+            tmem_read32(la + col + 64 * half + 32 * c, g);
+            if (border) {  // 0 * NaN
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (__uint_as_float(r[32 * c + e]) == 0.f) g[e] = 0u;
+              for (int e = 0; e < 32; ++e)
+                if (__uint_as_float(r[32 * c + e]) == 0.f) g[e] = 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x0 = __uint_as_float(r[32 * c + 2 * e]) * (__uint_as_float(g[2 * e]) - delta);
+              const float x1 = __uint_as_float(r[32 * c + 2 * e + 1]) * (__uint_as_float(g[2 * e + 1]) - delta);
+              pk[16 * c + e] = pack16<kBF16>(x0, x1);
+              if constexpr (split.value) lo[16 * c + e] = rest16<kBF16>(pk[16 * c + e], x0, x1);
+            }
           }
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            pk[16 * c + e] = pack16<kBF16>(__uint_as_float(r[32 * c + 2 * e]) * (__uint_as_float(g[2 * e]) - delta),
-                                           __uint_as_float(r[32 * c + 2 * e + 1]) * (__uint_as_float(g[2 * e + 1]) - delta));
-        }
+          if constexpr (split.value) tmem_st32(la + col + 64 * half + 32, lo);
+        };
+        if (fine) slopes(std::true_type()); else slopes(std::false_type());
         tmem_st32(la + col + 64 * half, pk);
         tmem_st_wait();
         tc_fence_before();
@@ -856,7 +964,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         return r.x >= r.y;
       }();
       const long long off = b * p.d0.sb + h * p.d0.sh + static_cast<long long>(row) * p.d0.ss;
-      store_acc<DP, kBF16>(la + kColD, half * (DP / 2), p.sm_scale, p.d0.p, off, p.D, live && !empty, steps > 0);
+      store_acc<DP, kBF16>(la + kColD, half * (DP / 2), p.sm_scale * lower, p.d0.p, off, p.D, live && !empty,
+                           steps > 0);
       if (live && empty) {
         const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int d0 = half * (DP / 2); d0 < min(p.D, (half + 1) * (DP / 2)); d0 += 8)
@@ -903,7 +1012,8 @@ int launch_bwd(const CUtensorMap* m, BwdParams p, const DenseArgs& a, cudaStream
 
 long long dense_backward_stats_bytes(int B, int H, int Sq, int Bm) {
   const long long rows = (static_cast<long long>(Sq) + dense::kTile - 1) / dense::kTile * dense::kTile;
-  return (static_cast<long long>(B) * H + Bm) * rows * 8;
+  const long long heads = static_cast<long long>(B) * H;
+  return (3 * heads + 2ll * Bm) * rows * 4 + heads * (rows / 16) * 4;
 }
 
 int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
@@ -937,14 +1047,15 @@ int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
   p.lse2 = a.stats;
   p.delta = a.stats + static_cast<long long>(a.B) * a.H * p.Sq_pad;
   p.rng = a.ranges ? reinterpret_cast<int2*>(a.stats + 2 * static_cast<long long>(a.B) * a.H * p.Sq_pad) : nullptr;
+  p.heads = a.B * a.H;
+  p.up = a.stats + (2ll * p.heads + (a.ranges ? 2ll * a.Bm : 0)) * p.Sq_pad;
   p.lse = a.lse;
   p.o = a.o;
   p.o_lo = a.o_lo;
   p.g = a.g;
-  if (static_cast<long long>(a.B) * a.H * p.q_tiles > INT_MAX || static_cast<long long>(a.B) * a.Hk * p.k_tiles > INT_MAX / 8 ||
-      static_cast<long long>(a.B) * a.H > 65535)
+  if (static_cast<long long>(a.B) * a.H * p.q_tiles > INT_MAX || static_cast<long long>(a.B) * a.Hk * p.k_tiles > INT_MAX / 8)
     return set_error(BSA_ERR_SHAPE, "too many row tiles for one launch");
-  const dim3 sgrid(p.Sq_pad / 16, a.B * a.H);
+  const dim3 sgrid(p.Sq_pad / 16, p.heads < 65535 ? p.heads : 65535);
   const bool bf = a.dtype == BSA_DTYPE_BF16, cap = a.softcap > 0.f;
   if (bf) stats_kernel<__nv_bfloat16><<<sgrid, 256, 0, stream>>>(p);
   else stats_kernel<__half><<<sgrid, 256, 0, stream>>>(p);

@@ -526,6 +526,50 @@ def test_gradients_of_a_padded_batch(cuda, bad, cap):
         assert (got[0][b, :, ql[b]:] == 0).all() and (got[1][b, :, kl[b]:] == 0).all() and (got[2][b, :, kl[b]:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hk,S", [(2, 2, 1), (4, 1, 7), (2, 1, 130), (1, 1, 500)])
+def test_short_gradients_round_once(cuda, dtype, H, Hk, S):
+    """Few steps: p and ds keep twice their type's bits, so that dv and, but for delta's share, dq and dk round once."""
+    from longcat_video.models.masked_attention import AttentionMask
+
+    q, k, v, g = (rand((2, n, S, 64), dtype, i, cuda) for i, n in enumerate((H, Hk, Hk, H)))
+    m = AttentionMask.build(S, S, causal=True, device=cuda)
+    _, got = gradients(q, k, v, g, m)
+    grads, ds, dl, fine, pg = ref_gradients(q, k, v, g, *rows_of(m), 0.125, 0.0)
+    u = unit(dtype)
+    tiny = 2.0 ** -24  # steps of fp16's subnormals, of the result and of what a rounding leaves over
+    for i in range(2):
+        x = (q if i else k).double().abs().amax() * 0.125 * S * H * tiny
+        check(got[i], grads[i], u * grads[i].abs() + u * u * ds[i] + u * dl[i] + SLACK * fine[i] + x + tiny)
+    # p is raised by 2^15 in fp16, and bf16 has no subnormals here
+    check(got[2], grads[2], u * grads[2].abs() + (u * u + SLACK) * pg + g.double().abs().amax() * S * H * tiny / 2 ** 15 + tiny)
+
+
+def test_small_gradients_in_fp16(cuda):
+    """Products of p and do far below fp16's normal numbers: raised by powers of two, they keep their bits."""
+    from longcat_video.models.masked_attention import AttentionMask
+
+    q, k, v = (rand((1, n, s, 64), torch.float16, i, cuda) for i, (n, s) in enumerate(((4, 600), (2, 2000), (2, 2000))))
+    g = rand((1, 4, 600, 64), torch.float16, 3, cuda) * 2.0 ** -8
+    m = AttentionMask.build(600, 2000, prefix=100, causal=True, device=cuda)
+    _, got = gradients(q, k, v, g, m)
+    grads, ds, dl, fine, pg = ref_gradients(q, k, v, g, *rows_of(m), 0.125, 0.0)
+    u, tiny = unit(torch.float16), 2.0 ** -24
+    assert g.float().norm(dim=-1).max() < 2.0 ** -4  # so ds is raised by 2^7 at least (2^7 |do| < 2^3)
+    for i in range(2):
+        x = (q if i else k).double().abs().amax() * 0.125 * (1200 if i else 2000) * tiny / 2 ** 7
+        check(got[i], grads[i], u * grads[i].abs() + u * ds[i] + u * dl[i] + SLACK * fine[i] + x + tiny)
+    x = g.double().abs().amax() * 1200 * tiny / 2 ** 15
+    check(got[2], grads[2], u * grads[2].abs() + (u + SLACK) * pg + x + tiny)
+
+
+def test_gradients_of_many_heads(cuda):
+    q, k, v, g = (rand((1, n, s, 8), torch.bfloat16, i, cuda)
+                  for i, (n, s) in enumerate(((70000, 2), (35000, 3), (35000, 3), (70000, 2))))
+    _, got = gradients(q, k, v, g, None)
+    check_gradients(got, q, k, v, g, *full(2, 3, cuda), 8 ** -0.5)
+
+
 def test_attention_gradient_against_differences(cuda):
     from longcat_video.models.masked_attention import AttentionMask, masked_attention
 
