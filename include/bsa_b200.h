@@ -230,8 +230,9 @@ int bsa_attention_ranges(int32_t* ranges, int32_t* table, int batch, int Sq, int
  * ([B, H, Sq] fp32, natural logarithm, NULL: not wanted).  out_rest ([B, H, Sq, D] in dtype, contiguous, NULL: not
  * wanted) receives what the rounding of out left over; the backward needs it.  scratch:
  * bsa_masked_attention_scratch_bytes() bytes (0: none needed).  Scores of unseen keys never count, whatever they
- * hold; nor do values of keys that no row of the same 128 rows sees.  A value that is infinite or NaN and seen by
- * one row can reach another row of the same 128. */
+ * hold; nor do values of keys in front of, or behind, what the same 128 rows see.  A value that is infinite or NaN
+ * and lies between those can reach all of the 128 rows.  At most 2^30 tokens.  out may be q; it
+ * overlaps no input otherwise. */
 int64_t bsa_masked_attention_scratch_bytes(int B, int H, int Sq, int Sk, int D);
 int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype, int B, int H, int Hk, int Sq, int Sk,
                          int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
@@ -240,8 +241,9 @@ int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype,
                          void* stream);
 
 /* bsa_masked_attention_backward: gradients of that call from its out, out_rest and lse and the gradient of out.
- * dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may be NULL.  Shared key heads sum over their query heads; keys no row sees get zeros.  No atomics: the same bits
- * every time.  scratch: bsa_masked_attention_backward_scratch_bytes() bytes (ranges_batch 0 without ranges). */
+ * dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may be NULL.  Shared key heads sum
+ * over their query heads; keys no row sees get zeros.  No atomics: the same bits every time.  scratch:
+ * bsa_masked_attention_backward_scratch_bytes() bytes (ranges_batch 0 without ranges). */
 int64_t bsa_masked_attention_backward_scratch_bytes(int B, int H, int Sq, int ranges_batch);
 int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
                                   const void* grad, const float* lse, int dtype, int B, int H, int Hk, int Sq, int Sk, int D,

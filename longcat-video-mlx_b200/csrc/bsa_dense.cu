@@ -23,9 +23,9 @@
 // P is rounded to the input type for the tensor cores, and o is divided by the sum of the rounded values: the weights
 // then sum to 1 and their rounding errors count against v_j - o_i instead of v_j.  lse comes from the fp32 values.
 //
-// Masked places never reach a result: scores are replaced by -inf whatever they hold, and V rows that no row
-// of the CTA sees are zeroed in shared memory (0 * NaN would be NaN).  Tiles outside the union of the rows'
-// intervals are not loaded; tiles inside all of them are not compared.
+// Masked places never reach a result: scores are replaced by -inf whatever they hold, and V rows in front of or behind
+// all of the CTA's intervals are zeroed in shared memory (0 * NaN would be NaN).  Tiles there are not loaded; tiles
+// inside all of the intervals are not compared.
 // Every wait is bounded (bsa_ptx.cuh).
 #include <climits>
 #include <mutex>

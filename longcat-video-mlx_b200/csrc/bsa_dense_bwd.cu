@@ -21,7 +21,7 @@
 //   dq : S(0) dP(0) [S(j) read] S(j+1) dP(j+1) [dS(j) ready] dQ(j) ...
 //
 // Masked places: p and ds are set to 0 by comparison, whatever the scores hold; rows of empty queries (dkv) and keys
-// that no row of the tile sees (dq) are zeroed in shared memory, since 0 * NaN would be NaN.
+// in front of or behind all of the tile's intervals (dq) are zeroed in shared memory, since 0 * NaN would be NaN.
 // Every wait is bounded (bsa_ptx.cuh).
 #include <climits>
 #include <type_traits>

@@ -23,6 +23,8 @@ Tensor4 tensor(const void* p, const int64_t* st) {
   return t;
 }
 
+constexpr int kMostRows = 1 << 30;  // tokens of a sequence: places and tile borders stay within 32 bits
+
 int elt(int dtype) { return dtype == BSA_DTYPE_F32 ? 4 : 2; }
 
 // base and strides (of axes that are walked) in multiples of 16 bytes
@@ -123,6 +125,7 @@ int dense_plan(bsa::DenseArgs& a, const void* q, const void* k, const void* v, i
   int rc = check_16bit(dtype);
   if (rc) return rc;
   if (B <= 0 || H <= 0 || Hk <= 0 || Sq <= 0 || Sk <= 0) return set_error(BSA_ERR_SHAPE, "empty tensor");
+  if (Sq > kMostRows || Sk > kMostRows) return set_error(BSA_ERR_SHAPE, "more than %d tokens", kMostRows);
   if (H % Hk) return set_error(BSA_ERR_SHAPE, "%d query heads are no multiple of %d key heads", H, Hk);
   if ((rc = check_head_dim(D))) return rc;
   if (!(sm_scale > 0.f) || std::isinf(sm_scale)) return set_error(BSA_ERR_ARG, "sm_scale must be positive and finite");
@@ -189,6 +192,7 @@ int bsa_norm_rope_backward(const void* x0, const int64_t* x0_strides, const void
   if (rc) return rc;
   if (!x0_strides || !g0_strides || !dx0 || (x1 && (!x1_strides || !g1_strides || !dx1)))
     return set_error(BSA_ERR_ARG, "null pointer");
+  if (!aligned(scratch, 4)) return set_error(BSA_ERR_ALIGN, "scratch must be 4-byte aligned");
   if ((dw0 || dw1) && !scratch) return set_error(BSA_ERR_ARG, "weight gradients need scratch");
   a.sides = x1 ? 2 : 1;
   for (int i = 0; i < a.sides; ++i) {
@@ -214,6 +218,9 @@ int bsa_attention_ranges(int32_t* ranges, int32_t* table, int batch, int Sq, int
                          int documents, const int32_t* q_lengths, const int32_t* k_lengths, int k_add, void* stream) {
   if (!ranges || !table) return set_error(BSA_ERR_ARG, "null pointer");
   if (batch <= 0 || Sq <= 0 || Sk < 0) return set_error(BSA_ERR_SHAPE, "empty ranges");
+  if (Sq > kMostRows || Sk > kMostRows) return set_error(BSA_ERR_SHAPE, "more than %d tokens", kMostRows);
+  if (static_cast<long long>(batch) * ((Sq + 127) / 128) > INT_MAX)
+    return set_error(BSA_ERR_SHAPE, "too many rows for one launch");
   if ((q_offsets == nullptr) != (k_offsets == nullptr)) return set_error(BSA_ERR_ARG, "q_offsets come with k_offsets");
   if (q_offsets && documents <= 0) return set_error(BSA_ERR_SHAPE, "no documents");
   if (q_offsets && (q_lengths || k_lengths)) return set_error(BSA_ERR_ARG, "documents or lengths, not both");
@@ -256,6 +263,7 @@ int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype,
   a.splits = bsa::dense_pick_splits(sms, B, H, Sq, Sk);
   if (a.splits > 1) {
     if (!scratch) return set_error(BSA_ERR_ARG, "scratch is required (bsa_masked_attention_scratch_bytes)");
+    if (!aligned(scratch, 16)) return set_error(BSA_ERR_ALIGN, "scratch must be 16-byte aligned");
     a.part = static_cast<float*>(scratch);
   }
   return bsa::launch_dense(a, sms, static_cast<cudaStream_t>(stream));
@@ -365,6 +373,7 @@ int bsa_kv8_attention(const void* q, int dtype, int B, int H, int Sq, const int6
   a.splits = cache_splits(sm_count(), B, Hk, static_cast<int>(rows), capacity);
   if (a.splits > 1) {
     if (!scratch) return set_error(BSA_ERR_ARG, "scratch is required (bsa_kv8_attention_scratch_bytes)");
+    if (!aligned(scratch, 16)) return set_error(BSA_ERR_ALIGN, "scratch must be 16-byte aligned");
     a.part = static_cast<float*>(scratch);
   }
   return launched(bsa::launch_cache_attention(a, static_cast<cudaStream_t>(stream)), "cache attention");

@@ -97,7 +97,6 @@ int launch_ranges(const RangesArgs& a, cudaStream_t stream) {
   p.Sq = a.Sq; p.Sk = a.Sk; p.causal = a.causal; p.prefix = a.prefix; p.docs = a.docs; p.k_add = a.k_add;
   p.tiles = (a.Sq + ranges::kTile - 1) / ranges::kTile;
   const long long grid = static_cast<long long>(a.Bm) * p.tiles;
-  if (grid > INT_MAX) return BSA_ERR_SHAPE;
   ranges::ranges_kernel<<<static_cast<int>(grid), ranges::kTile, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
 }

@@ -6,6 +6,8 @@
 // The entries are looked up in the engine's library, which Python has loaded; errors of the C ABI come back as
 // ValueError (arguments) or BSAError, with its message.
 #include <dlfcn.h>
+#include <ATen/MemoryOverlap.h>
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <optional>
@@ -84,6 +86,12 @@ void check(int rc, const char* what) {
   throw CudaFailure(std::string(what) + " failed (code " + std::to_string(rc) + "): " + msg);
 }
 
+// The C ABI's sizes are 32-bit.
+void small(const Tensor& t) {
+  for (const int64_t n : t.sizes())
+    if (n > INT32_MAX) refuse("a size of " + std::to_string(n) + " does not fit 32 bits");
+}
+
 int dtype_code(at::ScalarType t) {
   if (t == at::kBFloat16) return BSA_DTYPE_BF16;
   if (t == at::kHalf) return BSA_DTYPE_F16;
@@ -154,11 +162,13 @@ void check_pair(const Tensor& q, const OptTensor& k) {
   on_cuda(q);
   dtype_code(q.scalar_type());
   if (q.dim() != 4) refuse("expected tensors of shape [B, H, S, D]");
+  small(q);
   if (k) {
     same_place(q, *k);
     if (k->scalar_type() != q.scalar_type() || k->dim() != 4 || k->size(0) != q.size(0) || k->size(2) != q.size(2) ||
         k->size(3) != q.size(3))
       refuse("q and k must share dtype, batch, length and head_dim");
+    small(*k);
   }
 }
 
@@ -335,6 +345,7 @@ py::tuple attention_ranges(const py::object& device, int64_t Sq, int64_t Sk, int
                            OptTensor q_lengths, OptTensor k_lengths, int64_t k_add) {
   if (Sq < 0 || Sk < 0 || Sq > INT32_MAX || Sk > INT32_MAX) refuse("lengths must be >= 0 and fit 32 bits");
   if (prefix < 0) refuse("prefix must be >= 0");
+  prefix = std::min<int64_t>(prefix, INT32_MAX);
   if (q_offsets.has_value() != k_offsets.has_value()) refuse("q_offsets and k_offsets come together");
   if (q_offsets && (q_lengths || k_lengths)) refuse("give documents or lengths, not both");
   int64_t n = -1;
@@ -351,6 +362,8 @@ py::tuple attention_ranges(const py::object& device, int64_t Sq, int64_t Sk, int
   if (prefixes && n < 0) batch = n = prefixes->numel();
   if (prefixes && prefixes->dim() != 1) refuse("prefix must be one number or one for each document or entry");
   c10::Device dev(c10::kCUDA, -1);
+  for (const OptTensor* t : {&given, &prefixes, &q_offsets, &q_lengths, &k_lengths})
+    if (*t) small(**t);
   for (const OptTensor* t : {&given, &prefixes, &q_offsets, &q_lengths, &k_lengths})
     if (*t && device.is_none()) {
       on_cuda(**t);
@@ -402,6 +415,8 @@ void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
   same_place(q, v);
   if (q.dim() != 4 || k.dim() != 4) refuse("q, k and v must be [B, H, S, D]");
   if (k.sizes() != v.sizes()) refuse("k and v must have the same shape");
+  small(q);
+  small(k);
   const at::ScalarType t = q.scalar_type();
   if (k.scalar_type() != t || v.scalar_type() != t) refuse("q, k, v must share one dtype");
   if (t != at::kBFloat16 && t != at::kHalf) refuse(std::string("unsupported dtype ") + c10::toString(t) + " (bf16 or fp16)");
@@ -417,10 +432,19 @@ void check_scale(double sm_scale, double softcap) {
   if (!(softcap >= 0) || std::isinf(softcap)) refuse("softcap must be finite and >= 0");
 }
 
-void check_out(const Tensor& q, const OptTensor& out) {
+// The output may be q itself: a row of it is written by who has read that row of q.  It overlaps no input otherwise.
+void check_out(const Tensor& q, const OptTensor& out, std::initializer_list<const OptTensor*> others) {
   if (!out) return;
   same_place(q, *out);
   if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type()) refuse("out must have q's shape and dtype");
+  if (at::GradMode::is_enabled() && out->requires_grad()) refuse("out= is for calls without gradients");
+  bool over = at::get_overlap_status(*out, q) == at::MemOverlapStatus::Partial;
+  for (const OptTensor* t : others)
+    if (*t) {
+      const at::MemOverlapStatus s = at::get_overlap_status(*out, **t);
+      over = over || s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+    }
+  if (over) refuse("out overlaps an input");
 }
 
 // The caller's output where the kernels can write it, else a new tensor that is copied there at the end.
@@ -433,7 +457,10 @@ struct Output {
     for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
   }
   Tensor done(const OptTensor& out) {
-    if (copy) out->copy_(t);
+    if (copy)
+      out->copy_(t);
+    else if (out && !out->is_inference())
+      out->unsafeGetTensorImpl()->bump_version();  // what autograd saved of it is stale, as after any in-place write
     return out ? *out : t;
   }
 };
@@ -538,8 +565,8 @@ py::tuple masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     refuse("the mask is for " + std::to_string(mask_q) + " queries and " + std::to_string(mask_k) + " keys, got " +
            std::to_string(q.size(2)) + " and " + std::to_string(k.size(2)));
   const Mask m(q, mask, mask_batch, mask_table);
-  check_out(q, out);
   const OptTensor q0(q), k0(k), v0(v);
+  check_out(q, out, {&k0, &v0});
   if (any_grad({&q0, &k0, &v0})) {
     if (out) refuse("out= is for calls without gradients");
     const variable_list r = MaskedAttention::apply(q, k, v, mask, mask_batch, mask_table, sm_scale, softcap);
@@ -560,6 +587,7 @@ struct Cache {
     on_cuda(kc);
     for (const Tensor* t : {&ks, &vc, &vs, &len}) same_place(kc, *t);
     if (kc.dim() != 4 || kc.sizes() != vc.sizes()) refuse("codes must be [B, Hk, capacity, D]");
+    small(kc);
     B = kc.size(0), Hk = kc.size(1), cap = kc.size(2), D = kc.size(3);
     if (cap % 64 || cap == 0) refuse("capacity " + std::to_string(cap) + " must be a positive multiple of 64");
     if (D % 8 || D <= 0 || D > 128) refuse("head_dim D=" + std::to_string(D) + " must be a multiple of 8 and <= 128");
@@ -635,11 +663,11 @@ struct Cache {
       refuse("attention over a cache has no gradient");
     const double s = sm_scale ? *sm_scale : 1.0 / std::sqrt(static_cast<double>(D));
     check_scale(s, 0.0);
-    check_out(q, out);
+    check_out(q, out, {&k, &v});
     const c10::cuda::CUDAGuard guard(kc.device());
     if (!q.numel()) return out ? *out : like(q);
     const int64_t n = k ? k->size(2) : 0;
-    if (n == 0 && H / Hk * Sq <= few_rows) {
+    if (n == 0 && H / Hk * Sq <= few_rows && B * Hk * ((H / Hk * Sq + 15) / 16) <= 65535) {  // (a grid's height)
       Output o(q, out);
       const View a(q);
       OptTensor scratch;

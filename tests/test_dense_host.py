@@ -380,6 +380,33 @@ def test_norm_rope_refusals(lib, change, code):
     assert rc == code and msg
 
 
+@pytest.mark.parametrize("name,types,args", [
+    ("bsa_masked_attention", "pppiiiiiiisssppiffpspppp",
+     [FAKE, FAKE, FAKE, 2, 1, 1, 1, 64, 8192, 128, strides(*ST), strides(*ST), strides(*ST), None, None, 1, 0.1, 0.0, FAKE,
+      strides(*ST), None, None, FAKE + 8, None]),
+    ("bsa_kv8_attention", "piiiispppppiiiifpspp",
+     [FAKE, 2, 1, 4, 1, strides(*ST), FAKE, FAKE, FAKE, FAKE, FAKE, 2, 8192, 128, 0, 0.1, FAKE, strides(*ST), FAKE + 4, None])])
+def test_scratch_alignment(lib, name, types, args):
+    """Few rows over many keys are split and need scratch, which is read 16 bytes at a time."""
+    rc, msg = call(lib, name, types, args)
+    assert rc == 3 and "scratch" in msg
+    args[-2] = None
+    rc, msg = call(lib, name, types, args)
+    assert rc == 7 and "scratch" in msg
+
+
+def test_most_tokens(lib):
+    for Sq, Sk in ((2 ** 30 + 1, 1), (1, 2 ** 30 + 1)):
+        args = [FAKE, FAKE, FAKE, 2, 1, 1, 1, Sq, Sk, 8, strides(8, 8, 8), strides(8, 8, 8), strides(8, 8, 8), None, None, 1,
+                0.1, 0.0, FAKE, strides(8, 8, 8), None, None, None, None]
+        assert call(lib, "bsa_masked_attention", "pppiiiiiiisssppiffpspppp", args)[0] == 1
+        args = [FAKE, FAKE, 1, Sq, Sk, None, 0, 0, None, None, None, 0, None, None, 0, None]
+        assert call(lib, "bsa_attention_ranges", "ppiiipiipppippip", args)[0] == 1
+    args = [FAKE, FAKE, 2 ** 20, 2 ** 20, 1, None, 0, 0, None, None, None, 0, None, None, 0, None]
+    rc, msg = call(lib, "bsa_attention_ranges", "ppiiipiipppippip", args)
+    assert rc == 1 and "too many rows" in msg
+
+
 def test_host_tensors_are_refused():
     from longcat_video.models.kv_cache import KVCache8
     from longcat_video.models.masked_attention import AttentionMask, masked_attention

@@ -639,6 +639,47 @@ def test_training_step_in_a_graph(cuda):
         assert all(torch.equal(a, b) for a, b in zip(res, step()))
 
 
+def test_attention_output_refusals(cuda):
+    from longcat_video.models.kv_cache import KVCache8
+    from longcat_video.models.masked_attention import masked_attention
+
+    q, k, v = (rand((1, 2, 40, 64), torch.bfloat16, i, cuda) for i in range(3))
+    cache = KVCache8.from_kv(k, v)
+    for f in (lambda o: masked_attention(q, k, v, out=o), lambda o: cache.attend(q, out=o)):
+        wide = torch.empty((1, 2, 41, 64), dtype=torch.bfloat16, device=cuda).flatten()
+        q, bad = wide[:q.numel()].view_as(q).copy_(q), wide[64:64 + q.numel()].view_as(q)
+        for bad in (bad, torch.empty_like(q).requires_grad_()):
+            with pytest.raises(ValueError):
+                f(bad)
+        o = torch.zeros((1, 2, 40, 64), dtype=torch.bfloat16, device=cuda)
+        before = o._version
+        assert f(o) is o or f(o).data_ptr() == o.data_ptr()
+        assert o._version > before and torch.equal(o, f(None))
+        own = q.clone()
+        assert f(q) is not None and torch.equal(q, o)  # q itself
+        q = own
+    with pytest.raises(ValueError):
+        masked_attention(q, k, v, out=v)
+    w = torch.ones_like(q, requires_grad=True)
+    o = torch.zeros_like(q)
+    y = (w * o).sum()  # o is saved
+    masked_attention(q, k, v, out=o)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_lookup_of_many_heads(cuda):
+    """More 16-row tiles than a grid is high: the cache is unpacked."""
+    from longcat_video.models.kv_cache import KVCache8
+
+    k, v = (rand((1, 20000, 5, 8), torch.bfloat16, i, cuda) for i in range(2))
+    q = rand((1, 20000, 64, 8), torch.bfloat16, 2, cuda)
+    got = KVCache8.from_kv(k, v).attend(q)
+    part = KVCache8.from_kv(k[:, :50], v[:, :50]).attend(q[:, :50])
+    # two kernels: each rounds once (2^-8 of a value of at most max |v|) and weighs with 16-bit numbers (2^-8 again)
+    torch.testing.assert_close(got[:, :50].float(), part.float(), rtol=0, atol=4 * 2.0**-8 * v.abs().max().item())
+
+
 def test_gradient_refusals(cuda):
     """Second derivatives; a capture while an eager graph of the same leaf lives on another stream."""
     from longcat_video.models.masked_attention import masked_attention
