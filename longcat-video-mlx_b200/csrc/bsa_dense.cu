@@ -26,9 +26,14 @@
 // Masked places never reach a result: scores are replaced by -inf whatever they hold, and V rows in front of or behind
 // all of the CTA's intervals are zeroed in shared memory (0 * NaN would be NaN).  Tiles there are not loaded; tiles
 // inside all of the intervals are not compared.
+//
+// Measured: 20,280 rows x 8 heads, D 128, 6,240 of conditioning in front, 1.46 ms, 910 TFLOP/s of the visible pairs.
+// The card is then at its power limit (SM clock 1.65 of 1.97 GHz), and without the loads of K and V, which a tile of 128
+// rows makes for each step, it would take a tenth less.  Short calls are bound by their start: 2 us for one tile.
+// Tried and not faster (1.49 to 1.60 ms): two query tiles to a CTA with 8 or 16 softmax warps, three S buffers, two
+// issuing threads, half of the exponentials as polynomials.
 // Every wait is bounded (bsa_ptx.cuh).
 #include <climits>
-#include <mutex>
 #include "bsa_dense.cuh"
 
 namespace bsa {

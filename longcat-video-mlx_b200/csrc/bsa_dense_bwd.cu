@@ -20,6 +20,13 @@
 //   dkv: S(0) dP(0) [P(i) ready] dV(i) S(i+1) [dS(i) ready] dK(i) dP(i+1) ...
 //   dq : S(0) dP(0) [S(j) read] S(j+1) dP(j+1) [dS(j) ready] dQ(j) ...
 //
+// Where key tiles are few, the query heads of a key head are shared by the CTAs of a cluster, which add up their sums over
+// distributed shared memory, in the order of the CTAs.
+//
+// Measured, forward and backward: 9,360 rows x 8 heads, D 128, 1,560 of conditioning, 1.49 to 1.51 ms (930 TFLOP/s of
+// what is computed); 4,680 rows of 9 documents, 16 heads on 4, 0.33 ms (0.39 without clusters).  Bound by the port of
+// the shared memory, which the operands of the products pass, and by the arithmetic between the products.
+//
 // Masked places: p and ds are set to 0 by comparison, whatever the scores hold; rows of empty queries (dkv) and keys
 // in front of or behind all of the tile's intervals (dq) are zeroed in shared memory, since 0 * NaN would be NaN.
 // Every wait is bounded (bsa_ptx.cuh).
@@ -37,7 +44,8 @@ constexpr int kBwdThreads = 320;
 constexpr uint32_t kColA = 0, kColB = 128, kColC = 256, kColD = 384;  // tensor memory, 128 columns each
 // Up to this many steps of a CTA, p and ds go through the second products as their rounding and what it left over, so
 // that a gradient carries no error but its own rounding's.  Beyond, the one rounding of p and ds to the tensors' type adds
-// as much again (1.4 times the error).
+// as much again (1.4 times the error).  4 steps cost nothing measurable, 8 would cost 4,680 rows of 9 documents 1 % and
+// 1,000 rows x 32 heads 8 %, 16 would cost 3 % and, at 2,000 rows x 16 heads, 9 %.
 constexpr int kFineSteps = 4;
 
 struct BwdParams {

@@ -199,7 +199,7 @@ class Attention(torch.nn.Module):
         over the cache positions so that RoPE over the extended grid (T + num_cond_latents, H, W) gives
         q and k their global positions.  Q and KV lengths differ, so the hook takes its dense path.
         A :class:`KVCache8` (:meth:`quantize_kv_cache`) is read by the engine's kernels, whatever
-        ``dense_kernels`` says."""
+        ``dense_kernels`` says; what it holds is constant to a gradient."""
         B, N, C = x.shape
         qkv = self.qkv(x).reshape(B, N, 3, self.num_heads, self.head_dim).permute(2, 0, 3, 1, 4)
         q, k, v = qkv[0], qkv[1], qkv[2]
@@ -231,8 +231,13 @@ class Attention(torch.nn.Module):
         if isinstance(kv_cache, KVCache8):
             cache = kv_cache.expand(B)
             q, k = self._norm_rope(q, k, grid, start=num_cond_latents * Hl * Wl if rotated else 0)
+            if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+                # what is held goes behind the fresh tokens here: every query sees both, and so they are one interval
+                k_cache, v_cache = cache.dequantize(q.dtype)
+                mask = AttentionMask.build(N, N + cache.capacity, k_lengths=cache.lengths + N)
+                return self._project(q, torch.cat([k, k_cache], dim=2), torch.cat([v, v_cache], dim=2), mask)
             out = torch.empty((B, N, H, D), device=q.device, dtype=q.dtype)
-            cache.attend(q.detach(), k.detach(), v.detach(), sm_scale=self.scale, out=out.permute(0, 2, 1, 3))
+            cache.attend(q, k, v, sm_scale=self.scale, out=out.permute(0, 2, 1, 3))
             return self.proj(out.view(B, N, H * D))
         k_cache, v_cache = (t.expand(B, *t.shape[1:]) if t.shape[0] == 1 else t for t in kv_cache)
         n = k_cache.shape[2]

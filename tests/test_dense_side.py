@@ -1064,6 +1064,26 @@ def test_hook_continuation(cuda, B, cond):
         m.quantize_kv_cache(kv, (2, 6, 7), 1)
 
 
+@pytest.mark.parametrize("cond", [None, 2])
+def test_hook_continuation_gradients(cuda, cond):
+    """Over a cache in 8 bits: the gradients of the same step over what it holds, as tensors."""
+    m = hook(cuda)
+    m.dense_kernels = True
+    x0, x = rand((1, 84, 128), torch.bfloat16, 1, cuda), rand((2, 126, 128), torch.bfloat16, 2, cuda).requires_grad_()
+    g = rand((2, 126, 128), torch.bfloat16, 3, cuda)
+    with torch.no_grad():
+        _, kv = m(x0, (2, 6, 7), None, return_kv=True)
+        cache = m.quantize_kv_cache(kv, (2, 6, 7), cond)
+        eight = m.forward_with_kv_cache(x, (3, 6, 7), cond, cache)
+    leaves = [x, m.q_norm.weight, m.k_norm.weight, m.qkv.weight, m.proj.weight]
+    out = m.forward_with_kv_cache(x, (3, 6, 7), cond, cache)
+    near(out, eight, HOOK_REL)
+    got = torch.autograd.grad(out, leaves, g)
+    want = torch.autograd.grad(m.forward_with_kv_cache(x, (3, 6, 7), cond, kv), leaves, g)
+    for a, b in zip(got, want):
+        near(a, b, 2 * HOOK_REL + 4 * 2.0 ** -4)  # held keys and values in e4m3: half a step is 2^-4, in k and in v
+
+
 def test_hook_bsa_keeps_its_path(cuda):
     """dense_kernels leaves block-sparse calls alone, and serves the hook's fallback for odd shapes."""
     m = hook(cuda)
