@@ -94,11 +94,14 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // Rows in flight: 4 forward (8: 279 us at 720p x 16 heads, 4: 264, 2: 307); 2 backward, where they leave registers
-// for 4 CTAs to an SM (6 frames x 32 heads, both passes: 4 rows and 2 CTAs 213 us, 2 and 2 202, 2 and 4 181).
+// for 4 CTAs to an SM (6 frames x 32 heads, both passes: 4 rows and 2 CTAs 213 us, 2 and 2 202, 2 and 4 181).  Reading the
+// next rows before this step's arithmetic costs more registers than it hides (the same: 9 to 58 us more).
 template <typename T, int kLanes, bool kBackward>
 __global__ void __launch_bounds__(kThreads, kBackward && sizeof(T) == 2 ? 4 : 0) norm_rope_kernel(const Params p) {
   constexpr int kBatch = kBackward ? 2 : 4;
   constexpr int kRows = kThreads / kLanes;  // tokens of a tile
+  after_previous();
+  let_next_start();
   const int sub = threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
   const int d0 = 8 * lane;
@@ -270,6 +273,7 @@ __global__ void __launch_bounds__(kThreads, kBackward && sizeof(T) == 2 ? 4 : 0)
 __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* partial, int rows0, int rows1, int D, float* dw0,
                                                            float* dw1) {
   __shared__ float red[32][33];
+  after_previous();
   float* dst = blockIdx.y ? dw1 : dw0;
   if (!dst) return;
   const int c = threadIdx.x & 31, part = threadIdx.x >> 5;
@@ -340,11 +344,8 @@ int launch(const NormRopeArgs& a, int most, cudaStream_t stream, int* rows_out) 
     rows_out[0] = p.side[0].groups * p.chunks;
     rows_out[1] = p.side[1].groups * p.chunks;
   }
-  if (wide)
-    norm_rope_kernel<T, 16, kBackward><<<grid, kThreads, 0, stream>>>(p);
-  else
-    norm_rope_kernel<T, 8, kBackward><<<grid, kThreads, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+  auto* kernel = wide ? norm_rope_kernel<T, 16, kBackward> : norm_rope_kernel<T, 8, kBackward>;
+  return launch_behind(kernel, dim3(grid), dim3(kThreads), 0, stream, p) == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
 }
 
 }  // namespace nrope
@@ -372,9 +373,10 @@ int launch_norm_rope_backward(const NormRopeArgs& a, cudaStream_t stream) {
                  : a.dtype == BSA_DTYPE_F16 ? nrope::launch<__half, true>(a, most, stream, rows)
                                             : nrope::launch<__nv_bfloat16, true>(a, most, stream, rows);
   if (rc || !a.partial) return rc;
-  nrope::weight_grad_kernel<<<dim3((a.D + 31) / 32, a.sides), 1024, 0, stream>>>(
-      a.partial, rows[0], rows[1], a.D, a.side[0].dw, a.sides > 1 ? a.side[1].dw : nullptr);
-  return cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+  return launch_behind(nrope::weight_grad_kernel, dim3((a.D + 31) / 32, a.sides), dim3(1024), 0, stream, a.partial, rows[0],
+                       rows[1], a.D, a.side[0].dw, a.sides > 1 ? a.side[1].dw : nullptr) == cudaSuccess
+             ? BSA_OK
+             : BSA_ERR_CUDA;
 }
 
 }  // namespace bsa
