@@ -77,8 +77,7 @@ struct Params {
   int group;           // heads that run side by side
   int splits;          // CTAs along the keys
   float scale_log2;    // sm_scale log2(e)
-  float cap_in;        // 2 sm_scale log2(e) / cap
-  float cap_log2;      // cap log2(e)
+  Cap cap;
   void* out;
   long long ob, oh, os;
   void* out_lo;        // nullable: [B, H, Sq, D] contiguous, o - out in 16 bits
@@ -304,28 +303,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto prepare = [&](uint32_t* r, int key, bool border) {
         const uint32_t first = static_cast<uint32_t>(key - lo);
         if constexpr (kCap) {
-          float top = 0.f;
-          if (border) {  // what a masked place holds must not choose the form of tanh below
+          if (border) {  // what a masked place holds must not choose the form of tanh
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (first + e >= seen) r[e] = 0u;
           }
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
-          if (__all_sync(0xffffffffu, top * p.cap_in <= 2.f * 1.44269504f)) {  // |s| <= cap in all of the warp's rows
-            const float ci = p.cap_in * 0.34657359f;  // cap_in = 2 log2(e) sm_scale / cap
-            const uint64_t in2 = f2_pack(ci, ci), out2 = f2_pack(p.cap_log2, p.cap_log2);
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float a, c;
-              f2_unpack(f2_mul(tanh_poly2(f2_mul(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), in2)), out2), a, c);
-              r[e] = __float_as_uint(a);
-              r[e + 1] = __float_as_uint(c);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(p.cap_log2 * tanh_of(__uint_as_float(r[e]) * p.cap_in));
-          }
+          capped<32>(r, p.cap);
         }
         if (border) {
 #pragma unroll
@@ -640,10 +623,7 @@ int launch_dense(const DenseArgs& a, int sms, cudaStream_t stream) {
   const long long group = (40ll << 20) / kv_bytes * p.G;
   p.group = static_cast<int>(group < 1 ? 1 : (group < bh ? group : bh));
   p.scale_log2 = a.sm_scale * 1.4426950408889634f;
-  if (a.softcap > 0.f) {
-    p.cap_in = 2.f * p.scale_log2 / a.softcap;
-    p.cap_log2 = a.softcap * 1.4426950408889634f;
-  }
+  if (a.softcap > 0.f) p.cap = make_cap(p.scale_log2, a.softcap);
   p.out = a.o.p; p.ob = a.o.sb; p.oh = a.o.sh; p.os = a.o.ss;
   p.out_lo = a.o_lo;
   p.lse = a.lse;

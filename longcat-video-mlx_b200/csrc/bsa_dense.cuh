@@ -1,5 +1,7 @@
 // What the dense attention's forward and backward kernels share: tile geometry, tile loads, the tanh cap.
 #pragma once
+#include <cmath>
+#include <type_traits>
 #include "bsa_dense.h"
 #include "bsa_ptx.cuh"
 
@@ -158,17 +160,63 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ float max3_abs(float a, float b, float c) { return max3(a, fabsf(b), fabsf(c)); }
 
-// tanh of two values in [-1, 1]: a times a polynomial of degree 5 in a^2, fitted here for the smallest relative
-// error (5.9e-7)
-__device__ __forceinline__ uint64_t tanh_poly2(uint64_t a) {
-  const uint64_t u = f2_mul(a, a);
-  uint64_t y = f2_pack(-0.00306704058f, -0.00306704058f);
-  y = f2_fma(y, u, f2_pack(0.0167430621f, 0.0167430621f));
-  y = f2_fma(y, u, f2_pack(-0.0516056232f, -0.0516056232f));
-  y = f2_fma(y, u, f2_pack(0.132814318f, 0.132814318f));
-  y = f2_fma(y, u, f2_pack(-0.333290428f, -0.333290428f));
-  y = f2_fma(y, u, f2_pack(0.999999404f, 0.999999404f));
-  return f2_mul(y, a);
+// The cap: z log2(e) = cap log2(e) tanh(s / cap) of s = sm_scale q.k.  With x = q.k and a = s / cap, odd polynomials in a,
+// fitted here for the smallest relative error (5.5e-7 for |a| <= 1/2, 6.1e-7 for |a| <= 1), the factors of a and of the
+// result taken into their coefficients: x (c0 + c1 x^2 + ...).
+struct Cap {
+  float in;          // 2 sm_scale log2(e) / cap, of x
+  float log2;        // cap log2(e)
+  float near, most;  // |x| up to which |a| <= 1/2, and 1 (< 0: a coefficient would overflow)
+  float n[4], m[6];  // coefficients
+};
+inline Cap make_cap(float scale_log2, float cap) {
+  Cap c = {};
+  c.in = 2.f * scale_log2 / cap;
+  c.log2 = cap * 1.4426950408889634f;
+  const float n[4] = {0.999999464f, -0.333263189f, 0.131902963f, -0.0444022231f};
+  const float m[6] = {0.999999404f, -0.333290428f, 0.132814333f, -0.0516056716f, 0.0167431086f, -0.00306705665f};
+  const double a = c.in * 0.34657359027997264;  // in / (2 log2(e)): a = a x
+  double f = a * c.log2;
+  float largest = 0.f;
+  for (int i = 0; i < 6; ++i, f *= a * a) {
+    c.m[i] = static_cast<float>(m[i] * f);
+    if (i < 4) c.n[i] = static_cast<float>(n[i] * f);
+    largest = fmaxf(largest, fabsf(static_cast<float>(f)));
+  }
+  const float square = 1.2e18f;  // x^2 stays finite
+  c.most = largest < 1e37f ? fminf(static_cast<float>(1. / a), square) : -1.f;
+  c.near = 0.5f * c.most;
+  return c;
+}
+// N products q.k of a row through the cap, in the cheapest form that serves all of the warp's rows: 5 or 7 packed operations
+// a pair, or two of the exponential's unit a score, of which a step's exponentials take one each.
+template <int N>
+__device__ __forceinline__ void capped(uint32_t* r, const Cap& c) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+  auto series = [&](const float* k, auto terms) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const uint64_t x = f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+      const uint64_t v = f2_mul(x, x);
+      uint64_t y = f2_pack(k[terms.value - 1], k[terms.value - 1]);
+#pragma unroll
+      for (int i = terms.value - 2; i >= 0; --i) y = f2_fma(y, v, f2_pack(k[i], k[i]));
+      float a, b;
+      f2_unpack(f2_mul(y, x), a, b);
+      r[e] = __float_as_uint(a);
+      r[e + 1] = __float_as_uint(b);
+    }
+  };
+  if (__all_sync(0xffffffffu, top <= c.near)) {
+    series(c.n, std::integral_constant<int, 4>());
+  } else if (__all_sync(0xffffffffu, top <= c.most)) {
+    series(c.m, std::integral_constant<int, 6>());
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = __float_as_uint(c.log2 * tanh_of(__uint_as_float(r[e]) * c.in));
+  }
 }
 
 // 32 lanes x 32 columns store, counterpart of tmem_ld32

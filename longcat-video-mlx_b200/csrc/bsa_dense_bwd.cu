@@ -54,12 +54,13 @@ struct BwdParams {
   int Bm, H, Hk, G, Sq, Sk, D;
   int q_tiles, k_tiles, Sq_pad;
   int cluster;          // CTAs that share the query heads of a key tile (dkv)
-  float scale_log2, sm_scale, cap_in, cap_log2;
+  float scale_log2, sm_scale;
+  Cap cap;
   float* lse2;          // [B * H][Sq_pad]: lse in log2 (+inf: no keys)
   float* delta;         // [B * H][Sq_pad]
   float* up;            // fp16: [B * H][Sq_pad], what dq's row of ds is raised by (log2), then its least of 16 rows each
   int heads;            // B * H
-  float cap_inv, cap_mask;  // 1 / cap_log2, and a score below every capped one by 2^300
+  float cap_inv, cap_mask;  // 1 / cap.log2, and a score below every capped one by 2^300
   int2* rng;            // [Bm][Sq_pad]: ranges, padded with empty ones
   const float* lse;
   Tensor4 o, g;         // forward output, its gradient
@@ -145,27 +146,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                    smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
-}
-
-// 64 scores q.k through the cap, in log2 units; |s| <= cap in the whole warp: the polynomial form
-__device__ __forceinline__ void capped64(uint32_t* r, float cap_in, float cap_log2) {
-  float top = 0.f;
-#pragma unroll
-  for (int e = 0; e < 64; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
-  if (__all_sync(0xffffffffu, top * cap_in <= 2.f * 1.44269504f)) {
-    const float ci = cap_in * 0.34657359f;  // cap_in = 2 log2(e) sm_scale / cap
-    const uint64_t in2 = f2_pack(ci, ci), out2 = f2_pack(cap_log2, cap_log2);
-#pragma unroll
-    for (int e = 0; e < 64; e += 2) {
-      float a, c;
-      f2_unpack(f2_mul(tanh_poly2(f2_mul(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), in2)), out2), a, c);
-      r[e] = __float_as_uint(a);
-      r[e + 1] = __float_as_uint(c);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 64; ++e) r[e] = __float_as_uint(cap_log2 * tanh_of(__uint_as_float(r[e]) * cap_in));
-  }
 }
 
 __device__ __forceinline__ void put_masked(uint32_t* r, const uint32_t* seen, uint32_t v) {
@@ -563,7 +543,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           // what a masked place holds must not choose the form of tanh, nor reach anything else
           if constexpr (kCap) put_masked(r, seen, 0u);
         }
-        if constexpr (kCap) capped64(r, p.cap_in, p.cap_log2);
+        if constexpr (kCap) capped<64>(r, p.cap);
         if (border) put_masked(r, seen, __float_as_uint(kCap ? p.cap_mask : -INFINITY));
         uint32_t pk[32];
         auto weights = [&](auto split) {
@@ -911,7 +891,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             for (int e = 0; e < 64; ++e)
               if (d + e >= len) r[e] = 0u;
           }
-          capped64(r, p.cap_in, p.cap_log2);
+          capped<64>(r, p.cap);
         }
         if (border) {
           const uint32_t out = __float_as_uint(kCap ? p.cap_mask : -INFINITY);
@@ -1047,10 +1027,9 @@ int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
   p.scale_log2 = a.sm_scale * 1.4426950408889634f;
   p.sm_scale = a.sm_scale;
   if (a.softcap > 0.f) {
-    p.cap_in = 2.f * p.scale_log2 / a.softcap;
-    p.cap_log2 = a.softcap * 1.4426950408889634f;
-    p.cap_inv = 1.f / p.cap_log2;
-    p.cap_mask = -p.cap_log2 - 300.f;
+    p.cap = make_cap(p.scale_log2, a.softcap);
+    p.cap_inv = 1.f / p.cap.log2;
+    p.cap_mask = -p.cap.log2 - 300.f;
   }
   p.lse2 = a.stats;
   p.delta = a.stats + static_cast<long long>(a.B) * a.H * p.Sq_pad;
