@@ -24,7 +24,7 @@
 // distributed shared memory, in the order of the CTAs.
 //
 // Measured, forward and backward: 9,360 rows x 8 heads, D 128, 1,560 of conditioning, 1.49 to 1.51 ms (930 TFLOP/s of
-// what is computed); 4,680 rows of 9 documents, 16 heads on 4, 0.33 ms (0.39 without clusters).  Bound by the port of
+// what is computed); 4,680 rows of 9 documents, 16 heads on 4, 0.32 ms (0.05 more without clusters).  Bound by the port of
 // the shared memory, which the operands of the products pass, and by the arithmetic between the products.
 //
 // Masked places: p and ds are set to 0 by comparison, whatever the scores hold; rows of empty queries (dkv) and keys
