@@ -5,7 +5,7 @@
 // the scale makes three steps exact: x / s, the rescaling of a block whose largest value grew (up to codes
 // that become subnormal), and code * s in 16 bits.
 //
-// Append: one CTA for each touched block of one head and tensor.  Bound: HBM (2 bytes read, 1 written for a
+// Append: 256 threads for each touched block of one head and tensor.  Bound: HBM (2 bytes read, 1 written for a
 // value), at few tokens the launch.  A block that already holds tokens keeps its scale unless the new ones
 // need a larger one; then its codes are decoded and rounded again at the new scale.  6,240 tokens x 32 heads: 35 us,
 // 4.4 TB/s of 6.5; the maximum and the conversion, about 100 instructions for 8 values, are what is left.
@@ -79,30 +79,27 @@ struct AppendParams {
   const void* x[2];
   long long sb[2], sh[2], ss[2];
   const int32_t* counts;
-  int n;
+  int n, blocks;  // tokens, and the most blocks that they touch
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
-  after_previous();
-  let_next_start();
-  const int bh = blockIdx.y;
-  const int b = bh / p.c.Hk, h = bh - b * p.c.Hk;
-  const int which = blockIdx.z;
-  const int held = p.c.lengths[b];
+// 256 threads on one touched block of one head of K or V; `sync` is a barrier of theirs, `red` of 2 x 8 words
+template <typename T, typename Sync>
+__device__ __forceinline__ void append_block(const AppendParams& p, int b, int h, int which, int block, int held, int tid,
+                                             uint32_t (*red)[kAppendThreads / 32], Sync&& sync) {
+  const int bh = b * p.c.Hk + h;
   const int room = p.c.cap - held;
   int n = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
   if (held < 0 || n > room) {  // a device-side length the host could not check: keep what fits
-    if (threadIdx.x == 0) atomicCAS(&g_cache_err, 0, BSA_ERR_INDEX);
+    if (tid == 0) atomicCAS(&g_cache_err, 0, BSA_ERR_INDEX);
     n = held < 0 ? 0 : max(room, 0);
   }
   if (n <= 0) return;
-  const int blk = held / kCacheBlock + blockIdx.x;
+  const int blk = held / kCacheBlock + block;
   const int t0 = blk * kCacheBlock;
   if (t0 >= held + n) return;
   const int lanes = p.c.D >> 3;                // 8 values to a thread
   const int per = kAppendThreads / 16;         // rows of a pass (16 thread columns, D / 8 of them used)
-  const int col = threadIdx.x & 15, row0 = threadIdx.x >> 4;
+  const int col = tid & 15, row0 = tid >> 4;
   const bool live = col < lanes;
   const int nblk = p.c.cap / kCacheBlock;
   uint8_t* codes = (which ? p.c.v : p.c.k) + (static_cast<long long>(bh) * p.c.cap + t0) * p.c.D + 8 * col;
@@ -122,13 +119,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
       v[i].zero();
     }
   }
-  __shared__ uint32_t red[2][kAppendThreads / 32];
   constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   auto block_max = [&](uint32_t m, int k) {
     uint32_t one = max(m & 0xffffu, m >> 16);
     one = __reduce_max_sync(0xffffffffu, one);
-    if ((threadIdx.x & 31) == 0) red[k][threadIdx.x >> 5] = one;
-    __syncthreads();
+    if ((tid & 31) == 0) red[k][tid >> 5] = one;
+    sync();
 #pragma unroll
     for (int i = 0; i < kAppendThreads / 32; ++i) one = max(one, red[k][i]);
     return one;
@@ -170,7 +166,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
       *dst = encode8(f, inv);
     }
   }
-  if (threadIdx.x == 0) *sp = s;
+  if (tid == 0) *sp = s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+  __shared__ uint32_t red[2][kAppendThreads / 32];
+  after_previous();
+  let_next_start();
+  const int b = blockIdx.y / p.c.Hk, h = blockIdx.y - b * p.c.Hk;
+  append_block<T>(p, b, h, blockIdx.z, blockIdx.x, p.c.lengths[b], threadIdx.x, red, [] { __syncthreads(); });
 }
 
 // lengths[b] += what append_kernel wrote; a launch of its own, since every CTA above reads the old lengths
@@ -180,6 +185,34 @@ __global__ void advance_kernel(int32_t* lengths, const int32_t* counts, int n, i
     const int held = lengths[b];
     const int add = counts ? min(max(counts[b], 0), n) : n;
     if (held >= 0) lengths[b] = min(held + add, max(cap, held));
+  }
+}
+
+// Both in one launch where a batch entry's blocks fit a cluster of 8 CTAs of four blocks each (a token on up to 16 heads):
+// the length advances when all of the cluster has read it.  A second launch costs more there than the work does (a token
+// of 16 x 8 heads: 12.5 us a call with two, 10.7 with one).
+constexpr int kSide = 4, kMostCluster = 8;
+template <typename T>
+__global__ void __launch_bounds__(kSide * kAppendThreads) append_few_kernel(const AppendParams p, int cluster) {
+  __shared__ uint32_t red[kSide][2][kAppendThreads / 32];
+  after_previous();
+  const int b = blockIdx.x / cluster, rank = blockIdx.x - b * cluster;
+  const int side = threadIdx.x / kAppendThreads;
+  const int held = p.c.lengths[b];
+  const int item = rank * kSide + side;
+  if (item < p.blocks * p.c.Hk * 2) {
+    const int block = item / (2 * p.c.Hk), head = item - block * 2 * p.c.Hk;
+    append_block<T>(p, b, head >> 1, head & 1, block, held, threadIdx.x % kAppendThreads, red[side],
+                    [&] {
+                      __syncwarp();
+                      asm volatile("bar.sync %0, %1;" ::"r"(1 + side), "n"(kAppendThreads) : "memory");
+                    });
+  }
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (rank == 0 && threadIdx.x == 0 && held >= 0) {
+    const int add = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+    p.c.lengths[b] = min(held + add, max(p.c.cap, held));
   }
 }
 
@@ -670,8 +703,25 @@ int launch_cache_append(const AppendArgs& a, cudaStream_t stream) {
   kv8::set_pair(p, a.k, a.v);
   p.counts = a.counts;
   p.n = a.n;
-  // n tokens from any place in a block touch at most this many blocks
-  const dim3 grid((a.n + kCacheBlock - 2) / kCacheBlock + 1, a.c.B * a.c.Hk, 2);
+  p.blocks = (a.n + kCacheBlock - 2) / kCacheBlock + 1;  // from any place in a block
+  const int cluster = (p.blocks * a.c.Hk * 2 + kv8::kSide - 1) / kv8::kSide;
+  if (p.blocks <= kv8::kMostCluster * kv8::kSide && cluster <= kv8::kMostCluster) {
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.c.B * cluster);
+    cfg.blockDim = dim3(kv8::kSide * kv8::kAppendThreads);
+    cfg.stream = stream;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    auto* few = a.dtype == BSA_DTYPE_F16 ? kv8::append_few_kernel<__half> : kv8::append_few_kernel<__nv_bfloat16>;
+    return cudaLaunchKernelEx(&cfg, few, p, cluster) == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;
+  }
+  const dim3 grid(p.blocks, a.c.B * a.c.Hk, 2);
   auto* kernel = a.dtype == BSA_DTYPE_F16 ? kv8::append_kernel<__half> : kv8::append_kernel<__nv_bfloat16>;
   if (launch_behind(kernel, grid, dim3(kv8::kAppendThreads), 0, stream, p) != cudaSuccess ||
       launch_behind(kv8::advance_kernel, dim3(1), dim3(128), 0, stream, a.c.lengths, a.counts, a.n, a.c.cap, a.c.B) !=

@@ -827,6 +827,29 @@ def test_cache_append(cuda, dtype, B, H, D, steps):
         assert torch.equal(got.double(), torch.where(held[:, None, :, None], want, 0.0))
 
 
+@pytest.mark.parametrize("H,steps", [(1, [500, 1, 70]), (2, [60, 200, 3]), (5, [64, 1, 65]), (8, [1, 63, 64, 1]), (16, [1, 1, 2]),
+                                     (17, [1, 62, 1])])
+def test_cache_append_heads(cuda, H, steps):
+    """Few blocks and heads go in one launch, with the lengths; both sides of the border, and counts that run over."""
+    from longcat_video import _native
+    from longcat_video.models.kv_cache import KVCache8
+
+    cap = 576
+    cache, ref = KVCache8.allocate(3, H, cap, 16, cuda), RefCache(3, H, cap, 16, cuda)
+    for i, n in enumerate(steps):
+        k, v = (rand((3, H, n, 16), torch.bfloat16, 2 * i + j, cuda, scale=2.0 ** i) for j in range(2))
+        counts = [n, n // 2, 0] if i else [n] * 3
+        cache.append(k, v, torch.tensor(counts, dtype=torch.int32, device=cuda))
+        ref.append(k, v, counts)
+        same(cache, ref)
+    assert _native.device_error() == 0
+    cache.truncate(cap - 1)
+    k = rand((3, H, 2, 16), torch.bfloat16, 9, cuda)
+    cache.append(k, k)  # one fits
+    assert cache.lengths.tolist() == [cap] * 3 and _native.device_error(clear=True) != 0
+    assert _native.device_error() == 0
+
+
 def test_cache_extremes(cuda):
     """Largest and smallest values, infinities and NaN, zeros; a full cache; rows behind the last stay."""
     from longcat_video import _native
