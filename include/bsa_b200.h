@@ -258,7 +258,8 @@ int bsa_masked_attention_backward(const void* q, const void* k, const void* v, c
  * bsa_kv8_append: n new tokens (fp16 or bf16; counts [B]: only the first counts[b] of them) behind those held;
  * lengths advance.  Tokens past the capacity are dropped and reported by bsa_device_error (BSA_ERR_INDEX).
  * Rows behind the last token keep what they hold.
- * bsa_kv8_unpack: held tokens, then n fresh ones, then zeros, as [B, Hk, rows, D] in dtype.
+ * bsa_kv8_unpack: held tokens, then n fresh ones, then zeros (zeros = 0: rows left as they are, for a reader whose mask
+ * ends there), as [B, Hk, rows, D] in dtype.
  * bsa_kv8_attention: q [B, H, Sq, D] over the held tokens, straight from the codes; causal: query i sees
  * lengths[b] - Sq + i + 1 tokens.  Meant for few rows (H / Hk * Sq up to about 128): 16 rows are one pass over the
  * codes.  scratch: bsa_kv8_attention_scratch_bytes() bytes (0: none needed). */
@@ -267,7 +268,7 @@ int bsa_kv8_append(void* k_codes, float* k_scale, void* v_codes, float* v_scale,
                    const int64_t* v_strides, const int32_t* counts, void* stream);
 int bsa_kv8_unpack(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
                    int capacity, int D, const void* k, const void* v, int dtype, int n, const int64_t* k_strides,
-                   const int64_t* v_strides, void* k_out, void* v_out, int rows, void* stream);
+                   const int64_t* v_strides, void* k_out, void* v_out, int rows, int zeros, void* stream);
 int64_t bsa_kv8_attention_scratch_bytes(int B, int H, int Hk, int Sq, int capacity, int D);
 int bsa_kv8_attention(const void* q, int dtype, int B, int H, int Sq, const int64_t* q_strides, const void* k_codes,
                       const float* k_scale, const void* v_codes, const float* v_scale, const int32_t* lengths, int Hk,

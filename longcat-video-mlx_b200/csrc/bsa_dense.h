@@ -107,7 +107,7 @@ struct UnpackArgs {
   int dtype = 0, n = 0;
   void* ko = nullptr;                  // [B, Hk, rows, D] in dtype: held tokens, fresh tokens, zeros
   void* vo = nullptr;
-  int rows = 0;
+  int rows = 0, zeros = 1;             // zeros 0: nothing is written behind the fresh tokens
 };
 int launch_cache_unpack(const UnpackArgs& a, cudaStream_t stream);
 struct CacheAttnArgs {

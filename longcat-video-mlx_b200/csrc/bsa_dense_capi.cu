@@ -324,7 +324,7 @@ int bsa_kv8_append(void* k_codes, float* k_scale, void* v_codes, float* v_scale,
 
 int bsa_kv8_unpack(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
                    int capacity, int D, const void* k, const void* v, int dtype, int n, const int64_t* k_strides,
-                   const int64_t* v_strides, void* k_out, void* v_out, int rows, void* stream) {
+                   const int64_t* v_strides, void* k_out, void* v_out, int rows, int zeros, void* stream) {
   bsa::UnpackArgs a;
   int rc = cache_view(a.c, k_codes, k_scale, v_codes, v_scale, lengths, B, Hk, capacity, D);
   if (rc) return rc;
@@ -339,7 +339,7 @@ int bsa_kv8_unpack(void* k_codes, float* k_scale, void* v_codes, float* v_scale,
     if ((rc = check_tensor(a.v, dtype, B, Hk, n, "v"))) return rc;
   }
   if (!aligned(k_out, 16) || !aligned(v_out, 16)) return set_error(BSA_ERR_ALIGN, "outputs must be 16-byte aligned");
-  a.dtype = dtype; a.n = n; a.ko = k_out; a.vo = v_out; a.rows = rows;
+  a.dtype = dtype; a.n = n; a.ko = k_out; a.vo = v_out; a.rows = rows; a.zeros = zeros;
   return launched(bsa::launch_cache_unpack(a, static_cast<cudaStream_t>(stream)), "cache unpack");
 }
 

@@ -222,7 +222,7 @@ struct UnpackParams {
   const void* x[2];
   long long sb[2], sh[2], ss[2];
   void* out[2];
-  int n, rows;
+  int n, rows, zeros;
 };
 
 template <typename T>
@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(256) unpack_kernel(const UnpackParams p) {
   const int b = bh / p.c.Hk, h = bh - b * p.c.Hk;
   const int which = blockIdx.z;
   const int held = min(max(p.c.lengths[b], 0), p.c.cap);
+  const int rows = p.zeros ? p.rows : min(p.rows, held + (p.x[0] ? p.n : 0));
   const int lanes = p.c.D >> 3;
   const int nblk = p.c.cap / kCacheBlock;
   const uint8_t* codes = (which ? p.c.v : p.c.k) + static_cast<long long>(bh) * p.c.cap * p.c.D;
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(256) unpack_kernel(const UnpackParams p) {
   const float most = std::is_same<T, __half>::value ? 65504.f : 3.3895314e38f;  // the type's largest value
   const int j0 = blockIdx.x * 64 * lanes;
 #pragma unroll 2
-  for (int j = j0 + threadIdx.x; j < min(j0 + 64 * lanes, p.rows * lanes); j += 256) {
+  for (int j = j0 + threadIdx.x; j < min(j0 + 64 * lanes, rows * lanes); j += 256) {
     const int r = j / lanes, d0 = 8 * (j - r * lanes);
     float f[8];
     if (r < held) {
@@ -738,6 +739,7 @@ int launch_cache_unpack(const UnpackArgs& a, cudaStream_t stream) {
   p.out[1] = a.vo;
   p.n = a.n;
   p.rows = a.rows;
+  p.zeros = a.zeros;
   const dim3 grid((a.rows + 63) / 64, a.c.B * a.c.Hk, 2);
   if (a.dtype == BSA_DTYPE_F16)
     kv8::unpack_kernel<__half><<<grid, 256, 0, stream>>>(p);

@@ -626,8 +626,8 @@ struct Cache {
           "bsa_kv8_append");
   }
 
-  // (k, v) in 16 bits: the held tokens, the fresh ones, zeros up to capacity + fresh
-  std::pair<Tensor, Tensor> unpack(at::ScalarType dtype, const OptTensor& k, const OptTensor& v) {
+  // (k, v) in 16 bits: the held tokens, the fresh ones and, where asked for, zeros up to capacity + fresh
+  std::pair<Tensor, Tensor> unpack(at::ScalarType dtype, const OptTensor& k, const OptTensor& v, bool zeros) {
     if (dtype != at::kBFloat16 && dtype != at::kHalf) refuse("dequantize to bf16 or fp16");
     const c10::cuda::CUDAGuard guard(kc.device());
     const int64_t n = k ? k->size(2) : 0;
@@ -640,7 +640,7 @@ struct Cache {
     }
     check(api.bsa_kv8_unpack(ptr(kc), scale(ks), ptr(vc), scale(vs), lengths(), B, Hk, cap, D, a ? a->p() : nullptr,
                              b ? b->p() : nullptr, dtype_code(dtype), n, a ? a->strides : nullptr,
-                             b ? b->strides : nullptr, ptr(ko), ptr(vo), cap + n, stream_of(kc)),
+                             b ? b->strides : nullptr, ptr(ko), ptr(vo), cap + n, zeros, stream_of(kc)),
           "bsa_kv8_unpack");
     return {ko, vo};
   }
@@ -679,7 +679,8 @@ struct Cache {
             "bsa_kv8_attention");
       return o.done(out);
     }
-    const auto kv = n ? unpack(t, k, v) : unpack(t, std::nullopt, std::nullopt);
+    // what lies behind the last token is masked, whatever it holds
+    const auto kv = n ? unpack(t, k, v, false) : unpack(t, std::nullopt, std::nullopt, false);
     const py::tuple m = attention_ranges(py::cast(kc.device()), Sq, cap + n, B, std::nullopt, causal, 0, std::nullopt,
                                          std::nullopt, std::nullopt, std::nullopt, len, n);
     const OptTensor buf = py::cast<Tensor>(m[0]);
@@ -704,6 +705,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::class_<Cache>(m, "Cache")
       .def(py::init<Tensor, Tensor, Tensor, Tensor, Tensor>())
       .def("append", &Cache::append)
-      .def("unpack", &Cache::unpack)
+      .def("unpack", [](Cache& c, at::ScalarType dtype) { return c.unpack(dtype, std::nullopt, std::nullopt, true); })
       .def("attend", &Cache::attend);
 }

@@ -90,7 +90,7 @@ class KVCache8:
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
         """(k, v) [B, Hk, capacity, D]: the held tokens, zeros behind them."""
-        return self._cache.unpack(dtype, None, None)
+        return self._cache.unpack(dtype)
 
     def attend(self, q: torch.Tensor, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None, *,
                causal: bool = False, sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:

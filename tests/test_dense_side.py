@@ -668,6 +668,26 @@ def test_attention_output_refusals(cuda):
         y.backward()
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_lookup_in_a_long_cache(cuda, causal):
+    """Many rows over few tokens of a large cache: what its scratch holds behind them does not count."""
+    from longcat_video.models.kv_cache import KVCache8
+
+    k, v = (rand((2, 2, 150, 64), torch.bfloat16, i, cuda) for i in range(2))
+    q, fk, fv = (rand((2, n, 200, 64), torch.bfloat16, 3 + i, cuda) for i, n in enumerate((4, 2, 2)))
+    short, long = KVCache8.from_kv(k, v), KVCache8.from_kv(k, v, capacity=9000)
+    for c in (short, long):
+        c.truncate(torch.tensor([150, 70], dtype=torch.int32, device=cuda))
+    junk = [torch.full((2, 2, 9200, 64), math.nan, dtype=torch.bfloat16, device=cuda) for _ in range(4)]
+    del junk  # the allocator hands these bytes out again
+    # The longer one is split along its keys.  Either side is off by a rounding of the result, u |o|, and of the weights,
+    # u sum p |v - o| <= 2 u max |v|, so they differ by 6 u max |v| at most.
+    top = max(t.abs().max().item() for t in (v, fv))
+    for fresh in ((), (fk, fv)):
+        torch.testing.assert_close(long.attend(q, *fresh, causal=causal), short.attend(q, *fresh, causal=causal), rtol=0,
+                                   atol=6 * unit(torch.bfloat16) * top)
+
+
 def test_lookup_of_many_heads(cuda):
     """More 16-row tiles than a grid is high: the cache is unpacked."""
     from longcat_video.models.kv_cache import KVCache8
