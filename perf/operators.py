@@ -391,27 +391,22 @@ def _run_plain(st):
     return dict(out=_plain_attend(st))
 
 
-_package = []
+def _package():
+    import sys
+    from pathlib import Path
 
-
-def _framework():
-    """(KVCache8, AttentionMask, masked_attention, qk_norm_rope), imported at the first pass."""
-    if not _package:
-        import os
-        import sys
-
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "longcat-video-mlx_b200"))
-        from longcat_video.models.kv_cache import KVCache8
-        from longcat_video.models.masked_attention import AttentionMask, masked_attention
-        from longcat_video.models.rope_3d import qk_norm_rope
-
-        _package.extend((KVCache8, AttentionMask, masked_attention, qk_norm_rope))
-    return _package
+    here = str(Path(__file__).resolve().parent.parent / "longcat-video-mlx_b200")
+    if here not in sys.path:
+        sys.path.insert(0, here)
 
 
 def _run_own(st):
     c = st["case"]
-    KVCache8, AttentionMask, masked_attention, qk_norm_rope = _framework()
+    _package()
+    from longcat_video.models.kv_cache import KVCache8
+    from longcat_video.models.masked_attention import AttentionMask, masked_attention
+    from longcat_video.models.rope_3d import qk_norm_rope
+
     if c["op"] == "norm_rope":
         rope = (st["tables"], _axis_dims(c["D"]), _grid(c))
         if not c["train"]:
