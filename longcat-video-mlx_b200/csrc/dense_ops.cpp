@@ -200,20 +200,25 @@ std::pair<Tensor, OptTensor> norm_rope_forward(const Tensor& q, const OptTensor&
   Tensor y0 = like(q);
   OptTensor y1;
   if (k) y1 = like(*k);
-  if (q.numel() && (!k || k->numel())) {
-    const View x0(q);
+  // the sides that hold values: one or both, or none
+  const bool has_q = q.numel() > 0, has_k = k && k->numel() > 0;
+  if (has_q || has_k) {
+    const Tensor& first = has_q ? q : *k;
+    const bool both = has_q && has_k;
+    const View x0(first);
     std::optional<View> x1;
-    if (k) x1.emplace(*k);
-    check(api.bsa_norm_rope(x0.p(), x0.strides, q.size(1), ptr(wq), ptr(y0), x1 ? x1->p() : nullptr,
-                            x1 ? x1->strides : nullptr, k ? k->size(1) : 0, ptr(wk), ptr(y1), dtype_code(q.scalar_type()),
-                            wcode, q.size(0), q.size(2), q.size(3), static_cast<float>(eps), rope.p(), rope.dt, rope.dh,
-                            rope.dw, rope.T, rope.H, rope.W, rope.start, stream_of(q)),
+    if (both) x1.emplace(*k);
+    check(api.bsa_norm_rope(x0.p(), x0.strides, first.size(1), ptr(has_q ? wq : wk), ptr(has_q ? OptTensor(y0) : y1),
+                            both ? x1->p() : nullptr, both ? x1->strides : nullptr, both ? k->size(1) : 0,
+                            both ? ptr(wk) : nullptr, both ? ptr(y1) : nullptr, dtype_code(q.scalar_type()), wcode, q.size(0),
+                            q.size(2), q.size(3), static_cast<float>(eps), rope.p(), rope.dt, rope.dh, rope.dw, rope.T, rope.H,
+                            rope.W, rope.start, stream_of(q)),
           "bsa_norm_rope");
   }
   return {y0, y1};
 }
 
-// One or two sides (x, gradient, weight, whether its weight's gradient is wanted): [dx0, dw0, dx1, dw1]
+// One or two sides that hold values (x, gradient, weight, whether its weight's gradient is wanted): [dx0, dw0, dx1, dw1]
 std::array<Tensor, 4> norm_rope_backward(const Tensor& x0, const Tensor& g0, OptTensor w0, bool want0, const OptTensor& x1,
                                          const OptTensor& g1, OptTensor w1, bool want1, double eps, const Rope& rope) {
   const int wcode = weights(x0, w0, w1);
@@ -222,29 +227,23 @@ std::array<Tensor, 4> norm_rope_backward(const Tensor& x0, const Tensor& g0, Opt
   Tensor dx0 = like(x0);
   OptTensor dx1, dw0, dw1, scratch;
   if (x1) dx1 = like(*x1);
-  const bool empty = !x0.numel() || (x1 && !x1->numel());
-  auto grad = [&] {
-    return empty ? at::zeros({D}, x0.options().dtype(at::kFloat)) : at::empty({D}, x0.options().dtype(at::kFloat));
-  };
+  auto grad = [&] { return at::empty({D}, x0.options().dtype(at::kFloat)); };
   if (want0) dw0 = grad();
   if (want1) dw1 = grad();
-  if (!empty) {
-    if (want0 || want1)
-      scratch = bytes(x0, api.bsa_norm_rope_backward_scratch_bytes(x0.size(1), x1 ? x1->size(1) : 0, D));
-    const View a(x0), ga(g0);
-    std::optional<View> b, gb;
-    if (x1) {
-      b.emplace(*x1);
-      gb.emplace(*g1);
-    }
-    check(api.bsa_norm_rope_backward(
-              a.p(), a.strides, ga.p(), ga.strides, x0.size(1), ptr(w0), ptr(dx0), static_cast<float*>(ptr(dw0)),
-              b ? b->p() : nullptr, b ? b->strides : nullptr, gb ? gb->p() : nullptr, gb ? gb->strides : nullptr,
-              x1 ? x1->size(1) : 0, ptr(w1), ptr(dx1), static_cast<float*>(ptr(dw1)), dtype_code(x0.scalar_type()), wcode,
-              x0.size(0), x0.size(2), D, static_cast<float>(eps), rope.p(), rope.dt, rope.dh, rope.dw, rope.T, rope.H, rope.W,
-              rope.start, ptr(scratch), stream_of(x0)),
-          "bsa_norm_rope_backward");
+  if (want0 || want1) scratch = bytes(x0, api.bsa_norm_rope_backward_scratch_bytes(x0.size(1), x1 ? x1->size(1) : 0, D));
+  const View a(x0), ga(g0);
+  std::optional<View> b, gb;
+  if (x1) {
+    b.emplace(*x1);
+    gb.emplace(*g1);
   }
+  check(api.bsa_norm_rope_backward(
+            a.p(), a.strides, ga.p(), ga.strides, x0.size(1), ptr(w0), ptr(dx0), static_cast<float*>(ptr(dw0)),
+            b ? b->p() : nullptr, b ? b->strides : nullptr, gb ? gb->p() : nullptr, gb ? gb->strides : nullptr,
+            x1 ? x1->size(1) : 0, ptr(w1), ptr(dx1), static_cast<float*>(ptr(dw1)), dtype_code(x0.scalar_type()), wcode,
+            x0.size(0), x0.size(2), D, static_cast<float>(eps), rope.p(), rope.dt, rope.dh, rope.dw, rope.T, rope.H, rope.W,
+            rope.start, ptr(scratch), stream_of(x0)),
+        "bsa_norm_rope_backward");
   const Tensor none;
   return {dx0, dw0.value_or(none), dx1.value_or(none), dw1.value_or(none)};
 }
@@ -295,9 +294,16 @@ class NormRope : public torch::autograd::Function<NormRope> {
     bool need[4];
     for (int i = 0, edge = 0; i < 4; ++i) need[i] = saved[i].defined() && ctx->needs_input_grad(edge++);
     int sides[2], n = 0;
-    for (int i = 0; i < 2; ++i)
-      if (saved[i].defined() && grads[i].defined() && (need[i] || need[2 + i])) sides[n++] = i;
     variable_list res(7);
+    for (int i = 0; i < 2; ++i)
+      if (saved[i].defined() && grads[i].defined() && (need[i] || need[2 + i])) {
+        if (saved[i].numel()) {
+          sides[n++] = i;
+        } else {  // no tokens or no heads
+          if (need[i]) res[i] = at::empty(saved[i].sizes(), saved[i].options());
+          if (need[2 + i]) res[2 + i] = at::zeros(saved[2 + i].sizes(), saved[2 + i].options());
+        }
+      }
     if (n) {
       auto grad = [&](int i) { return grads[i].to(saved[i].scalar_type()); };
       const int a = sides[0], b = sides[n - 1];
