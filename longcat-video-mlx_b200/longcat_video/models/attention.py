@@ -103,10 +103,15 @@ class Attention(torch.nn.Module):
         return F.scaled_dot_product_attention(q, k, v, scale=self.scale)
 
     def _norm_rope(self, q: torch.Tensor, k: torch.Tensor, grid=None, start: int = 0, norm: bool = True):
-        """q_norm / k_norm and the RoPE over ``grid`` (None: none) from place ``start`` on, in one launch."""
+        """q_norm / k_norm and the RoPE over ``grid`` (None: none) from place ``start`` on, in one launch; in two
+        where the norms' eps differ."""
         rope = self.rope_3d.tables(grid, q.device) if grid is not None else None
-        wq, wk = (self.q_norm.weight, self.k_norm.weight) if norm else (None, None)
-        return qk_norm_rope(q, k, wq, wk, self.q_norm.eps, rope=rope, start=start)
+        nq, nk = self.q_norm, self.k_norm
+        if norm and nq.eps != nk.eps:
+            return (qk_norm_rope(q, None, nq.weight, eps=nq.eps, rope=rope, start=start),
+                    qk_norm_rope(k, None, nk.weight, eps=nk.eps, rope=rope, start=start))
+        wq, wk = (nq.weight, nk.weight) if norm else (None, None)
+        return qk_norm_rope(q, k, wq, wk, nq.eps, rope=rope, start=start)
 
     def forward(self, x: torch.Tensor, shape: Tuple[int, int, int],
                 num_cond_latents: Optional[int] = None, return_kv: bool = False):

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_dense_side import rand, rope_of
+from test_dense_side import hook, rand, rope_of
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,17 @@ def test_norm_rope_side_without_heads(cuda, heads):
     for i in range(2):
         assert torch.equal(got[i], want[i][1]) and torch.equal(got[2 + i], want[i][2])
         assert heads[i] or not got[2 + i].any()
+
+
+def test_hook_norms_with_their_own_eps(cuda):
+    """q and k are normalised with their own constants, in one call or two."""
+    from longcat_video.models.rope_3d import qk_norm_rope
+
+    m = hook(cuda)
+    m.k_norm.eps = 0.5
+    q, k = (rand((1, 2, 210, 64), torch.bfloat16, i, cuda) for i in range(2))
+    rope = m.rope_3d.tables((5, 6, 7), q.device)
+    with torch.no_grad():
+        got = m._norm_rope(q, k, (5, 6, 7))
+        for y, x, n in zip(got, (q, k), (m.q_norm, m.k_norm)):
+            assert torch.equal(y, qk_norm_rope(x, None, n.weight, eps=n.eps, rope=rope))
