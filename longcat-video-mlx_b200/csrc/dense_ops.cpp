@@ -13,6 +13,7 @@
 #include <optional>
 #include <string>
 #include <torch/extension.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -248,6 +249,13 @@ std::array<Tensor, 4> norm_rope_backward(const Tensor& x0, const Tensor& g0, Opt
   return {dx0, dw0.value_or(none), dx1.value_or(none), dw1.value_or(none)};
 }
 
+// Refused: inputs with a tangent (forward-mode derivatives), which these operators would drop
+void no_tangent(std::initializer_list<const OptTensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const OptTensor* t : ts)
+    if (*t && (*t)->_fw_grad(/*level=*/0).defined()) refuse("no forward-mode derivatives: an input has a tangent");
+}
+
 // Whether a graph has to be recorded.  Refused in a capture: a leaf whose gradient node an eager graph still holds.  Its
 // gradient is added up on that graph's stream, which the capture cannot reach; autograd then ends the process.
 bool any_grad(std::initializer_list<const OptTensor*> ts) {
@@ -327,6 +335,7 @@ py::object norm_rope(const Tensor& q, const OptTensor& k, const OptTensor& wq, c
   const Rope rope{tables, dt, dh, dw, T, H, W, start};
   rope.check(q);
   const OptTensor q0(q);
+  no_tangent({&q0, &k, &wq, &wk});
   if (any_grad({&q0, &k, &wq, &wk})) {
     const variable_list y = NormRope::apply(q, k, wq, wk, tables, eps, std::array<int, 7>{dt, dh, dw, T, H, W, start});
     return k ? py::object(py::make_tuple(y[0], y[1])) : py::cast(y[0]);
@@ -572,6 +581,7 @@ py::tuple masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
            std::to_string(q.size(2)) + " and " + std::to_string(k.size(2)));
   const Mask m(q, mask, mask_batch, mask_table);
   const OptTensor q0(q), k0(k), v0(v);
+  no_tangent({&q0, &k0, &v0, &out});
   check_out(q, out, {&k0, &v0});
   if (any_grad({&q0, &k0, &v0})) {
     if (out) refuse("out= is for calls without gradients");
@@ -667,6 +677,8 @@ struct Cache {
     }
     if (at::GradMode::is_enabled() && (q.requires_grad() || (k && (k->requires_grad() || v->requires_grad()))))
       refuse("attention over a cache has no gradient");
+    const OptTensor q0(q);
+    no_tangent({&q0, &k, &v, &out});
     const double s = sm_scale ? *sm_scale : 1.0 / std::sqrt(static_cast<double>(D));
     check_scale(s, 0.0);
     check_out(q, out, {&k, &v});

@@ -2,8 +2,8 @@
 
 The dense side of the attention hook on the engine's own kernels.  A mask is a key interval [lo, hi) for each
 query row (:class:`AttentionMask`), built once for a batch and used by every layer; no Sq x Sk tensor exists.
-``masked_attention`` is differentiable, once (``create_graph=True`` is refused); its gradients are computed without
-atomics, so two runs give the same bits.
+``masked_attention`` is differentiable, once (``create_graph=True`` is refused, and so is forward mode); its gradients
+are computed without atomics, so two runs give the same bits.
 """
 
 from __future__ import annotations

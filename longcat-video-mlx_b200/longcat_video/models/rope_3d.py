@@ -118,7 +118,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_weight: Op
     place.  A weight [D] turns its tensor's norm on.  ``rope``: :class:`RopeTables` or (tables, axis dims, grid); the
     tokens stand at places ``start`` .. ``start`` + S - 1 of the grid (t-major), so a continuation behind n cached
     tokens passes ``start=n``.  Sums are fp32 and the result is rounded once (the unfused form rounds after each
-    step).  Gradients are first-order (``create_graph=True`` is refused).  Returns contiguous tensors: (q, k), or q alone."""
+    step).  Gradients are first-order and reverse-mode (others are refused).  Returns contiguous tensors: (q, k), or q alone."""
     if q_weight is None and k_weight is None and rope is None:
         raise ValueError("nothing to do: give norm weights, rope tables or both")
     if k is None and k_weight is not None:

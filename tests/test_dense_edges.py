@@ -60,3 +60,25 @@ def test_hook_norms_with_their_own_eps(cuda):
         got = m._norm_rope(q, k, (5, 6, 7))
         for y, x, n in zip(got, (q, k), (m.q_norm, m.k_norm)):
             assert torch.equal(y, qk_norm_rope(x, None, n.weight, eps=n.eps, rope=rope))
+
+
+def test_forward_mode_is_refused(cuda):
+    """A tangent would be lost: every call that has one among its inputs says so."""
+    import torch.autograd.forward_ad as fwd
+
+    from longcat_video.models.kv_cache import KVCache8
+    from longcat_video.models.masked_attention import masked_attention
+    from longcat_video.models.rope_3d import qk_norm_rope
+
+    x = rand((1, 2, 20, 64), torch.bfloat16, 1, cuda)
+    w = torch.ones(64, device=cuda)
+    cache = KVCache8.from_kv(x, x)
+    with fwd.dual_level():
+        d, dw = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(w, torch.ones_like(w))
+        for f in (lambda: masked_attention(d, x, x), lambda: masked_attention(x, d, x), lambda: masked_attention(x, x, d),
+                  lambda: masked_attention(x, x, x, out=d), lambda: qk_norm_rope(d, q_weight=w),
+                  lambda: qk_norm_rope(x, d, w, w), lambda: qk_norm_rope(x, q_weight=dw), lambda: cache.attend(d),
+                  lambda: cache.attend(x, d, x), lambda: cache.attend(x, x, d)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                f()
+        masked_attention(x, x, x)  # without a tangent
