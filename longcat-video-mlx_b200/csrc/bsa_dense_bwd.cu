@@ -58,7 +58,10 @@ struct BwdParams {
   Cap cap;
   float* lse2;          // [B * H][Sq_pad]: lse in log2 (+inf: no keys)
   float* delta;         // [B * H][Sq_pad]
-  float* up;            // fp16: [B * H][Sq_pad], what dq's row of ds is raised by (log2), then its least of 16 rows each
+  int* up;              // fp16: [B * H][Sq_pad] powers of two above |do|, then of 16 rows each the most of those and of delta's
+  int* v_up;            // fp16: [B * Hk][kBins] powers of two above |v| of the keys that are seen, v_bin of them each
+  int v_bin, v_bins;
+  Tensor4 v;
   int heads;            // B * H
   float cap_inv, cap_mask;  // 1 / cap.log2, and a score below every capped one by 2^300
   int2* rng;            // [Bm][Sq_pad]: ranges, padded with empty ones
@@ -73,11 +76,86 @@ struct BwdParams {
 // few keys share a row, and with the rounded o alone dq and dk came out with twice the error of their own rounding
 // (0.0034 against 0.0017 on causal documents in bf16).
 //
-// fp16 keeps 11 bits only above 2^-14, and ds is a product of p, which falls with the number of keys, and of do, which may
-// be small altogether.  So p and ds are raised by powers of two, which their sums are lowered by again: p by 2^kUp, ds of
-// a row by the 2^n, 0 <= n <= kUp, that brings |do_i| below 2^3 (dkv: the least of a CTA's rows).  |ds_ij| is at
-// most 2 |do_i| |v_j|, so it stays below 65504 with |v_j| up to 4,000.
-constexpr int kUp = 15;
+// fp16 keeps 11 bits only between 2^-14 and 2^16, and ds is a product of p, which falls with the number of keys, of do and
+// of v, which may be small or large altogether.  So p and ds are multiplied by powers of two, which their sums are divided
+// by again: p by 2^kUp, ds by 2^n, n <= kUp, such that 2^n |ds_ij| <= 2^n (|do_i| |v_j| + |delta_i|) < 2^15 by the
+// norms of the rows.  dq, whose rows are queries, takes n for each query, with the largest |v_j| of the keys that its tile
+// sees; dk, whose rows are keys, for each key, with the largest |do_i| and |delta_i| of its CTA's queries.  Rows that are
+// not finite choose nothing: what they touch is not finite either.
+constexpr int kUp = 15, kBelow = 14;
+constexpr int kBins = 128;  // runs of keys of a head, at least 64 keys each
+
+// The least e with |x| < 2^e; -126 for 0 and for what is not finite
+__device__ __forceinline__ int log2_above(float x) {
+  const int e = static_cast<int>((__float_as_uint(x) >> 23) & 255u);
+  return e == 255 ? -126 : e - 126;
+}
+// ... of a vector whose square is x
+__device__ __forceinline__ int log2_above_root(float x) { return (log2_above(x) + 1) >> 1; }
+__device__ __forceinline__ int pack_most(int g, int d) { return (g + 256) << 16 | (d + 256); }
+__device__ __forceinline__ int most_g(int m) { return (m >> 16) - 256; }
+__device__ __forceinline__ int most_d(int m) { return (m & 0xffff) - 256; }
+
+// The power of two above |v| of the keys of run blockIdx.x that some row may see (that lie between the first and the last key
+// of some 128 rows: what lies elsewhere must not choose anything).  16 lanes to a key, all threads of the CTA.
+__device__ __forceinline__ void values_above(const BwdParams& p, int b, int hk, uint32_t (*top)[8]) {
+  const int first = blockIdx.x * p.v_bin, end = min(p.Sk, first + p.v_bin);
+  const int lane = threadIdx.x & 15;
+  __shared__ uint32_t seen[2];
+  float most = 0.f;
+  for (int base = first; base < end; base += 64) {
+    uint64_t mask = ~0ull;
+    if (p.table) {
+      if (threadIdx.x < 2) seen[threadIdx.x] = 0u;
+      __syncthreads();
+      uint64_t mine = 0ull;
+      for (int i = threadIdx.x; i < p.q_tiles; i += 256) {
+        const int4 t = p.table[static_cast<long long>(p.Bm > 1 ? b : 0) * p.q_tiles + i];
+        const int lo = max(t.x, base), hi = min(t.y, base + 64);
+        if (lo < hi) mine |= (~0ull >> (64 - (hi - lo))) << (lo - base);
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t any = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine >> (32 * w)));
+        if ((threadIdx.x & 31) == 0 && any) atomicOr(&seen[w], any);
+      }
+      __syncthreads();
+      mask = static_cast<uint64_t>(seen[1]) << 32 | seen[0];
+      __syncthreads();
+    }
+    float n2[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int at = 16 * u + (threadIdx.x >> 4);
+      n2[u] = 0.f;
+      if (base + at < end && 8 * lane < p.D && (mask >> at & 1u)) {
+        Row8<__half> v;
+        v.load(static_cast<const __half*>(p.v.p) + b * p.v.sb + hk * p.v.sh + (base + at) * p.v.ss + 8 * lane);
+        float f[8];
+        v.get(f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n2[u] = fmaf(f[e], f[e], n2[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) n2[u] += __shfl_xor_sync(0xffffffffu, n2[u], o);
+      if (n2[u] < INFINITY) most = fmaxf(most, n2[u]);
+    }
+  }
+  const uint32_t warp = __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // >= 0: ordered as its bits
+  if ((threadIdx.x & 31) == 0) (*top)[threadIdx.x >> 5] = warp;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t m = (*top)[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) m = max(m, (*top)[w]);
+    p.v_up[(static_cast<long long>(b) * p.Hk + hk) * kBins + blockIdx.x] = log2_above_root(__uint_as_float(m));
+  }
+  __syncthreads();
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) stats_kernel(const BwdParams p) {
   constexpr int kLanes = 16;
@@ -85,9 +163,13 @@ __global__ void __launch_bounds__(256) stats_kernel(const BwdParams p) {
   const int row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
   const bool on = row < p.Sq;
-  __shared__ int least[8];
+  __shared__ uint32_t most[8];
   for (int bh = blockIdx.y; bh < p.heads; bh += gridDim.y) {
     const int b = bh / p.H, h = bh - b * p.H;
+    if constexpr (kHalf) {
+      if (static_cast<int>(blockIdx.x) < p.v_bins && h % p.G == 0) values_above(p, b, h / p.G, &most);
+      if (static_cast<int>(blockIdx.x) >= p.Sq_pad / 16) continue;
+    }
     const long long at = static_cast<long long>(bh) * p.Sq_pad + row;
     float dot = 0.f, norm2 = 0.f;
     if (on && 8 * lane < p.D) {
@@ -122,19 +204,20 @@ __global__ void __launch_bounds__(256) stats_kernel(const BwdParams p) {
             on ? p.ranges[static_cast<long long>(b) * p.Sq + row] : make_int2(0, 0);
     }
     if constexpr (kHalf) {
-      // |do|^2 < 2^(e + 1): n = floor(3 - (e + 1) / 2)
-      const int e = static_cast<int>(__float_as_uint(norm2) >> 23) - 127;
-      const int n = keys ? min(max((5 - e) >> 1, 0), kUp) : kUp;
-      if (lane == 0) p.up[at] = static_cast<float>(n);
-      const int both = __reduce_min_sync(0xffffffffu, n);
-      if ((threadIdx.x & 31) == 0) least[threadIdx.x >> 5] = both;
+      const int eg = keys ? log2_above_root(norm2) : -126, ed = keys ? log2_above(dot) : -126;
+      if (lane == 0) p.up[at] = eg;
+      const int mg = __reduce_max_sync(0xffffffffu, eg), md = __reduce_max_sync(0xffffffffu, ed);
+      if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = pack_most(mg, md);
       __syncthreads();
       if (threadIdx.x == 0) {
-        int m = least[0];
+        int g = -126, d = -126;
 #pragma unroll
-        for (int w = 1; w < 8; ++w) m = min(m, least[w]);
+        for (int w = 0; w < 8; ++w) {
+          g = max(g, most_g(most[w]));
+          d = max(d, most_d(most[w]));
+        }
         (p.up + static_cast<long long>(p.heads) * p.Sq_pad)[static_cast<long long>(bh) * (p.Sq_pad / 16) + blockIdx.x] =
-            static_cast<float>(m);
+            pack_most(g, d);
       }
       __syncthreads();
     }
@@ -276,7 +359,7 @@ struct DkvSmem {
   uint32_t tmem;
   int abort_flag;
   int first, last;
-  int up;  // fp16: what ds is raised by (log2)
+  int most[2];  // fp16: powers of two above |do| and |delta| of the CTA's queries
 };
 template <int DP>
 constexpr int dkv_smem_bytes() { return DkvSmem<DP>::kTiles + static_cast<int>(sizeof(DkvSmem<DP>)) + 1024; }
@@ -323,7 +406,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     ss.abort_flag = 0;
     ss.first = table ? INT_MAX : 0;
     ss.last = table ? -1 : p.q_tiles - 1;
-    ss.up = kUp;
+    ss.most[0] = ss.most[1] = -126;
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -351,12 +434,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if constexpr (!kBF16) {
     if (some) {
       const int runs = 8 * (last - first + 1);
-      const float* from = p.up + static_cast<long long>(p.heads) * p.Sq_pad +
-                          (static_cast<long long>(b) * p.H + hk * p.G + g_first) * (p.Sq_pad / 16) + 8 * first;
-      float least = kUp;
+      const int* from = p.up + static_cast<long long>(p.heads) * p.Sq_pad +
+                        (static_cast<long long>(b) * p.H + hk * p.G + g_first) * (p.Sq_pad / 16) + 8 * first;
+      int mg = -126, md = -126;
       for (int g = 0; g < g_count; ++g)
-        for (int i = tid; i < runs; i += kBwdThreads) least = fminf(least, from[g * static_cast<long long>(p.Sq_pad / 16) + i]);
-      atomicMin(&ss.up, static_cast<int>(least));
+        for (int i = tid; i < runs; i += kBwdThreads) {
+          const int m = from[g * static_cast<long long>(p.Sq_pad / 16) + i];
+          mg = max(mg, most_g(m));
+          md = max(md, most_d(m));
+        }
+      atomicMax(&ss.most[0], mg);
+      atomicMax(&ss.most[1], md);
     }
     __syncthreads();
   }
@@ -513,9 +601,31 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int half = warp >> 2;
     const uint32_t la = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     const int key = key0 + 32 * (warp & 3) + lane;
-    const float raise = kBF16 ? 1.f : __uint_as_float(static_cast<uint32_t>(127 + ss.up - kUp) << 23);  // of ds over p's
     bool ok = true;
-    if (some) {
+    int up = kUp;  // what ds is raised by (log2), and by which factor over p's
+    float raise = 1.f;
+    if constexpr (!kBF16) {
+      if (some) {
+        ok = bar_wait(&ss.kv_full, 0, abort_flag, err, 425);
+        ok = __all_sync(0xffffffffu, ok);
+        float n2 = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < DP / 8; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(
+              sV + (c >> 3) * kHalfBytes + sw128_offset(static_cast<uint32_t>(32 * (warp & 3) + lane), c & 7));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x0, x1;
+            unpack16<false>(w[e], x0, x1);
+            n2 = fmaf(x0, x0, fmaf(x1, x1, n2));
+          }
+        }
+        up = min(kUp, kBelow - max(ss.most[0] + log2_above_root(n2), ss.most[1]));
+        raise = __uint_as_float(static_cast<uint32_t>(127 + up - kUp) << 23);
+      }
+    }
+    if (some && ok) {
       Ring<S::kQ> rq;
       int n = 0;
       ok = walk([&](int, int, const int4& t) {
@@ -630,7 +740,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     // what p and ds were raised by
     const float lower_p = kBF16 ? 1.f : __uint_as_float((127u - kUp) << 23);
-    const float lower_ds = kBF16 ? 1.f : __uint_as_float(static_cast<uint32_t>(127 - ss.up) << 23);
+    const float lower_ds = kBF16 ? 1.f : __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
     if (p.cluster > 1) {  // this CTA's sums to shared memory: its tiles are done with
       to_shared<DP>(la + kColD, half, 32 * (warp & 3) + lane, lower_ds, smem, ok && some);
       to_shared<DP>(la + kColC, half, 32 * (warp & 3) + lane, lower_p, smem + kTile * DP * 4, ok && some);
@@ -858,12 +968,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     float lower = 1.f;
     if (steps > 0) {
       float lse2 = p.lse2[static_cast<long long>(bh) * p.Sq_pad + row];
-      if constexpr (!kBF16) {  // p raised by 2^kUp there; here p, and so ds, by what the row's do allows
-        const float n = p.up[static_cast<long long>(bh) * p.Sq_pad + row];
-        lse2 += kUp - n;
-        lower = __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(n)) << 23);
-      }
       const float delta = p.delta[static_cast<long long>(bh) * p.Sq_pad + row];
+      if constexpr (!kBF16) {  // p raised by 2^kUp there; here p, and so ds, by what the row allows
+        const int* bins = p.v_up + (static_cast<long long>(b) * p.Hk + hk) * kBins;
+        int above = -126;
+        for (int i = tab.x / p.v_bin + lane; i <= (tab.y - 1) / p.v_bin; i += 32) above = max(above, bins[i]);
+        above = __reduce_max_sync(0xffffffffu, above);
+        const int n = min(kUp, kBelow - max(p.up[static_cast<long long>(bh) * p.Sq_pad + row] + above, log2_above(delta)));
+        lse2 += static_cast<float>(kUp - n);
+        lower = __uint_as_float(static_cast<uint32_t>(127 - n) << 23);
+      }
       int lo = 0, hi = live ? p.Sk : 0;  // rows behind the last see nothing, and choose nothing
       if (p.ranges && live) {
         const int2 r = p.ranges[static_cast<long long>(bm) * p.Sq + row];
@@ -1001,7 +1115,7 @@ int launch_bwd(const CUtensorMap* m, BwdParams p, const DenseArgs& a, cudaStream
 long long dense_backward_stats_bytes(int B, int H, int Sq, int Bm) {
   const long long rows = (static_cast<long long>(Sq) + dense::kTile - 1) / dense::kTile * dense::kTile;
   const long long heads = static_cast<long long>(B) * H;
-  return (3 * heads + 2ll * Bm) * rows * 4 + heads * (rows / 16) * 4;
+  return (3 * heads + 2ll * Bm) * rows * 4 + heads * (rows / 16) * 4 + heads * dense::kBins * 4;
 }
 
 int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
@@ -1035,15 +1149,20 @@ int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
   p.delta = a.stats + static_cast<long long>(a.B) * a.H * p.Sq_pad;
   p.rng = a.ranges ? reinterpret_cast<int2*>(a.stats + 2 * static_cast<long long>(a.B) * a.H * p.Sq_pad) : nullptr;
   p.heads = a.B * a.H;
-  p.up = a.stats + (2ll * p.heads + (a.ranges ? 2ll * a.Bm : 0)) * p.Sq_pad;
+  p.up = reinterpret_cast<int*>(a.stats + (2ll * p.heads + (a.ranges ? 2ll * a.Bm : 0)) * p.Sq_pad);
+  p.v_up = p.up + static_cast<long long>(p.heads) * (p.Sq_pad + p.Sq_pad / 16);
+  p.v_bin = 64 * ((a.Sk + 64 * kBins - 1) / (64 * kBins));
+  p.v_bins = (a.Sk + p.v_bin - 1) / p.v_bin;
+  p.v = a.v;
   p.lse = a.lse;
   p.o = a.o;
   p.o_lo = a.o_lo;
   p.g = a.g;
   if (static_cast<long long>(a.B) * a.H * p.q_tiles > INT_MAX || static_cast<long long>(a.B) * a.Hk * p.k_tiles > INT_MAX / 8)
     return set_error(BSA_ERR_SHAPE, "too many row tiles for one launch");
-  const dim3 sgrid(p.Sq_pad / 16, p.heads < 65535 ? p.heads : 65535);
   const bool bf = a.dtype == BSA_DTYPE_BF16, cap = a.softcap > 0.f;
+  const int runs = p.Sq_pad / 16;
+  const dim3 sgrid(bf || runs > p.v_bins ? runs : p.v_bins, p.heads < 65535 ? p.heads : 65535);
   if (bf) stats_kernel<__nv_bfloat16><<<sgrid, 256, 0, stream>>>(p);
   else stats_kernel<__half><<<sgrid, 256, 0, stream>>>(p);
   rc = cudaGetLastError() == cudaSuccess ? BSA_OK : BSA_ERR_CUDA;

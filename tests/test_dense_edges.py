@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_dense_side import hook, rand, rope_of
+from test_dense_side import (SLACK, check, check_gradients, full, gradients, hook, rand, ref_gradients, rope_of, unit)
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,52 @@ def test_forward_mode_is_refused(cuda):
             with pytest.raises(ValueError, match="forward-mode"):
                 f()
         masked_attention(x, x, x)  # without a tangent
+
+
+def fp16_case(H, Hk, Sq, Sk, gs, vs, device, seed=0):
+    q, k = rand((1, H, Sq, 128), torch.float16, seed, device, 0.5), rand((1, Hk, Sk, 128), torch.float16, seed + 1, device, 0.5)
+    v = rand((1, Hk, Sk, 128), torch.float16, seed + 2, device, vs)
+    # gradients along the values, so that their products are as large as their norms allow
+    g = v[:, :1, torch.arange(Sq, device=device) % Sk].expand(1, H, Sq, 128).float() * (gs / vs)
+    return q, k, v, g.half()
+
+
+@pytest.mark.parametrize("H,Hk,Sq,Sk,gs,vs", [(2, 1, 6, 5, 6000.0, 1.0), (2, 2, 7, 3, 0.12, 8000.0), (4, 1, 300, 6, 60.0, 100.0),
+                                              (1, 1, 130, 300, 12000.0, 3.0), (2, 1, 1, 2, 15000.0, 1.0)])
+def test_large_gradients_in_fp16(cuda, H, Hk, Sq, Sk, gs, vs):
+    """Products of p, do and v beyond fp16's largest number, of a gradient that is not: finite, with their bits."""
+    from longcat_video.models.masked_attention import AttentionMask
+
+    q, k, v, g = fp16_case(H, Hk, Sq, Sk, gs, vs, cuda)
+    scale = 2.0 ** -8
+    for m in (None, AttentionMask.build(Sq, Sk, causal=True, device=cuda)):
+        rows = full(Sq, Sk, cuda) if m is None else (m.ranges[..., 0].long(), m.ranges[..., 1].long())
+        _, got = gradients(q, k, v, g, m, sm_scale=scale)
+        want = ref_gradients(q, k, v, g, *rows, scale, 0.0)[0]
+        assert all(w.abs().max() < 65504 for w in want)  # the result itself fits
+        check_gradients(got, q, k, v, g, *rows, scale)
+
+
+def test_large_values_do_not_cost_other_rows_their_bits(cuda):
+    """A row's dq depends on its own gradient's size, a key's dk on its own value's: the others keep their precision.
+
+    dq of rows with small gradients beside rows with large ones; values behind the padded length that are large but finite."""
+    from longcat_video.models.masked_attention import AttentionMask
+
+    q, k, v, g = (rand((1, 2, n, 64), torch.float16, i, cuda) for i, n in enumerate((200, 400, 400, 200)))
+    g = g * torch.where(torch.arange(200, device=cuda) % 2 == 0, 8000.0, 2.0 ** -6)[:, None].half()
+    m = AttentionMask.build(200, 400, k_lengths=torch.tensor([300], dtype=torch.int32, device=cuda))
+    rows = (m.ranges[..., 0].long(), m.ranges[..., 1].long())
+    _, want = gradients(q, k, v, g, m)
+    check_gradients(want, q, k, v, g, *rows, 0.125)
+    grads, ds, dl, fine, _ = ref_gradients(q, k, v, g, *rows, 0.125, 0.0)
+    u, odd = unit(torch.float16), slice(1, None, 2)
+    # the small rows' ds is raised by 2^10 at least (2^-6 * 8 * 2^4 * 2^10 < 2^12): steps of 2^-34 over the row's 300 keys
+    x = k.double().abs().amax() * 0.125 * 300 * 2.0 ** -34
+    part = lambda t: t[:, :, odd]  # noqa: E731
+    check(part(want[0]), part(grads[0]), u * part(grads[0]).abs() + u * part(ds[0]) + u * part(dl[0]) + SLACK * part(fine[0])
+          + x + 2.0 ** -24)
+    k2, v2 = k.clone(), v.clone()
+    k2[:, :, 300:], v2[:, :, 300:] = 60000.0, 60000.0
+    _, got = gradients(q, k2, v2, g, m)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
