@@ -3,7 +3,9 @@
 //   s = the smallest 2^n with max|x| / s <= 448,   code = e4m3(x / s) to nearest even,   x ~ code * s
 // A floating-point code loses no precision by a power-of-two scale (only the codes' subnormals move), and
 // the scale makes three steps exact: x / s, the rescaling of a block whose largest value grew (up to codes
-// that become subnormal), and code * s in 16 bits.
+// that become subnormal), and code * s in 16 bits within the type's range: fp16 holds every code exactly for s >= 2^-15 (the
+// last place of a code is 2^-9 s, fp16's 2^-24), bf16 for s >= 2^-124 (2^-133), up to the type's largest value.  Outside,
+// unpacking rounds and clamps where the lookup of few rows, which takes s in fp32, does not.
 //
 // Append: 256 threads for each touched block of one head and tensor.  Bound: HBM (2 bytes read, 1 written for a
 // value), at few tokens the launch.  A block that already holds tokens keeps its scale unless the new ones
@@ -131,7 +133,9 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int b, int h
   };
   const float was = *sp;
   uint32_t largest = block_max(top, 0);
+  float least = 0.f;
   if (largest >= kInf) {  // neither infinity nor NaN sets a scale: once more without them
+    least = 1.17549435e-38f;  // 2^-126, so that infinity * (1 / s) is infinity where there is nothing but zeros beside it
     top = 0u;
 #pragma unroll
     for (int i = 0; i < kCacheBlock / per; ++i) {
@@ -147,7 +151,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int b, int h
   float amax, none;
   unpack_pair(largest, amax, none, T());
   const float old = t0 < held ? was : 0.f;     // a block without tokens has no scale to keep
-  const float s = fmaxf(old, scale_of(amax));
+  const float s = fmaxf(fmaxf(old, least), scale_of(amax));
   const float inv = inverse_of(s);
 #pragma unroll
   for (int i = 0; i < kCacheBlock / per; ++i) {

@@ -131,3 +131,27 @@ def test_large_values_do_not_cost_other_rows_their_bits(cuda):
     k2[:, :, 300:], v2[:, :, 300:] = 60000.0, 60000.0
     _, got = gradients(q, k2, v2, g, m)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinities_in_a_block_of_zeros(cuda, dtype):
+    """Infinities are the block's largest code whatever else it holds; NaN stays; a lookup stays finite."""
+    from longcat_video.models.kv_cache import KVCache8
+
+    x = torch.zeros((1, 3, 70, 16), dtype=dtype, device=cuda)
+    x[0, 0, 3, 4], x[0, 0, 9, 9] = math.inf, -math.inf
+    x[0, 1, 65, 1] = math.inf
+    x[0, 2, 5, 5] = math.nan
+    cache = KVCache8.from_kv(x, x)
+    codes = cache.k_codes.float()
+    assert codes[0, 0, 3, 4] == 448 and codes[0, 0, 9, 9] == -448 and codes[0, 1, 65, 1] == 448
+    assert codes[0, 2, 5, 5].isnan() and codes.nan_to_num(0).count_nonzero() == 3
+    assert torch.equal(cache.k_codes.view(torch.uint8), cache.v_codes.view(torch.uint8))
+    out = cache.attend(rand((1, 3, 1, 16), dtype, 1, cuda))
+    assert torch.isfinite(out[:, :2]).all()
+    kd, _ = cache.dequantize(dtype)
+    assert torch.isfinite(kd[:, :2]).all()
+    one = torch.ones((1, 3, 1, 16), dtype=dtype, device=cuda)  # a finite value sets the scale as ever
+    cache.append(one, one)
+    assert cache.k_scale[0, :, 1].tolist() == [2.0 ** -8] * 3
+    assert (cache.dequantize(dtype)[0][:, :, 70] == 1).all()
