@@ -2,7 +2,8 @@
 
 Keys and values are held as e4m3 codes with one power-of-two scale for each 64 tokens of a head: half of the
 bf16 cache's memory and, where few rows attend, half of its traffic.  A floating-point code loses no precision
-by a power-of-two scale, and decoding a code to 16 bits is exact.
+by a power-of-two scale, and decoding a code to 16 bits is exact within the type's range (in fp16 for scales of 2^-15
+and above, where the block's largest value is above 0.0068; smaller ones fall into fp16's subnormals and are rounded).
 """
 
 from __future__ import annotations
