@@ -19,7 +19,9 @@
 //   warp 8    : issues the products: P(j) V first, which the next step's P waits for, then S(j+3)
 //   warp 9    : loads; one ring for K and V tiles in the order of their use (warps 10, 11: idle)
 // The maximum is raised, and O and l rescaled, only when a score exceeds it by more than 2^8 (log2 8): P stays within
-// fp16's range and rounding is relative, so the result is as exact as with the true maximum.
+// fp16's range and rounding is relative, so the result is as exact as with the true maximum.  fp16's P is multiplied by 2^7
+// (and so is l), up to 2^15: weights keep their bits down to 2^-21 of the largest and vanish below 2^-32, where 2^-25 without
+// it would cost a row with a few heavy keys the sum of a long tail.
 // P is rounded to the input type for the tensor cores, and o is divided by the sum of the rounded values: the weights
 // then sum to 1 and their rounding errors count against v_j - o_i instead of v_j.  lse comes from the fp32 values.
 //
@@ -45,6 +47,8 @@ constexpr int kThreads = 384;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kIssue = kSoftmaxWarps, kLoad = kSoftmaxWarps + 1;  // warps
 constexpr float kRescale = 8.f;  // log2
+template <bool kBF16>
+constexpr float kRaise = kBF16 ? 0.f : 7.f;  // log2: of P
 constexpr uint32_t kTmemCols = 512;
 __host__ __device__ constexpr uint32_t col_s(int b) { return 128u * static_cast<uint32_t>(b); }
 constexpr uint32_t kColO = 256, kColQ = 384, kColP = 448;
@@ -414,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (!ok) continue;
-        const float nm = m == -INFINITY ? 0.f : -m;
+        const float nm = m == -INFINITY ? 0.f : kRaise<kBF16> - m;
         const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(nm, nm);
         const bool more = j + 1 < steps;
         uint32_t pk[16];
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok) {
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
-        const float lse2 = lt == 0.f ? -INFINITY : m + log2f(lt);
+        const float lse2 = lt == 0.f ? -INFINITY : log2f(lt) - (kRaise<kBF16> - m);
         const long long flat = static_cast<long long>(bh) * p.Sq + row;
         float* part = p.splits > 1 ? p.part + (split * p.rows + flat) * p.D : nullptr;
         const long long off = b * p.ob + h * p.oh + static_cast<long long>(row) * p.os;

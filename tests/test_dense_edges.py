@@ -7,7 +7,8 @@ import math
 import pytest
 import torch
 
-from test_dense_side import (SLACK, check, check_gradients, full, gradients, hook, rand, ref_gradients, rope_of, unit)
+from test_dense_side import (SLACK, check, check_gradients, full, gradients, hook, rand, ref_attention, ref_gradients, rope_of,
+                             unit)
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +156,36 @@ def test_infinities_in_a_block_of_zeros(cuda, dtype):
     cache.append(one, one)
     assert cache.k_scale[0, :, 1].tolist() == [2.0 ** -8] * 3
     assert (cache.dequantize(dtype)[0][:, :, 70] == 1).all()
+
+
+def sink(dtype, rows, n, device):
+    """A key 18 nats above n - 1 others, whose values alone count: (q, k, v, the result in 64 bits)."""
+    q = torch.zeros((1, 1, rows, 16), dtype=dtype, device=device)
+    q[..., 0] = 1
+    k = torch.zeros((1, 1, n, 16), dtype=dtype, device=device)
+    k[0, 0, 777, 0] = 18
+    v = torch.ones((1, 1, n, 16), dtype=dtype, device=device)
+    v[0, 0, 777] = 0
+    return q, k, v, ref_attention(q[:, :, :1], k, v, *full(1, n, device), 1.0)[:3]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 130])
+def test_long_tail_under_a_sink(cuda, dtype, rows):
+    """20,000 keys 18 nats below one: each weighs 2^-26, together they are the result.
+
+    Beside the roundings that check_attention counts, a weight may be off by half of a subnormal step of fp16, 2^-25, of what
+    it is raised by, 2^7 at least: 2^-32 a key of the largest weight, of which the row's sum is one at least.  80 heads
+    leave no split along the keys, which would part the sink from most of the others."""
+    from longcat_video.models.kv_cache import KVCache8
+    from longcat_video.models.masked_attention import masked_attention
+
+    n = 20_000
+    q, k, v, (o, lse, size) = sink(dtype, rows, n, cuda)
+    bound = (2.0 ** -11 + unit(dtype) + SLACK) * size + unit(dtype) * o.abs() + n * 2.0 ** -32
+    wide = lambda t: t.expand(1, 80, *t.shape[2:])  # noqa: E731
+    got, l = masked_attention(wide(q), k, v, sm_scale=1.0, return_lse=True)
+    check(got, o.expand(got.shape), bound)
+    check(l, lse.expand(l.shape), 2.0 ** -16 * (1 + lse.abs()))
+    if rows > 128:  # the cache is unpacked
+        check(KVCache8.from_kv(wide(k), wide(v)).attend(wide(q), sm_scale=1.0), o.expand(got.shape), bound)
