@@ -18,8 +18,9 @@
 // cp.async (K and V of a block are separate groups in a ring of three, so loads run behind the arithmetic),
 // and widens them to fp16 in registers, which is exact, for mma.m16n8k16 with fp32 sums.  The queries go
 // through fp16 too: bf16's 8 bits fit fp16's 11, and each row is scaled by a power of two to its largest
-// value, so only elements 2^-14 below it lose bits.  The scales of the blocks are applied in fp32: K's to the
-// scores, V's where a block's P V is added to the output.  The tensor cores' newer path does not pay here:
+// value, so only elements 2^-14 below it lose bits.  P, at most 1, is multiplied by 2^15 in fp16, so that a long tail of
+// small weights keeps its bits (2^-29 of the largest) and its sum.  The scales of the blocks are applied in fp32: K's to the
+// scores, V's, with P's 2^-15, where a block's P V is added to the output.  The tensor cores' newer path does not pay here:
 // 16 rows fill an eighth of its smallest tile, and its operands would have to pass through shared memory.
 // One token, 8 sequences of up to 32,000 tokens, 32 heads on 8: 78 us, 4.7 TB/s of 6.5.
 #include <climits>
@@ -276,6 +277,7 @@ constexpr int kRowBytes = 128;                       // a token's codes in share
 constexpr int kSlotBytes = kCacheBlock * kRowBytes;  // K or V of one block
 constexpr int kSlots = 3;
 constexpr int kAttnSmem = kWarps * kSlots * kSlotBytes;
+constexpr float kRaise = 15.f, kLower = 1.f / 32768.f;  // of P: log2, and what its sums are multiplied by
 
 __device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   int slot = 0;
   for (; blk < blk_end; blk += kWarps) {
-    const float kscale = ksc[blk], vscale = vsc[blk];
+    const float kscale = ksc[blk], vscale = vsc[blk] * kLower;
     fetch(kc, blk + kWarps);  // into the slot of the last V read
     asm volatile("cp.async.wait_group 2;" ::: "memory");
     __syncwarp();
@@ -504,16 +506,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) cache_attn_kernel(const AttnP
       const float base = mn == -INFINITY ? 0.f : mn;
       alpha[hf] = ex2(m[hf] - base);
       m[hf] = mn;
+      const float below = base - kRaise;
       float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 8; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& v = s[t][2 * hf + e];
-          v = ex2(v - base);
+          v = ex2(v - below);
           sum += v;
         }
-      l[hf] = l[hf] * alpha[hf] + sum;
+      l[hf] = l[hf] * alpha[hf] + sum * kLower;
     }
     // P as A fragments: the scores' layout is the A layout of k-steps of 16 tokens
     uint32_t pa[4][4];

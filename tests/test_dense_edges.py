@@ -189,3 +189,14 @@ def test_long_tail_under_a_sink(cuda, dtype, rows):
     check(l, lse.expand(l.shape), 2.0 ** -16 * (1 + lse.abs()))
     if rows > 128:  # the cache is unpacked
         check(KVCache8.from_kv(wide(k), wide(v)).attend(wide(q), sm_scale=1.0), o.expand(got.shape), bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lookup_of_a_long_tail_under_a_sink(cuda, dtype):
+    """As above from the codes, which hold these keys and values exactly; 900 key heads leave no split."""
+    from longcat_video.models.kv_cache import KVCache8
+
+    q, k, v, (o, _, size) = sink(dtype, 1, 20_000, cuda)
+    wide = lambda t: t.expand(1, 900, *t.shape[2:])  # noqa: E731
+    got = KVCache8.from_kv(wide(k), wide(v)).attend(wide(q), sm_scale=1.0)
+    check(got, o.expand(got.shape), (2.0 ** -11 + SLACK) * size + unit(dtype) * o.abs() + 20_000 * 2.0 ** -32)
