@@ -188,10 +188,10 @@ inline Cap make_cap(float scale_log2, float cap) {
   c.near = 0.5f * c.most;
   return c;
 }
-// N products q.k of a row through the cap, in the cheapest form that serves all of the warp's rows: 5 or 7 packed operations
-// a pair, or two of the exponential's unit a score, of which a step's exponentials take one each.
+// N products q.k of a row through the cap where a polynomial serves all of the warp's rows, 5 or 7 packed operations a pair;
+// else they stay as they are, and false.
 template <int N>
-__device__ __forceinline__ void capped(uint32_t* r, const Cap& c) {
+__device__ __forceinline__ bool capped_near(uint32_t* r, const Cap& c) {
   float top = 0.f;
 #pragma unroll
   for (int e = 0; e < N; e += 2) top = max3_abs(top, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
@@ -214,9 +214,31 @@ __device__ __forceinline__ void capped(uint32_t* r, const Cap& c) {
   } else if (__all_sync(0xffffffffu, top <= c.most)) {
     series(c.m, std::integral_constant<int, 6>());
   } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) r[e] = __float_as_uint(c.log2 * tanh_of(__uint_as_float(r[e]) * c.in));
+    return false;
   }
+  return true;
+}
+// ... or through the exponential: two operations of its unit a score, of which a step's exponentials take one each.
+template <int N>
+__device__ __forceinline__ void capped(uint32_t* r, const Cap& c) {
+  if (capped_near<N>(r, c)) return;
+#pragma unroll
+  for (int e = 0; e < N; ++e) r[e] = __float_as_uint(c.log2 * tanh_of(__uint_as_float(r[e]) * c.in));
+}
+// ... or, where the slope is wanted too, as w = 1 - |tanh| with the product's sign, which keeps its digits where tanh rounds
+// to 1: with e = 2^-|2 a log2(e)|, w = 2 e / (1 + e), z = +-(1 - w) and 1 - tanh^2 = w (2 - w).
+template <int N>
+__device__ __forceinline__ void capped_rest(uint32_t* r, const Cap& c) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float a2 = __uint_as_float(r[e]) * c.in, x = ex2_approx(-fabsf(a2));
+    r[e] = __float_as_uint(copysignf(2.f * x * rcp_approx(1.f + x), a2));
+  }
+}
+// z log2(e) of a rest, and the slope (0 for a masked place, which is a rest above 2)
+__device__ __forceinline__ float capped_of(float w, const Cap& c, float& slope) {
+  slope = fmaxf(fabsf(w) * (2.f - fabsf(w)), 0.f);
+  return fmaf(-c.log2, w, copysignf(c.log2, w));
 }
 
 // 32 lanes x 32 columns store, counterpart of tmem_ld32

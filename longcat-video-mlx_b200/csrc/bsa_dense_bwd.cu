@@ -64,6 +64,7 @@ struct BwdParams {
   Tensor4 v;
   int heads;            // B * H
   float cap_inv, cap_mask;  // 1 / cap.log2, and a score below every capped one by 2^300
+  float cap_mask_rest;      // a rest with such a score
   int2* rng;            // [Bm][Sq_pad]: ranges, padded with empty ones
   const float* lse;
   Tensor4 o, g;         // forward output, its gradient
@@ -653,10 +654,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           // what a masked place holds must not choose the form of tanh, nor reach anything else
           if constexpr (kCap) put_masked(r, seen, 0u);
         }
-        if constexpr (kCap) capped<64>(r, p.cap);
-        if (border) put_masked(r, seen, __float_as_uint(kCap ? p.cap_mask : -INFINITY));
+        bool far = false;  // scores beyond the cap's polynomials: as rests
+        if constexpr (kCap) {
+          far = !capped_near<64>(r, p.cap);
+          if (far) capped_rest<64>(r, p.cap);
+        }
+        if (border) put_masked(r, seen, __float_as_uint(!kCap ? -INFINITY : far ? p.cap_mask_rest : p.cap_mask));
         uint32_t pk[32];
-        auto weights = [&](auto split) {
+        auto weights = [&](auto split, auto far) {
           uint32_t lo[32];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -666,9 +671,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const float s = __uint_as_float(r[4 * e + c]);
-              x[c] = ex2_approx(kCap ? s - lv[c] : fmaf(s, p.scale_log2, -lv[c]));
-              const float u = s * p.cap_inv;  // tanh
-              r[4 * e + c] = __float_as_uint(kCap ? x[c] * fmaf(-u, u, 1.f) : x[c]);
+              if constexpr (far.value) {
+                float slope;
+                x[c] = ex2_approx(capped_of(s, p.cap, slope) - lv[c]);
+                r[4 * e + c] = __float_as_uint(x[c] * slope);
+              } else {
+                x[c] = ex2_approx(kCap ? s - lv[c] : fmaf(s, p.scale_log2, -lv[c]));
+                const float u = s * p.cap_inv;  // tanh, at most tanh(1) in size
+                r[4 * e + c] = __float_as_uint(kCap ? x[c] * fmaf(-u, u, 1.f) : x[c]);
+              }
             }
             pk[2 * e] = pack16<kBF16>(x[0], x[1]);
             pk[2 * e + 1] = pack16<kBF16>(x[2], x[3]);
@@ -679,7 +690,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
           if constexpr (split.value) tmem_st32(la + kColA + 64 * half + 32, lo);
         };
-        if (fine) weights(std::true_type()); else weights(std::false_type());
+        auto all_weights = [&](auto far) {
+          if (fine) weights(std::true_type(), far); else weights(std::false_type(), far);
+        };
+        if constexpr (kCap) {
+          if (far) all_weights(std::true_type()); else all_weights(std::false_type());
+        } else {
+          all_weights(std::false_type());
+        }
         tmem_st32(la + kColA + 64 * half, pk);
         tmem_st_wait();
         tc_fence_before();
@@ -999,26 +1017,37 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int key0 = (n0 + n) * kTile;
         const bool border = key0 < tab.z || key0 + kTile > tab.w;
         const uint32_t d = static_cast<uint32_t>(key0 + 64 * half - lo);
+        bool far = false;  // scores beyond the cap's polynomials: as rests
         if constexpr (kCap) {
           if (border) {  // what a masked place holds must not choose the form of tanh
 #pragma unroll
             for (int e = 0; e < 64; ++e)
               if (d + e >= len) r[e] = 0u;
           }
-          capped<64>(r, p.cap);
+          far = !capped_near<64>(r, p.cap);
+          if (far) capped_rest<64>(r, p.cap);
         }
         if (border) {
-          const uint32_t out = __float_as_uint(kCap ? p.cap_mask : -INFINITY);
+          const uint32_t out = __float_as_uint(!kCap ? -INFINITY : far ? p.cap_mask_rest : p.cap_mask);
 #pragma unroll
           for (int e = 0; e < 64; ++e)
             if (d + e >= len) r[e] = out;
         }
+        if (kCap && far) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          const float s = __uint_as_float(r[e]);
-          const float x = ex2_approx(kCap ? s - lse2 : fmaf(s, p.scale_log2, -lse2));
-          const float u = s * p.cap_inv;  // tanh
-          r[e] = __float_as_uint(kCap ? x * fmaf(-u, u, 1.f) : x);
+          for (int e = 0; e < 64; ++e) {
+            float slope;
+            const float x = ex2_approx(capped_of(__uint_as_float(r[e]), p.cap, slope) - lse2);
+            r[e] = __float_as_uint(x * slope);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            const float s = __uint_as_float(r[e]);
+            const float x = ex2_approx(kCap ? s - lse2 : fmaf(s, p.scale_log2, -lse2));
+            const float u = s * p.cap_inv;  // tanh, at most tanh(1) in size
+            r[e] = __float_as_uint(kCap ? x * fmaf(-u, u, 1.f) : x);
+          }
         }
         const uint32_t col = (n & 1) ? kColC : kColB;
         ok = bar_wait(&ss.dp_full[n & 1], static_cast<uint32_t>((n >> 1) & 1), abort_flag, err, 472);
@@ -1144,6 +1173,7 @@ int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
     p.cap = make_cap(p.scale_log2, a.softcap);
     p.cap_inv = 1.f / p.cap.log2;
     p.cap_mask = -p.cap.log2 - 300.f;
+    p.cap_mask_rest = 4.f + 300.f * p.cap_inv;
   }
   p.lse2 = a.stats;
   p.delta = a.stats + static_cast<long long>(a.B) * a.H * p.Sq_pad;

@@ -200,3 +200,25 @@ def test_lookup_of_a_long_tail_under_a_sink(cuda, dtype):
     wide = lambda t: t.expand(1, 900, *t.shape[2:])  # noqa: E731
     got = KVCache8.from_kv(wide(k), wide(v)).attend(wide(q), sm_scale=1.0)
     check(got, o.expand(got.shape), (2.0 ** -11 + SLACK) * size + unit(dtype) * o.abs() + 20_000 * 2.0 ** -32)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("times", [2.0, 6.0, 9.0, 12.0])
+@pytest.mark.parametrize("Sq,Sk", [(3, 5), (140, 700)])
+def test_slope_of_the_cap_far_out(cuda, times, sign, Sq, Sk):
+    """Scores at several times the cap: 1 - tanh^2 falls like 4 e^(-2 |s| / cap) and keeps its digits."""
+    from longcat_video.models.masked_attention import AttentionMask
+
+    q, k, v, g = (rand((1, 2, n, 64), torch.bfloat16, i, cuda, 0.02 if i < 2 else 1.0) for i, n in enumerate((Sq, Sk, Sk, Sq)))
+    cap = 4.0
+    q[..., 0], k[..., 0] = times, sign
+    scale = cap  # scores near times * cap
+    for m in (None, AttentionMask.build(Sq, Sk, causal=True, device=cuda)):
+        rows = full(Sq, Sk, cuda) if m is None else (m.ranges[..., 0].long(), m.ranges[..., 1].long())
+        _, got = gradients(q, k, v, g, m, softcap=cap, sm_scale=scale)
+        grads, ds, dl, fine, _ = ref_gradients(q, k, v, g, *rows, scale, cap)
+        u = unit(torch.bfloat16)
+        # 2 |s| / cap in fp32: an error of 2^-20 of it (sums, scale and the exponential) is one of the slope
+        e = SLACK + 2.0 ** -18 * 2 * (times + 1)
+        for i in range(2):
+            check(got[i], grads[i], u * grads[i].abs() + (u + e) * ds[i] + u * dl[i] + SLACK * fine[i] + 1e-37)
