@@ -654,12 +654,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           // what a masked place holds must not choose the form of tanh, nor reach anything else
           if constexpr (kCap) put_masked(r, seen, 0u);
         }
-        bool far = false;  // scores beyond the cap's polynomials: as rests
-        if constexpr (kCap) {
-          far = !capped_near<64>(r, p.cap);
-          if (far) capped_rest<64>(r, p.cap);
-        }
-        if (border) put_masked(r, seen, __float_as_uint(!kCap ? -INFINITY : far ? p.cap_mask_rest : p.cap_mask));
+        bool far = false;  // scores beyond the cap's polynomials
+        if constexpr (kCap) far = !capped_near<64>(r, p.cap);
         uint32_t pk[32];
         auto weights = [&](auto split, auto far) {
           uint32_t lo[32];
@@ -690,13 +686,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
           if constexpr (split.value) tmem_st32(la + kColA + 64 * half + 32, lo);
         };
-        auto all_weights = [&](auto far) {
-          if (fine) weights(std::true_type(), far); else weights(std::false_type(), far);
-        };
-        if constexpr (kCap) {
-          if (far) all_weights(std::true_type()); else all_weights(std::false_type());
+        if (kCap && far) [[unlikely]] {
+          capped_rest<64>(r, p.cap);
+          if (border) put_masked(r, seen, __float_as_uint(p.cap_mask_rest));
+          weights(std::true_type(), std::bool_constant<kCap>());  // what is left over is used where `fine`
         } else {
-          all_weights(std::false_type());
+          if (border) put_masked(r, seen, __float_as_uint(kCap ? p.cap_mask : -INFINITY));
+          if (fine) weights(std::true_type(), std::false_type()); else weights(std::false_type(), std::false_type());
         }
         tmem_st32(la + kColA + 64 * half, pk);
         tmem_st_wait();
@@ -1017,23 +1013,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int key0 = (n0 + n) * kTile;
         const bool border = key0 < tab.z || key0 + kTile > tab.w;
         const uint32_t d = static_cast<uint32_t>(key0 + 64 * half - lo);
-        bool far = false;  // scores beyond the cap's polynomials: as rests
-        if constexpr (kCap) {
-          if (border) {  // what a masked place holds must not choose the form of tanh
+        auto mask = [&](float v) {
+          if (border) {
 #pragma unroll
             for (int e = 0; e < 64; ++e)
-              if (d + e >= len) r[e] = 0u;
+              if (d + e >= len) r[e] = __float_as_uint(v);
           }
+        };
+        bool far = false;  // scores beyond the cap's polynomials
+        if constexpr (kCap) {
+          mask(0.f);  // what a masked place holds must not choose the form of tanh
           far = !capped_near<64>(r, p.cap);
-          if (far) capped_rest<64>(r, p.cap);
         }
-        if (border) {
-          const uint32_t out = __float_as_uint(!kCap ? -INFINITY : far ? p.cap_mask_rest : p.cap_mask);
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (d + e >= len) r[e] = out;
-        }
-        if (kCap && far) {
+        if (kCap && far) [[unlikely]] {
+          capped_rest<64>(r, p.cap);
+          mask(p.cap_mask_rest);
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
             float slope;
@@ -1041,6 +1035,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             r[e] = __float_as_uint(x * slope);
           }
         } else {
+          mask(kCap ? p.cap_mask : -INFINITY);
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
             const float s = __uint_as_float(r[e]);
