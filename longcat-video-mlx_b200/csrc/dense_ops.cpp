@@ -6,7 +6,6 @@
 // The entries are looked up in the engine's library, which Python has loaded; errors of the C ABI come back as
 // ValueError (arguments) or BSAError, with its message.
 #include <dlfcn.h>
-#include <ATen/MemoryOverlap.h>
 #include <algorithm>
 #include <array>
 #include <cmath>
@@ -447,19 +446,108 @@ void check_scale(double sm_scale, double softcap) {
   if (!(softcap >= 0) || std::isinf(softcap)) refuse("softcap must be finite and >= 0");
 }
 
-// The output may be q itself: a row of it is written by who has read that row of q.  It overlaps no input otherwise.
-void check_out(const Tensor& q, const OptTensor& out, std::initializer_list<const OptTensor*> others) {
-  if (!out) return;
+// Whether views share bytes.  A place of a view is its base and a sum of strides times indexes, so two views meet where
+// sum step_i x_i = distance has a solution with lo_i <= x_i <= hi_i.  Steps are tried from the largest down; what the smaller
+// ones can still reach leaves two or three x_i each for views of one layout.
+enum class Meet { kNo, kYes, kUnknown };
+
+class Steps {
+ public:
+  void add(int64_t step, int64_t lo, int64_t hi) {
+    if (lo == hi) return;
+    for (int i = 0; i < n_; ++i)
+      if (axis_[i].step == step) {
+        axis_[i].lo += lo;
+        axis_[i].hi += hi;
+        return;
+      }
+    axis_[n_++] = {step, lo, hi};
+  }
+  // whether there are `want` solutions
+  Meet reach(int64_t distance, int want) {
+    std::sort(axis_, axis_ + n_, [](const Axis& a, const Axis& b) { return a.step > b.step; });
+    lo_[n_] = hi_[n_] = 0;
+    for (int i = n_ - 1; i >= 0; --i) {
+      lo_[i] = lo_[i + 1] + axis_[i].step * axis_[i].lo;
+      hi_[i] = hi_[i + 1] + axis_[i].step * axis_[i].hi;
+    }
+    left_ = 1 << 16;
+    missing_ = want;
+    search(0, distance);
+    return missing_ <= 0 ? Meet::kYes : left_ < 0 ? Meet::kUnknown : Meet::kNo;
+  }
+
+ private:
+  struct Axis {
+    int64_t step, lo, hi;
+  };
+  void search(int i, int64_t distance) {
+    if (distance < lo_[i] || distance > hi_[i] || missing_ <= 0 || --left_ < 0) return;
+    if (i == n_) {
+      --missing_;
+      return;
+    }
+    const Axis& a = axis_[i];
+    auto floor_div = [](int64_t x, int64_t d) { return x >= 0 ? x / d : -((-x + d - 1) / d); };
+    const int64_t first = std::max(a.lo, -floor_div(hi_[i + 1] - distance, a.step));
+    const int64_t last = std::min(a.hi, floor_div(distance - lo_[i + 1], a.step));
+    for (int64_t x = first; x <= last && missing_ > 0 && left_ >= 0; ++x) search(i + 1, distance - x * a.step);
+  }
+  Axis axis_[12];
+  int n_ = 0, missing_ = 0, left_ = 0;
+  int64_t lo_[13], hi_[13];
+};
+
+bool same_view(const Tensor& a, const Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
+}
+
+Meet meet(const Tensor& a, const Tensor& b) {
+  if (!a.numel() || !b.numel()) return Meet::kNo;
+  const int64_t size[2] = {a.element_size(), b.element_size()};
+  const int64_t distance = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+  Steps s;
+  for (int i = 0; i < 4; ++i) {
+    if (a.stride(i)) s.add(a.stride(i) * size[0], 0, a.size(i) - 1);
+    if (b.stride(i)) s.add(b.stride(i) * size[1], 1 - b.size(i), 0);
+  }
+  s.add(1, 1 - size[1], size[0] - 1);
+  return s.reach(distance, 1);
+}
+
+Meet meets_itself(const Tensor& t) {
+  if (!t.numel()) return Meet::kNo;
+  Steps s;
+  for (int i = 0; i < 4; ++i) {
+    if (t.size(i) > 1 && !t.stride(i)) return Meet::kYes;
+    s.add(t.stride(i), 1 - t.size(i), t.size(i) - 1);
+  }
+  // axes of one step meet, and are one axis to the search below, which looks for a way to 0 beside zeros alone
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      if (t.size(i) > 1 && t.size(j) > 1 && t.stride(i) == t.stride(j)) return Meet::kYes;
+  return s.reach(0, 2);
+}
+
+// The output may be q itself: a row of it is written by who has read that row of q.  It overlaps no input otherwise, nor
+// itself.  True: views too entangled to tell, whose result is computed aside.
+bool check_out(const Tensor& q, const OptTensor& out, std::initializer_list<const OptTensor*> others) {
+  if (!out) return false;
   same_place(q, *out);
   if (out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type()) refuse("out must have q's shape and dtype");
   if (at::GradMode::is_enabled() && out->requires_grad()) refuse("out= is for calls without gradients");
-  bool over = at::get_overlap_status(*out, q) == at::MemOverlapStatus::Partial;
+  Meet m = meets_itself(*out);
+  if (m == Meet::kYes) refuse("out overlaps itself");
+  bool aside = m == Meet::kUnknown;
+  auto against = [&](const Tensor& t) {
+    m = meet(*out, t);
+    if (m == Meet::kYes) refuse("out overlaps an input");
+    aside = aside || m == Meet::kUnknown;
+  };
+  if (!same_view(*out, q)) against(q);
   for (const OptTensor* t : others)
-    if (*t) {
-      const at::MemOverlapStatus s = at::get_overlap_status(*out, **t);
-      over = over || s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
-    }
-  if (over) refuse("out overlaps an input");
+    if (*t) against(**t);
+  return aside;
 }
 
 // The caller's output where the kernels can write it, else a new tensor that is copied there at the end.
@@ -467,7 +555,7 @@ struct Output {
   Tensor t;
   bool copy;
   int64_t strides[3];
-  Output(const Tensor& q, const OptTensor& out) : copy(out && !readable(*out)) {
+  Output(const Tensor& q, const OptTensor& out, bool aside) : copy(out && (aside || !readable(*out))) {
     t = out && !copy ? *out : like(q);
     for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
   }
@@ -486,10 +574,10 @@ struct Attended {
 };
 
 Attended attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Mask& m, double sm_scale, double softcap,
-                           const OptTensor& out, bool want_lse, bool want_rest) {
+                           const OptTensor& out, bool aside, bool want_lse, bool want_rest) {
   const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1), Sk = k.size(2);
   const c10::cuda::CUDAGuard guard(q.device());
-  Output o(q, out);
+  Output o(q, out, aside);
   OptTensor lse, rest;
   if (want_lse) lse = at::empty({B, H, Sq}, q.options().dtype(at::kFloat));
   if (want_rest) rest = like(q);
@@ -544,7 +632,7 @@ class MaskedAttention : public torch::autograd::Function<MaskedAttention> {
                                const OptTensor& mask, int64_t mask_batch, int64_t mask_table, double sm_scale,
                                double softcap) {
     const Attended a = attention_forward(q, k, v, Mask(q, mask, mask_batch, mask_table), sm_scale, softcap, std::nullopt,
-                                         true, true);
+                                         false, true, true);
     ctx->save_for_backward({q, k, v, a.out, *a.rest, *a.lse, mask.value_or(Tensor())});
     ctx->saved_data["mask"] = std::vector<int64_t>{mask_batch, mask_table};
     ctx->saved_data["scale"] = std::vector<double>{sm_scale, softcap};
@@ -582,13 +670,13 @@ py::tuple masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
   const Mask m(q, mask, mask_batch, mask_table);
   const OptTensor q0(q), k0(k), v0(v);
   no_tangent({&q0, &k0, &v0, &out});
-  check_out(q, out, {&k0, &v0});
+  const bool aside = check_out(q, out, {&k0, &v0});
   if (any_grad({&q0, &k0, &v0})) {
     if (out) refuse("out= is for calls without gradients");
     const variable_list r = MaskedAttention::apply(q, k, v, mask, mask_batch, mask_table, sm_scale, softcap);
     return py::make_tuple(r[0], r[1]);
   }
-  const Attended a = attention_forward(q, k, v, m, sm_scale, softcap, out, want_lse, false);
+  const Attended a = attention_forward(q, k, v, m, sm_scale, softcap, out, aside, want_lse, false);
   return py::make_tuple(a.out, a.lse);
 }
 
@@ -681,12 +769,12 @@ struct Cache {
     no_tangent({&q0, &k, &v, &out});
     const double s = sm_scale ? *sm_scale : 1.0 / std::sqrt(static_cast<double>(D));
     check_scale(s, 0.0);
-    check_out(q, out, {&k, &v});
+    const bool aside = check_out(q, out, {&k, &v});
     const c10::cuda::CUDAGuard guard(kc.device());
     if (!q.numel()) return out ? *out : like(q);
     const int64_t n = k ? k->size(2) : 0;
     if (n == 0 && H / Hk * Sq <= few_rows && B * Hk * ((H / Hk * Sq + 15) / 16) <= 65535) {  // (a grid's height)
-      Output o(q, out);
+      Output o(q, out, aside);
       const View a(q);
       OptTensor scratch;
       const int64_t need = api.bsa_kv8_attention_scratch_bytes(B, H, Hk, Sq, cap, D);
@@ -702,7 +790,8 @@ struct Cache {
     const py::tuple m = attention_ranges(py::cast(kc.device()), Sq, cap + n, B, std::nullopt, causal, 0, std::nullopt,
                                          std::nullopt, std::nullopt, std::nullopt, len, n);
     const OptTensor buf = py::cast<Tensor>(m[0]);
-    return attention_forward(q, kv.first, kv.second, Mask(q, buf, B, py::cast<int64_t>(m[2])), s, 0.0, out, false, false).out;
+    return attention_forward(q, kv.first, kv.second, Mask(q, buf, B, py::cast<int64_t>(m[2])), s, 0.0, out, aside, false, false)
+        .out;
   }
 };
 

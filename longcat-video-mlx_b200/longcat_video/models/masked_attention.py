@@ -82,7 +82,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     bf16 or fp16 CUDA tensors, D a multiple of 8 up to 128, any strides (views that the kernels cannot read in place
     are copied once).  sm_scale defaults to 1 / sqrt(D).  Rows that see no key give zeros, and -inf in the
     log-sum-exp [B, H, Sq] (fp32, natural) that ``return_lse`` adds; it carries no gradient.  ``out``: a
-    preallocated [B, H, Sq, D] result, which may be q but overlaps no other input (not with gradients).
+    preallocated [B, H, Sq, D] result, which may be q; over another input, or itself, it is refused (so with gradients).
 
     What masked places hold does not matter, with one limit: a value that is infinite or NaN, in a row of v (for
     gradients, of k too) between the first and the last key that some row of the same 128 queries sees, can reach all

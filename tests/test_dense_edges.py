@@ -222,3 +222,88 @@ def test_slope_of_the_cap_far_out(cuda, times, sign, Sq, Sk):
         e = SLACK + 2.0 ** -18 * 2 * (times + 1)
         for i in range(2):
             check(got[i], grads[i], u * grads[i].abs() + (u + e) * ds[i] + u * dl[i] + SLACK * fine[i] + 1e-37)
+
+
+def test_outputs_over_packed_inputs(cuda):
+    """Slots of one packed projection: over q in place, over k or v refused, beside them in place."""
+    from longcat_video.models.kv_cache import KVCache8
+    from longcat_video.models.masked_attention import masked_attention
+
+    for H, N in ((3, 210), (4, 64)):
+        packed = rand((2, N, 4, H, 64), torch.bfloat16, 1, cuda)
+        q, k, v, free = packed.permute(2, 0, 3, 1, 4)
+        want = masked_attention(q, k, v)
+        cache = KVCache8.from_kv(k, v)
+        held = cache.attend(q, k, v)
+        for bad in (k, v):
+            with pytest.raises(ValueError, match="overlaps"):
+                masked_attention(q, k, v, out=bad)
+            with pytest.raises(ValueError, match="overlaps"):
+                cache.attend(q, k, v, out=bad)
+        before = packed.clone()
+        masked_attention(q, k, v, out=free)
+        assert torch.equal(free, want) and torch.equal(packed[:, :, :3], before[:, :, :3])
+        cache.attend(q, k, v, out=free)
+        assert torch.equal(free, held) and torch.equal(packed[:, :, :3], before[:, :, :3])
+        masked_attention(q, k, v, out=q)
+        assert torch.equal(q, want) and torch.equal(packed[:, :, 1:3], before[:, :, 1:3])
+
+
+def test_outputs_that_shift_or_turn_an_input(cuda):
+    from longcat_video.models.masked_attention import masked_attention
+
+    row = rand((1, 2 * 41, 2, 64), torch.bfloat16, 1, cuda)
+    q = row[:, 0:80:2].transpose(1, 2)  # every second token of both heads
+    k = rand((1, 2, 50, 64), torch.bfloat16, 2, cuda)
+    want = masked_attention(q, k, k)
+    for bad in (row[:, 2:82:2].transpose(1, 2), row[:, 1:41].transpose(1, 2)):  # shifted, and of another step
+        with pytest.raises(ValueError, match="overlaps"):
+            masked_attention(q, k, k, out=bad)
+    odd = row[:, 1:81:2].transpose(1, 2)  # the tokens between
+    assert torch.equal(masked_attention(q, k, k, out=odd), want)
+    square = rand((1, 6, 6, 64), torch.bfloat16, 3, cuda)
+    with pytest.raises(ValueError, match="overlaps"):
+        masked_attention(square, square.clone(), square.clone(), out=square.transpose(1, 2))
+    flat = torch.zeros(4096, dtype=torch.bfloat16, device=cuda)
+    for bad in (flat.as_strided((1, 2, 40, 64), (8192, 2048, 32, 1)), flat[:64].expand(1, 2, 40, 64)):  # rows over one another
+        with pytest.raises(ValueError, match="overlaps"):
+            masked_attention(q.contiguous(), k, k, out=bad)
+
+
+def test_overlaps_of_views_against_their_places(cuda):
+    """Random views into one buffer: refused where, and only where, a place of the output is one of an input or its own."""
+    import random
+
+    from longcat_video.models.masked_attention import masked_attention
+
+    r = random.Random(5)
+    buf = torch.zeros(6000, dtype=torch.bfloat16, device=cuda)
+    index = torch.arange(6000)
+
+    def view(S):
+        while True:
+            H = r.choice([1, 2, 2, 3])
+            step = [8 * r.choice([0, 1, 1, 2, 3, 4, 5, 12, 20, 40, 41]) if r.random() < 0.9 else r.randint(1, 70) for _ in range(3)]
+            at, shape = r.choice([8 * r.randint(0, 200), r.randint(0, 1000)]), (2, H, S, 8)
+            if at + sum((n - 1) * s for n, s in zip(shape, step)) + 8 <= 6000:
+                return lambda t: t.as_strided(shape, (*step, 1), at)
+
+    seen = {True: 0, False: 0}
+    for _ in range(400):
+        make = [view(5), view(7)]
+        out = make[0](buf)
+        q = torch.ones_like(out)
+        k, H = make[1](buf), out.shape[1]
+        if H % k.shape[1]:
+            continue
+        own, other = make[0](index).flatten().tolist(), set(make[1](index).flatten().tolist())
+        meets = len(set(own)) < len(own) or not other.isdisjoint(own)
+        seen[meets] += 1
+        if meets:
+            with pytest.raises(ValueError, match="overlaps"):
+                masked_attention(q, k, torch.ones_like(k), out=out)
+        else:
+            masked_attention(q, k, torch.ones_like(k), out=out)
+            assert (out == 1).all() and buf.count_nonzero() == out.numel()
+            buf.zero_()
+    assert min(seen.values()) > 40
