@@ -693,6 +693,7 @@ struct Cache {
     if (kc.dim() != 4 || kc.sizes() != vc.sizes()) refuse("codes must be [B, Hk, capacity, D]");
     small(kc);
     B = kc.size(0), Hk = kc.size(1), cap = kc.size(2), D = kc.size(3);
+    if (Hk == 0) refuse("a cache needs key heads");
     if (cap % 64 || cap == 0) refuse("capacity " + std::to_string(cap) + " must be a positive multiple of 64");
     if (D % 8 || D <= 0 || D > 128) refuse("head_dim D=" + std::to_string(D) + " must be a multiple of 8 and <= 128");
     for (const Tensor* t : {&kc, &vc})

@@ -307,3 +307,12 @@ def test_overlaps_of_views_against_their_places(cuda):
             assert (out == 1).all() and buf.count_nonzero() == out.numel()
             buf.zero_()
     assert min(seen.values()) > 40
+
+
+def test_cache_without_heads_is_refused(cuda):
+    from longcat_video.models.kv_cache import KVCache8
+
+    with pytest.raises(ValueError, match="heads"):
+        KVCache8.allocate(1, 0, 64, 64, cuda)
+    with pytest.raises(ValueError, match="heads"):
+        KVCache8.from_kv(*(torch.empty((1, 0, 5, 64), dtype=torch.bfloat16, device=cuda) for _ in range(2)))
