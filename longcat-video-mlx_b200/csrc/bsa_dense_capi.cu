@@ -80,6 +80,11 @@ int norm_rope_plan(bsa::NormRopeArgs& a, int dtype, int w_dtype, int B, int S, i
         static_cast<long long>(start) + S > static_cast<long long>(rope_T) * rope_H * rope_W)
       return set_error(BSA_ERR_SHAPE, "rope grid (%d, %d, %d) does not cover tokens %d to %lld", rope_T, rope_H, rope_W,
                        start, static_cast<long long>(start) + S);
+    // an axis's cosines are indexed in 32 bits
+    const int n[3] = {rope_T, rope_H, rope_W}, d[3] = {rope_dt, rope_dh, rope_dw};
+    for (int i = 0; i < 3; ++i)
+      if (static_cast<long long>(n[i]) * (d[i] / 2) > INT_MAX)
+        return set_error(BSA_ERR_SHAPE, "a rope table of %d places of %d angles is too large", n[i], d[i] / 2);
   }
   a.dtype = dtype; a.w_dtype = w_dtype; a.B = B; a.S = S; a.D = D; a.eps = eps;
   a.rope = rope; a.dt = rope_dt; a.dh = rope_dh; a.dw = rope_dw;
