@@ -80,6 +80,8 @@ int norm_rope_plan(bsa::NormRopeArgs& a, int dtype, int w_dtype, int B, int S, i
         static_cast<long long>(start) + S > static_cast<long long>(rope_T) * rope_H * rope_W)
       return set_error(BSA_ERR_SHAPE, "rope grid (%d, %d, %d) does not cover tokens %d to %lld", rope_T, rope_H, rope_W,
                        start, static_cast<long long>(start) + S);
+    if (static_cast<long long>(start) + S > INT_MAX)
+      return set_error(BSA_ERR_SHAPE, "places %d to %lld do not fit 32 bits", start, static_cast<long long>(start) + S);
     // an axis's cosines are indexed in 32 bits
     const int n[3] = {rope_T, rope_H, rope_W}, d[3] = {rope_dt, rope_dh, rope_dw};
     for (int i = 0; i < 3; ++i)

@@ -17,3 +17,11 @@ def test_rope_tables_beyond_32_bits(lib, dims, grid):  # noqa: F811
             1e-6, *rope, None, None]
     rc, msg = call(lib, "bsa_norm_rope_backward", "pspsippppspsipppiiiiifpiiiiiiipp", args)
     assert rc == 1 and "table" in msg
+
+
+def test_rope_places_beyond_32_bits(lib):  # noqa: F811
+    """A grid may hold more than 2^31 places; the tokens' own stay within 32 bits."""
+    rope = [FAKE, 44, 42, 42, 2 ** 11, 2 ** 10, 2 ** 11, 2 ** 31 - 32]
+    args = [FAKE, strides(*ST), 2, FAKE, FAKE, None, None, 0, None, None, 2, 0, 1, 64, 128, 1e-6, *rope, None]
+    rc, msg = call(lib, "bsa_norm_rope", "psipppsippiiiiifpiiiiiiip", args)
+    assert rc == 1 and "32 bits" in msg
