@@ -67,7 +67,8 @@ int norm_rope_plan(bsa::NormRopeArgs& a, int dtype, int w_dtype, int B, int S, i
   if (w_dtype != BSA_DTYPE_F32 && w_dtype != BSA_DTYPE_F16 && w_dtype != BSA_DTYPE_BF16)
     return set_error(BSA_ERR_DTYPE, "unsupported weight dtype code %d", w_dtype);
   if (B <= 0 || S <= 0) return set_error(BSA_ERR_SHAPE, "empty tensor");
-  if (static_cast<long long>(B) * (S / 16 + 1) >= INT_MAX) return set_error(BSA_ERR_SHAPE, "too many tokens for one launch");
+  if (S > INT_MAX - 64 || static_cast<long long>(B) * (S / 16 + 1) >= INT_MAX)  // a tile's rows go past the last token
+    return set_error(BSA_ERR_SHAPE, "too many tokens for one launch");
   int rc = check_head_dim(D);
   if (rc) return rc;
   if (!(eps >= 0.f)) return set_error(BSA_ERR_ARG, "norm eps must be >= 0");

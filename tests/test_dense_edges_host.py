@@ -25,3 +25,11 @@ def test_rope_places_beyond_32_bits(lib):  # noqa: F811
     args = [FAKE, strides(*ST), 2, FAKE, FAKE, None, None, 0, None, None, 2, 0, 1, 64, 128, 1e-6, *rope, None]
     rc, msg = call(lib, "bsa_norm_rope", "psipppsippiiiiifpiiiiiiip", args)
     assert rc == 1 and "32 bits" in msg
+
+
+def test_tokens_at_the_32_bit_border(lib):  # noqa: F811
+    """The last tile's rows behind the last token are counted in 32 bits too."""
+    args = [FAKE, strides(8, 8, 8), 1, FAKE, FAKE, None, None, 0, None, None, 2, 0, 1, 2 ** 31 - 3, 8, 1e-6, None, 0, 0, 0, 0, 0, 0, 0,
+            None]
+    rc, msg = call(lib, "bsa_norm_rope", "psipppsippiiiiifpiiiiiiip", args)
+    assert rc == 1 and "too many tokens" in msg
