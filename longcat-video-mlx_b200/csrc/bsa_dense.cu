@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       int slot = 0, issued = 0, fixes = 0;
       uint32_t phase = 0;
-      bool ok = true;
+      bool ok = true, fixing = false;
       // in the order of use: K(0) K(1) K(2), then V(j) K(j+3)
       int ik = 0, iv = 0;
       for (int i = 0; i < 2 * steps && ok; ++i) {
@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           ok = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 302);
           ok = __all_sync(0xffffffffu, ok);
+          fixing = !ok;
           if (!ok) break;
           ++fixes;
           for (int r = 0; r < kTile; ++r)
@@ -218,15 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase ^= 1u;
         }
       }
-      if (!ok && lane == 0) {
-        // wind-down after an expired wait: no load into this CTA's shared memory may still be in flight
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(&ss.q_full, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
-        }
-        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-          while (!mbar_try_wait(&ss.full[i % kStages], static_cast<uint32_t>((i / kStages) & 1)) &&
-                 globaltimer_ns() - t0 < kWaitLimitNs) {
-          }
+      if (lane == 0) {
+        drain(&ss.q_full, 0);
+        drain_ring(ss.full, kStages, issued);
+        if (fixing) drain(&ss.fix, static_cast<uint32_t>(fixes & 1));
       }
     }
     __syncwarp();

@@ -62,6 +62,19 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, ui
   for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * kHalfBytes, m, bar, 64 * c, row, h, b);
 }
 
+// The loading warp's end, by one lane: every load that it issued has landed before the CTA may end and its shared memory go to
+// another, whether or not their readers are still there.  `issued` tiles of a ring of `stages` have signalled, or will, on
+// `full`; a load of a tile that this warp mends before it hands it on signals on a barrier of its own.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < kWaitLimitNs) {
+  }
+}
+__device__ __forceinline__ void drain_ring(uint64_t* full, int stages, int issued) {
+  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+    drain(&full[i % stages], static_cast<uint32_t>((i / stages) & 1));
+}
+
 // Zeros in row r of a tile, by the 32 lanes of a warp: lanes split the row's 16-byte chunks.
 template <int DP>
 __device__ __forceinline__ void zero_row(uint8_t* tile, int r, int lane) {

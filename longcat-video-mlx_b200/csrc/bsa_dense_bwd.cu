@@ -250,15 +250,6 @@ struct Ring {
   }
 };
 
-// Waits that every load issued into a ring has landed (after an expired wait, before the CTA ends).
-__device__ __forceinline__ void drain_ring(uint64_t* full, int stages, int issued) {
-  const uint64_t t0 = globaltimer_ns();
-  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
-    while (!mbar_try_wait(&full[i % stages], static_cast<uint32_t>((i / stages) & 1)) &&
-           globaltimer_ns() - t0 < kWaitLimitNs) {
-    }
-}
-
 // Products of a 128 x N accumulator: A and B along d (K-major both), or A in tensor memory (two runs of 32 columns at
 // `a` and `a` + 64, 64 values of K each) and B by rows.
 template <int DP>
@@ -475,11 +466,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       Ring<S::kQ> rq;
       Ring<S::kG> rg;
-      int n = 0, fixes = 0;
-      const bool ok = walk([&](int g, int i, const int4& t) {
+      int nq = 0, ng = 0, fixes = 0;
+      bool fixing = false;
+      walk([&](int g, int i, const int4& t) {
         const int h = hk * p.G + g;
         bool w = true;
-        if (n >= S::kQ) w = bar_wait(&ss.q_empty[rq.slot], rq.phase ^ 1u, abort_flag, err, 401);
+        if (nq >= S::kQ) w = bar_wait(&ss.q_empty[rq.slot], rq.phase ^ 1u, abort_flag, err, 401);
         if (!__all_sync(0xffffffffu, w)) return false;
         const bool fix = t.w <= 0;  // rows without keys, whose q and do may hold anything
         uint8_t* q = sQ + rq.slot * kBytes;
@@ -498,7 +490,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (fix) {
           __syncwarp();
           w = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 402);
-          if (!__all_sync(0xffffffffu, w)) return false;
+          fixing = !__all_sync(0xffffffffu, w);
+          if (fixing) return false;
           ++fixes;
           for (int r = 0; r < kTile; ++r)
             if (ss.rng[rq.slot][r].x >= ss.rng[rq.slot][r].y) zero_row<DP>(q, r, lane);
@@ -506,7 +499,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&ss.q_full[rq.slot]);
         }
-        if (n >= S::kG) w = bar_wait(&ss.g_empty[rg.slot], rg.phase ^ 1u, abort_flag, err, 403);
+        ++nq;
+        if (ng >= S::kG) w = bar_wait(&ss.g_empty[rg.slot], rg.phase ^ 1u, abort_flag, err, 403);
         if (!__all_sync(0xffffffffu, w)) return false;
         uint8_t* go = sG + rg.slot * kBytes;
         if (elect_one()) {
@@ -517,7 +511,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (fix) {
           __syncwarp();
           w = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 404);
-          if (!__all_sync(0xffffffffu, w)) return false;
+          fixing = !__all_sync(0xffffffffu, w);
+          if (fixing) return false;
           ++fixes;
           for (int r = 0; r < kTile; ++r)
             if (ss.rng[rq.slot][r].x >= ss.rng[rq.slot][r].y) zero_row<DP>(go, r, lane);
@@ -525,15 +520,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&ss.g_full[rg.slot]);
         }
-        ++n;
+        ++ng;
         rq.next();
         rg.next();
         return true;
       });
-      if (!ok && lane == 0) {
-        drain_ring(&ss.kv_full, 1, 1);
-        drain_ring(ss.q_full, S::kQ, n + 1);
-        drain_ring(ss.g_full, S::kG, n);
+      if (lane == 0) {
+        drain(&ss.kv_full, 0);
+        drain_ring(ss.q_full, S::kQ, nq);
+        drain_ring(ss.g_full, S::kG, ng);
+        if (fixing) drain(&ss.fix, static_cast<uint32_t>(fixes & 1));
       }
     }
     __syncwarp();
@@ -882,9 +878,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       Ring<S::kK> rk;
       Ring<S::kV> rv;
-      int n = 0, fixes = 0;
-      bool ok = true;
-      for (; n < steps; ++n) {
+      int nk = 0, nv = 0, fixes = 0;
+      bool ok = true, fixing = false;
+      for (int n = 0; n < steps; ++n) {
         if (n >= S::kK) ok = bar_wait(&ss.k_empty[rk.slot], rk.phase ^ 1u, abort_flag, err, 451);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -900,6 +896,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           __syncwarp();
           ok = bar_wait(&ss.fix, static_cast<uint32_t>(fixes & 1), abort_flag, err, 452);
           ok = __all_sync(0xffffffffu, ok);
+          fixing = !ok;
           if (!ok) break;
           ++fixes;
           for (int r = 0; r < kTile; ++r)
@@ -908,6 +905,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&ss.k_full[rk.slot]);
         }
+        ++nk;
         if (n >= S::kV) ok = bar_wait(&ss.v_empty[rv.slot], rv.phase ^ 1u, abort_flag, err, 453);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -915,13 +913,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           mbar_arrive_expect_tx(&ss.v_full[rv.slot], kBytes);
           load_tile<DP>(sV + rv.slot * kBytes, &tm_v, &ss.v_full[rv.slot], row, hk, b);
         }
+        ++nv;
         rk.next();
         rv.next();
       }
-      if (!ok && lane == 0) {
-        drain_ring(&ss.qg_full, 1, 1);
-        drain_ring(ss.k_full, S::kK, n + 1);
-        drain_ring(ss.v_full, S::kV, n);
+      if (lane == 0) {
+        drain(&ss.qg_full, 0);
+        drain_ring(ss.k_full, S::kK, nk);
+        drain_ring(ss.v_full, S::kV, nv);
+        if (fixing) drain(&ss.fix, static_cast<uint32_t>(fixes & 1));
       }
     }
     __syncwarp();
