@@ -67,7 +67,7 @@ __device__ __forceinline__ void load_weight(const void* w, int w_dtype, int d0, 
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (w_dtype == BSA_DTYPE_F32)
-      f[e] = __ldg(static_cast<const float*>(w) + d0 + e);
+      f[e] = static_cast<const float*>(w)[d0 + e];
     else if (w_dtype == BSA_DTYPE_F16)
       f[e] = __half2float(static_cast<const __half*>(w)[d0 + e]);
     else
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, kBackward && sizeof(T) == 2 ? 4 : 0)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float* at = cos_at[e] + (axis[e] == 0 ? t : axis[e] == 1 ? h : w) * step[e];
-        const float c = __ldg(at), sn = __ldg(at + sin_off[e]);
+        const float c = at[0], sn = at[sin_off[e]];
         cw[e] = f2_pack(c, c);
         sw[e] = kBackward ? f2_pack(sn, -sn) : f2_pack(-sn, sn);
       }

@@ -1,4 +1,5 @@
-// Eight consecutive values of a row: 16-byte loads and stores, fp32 in registers.
+// Eight consecutive values of a row: 16-byte loads and stores, fp32 in registers.  The loads are plain ones: a kernel that
+// begins before the one in front of it has ended (bsa_dense.h) may read what that one writes.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -29,7 +30,7 @@ __device__ __forceinline__ void unpack_pair(uint32_t u, float& lo, float& hi, __
 template <typename T>
 struct Row8 {
   uint4 u;
-  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float* f) const {
     unpack_pair(u.x, f[0], f[1], T());
@@ -64,8 +65,8 @@ template <>
 struct Row8<float> {
   float4 a, b;
   __device__ __forceinline__ void load(const float* p) {
-    a = __ldg(reinterpret_cast<const float4*>(p));
-    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
   }
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void get(float* f) const {

@@ -336,3 +336,16 @@ def test_the_model_sees_a_load_left_behind(kernel, stages):
         except AssertionError:
             found += 1
     assert found
+
+
+def test_kernels_behind_another_read_coherently():
+    """A kernel that may begin before the one in front of it has ended reads what that one wrote: its loads are ordered by
+    after_previous().  Loads of read-only memory are not, and may be moved in front of it."""
+    import os
+
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "longcat-video-mlx_b200", "csrc")
+    behind = [f for f in os.listdir(src) if f.endswith(".cu") and "after_previous()" in open(os.path.join(src, f)).read()]
+    assert {"bsa_normrope.cu", "bsa_kv8.cu", "bsa_dense.cu"} <= set(behind)
+    for f in (*behind, "bsa_rows.cuh", "bsa_dense.cuh"):
+        text = open(os.path.join(src, f)).read()
+        assert "__ldg" not in text and ".nc." not in text and "__restrict__" not in text, f
