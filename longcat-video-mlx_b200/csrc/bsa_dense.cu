@@ -11,13 +11,13 @@
 // both products and the loads of K and V move 128 KB a step through shared memory, 160 KB with Q there too.  S(j+3)
 // is issued when S(j+1) has been read, behind P(j) V, two steps before it is needed.
 //
-// Roles (384 threads, one CTA to an SM):
+// Roles (320 threads, one CTA to an SM):
 //   warps 0-7 : softmax, warps 0-3 on the keys 0-63 of a step, 4-7 on 64-127, a thread on half a row.  The two threads
 //               of a row need one maximum only when one of them finds it exceeded (below), which a barrier with a vote
 //               tells; their sums join at the end.  Of its 64 scores a thread reads the next step's first 32 before
 //               it computes the exponentials of this step's last 32, so their maximum is found beside those
 //   warp 8    : issues the products: P(j) V first, which the next step's P waits for, then S(j+3)
-//   warp 9    : loads; one ring for K and V tiles in the order of their use (warps 10, 11: idle)
+//   warp 9    : loads; one ring for K and V tiles in the order of their use
 // The maximum is raised, and O and l rescaled, only when a score exceeds it by more than 2^8 (log2 8): P stays within
 // fp16's range and rounding is relative, so the result is as exact as with the true maximum.  fp16's P is multiplied by 2^7
 // (and so is l), up to 2^15: weights keep their bits down to 2^-21 of the largest and vanish below 2^-32, where 2^-25 without
@@ -43,7 +43,7 @@ namespace dense {
 
 __device__ int g_dense_err;
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 320;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kIssue = kSoftmaxWarps, kLoad = kSoftmaxWarps + 1;  // warps
 constexpr float kRescale = 8.f;  // log2

@@ -10,8 +10,7 @@ namespace dense {
 
 constexpr int kTile = 128;  // rows of a query tile and of a key tile
 
-// Bounded wait like mbar_wait, wholly inline: a kernel that gives its registers from one group of warps to another
-// (setmaxnreg) cannot hold them across calls.
+// Bounded wait like mbar_wait, wholly inline: a call would spill what the softmax warps hold in registers.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int site) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
