@@ -47,6 +47,16 @@ int check_16bit(int dtype) {
   return BSA_OK;
 }
 
+// The kernels take sm_scale log2(e), twice its quotient by the cap, and cap log2(e) in fp32
+int check_scales(float sm_scale, float softcap) {
+  if (!(sm_scale > 0.f) || std::isinf(sm_scale)) return set_error(BSA_ERR_ARG, "sm_scale must be positive and finite");
+  if (!(softcap >= 0.f) || std::isinf(softcap)) return set_error(BSA_ERR_ARG, "softcap must be finite and >= 0");
+  const float log2e = 1.4426950408889634f, scale_log2 = sm_scale * log2e;
+  if (std::isinf(scale_log2) || (softcap > 0.f && (std::isinf(2.f * scale_log2 / softcap) || std::isinf(softcap * log2e))))
+    return set_error(BSA_ERR_ARG, "sm_scale %g with softcap %g is out of fp32's range", sm_scale, softcap);
+  return BSA_OK;
+}
+
 int sm_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -136,8 +146,7 @@ int dense_plan(bsa::DenseArgs& a, const void* q, const void* k, const void* v, i
   if (Sq > kMostRows || Sk > kMostRows) return set_error(BSA_ERR_SHAPE, "more than %d tokens", kMostRows);
   if (H % Hk) return set_error(BSA_ERR_SHAPE, "%d query heads are no multiple of %d key heads", H, Hk);
   if ((rc = check_head_dim(D))) return rc;
-  if (!(sm_scale > 0.f) || std::isinf(sm_scale)) return set_error(BSA_ERR_ARG, "sm_scale must be positive and finite");
-  if (!(softcap >= 0.f) || std::isinf(softcap)) return set_error(BSA_ERR_ARG, "softcap must be finite and >= 0");
+  if ((rc = check_scales(sm_scale, softcap))) return rc;
   if ((ranges == nullptr) != (table == nullptr)) return set_error(BSA_ERR_ARG, "ranges come with their table");
   if (ranges && ranges_batch != 1 && ranges_batch != B)
     return set_error(BSA_ERR_SHAPE, "ranges of %d batch entries for a batch of %d", ranges_batch, B);
@@ -369,7 +378,7 @@ int bsa_kv8_attention(const void* q, int dtype, int B, int H, int Sq, const int6
   if (!q_strides || !out_strides) return set_error(BSA_ERR_ARG, "null pointer");
   if (H <= 0 || Sq <= 0) return set_error(BSA_ERR_SHAPE, "empty tensor");
   if (H % Hk) return set_error(BSA_ERR_SHAPE, "%d query heads are no multiple of %d key heads", H, Hk);
-  if (!(sm_scale > 0.f) || std::isinf(sm_scale)) return set_error(BSA_ERR_ARG, "sm_scale must be positive and finite");
+  if ((rc = check_scales(sm_scale, 0.f))) return rc;
   const long long rows = static_cast<long long>(H / Hk) * Sq;
   if (rows > INT_MAX || static_cast<long long>(B) * Hk * ((rows + 15) / 16) > 65535)
     return set_error(BSA_ERR_SHAPE, "too many query rows for the cache's few-row kernel");

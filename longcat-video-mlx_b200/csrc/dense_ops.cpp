@@ -444,6 +444,7 @@ void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v) {
 void check_scale(double sm_scale, double softcap) {
   if (!(sm_scale > 0) || std::isinf(sm_scale)) refuse("sm_scale must be positive and finite");
   if (!(softcap >= 0) || std::isinf(softcap)) refuse("softcap must be finite and >= 0");
+  if (softcap > 0 && static_cast<float>(softcap) == 0.f) refuse("softcap is out of fp32's range");
 }
 
 // Whether views share bytes.  A place of a view is its base and a sum of strides times indexes, so two views meet where

@@ -316,3 +316,12 @@ def test_cache_without_heads_is_refused(cuda):
         KVCache8.allocate(1, 0, 64, 64, cuda)
     with pytest.raises(ValueError, match="heads"):
         KVCache8.from_kv(*(torch.empty((1, 0, 5, 64), dtype=torch.bfloat16, device=cuda) for _ in range(2)))
+
+
+def test_a_cap_below_every_float_is_refused(cuda):
+    """It would be rounded to 0, which means no cap."""
+    from longcat_video.models.masked_attention import masked_attention
+
+    x = rand((1, 1, 4, 16), torch.bfloat16, 1, cuda)
+    with pytest.raises(ValueError, match="softcap"):
+        masked_attention(x, x, x, softcap=1e-60)

@@ -349,3 +349,19 @@ def test_kernels_behind_another_read_coherently():
     for f in (*behind, "bsa_rows.cuh", "bsa_dense.cuh"):
         text = open(os.path.join(src, f)).read()
         assert "__ldg" not in text and ".nc." not in text and "__restrict__" not in text, f
+
+
+@pytest.mark.parametrize("scale,cap", [(3e38, 0.0), (1.0, 1e-39), (1e30, 1e-12), (1.0, 3e38)])
+def test_scales_whose_products_overflow(lib, scale, cap):  # noqa: F811
+    """sm_scale log2(e), its quotient by the cap and cap log2(e) are fp32: an infinite one would make NaN of a score of 0."""
+    st = strides(*ST)
+    args = [FAKE, FAKE, FAKE, 2, 1, 1, 1, 64, 64, 128, st, st, st, None, None, 1, scale, cap, FAKE, st, None, None, None, None]
+    rc, msg = call(lib, "bsa_masked_attention", "pppiiiiiiisssppiffpspppp", args)
+    assert rc == 7 and "range" in msg
+    args = [*args[:3], FAKE, FAKE, FAKE, FAKE, *args[3:13], st, st, None, None, 1, scale, cap, FAKE, FAKE, FAKE, FAKE, None]
+    rc, msg = call(lib, "bsa_masked_attention_backward", "pppppppiiiiiiisssssppiffppppp", args)
+    assert rc == 7 and "range" in msg
+    if not cap:
+        args = [FAKE, 2, 1, 4, 1, st, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 128, 128, 0, scale, FAKE, st, FAKE, None]
+        rc, msg = call(lib, "bsa_kv8_attention", "piiiispppppiiiifpspp", args)
+        assert rc == 7 and "range" in msg
