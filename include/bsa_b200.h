@@ -232,7 +232,7 @@ int bsa_attention_ranges(int32_t* ranges, int32_t* table, int batch, int Sq, int
  * bsa_masked_attention_scratch_bytes() bytes (0: none needed).  Scores of unseen keys never count, whatever they
  * hold; nor do values of keys in front of, or behind, what the same 128 rows see.  A value that is infinite or NaN
  * and lies between those can reach all of the 128 rows.  At most 2^30 tokens.  out may be q; it
- * overlaps no input otherwise. */
+ * overlaps no input otherwise.  sm_scale and softcap: their products and quotient (times 2 log2(e)) are finite in fp32. */
 int64_t bsa_masked_attention_scratch_bytes(int B, int H, int Sq, int Sk, int D);
 int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype, int B, int H, int Hk, int Sq, int Sk,
                          int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
@@ -242,7 +242,9 @@ int bsa_masked_attention(const void* q, const void* k, const void* v, int dtype,
 
 /* bsa_masked_attention_backward: gradients of that call from its out, out_rest and lse and the gradient of out.
  * dq [B, H, Sq, D] and dk, dv [B, Hk, Sk, D] are contiguous; dq, or dk and dv, may be NULL.  Shared key heads sum
- * over their query heads; keys no row sees get zeros.  No atomics: the same bits every time.  scratch:
+ * over their query heads; keys no row sees get zeros.  No atomics: the same bits every time.  A value of q or grad that is
+ * infinite or NaN, in a row that sees a key, can reach dk and dv of all keys in the runs of 128 that its 128 rows see; one of k
+ * or v reaches dq as v reaches out.  fp16: finite results do not overflow on the way, whatever grad and v hold.  scratch:
  * bsa_masked_attention_backward_scratch_bytes() bytes (ranges_batch 0 without ranges). */
 int64_t bsa_masked_attention_backward_scratch_bytes(int B, int H, int Sq, int ranges_batch);
 int bsa_masked_attention_backward(const void* q, const void* k, const void* v, const void* out, const void* out_rest,
@@ -253,8 +255,9 @@ int bsa_masked_attention_backward(const void* q, const void* k, const void* v, c
                                   void* dk, void* dv, void* scratch, void* stream);
 
 /* 8-bit key/value cache: codes [B, Hk, capacity, D] e4m3, contiguous, 16-byte aligned; scales
- * [B, Hk, capacity / 64] fp32, each the smallest power of two that keeps the block's codes within 448 (0: a block
- * of zeros); lengths [B] int32: tokens held.  capacity is a multiple of 64.
+ * [B, Hk, capacity / 64] fp32, each the smallest power of two that keeps the block's finite codes within 448 (0: a block
+ * of zeros; 2^-126 at least where a value is infinite, held as +-448, or NaN); lengths [B] int32: tokens held.  capacity is a
+ * multiple of 64.
  * bsa_kv8_append: n new tokens (fp16 or bf16; counts [B]: only the first counts[b] of them) behind those held;
  * lengths advance.  Tokens past the capacity are dropped and reported by bsa_device_error (BSA_ERR_INDEX).
  * Rows behind the last token keep what they hold.
@@ -262,7 +265,8 @@ int bsa_masked_attention_backward(const void* q, const void* k, const void* v, c
  * ends there), as [B, Hk, rows, D] in dtype.
  * bsa_kv8_attention: q [B, H, Sq, D] over the held tokens, straight from the codes; causal: query i sees
  * lengths[b] - Sq + i + 1 tokens.  Meant for few rows (H / Hk * Sq up to about 128): 16 rows are one pass over the
- * codes.  scratch: bsa_kv8_attention_scratch_bytes() bytes (0: none needed). */
+ * codes, and a value of NaN that one of them sees can reach all 16.  scratch: bsa_kv8_attention_scratch_bytes() bytes
+ * (0: none needed). */
 int bsa_kv8_append(void* k_codes, float* k_scale, void* v_codes, float* v_scale, int32_t* lengths, int B, int Hk,
                    int capacity, int D, const void* k, const void* v, int dtype, int n, const int64_t* k_strides,
                    const int64_t* v_strides, const int32_t* counts, void* stream);

@@ -12,7 +12,8 @@ kernel instead of being applied as a separate pass.
 
 With ``dense_kernels`` on, what is not block-sparse runs on the engine's own kernels too, with gradients:
 q/k norm and RoPE in one launch, dense attention, the conditioning branch as one call under a prefix
-mask, and the chunked continuation over a :class:`KVCache8`.
+mask, and the chunked continuation over a :class:`KVCache8`.  With BSA and conditioning frames both, the frames' part of the
+attention is the engine's, norm and RoPE stay separate passes.
 """
 
 from __future__ import annotations

@@ -74,7 +74,8 @@ class KVCache8:
 
         A block whose largest value grows takes a larger scale, and its codes are rounded again at it.  Tokens that
         do not fit are dropped, and ``_native.device_error()`` then reports it; more tokens than the whole capacity
-        are refused here.  Infinities are held as the block's largest code, NaN as NaN; neither sets a scale."""
+        are refused here.  Infinities are held as the block's largest code, NaN as NaN; neither sets a scale, but that a
+        block with either has the smallest one (2^-126) at least.  What is held is constant to gradients."""
         self._cache.append(k, v, counts)
 
     def truncate(self, lengths: Union[int, torch.Tensor]) -> None:
@@ -100,5 +101,7 @@ class KVCache8:
 
         ``causal``: the last query sees every key (held, then fresh), the one before it one less, and so on.
         sm_scale defaults to 1 / sqrt(D).  Sequences without a key give zeros.  Few rows read the codes as they are;
-        many rows, or fresh keys, unpack the cache into 16-bit scratch first."""
+        many rows, or fresh keys, unpack the cache into 16-bit scratch first.  What lies behind the held tokens does not
+        matter; a value of NaN that is held, or infinite or NaN among the fresh ones, reaches the rows that see it and,
+        with ``causal``, can reach earlier rows of the same pass: 16 of them, or 128 where the cache is unpacked."""
         return self._cache.attend(q, k, v, causal, sm_scale, out, FEW_ROWS)

@@ -1,7 +1,8 @@
 """Dense attention over key intervals: document, prefix, causal and padding masks, scores capped by a tanh.
 
 The dense side of the attention hook on the engine's own kernels.  A mask is a key interval [lo, hi) for each
-query row (:class:`AttentionMask`), built once for a batch and used by every layer; no Sq x Sk tensor exists.
+query row (:class:`AttentionMask`), which one build (a small launch) makes for as many calls as share it; no Sq x Sk
+tensor exists.
 ``masked_attention`` is differentiable, once (``create_graph=True`` is refused, and so is forward mode); its gradients
 are computed without atomics, so two runs give the same bits.
 """
@@ -84,9 +85,10 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Op
     log-sum-exp [B, H, Sq] (fp32, natural) that ``return_lse`` adds; it carries no gradient.  ``out``: a
     preallocated [B, H, Sq, D] result, which may be q; over another input, or itself, it is refused (so with gradients).
 
-    What masked places hold does not matter, with one limit: a value that is infinite or NaN, in a row of v (for
-    gradients, of k too) between the first and the last key that some row of the same 128 queries sees, can reach all
-    of those queries."""
+    What masked places hold does not matter, with limits for values that are infinite or NaN: in a row of v (for
+    gradients, of k too) between the first and the last key that some row of the same 128 queries sees, they can reach all
+    of those queries; in a row of q or of the output's gradient that sees a key, they can reach the gradients of all keys
+    in the runs of 128 that some row of the same 128 queries sees.  Rows that see nothing may hold anything."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale
     args = _NO_MASK if mask is None else mask._args()
     o, lse = _dense.ops().masked_attention(q, k, v, *args, scale, softcap, out, return_lse)
