@@ -11,7 +11,7 @@
 // for D > 64, else 8) holds one row, 8 values (16 bytes of bf16) to a lane, as pairs for the packed fp32
 // instructions.  A CTA keeps to one group of kHeads heads and walks over tokens, so that the weights, and what a lane
 // needs of the angle tables, stay in registers, and a token's angles are used for all heads of the group:
-// with w folded into them a row costs 3 packed operations a pair.  86,400 tokens x 32 heads: 5.35 TB/s of 6.54 measured (with
+// with w folded into them a row costs 3 packed operations a pair.  86,400 tokens x 32 heads: 5.4 TB/s of 6.54 measured (with
 // the addresses worked out for each token and 4 heads, and scalar arithmetic, 240 instructions a row and warp: 4.1).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -93,9 +93,9 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// Rows in flight: 4 forward (8: 279 us at 720p x 16 heads, 4: 264, 2: 307); 2 backward, where they leave registers
-// for 4 CTAs to an SM (6 frames x 32 heads, both passes: 4 rows and 2 CTAs 213 us, 2 and 2 202, 2 and 4 181).  Reading the
-// next rows before this step's arithmetic costs more registers than it hides (the same: 9 to 58 us more).
+// Rows in flight: 4 forward (8: 306 us at 720p x 16 heads, 4: 263, 2: 301); 2 backward, where they leave registers
+// for 4 CTAs to an SM (6 frames x 32 heads, both passes: 2 rows and 2 CTAs 174 us, 2 and 4 162 to 167, 4 and 2 162).  Reading
+// the next rows before this step's arithmetic costs more registers than it hides (the same: 9 to 58 us more).
 template <typename T, int kLanes, bool kBackward>
 __global__ void __launch_bounds__(kThreads, kBackward && sizeof(T) == 2 ? 4 : 0) norm_rope_kernel(const Params p) {
   constexpr int kBatch = kBackward ? 2 : 4;
