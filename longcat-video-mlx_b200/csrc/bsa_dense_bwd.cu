@@ -1178,7 +1178,7 @@ int launch_dense_backward(const DenseArgs& a, int sms, cudaStream_t stream) {
   p.up = reinterpret_cast<int*>(a.stats + (2ll * p.heads + (a.ranges ? 2ll * a.Bm : 0)) * p.Sq_pad);
   p.v_up = p.up + static_cast<long long>(p.heads) * (p.Sq_pad + p.Sq_pad / 16);
   p.v_bin = 64 * ((a.Sk + 64 * kBins - 1) / (64 * kBins));
-  p.v_bins = (a.Sk + p.v_bin - 1) / p.v_bin;
+  p.v_bins = a.dq.p ? (a.Sk + p.v_bin - 1) / p.v_bin : 0;  // only dq reads them
   p.v = a.v;
   p.lse = a.lse;
   p.o = a.o;
